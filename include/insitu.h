@@ -195,6 +195,19 @@ int insitu_attend_causal_head(insitu_cache *cache, int32_t seq, int32_t kv_head,
                               int64_t n_q, const int32_t *q_rot_dev, int32_t *out_dev, int32_t mode,
                               insitu_stats *stats_host);
 
+/* The queries of a tree of drafted tokens, for every sequence at once (speculative decoding; no
+ * counterpart in the reference). The last n rows of every sequence are the tree's nodes, appended
+ * in an order where each parent comes before its children: node i attends the rows before the n and,
+ * of the n, its ancestors and itself, in row order, exactly as decode steps along its path would
+ * (SEQUENTIAL and SPLIT, or TWO_PASS; SERIAL token by token). n is 1 .. 256. parents_dev int32 (n),
+ * or (batch, n) with per_sequence = 1: the parent's number, or -1 for a child of the context; any
+ * other value counts as -1 and as a range error (statistics). q_rot_dev int32 (batch, n, n_q_heads,
+ * d) rotated; out_dev int32, the same shape, Q16. EBADLEN when a sequence holds fewer than n rows.
+ * stats_host may be NULL: then nothing synchronises, and once a call of the shape has allocated the
+ * cache's scratch nothing allocates either. */
+int insitu_attend_tree(insitu_cache *cache, int32_t n, const int32_t *parents_dev, int32_t per_sequence,
+                       const int32_t *q_rot_dev, int32_t *out_dev, int32_t mode, insitu_stats *stats_host);
+
 /* insitu_attend_causal without allocating: no counterpart in the reference; for callers
  * that cannot call hipMalloc (tight serving loops, harnesses that forbid it). The same
  * launches and results as insitu_attend_causal, but the chunk scratch and the lengths of
@@ -247,6 +260,32 @@ int insitu_project_seam(insitu_ctx *ctx, const uint16_t *w_dev, int32_t in_f, co
                         int32_t frac, double attn_scale, int32_t cast_after_rope, float *p_dev, int32_t *q_dev,
                         int32_t *k_dev, int32_t *v_dev, unsigned long long *counts_host);
 
+/* insitu_seam_wire for the models whose queries and keys are normed a head and for the other forms of
+ * rotary positions (no counterpart in the reference's seam; its QK-norm is ops/norm.py). */
+typedef struct {
+    int32_t n_q, n_kv, d;          /* d a power of two in 16..128                              */
+    int32_t rotary_dim;            /* channels 0 .. rotary_dim - 1 of a head are rotated, the
+                                      others only cast: even, 2 .. d                           */
+    int32_t interleaved;           /* 0: channel j pairs with j + rotary_dim / 2; 1: 2 j with
+                                      2 j + 1                                                  */
+    int32_t frac, cast_after_rope; /* as insitu_seam_wire                                      */
+    double attn_scale, norm_eps;   /* norm_eps > 0 where there are norms                       */
+    const float *bias_dev;         /* ((n_q + 2 n_kv) d) or NULL                               */
+    const float *q_norm_dev;       /* (d) the norm's weights of every query head, or NULL: none */
+    const float *k_norm_dev;       /* the keys'                                                */
+    const int64_t *cos_dev;        /* (max_pos, rotary_dim / 2) Q(frac)                        */
+    const int64_t *sin_dev;
+    int64_t max_pos;
+} insitu_seam_desc;
+/* p_dev fp32 (n, (n_q + 2 n_kv) d), the q|k|v projections; a query or key head becomes
+ * x / sqrt(mean(x^2) + norm_eps) * weight in float64 (x the projection plus the bias in fp32),
+ * then the attention scale on q, the rotation and the cast as insitu_seam_wire, whose rows it
+ * gives bit for bit where there are no norms and rotary_dim = d in half pairs. pos_dev, pos0,
+ * q/k/v_dev and counts_host as there; outputs do not overlap inputs. n (n_q + 2 n_kv) < 2^31. */
+int insitu_seam_heads(insitu_ctx *ctx, const insitu_seam_desc *desc, const float *p_dev, int64_t n,
+                      const int64_t *pos_dev, int64_t pos0, int32_t *q_dev, int32_t *k_dev, int32_t *v_dev,
+                      unsigned long long *counts_host);
+
 /* The output side (kernel.py:348-356): out_dev int32 (n, width) Q(frac) -> float ->
  * fp16, then y_dev fp32 (n, hidden) = that @ wo_dev^T + bias_dev with W_o' fp16
  * (hidden, width), R^-1 folded in (ops/output.py:49-78). bias_dev may be NULL. */
@@ -265,6 +304,22 @@ int insitu_read_rows(insitu_cache *cache, int32_t seq, int32_t head, int64_t t0,
                      uint8_t *rows_host);
 int insitu_load_rows(insitu_cache *cache, int32_t seq, int32_t head, int64_t t0, int64_t n,
                      const uint8_t *rows_host);
+
+/* Sequences that continue others (n-best answers, beams, branches of a draft; no counterpart in the
+ * reference, whose cache holds one sequence). Sequence dst_host[i] becomes a copy of sequence
+ * src_host[i], i < n_copies: all its rows (n = 0), or the rows before its last n and then, in the
+ * order given, counts_host[i] of those n, row rows_dev[i * rows_stride + j] as number j (0 .. n - 1;
+ * a value outside is taken as the nearest one inside). rows_stride 0: one list for all. The
+ * destinations are different sequences, none of them a source. Rows behind the new length stay as
+ * they are. Stream-ordered; nothing synchronises. */
+int insitu_cache_fork(insitu_cache *cache, int32_t n_copies, const int32_t *src_host, const int32_t *dst_host,
+                      int64_t n, const int32_t *rows_dev, int64_t rows_stride, const int64_t *counts_host);
+/* Of the last n rows of every sequence, the listed ones (as insitu_cache_fork's lists, a list a
+ * sequence, in any order) become the first, in place, and the sequence ends behind them: the accepted
+ * path of a draft. counts_host (batch), or NULL: none is kept and rows_dev is not read. More than
+ * 1,024 rows of a sequence go through a buffer of the cache, which the first such call allocates. */
+int insitu_cache_keep(insitu_cache *cache, int64_t n, const int32_t *rows_dev, int64_t rows_stride,
+                      const int64_t *counts_host);
 
 /* The raw plane image of one sequence (DdrLayout.image / CMD_LOAD, ddr_layout.py:227-248):
  * nbytes must equal insitu_layout.seq_stride. Synchronous. */

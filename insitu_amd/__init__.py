@@ -12,6 +12,10 @@ Python host side that mirrors the reference's interfaces:
     CompressedAttention, AttentionStats     ops/attention.py
     AttentionBlock, StepReport              kernel.py (forward, both halves)
     Weights, HostHalf, RoPE, RopeScaling    weights.py, ops/rope.py, kernel.py:198-249
+
+and beside them Seam, LinearScaling and YarnScaling (norms of queries and keys, the other
+forms of rotary positions), CompressedAttention.attend_tree, CompressedCache.fork and keep
+and AttentionBlock.forward_tree and accept (drafted tokens).
 """
 
 from .config import FixedFormat, ModelConfig, QuantConfig
@@ -20,7 +24,7 @@ from .codebook import Codebook
 __all__ = ["FixedFormat", "ModelConfig", "QuantConfig", "Codebook", "Rotation",
            "KVCache", "CompressedCache", "CompressedKV", "CompressedAttention",
            "AttentionStats", "AttentionBlock", "StepReport", "Weights", "HostHalf", "RoPE",
-           "RopeScaling"]
+           "RopeScaling", "LinearScaling", "YarnScaling", "Seam"]
 
 
 def __getattr__(name):
@@ -38,7 +42,7 @@ def __getattr__(name):
     if name in ("AttentionBlock", "StepReport"):
         from . import block
         return getattr(block, name)
-    if name in ("Weights", "HostHalf", "RoPE", "RopeScaling"):
+    if name in ("Weights", "HostHalf", "RoPE", "RopeScaling", "LinearScaling", "YarnScaling", "Seam"):
         from . import host
         return getattr(host, name)
     raise AttributeError(name)

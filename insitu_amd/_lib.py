@@ -31,7 +31,7 @@ EXPORTS = (
     "insitu_cache_create", "insitu_cache_destroy", "insitu_cache_reset", "insitu_cache_length",
     "insitu_cache_set_length", "insitu_cache_layout", "insitu_append", "insitu_append_seq",
     "insitu_append_wire", "insitu_attend", "insitu_attend_causal", "insitu_attend_causal_head", "insitu_attend_causal_static", "insitu_step", "insitu_project", "insitu_seam_wire",
-    "insitu_project_seam",
+    "insitu_project_seam", "insitu_seam_heads", "insitu_attend_tree", "insitu_cache_fork", "insitu_cache_keep",
     "insitu_output_projection", "insitu_read_rows", "insitu_load_rows", "insitu_read_image",
     "insitu_load_image", "insitu_probe_read", "insitu_probe_empty", "insitu_cache_debug",
     "insitu_cache_stats",
@@ -84,6 +84,16 @@ class Stats(ctypes.Structure):
         "max_abs_acc", "range_errors", "serial_fallbacks")]
 
 
+class SeamDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_q", "n_kv", "d", "rotary_dim", "interleaved", "frac",
+                                              "cast_after_rope")] + \
+        [("attn_scale", ctypes.c_double), ("norm_eps", ctypes.c_double)] + \
+        [(n, ctypes.c_void_p) for n in ("bias_dev", "q_norm_dev", "k_norm_dev", "cos_dev", "sin_dev")] + \
+        [("max_pos", ctypes.c_int64)]
+
+
+TREE_NODES = 256         # nodes of a tree of drafted tokens, at most
+
 _lib = None
 
 
@@ -130,6 +140,10 @@ def load(path: str | None = None):
                                    ctypes.c_double, i32, vp, vp, vp, P(ctypes.c_uint64)]),
         "insitu_project_seam": (i32, [vp, vp, i32, vp, i64, vp, i32, i32, i32, vp, i64, vp, vp, i64, i32,
                                       ctypes.c_double, i32, vp, vp, vp, vp, P(ctypes.c_uint64)]),
+        "insitu_seam_heads": (i32, [vp, P(SeamDesc), vp, i64, vp, i64, vp, vp, vp, P(ctypes.c_uint64)]),
+        "insitu_attend_tree": (i32, [vp, i32, vp, i32, vp, vp, i32, P(Stats)]),
+        "insitu_cache_fork": (i32, [vp, i32, P(i32), P(i32), i64, vp, i64, P(i64)]),
+        "insitu_cache_keep": (i32, [vp, i64, vp, i64, P(i64)]),
         "insitu_output_projection": (i32, [vp, vp, i64, i32, i32, vp, i32, vp, vp]),
         "insitu_step": (i32, [vp, vp, vp, vp, vp, i32, P(Stats)]),
         "insitu_read_rows": (i32, [vp, i32, i32, i64, i64, vp]),

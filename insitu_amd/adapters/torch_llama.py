@@ -27,12 +27,14 @@ the reference keeps it:
 Differences from the reference, by construction: the host half runs its fp32
 GEMVs on the GPU, so a wire row can differ from the reference's numpy float
 order by up to 2 Q8.16 LSB in a few lanes (below the seam everything is
-bit-exact for the same wire rows); QK-norm models, the dense fp16 baseline
-(compressed=False) and the reference's hardware model (hw) are refused with
-NotImplementedError rather than approximated.
+bit-exact for the same wire rows); the dense fp16 baseline (compressed=False),
+the reference's hardware model (hw) and norms of queries and keys that are not an
+RMS norm of each head are refused with NotImplementedError rather than approximated.
 """
 
 from __future__ import annotations
+
+import dataclasses
 
 import numpy as np
 import torch
@@ -98,6 +100,35 @@ class KernelAttention(nn.Module):
         self.kernel.reset()
 
 
+def _head_norms(attn_module, m: ModelConfig):
+    """The module's q_norm and k_norm as (weights or None, weights or None, eps). Each has to be
+    x / sqrt(mean(x^2) + eps) * weight over a head's channels, which one row shows: there are norms
+    with a mean, a bias, 1 + weight or a whole projection's width."""
+    weights, eps = [], []
+    for name in ("q_norm", "k_norm"):
+        norm = getattr(attn_module, name, None)
+        if norm is None:
+            weights.append(None)
+            continue
+        w = getattr(norm, "weight", None)
+        e = next((float(getattr(norm, a)) for a in ("variance_epsilon", "eps") if getattr(norm, a, None) is not None),
+                 None)
+        if w is None or tuple(w.shape) != (m.head_dim,) or e is None or not e > 0:
+            raise NotImplementedError(f"QK-norm: {name} ({type(norm).__name__}) is not an RMS norm of each head")
+        x = torch.linspace(-1.0, 2.0, m.head_dim, dtype=torch.float32)
+        with torch.no_grad():
+            got = norm(x.to(device=w.device, dtype=w.dtype)).float().cpu()
+        want = x.to(w.dtype).float()
+        want = want * torch.rsqrt(want.square().mean() + e) * w.detach().float().cpu()
+        if not torch.allclose(got, want, rtol=8 * torch.finfo(w.dtype).eps, atol=8 * torch.finfo(w.dtype).eps):
+            raise NotImplementedError(f"QK-norm: {name} ({type(norm).__name__}) is not an RMS norm of each head")
+        weights.append(w)
+        eps.append(e)
+    if len(set(eps)) > 1:
+        raise NotImplementedError(f"QK-norm: queries and keys with different eps {eps}")
+    return weights[0], weights[1], eps[0] if eps else m.qk_norm_eps
+
+
 def build_from_layer(attn_module, model_config, *, quant: QuantConfig | None = None,
                      fmt: FixedFormat | None = None, hw=None, capacity: int = 4096,
                      compressed: bool = True, layer_idx: int = 0, softmax: str = "two_pass",
@@ -113,9 +144,9 @@ def build_from_layer(attn_module, model_config, *, quant: QuantConfig | None = N
     if hw is not None:
         raise NotImplementedError("hw configures the reference's systolic-array model; the GPU "
                                   "block has no counterpart")
-    if getattr(attn_module, "q_norm", None) is not None or getattr(attn_module, "k_norm", None) is not None:
-        raise NotImplementedError("QK-norm (q_norm / k_norm) is not modelled by the GPU host half")
     m = ModelConfig.from_hf(model_config)
+    q_norm, k_norm, eps = _head_norms(attn_module, m)
+    m = dataclasses.replace(m, qk_norm_eps=eps)
     block = AttentionBlock(m, quant or QuantConfig(), fmt, capacity=capacity, softmax=softmax, ctx=ctx)
 
     def w(name):
@@ -125,7 +156,8 @@ def build_from_layer(attn_module, model_config, *, quant: QuantConfig | None = N
         return getattr(attn_module, f"{name}_proj").bias
 
     block.weights = Weights(w("q"), w("k"), w("v"), w("o"), m, block.rotation,
-                            q_bias=b("q"), k_bias=b("k"), v_bias=b("v"), o_bias=b("o"), ctx=block.ctx)
+                            q_bias=b("q"), k_bias=b("k"), v_bias=b("v"), o_bias=b("o"),
+                            q_norm=q_norm, k_norm=k_norm, ctx=block.ctx)
     return KernelAttention(block, layer_idx=layer_idx)
 
 

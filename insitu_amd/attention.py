@@ -82,6 +82,55 @@ class CompressedAttention:
         self._keep = q
         return out, (AttentionStats.from_c(st) if st is not None else None)
 
+    # -- a tree of drafted tokens -------------------------------------------------
+
+    def check_parents(self, parents, n: int):
+        """A tree's parents, (n,) or (batch, n), as attend_tree takes them: int32 on the device."""
+        import torch
+        if not isinstance(parents, torch.Tensor) or not parents.is_cuda:
+            host = np.asarray(parents, dtype=np.int64)
+            if host.shape and (np.any(host >= np.arange(host.shape[-1])) or np.any(host < -1)):
+                raise ValueError("a node's parent is an earlier node, or -1")
+            parents = host
+        par = self.ctx.to_device(parents, torch.int32)
+        if tuple(par.shape) not in ((n,), (self.cache.batch, n)):
+            raise ValueError(f"parents must be ({n},) or ({self.cache.batch}, {n}), got {tuple(par.shape)}")
+        return par
+
+    def attend_tree(self, q_rot, parents, mode: str = "online", out=None, stats: bool = True):
+        """The queries of a tree of drafted tokens whose rows are the last n of every sequence, in an
+        order where parents come first: q_rot (batch, n, n_q_heads, d) rotated, or (n, n_q_heads, d)
+        of a batch of one; parents (n,) for every sequence or (batch, n): the parent's number, or -1
+        for a child of the context (at most 256 nodes). Node i attends the rows before the n, its
+        ancestors and itself: the integers that decode steps along its path would give, in
+        every mode. Returns (out torch int32 of q_rot's shape, AttentionStats or None).
+        Host parents are checked; a device tensor's bad values count as -1 (range_errors). With
+        stats=False nothing synchronises."""
+        import torch
+        c = self.cache
+        q = self.ctx.to_device(q_rot, torch.int32)
+        lone = q.dim() == 3 and c.batch == 1
+        if lone:
+            q = q.unsqueeze(0)
+        if q.dim() != 4 or q.shape[0] != c.batch or tuple(q.shape[2:]) != (c.n_q_heads, c.head_dim):
+            raise ValueError(f"q_rot must be ({c.batch}, n, {c.n_q_heads}, {c.head_dim}), got {tuple(q.shape)}")
+        n = int(q.shape[1])
+        par = self.check_parents(parents, n)
+        if out is None:
+            out = torch.empty_like(q)
+        elif tuple(out.shape) not in (tuple(q.shape), tuple(q.shape[1:]) if lone else ()) or \
+                out.dtype != torch.int32 or not out.is_contiguous() or out.device != q.device:
+            raise ValueError(f"out must be a contiguous int32 tensor {tuple(q.shape)} on {q.device}")
+        st = _lib.Stats() if stats else None
+        with self.ctx.ordered(q, par, out):
+            _lib.check(self.ctx.lib.insitu_attend_tree(c.handle, n, ptr(par), 1 if par.dim() == 2 else 0, ptr(q),
+                                                       ptr(out), _lib.MODES[mode],
+                                                       ctypes.byref(st) if st is not None else None))
+        self._keep = (q, par)
+        if lone and out.dim() == 4:
+            out = out[0]
+        return out, (AttentionStats.from_c(st) if st is not None else None)
+
     # -- one KV head: the reference's call forms (kernel.py:317-331, 385-392) --------
 
     score_mode = "fused"     # attention.py:323: scores on the codes (architecture B)

@@ -147,6 +147,73 @@ class AttentionBlock:
         self.last_stats = st
         return out.reshape(n, m.num_heads * m.head_dim)
 
+    def step_tree(self, qi, ki, vi, parents, *, stats: bool = True):
+        """A draft of n nodes for every sequence: qi (batch, n, num_heads, d), ki/vi (batch, n,
+        num_kv_heads, d) wire Q8.16, in an order where parents come first; parents as
+        CompressedAttention.attend_tree takes them. Rotates all three, appends the n rows, then each
+        node attends the context, its ancestors and itself: the integers of decode steps along
+        its path. Returns (batch, n, num_heads * d) Q16, a torch int32 tensor; accept() then keeps
+        the rows of the path that is taken."""
+        import torch
+        m = self.model
+        q = self.ctx.to_device(qi, torch.int32)
+        n = int(q.shape[1]) if q.dim() == 4 else -1
+        if tuple(q.shape) != (self.batch, n, m.num_heads, m.head_dim):
+            raise ValueError(f"qi must be ({self.batch}, n, {m.num_heads}, {m.head_dim}), got {tuple(q.shape)}")
+        if not 1 <= n <= _lib.TREE_NODES:
+            raise ValueError(f"a tree has 1 to {_lib.TREE_NODES} nodes, got {n}")
+        k = self.ctx.to_device(ki, torch.int32).reshape(self.batch, n, m.num_kv_heads, m.head_dim)
+        v = self.ctx.to_device(vi, torch.int32).reshape(self.batch, n, m.num_kv_heads, m.head_dim)
+        parents = self.attn.check_parents(parents, n)       # before the rows are written
+        qr = self.rotation.apply(q, self.ctx)
+        if self.rotation.rounds:
+            self.cache.append_wire(k, v) if self.batch > 1 else self.cache.append_wire(k[0], v[0], seq=0)
+        else:
+            self.cache.append_rotated(k, v) if self.batch > 1 else self.cache.append_rotated(k[0], v[0], seq=0)
+        out, self.last_stats = self.attn.attend_tree(qr, parents, self.softmax, stats=stats)
+        return out.reshape(self.batch, n, m.num_heads * m.head_dim)
+
+    def forward_tree(self, hidden_states, parents, *, stats: bool = True):
+        """batch == 1: forward of a draft's n nodes, hidden_states (n, hidden) in an order where
+        parents come first, parents (n,) host values: the parent's number, or -1 for a child of the
+        context. A node's position is the context's length plus its depth. Returns (n, hidden)
+        float32 and a StepReport, as forward does; accept(path) keeps the taken path's rows, and
+        the cache is then what decode steps along it leave."""
+        import torch
+        m = self.model
+        if self.batch != 1:
+            raise ValueError("forward_tree drives a batch-1 block")
+        x = self.ctx.to_device(hidden_states, torch.float32)
+        if x.dim() != 2 or x.shape[-1] != m.hidden_size:
+            raise ValueError(f"hidden_states must be (n, {m.hidden_size}), got {tuple(x.shape)}")
+        n = int(x.shape[0])
+        if isinstance(parents, torch.Tensor):
+            parents = parents.cpu().numpy()
+        parents = np.asarray(parents, dtype=np.int64)
+        if parents.shape != (n,):
+            raise ValueError(f"parents must be ({n},), got {parents.shape}")
+        parents_dev = self.attn.check_parents(parents, n)
+        depth = np.zeros(n, dtype=np.int64)
+        for i, p in enumerate(parents):
+            if p >= 0:
+                depth[i] = depth[p] + 1
+        base = self.cache.length
+        host = self.host
+        qi, ki, vi = host.wire(x, base + depth, counts=stats)
+        self.taps = {"wire.q": qi, "wire.k": ki, "wire.v": vi}
+        out = self.step_tree(qi[None], ki[None], vi[None], parents_dev, stats=stats)[0]
+        self.taps["out"] = out
+        report = StepReport(n_tokens=n, context=base + n, attention=self.last_stats)
+        if stats:
+            report.saturated = host.last_saturated
+            report.conversions = n * (m.num_heads + 2 * m.num_kv_heads) * m.head_dim
+        return host.output(out), report
+
+    def accept(self, n: int, rows=None, *, counts=None) -> None:
+        """After a draft of n nodes: of every sequence's, the listed rows stay (the taken path's nodes
+        in order; CompressedCache.keep), or none."""
+        self.cache.keep(n, rows, counts=counts)
+
     def forward_seam(self, qi, ki, vi, *, force_token_loop: bool = False) -> np.ndarray:
         """batch == 1: (tokens, heads, d) wire tensors.
 

@@ -179,6 +179,15 @@ def unpack_rows(buf: np.ndarray, d: int, key_bits: int, value_bits: int,
     return CompressedKV(k_idx, k_norm, v_idx, v_norm)
 
 
+class _Memory:
+    """Device bytes as torch.as_tensor takes them."""
+
+    def __init__(self, owner, address: int, shape) -> None:
+        self.owner = owner
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "|u1", "data": (address, False),
+                                         "version": 2, "strides": None}
+
+
 class CompressedCache(KVCache):
     """cache/compressed.py:42-132 on the GPU, for `batch` sequences.
 
@@ -339,6 +348,76 @@ class CompressedCache(KVCache):
         _lib.check(self.ctx.lib.insitu_append_wire(self.handle, -1 if seq is None else seq,
                                                    ptr(k), ptr(v), n))
         self._keep = (k, v)     # keep inputs alive until the stream has consumed them
+
+    # -- sequences that continue others, and drafts ------------------------------
+
+    def _kept(self, n: int, rows, lists: int, counts):
+        """(device int32 lists (lists, m) or (m,), entries from list to list, entries of each): host
+        lists are checked, a device tensor's values are the caller's."""
+        import torch
+        if rows is None:
+            if counts is not None and any(counts):
+                raise ValueError("counts without rows")
+            return None, 0, [0] * lists
+        if not isinstance(rows, torch.Tensor) or not rows.is_cuda:
+            if isinstance(rows, torch.Tensor):
+                rows = rows.numpy()
+            if isinstance(rows, (list, tuple)) and rows and isinstance(rows[0], (list, tuple, np.ndarray)):
+                if counts is None:
+                    counts = [len(r) for r in rows]
+                wide = max(len(r) for r in rows)
+                rows = np.array([list(r) + [0] * (wide - len(r)) for r in rows], dtype=np.int64).reshape(len(rows), wide)
+            rows = np.asarray(rows, dtype=np.int64)
+            if rows.size and (rows.min() < 0 or rows.max() >= n):
+                raise ValueError(f"rows are numbers of the last {n} rows, 0 .. {n - 1}")
+        rows = self.ctx.to_device(rows, torch.int32)
+        if rows.dim() not in (1, 2) or (rows.dim() == 2 and rows.shape[0] != lists):
+            raise ValueError(f"rows must be (m,) or ({lists}, m), got {tuple(rows.shape)}")
+        m = int(rows.shape[-1])
+        counts = [m] * lists if counts is None else [int(c) for c in counts]
+        if len(counts) != lists or any(not 0 <= c <= m for c in counts):
+            raise ValueError(f"counts must be {lists} values of 0 .. {m}")
+        return rows, m if rows.dim() == 2 else 0, counts
+
+    def fork(self, src, dst, *, n: int = 0, rows=None, counts=None) -> None:
+        """Sequences `dst` (a list) become copies of sequence `src` (or of src[i], a list as long):
+        every row, or with n the rows before the last n and then, in the order given, the listed of
+        those n: rows (m,) for all or (len(dst), m) numbers of 0 .. n - 1, counts of them each
+        (default m). Lists of lists may differ in length. No destination is a source or comes
+        twice. Rows behind a copy's end stay as they are. Stream-ordered."""
+        dst = [int(b) for b in np.atleast_1d(dst)]
+        srcs = [int(b) for b in np.broadcast_to(np.asarray(src, dtype=np.int64), (len(dst),))] if np.ndim(src) == 0 \
+            else [int(b) for b in src]
+        if len(srcs) != len(dst):
+            raise ValueError(f"{len(srcs)} sources for {len(dst)} destinations")
+        if n == 0 and (rows is not None or counts is not None):
+            raise ValueError("rows and counts select from the last n rows: n is 0")
+        rows, stride, counts = self._kept(n, rows, len(dst), counts)
+        arr = lambda t, v: (t * max(1, len(v)))(*v)
+        with self.ctx.ordered(rows):
+            _lib.check(self.ctx.lib.insitu_cache_fork(
+                self.handle, len(dst), arr(ctypes.c_int32, srcs), arr(ctypes.c_int32, dst), n,
+                ptr(rows) if rows is not None else None, stride, arr(ctypes.c_int64, counts) if n else None))
+        self._keep_rows = rows
+
+    def keep(self, n: int, rows=None, *, counts=None) -> None:
+        """Of the last n rows of every sequence only the listed ones stay, in the order given, and the
+        sequence ends behind them: the accepted path of a draft (rows (m,) for all or (batch, m), as
+        fork takes them), or none of it (rows None: a rejected draft). In place, stream-ordered."""
+        rows, stride, counts = self._kept(n, rows, self.batch, counts)
+        with self.ctx.ordered(rows):
+            _lib.check(self.ctx.lib.insitu_cache_keep(self.handle, n, ptr(rows) if rows is not None else None, stride,
+                                                      (ctypes.c_int64 * self.batch)(*counts)))
+        self._keep_rows = rows
+
+    def device_image(self):
+        """The plane image of every sequence where it lies: a uint8 tensor (batch, seq_stride) over the
+        cache's own memory (layout() gives the planes), written by the calls that follow. It keeps
+        the cache alive; close() ends it."""
+        import torch
+        lay = self._layout
+        memory = _Memory(self, int(lay.device_base), (self.batch, int(lay.seq_stride)))
+        return torch.as_tensor(memory, device=self.ctx.torch_device)
 
     def append(self, k, v, positions, trace=None) -> None:
         raise NotImplementedError(

@@ -22,7 +22,11 @@ class ModelConfig:
     head_dim: int | None = None
     rope_theta: float = 10000.0
     max_position: int = 4096
-    rope_scaling: object | None = None     # insitu_amd.host.RopeScaling, or None for plain RoPE
+    rope_scaling: object | None = None     # insitu_amd.host.RopeScaling (or Linear-, YarnScaling), or None
+    # forms beside the reference's (insitu_amd.host.Seam):
+    rotary_dim: int | None = None          # channels of a head that RoPE rotates; None: all of them
+    rope_interleaved: bool = False         # channel pairs (2 j, 2 j + 1) instead of (j, j + rotary_dim / 2)
+    qk_norm_eps: float = 1e-6              # of the query and key norms, where the weights have them
 
     def __post_init__(self) -> None:
         d = self.head_dim if self.head_dim is not None else self.hidden_size // self.num_heads
@@ -35,6 +39,12 @@ class ModelConfig:
                              f"Walsh-Hadamard butterfly")
         if d % 2:
             raise ValueError(f"head_dim={d} must be even")
+        r = d if self.rotary_dim is None else self.rotary_dim
+        object.__setattr__(self, "rotary_dim", r)
+        if r % 2 or not 2 <= r <= d:
+            raise ValueError(f"rotary_dim={r} must be even, from 2 to head_dim={d}")
+        if not self.qk_norm_eps > 0:
+            raise ValueError(f"qk_norm_eps={self.qk_norm_eps} must be positive")
 
     @property
     def kv_groups(self) -> int:
@@ -52,9 +62,10 @@ class ModelConfig:
     def from_hf(cls, hf_config) -> "ModelConfig":
         """config.py:78-120: from a transformers config (or anything duck-typed, a
         dict included). rope_theta is read top-level or from rope_parameters and
-        never defaulted; "default" and "llama3" RoPE are modelled, any other
-        scaling type is refused."""
-        from .host import RopeScaling
+        never defaulted; "default", "llama3", "linear" and "yarn" RoPE (this one with
+        its original_max_position_embeddings) are modelled, any other scaling type is
+        refused. partial_rotary_factor and rms_norm_eps are read where they are there."""
+        from .host import LinearScaling, RopeScaling, YarnScaling
         get = (lambda k, d=None: hf_config.get(k, d)) if isinstance(hf_config, dict) \
             else (lambda k, d=None: getattr(hf_config, k, d))
         theta = get("rope_theta")
@@ -70,14 +81,25 @@ class ModelConfig:
         rope_type = params.get("rope_type") or params.get("type") or "default"
         if rope_type == "llama3":
             scaling = RopeScaling.from_hf(params)
+        elif rope_type == "linear":
+            scaling = LinearScaling(float(params["factor"]))
+        elif rope_type == "yarn" and params.get("original_max_position_embeddings"):
+            scaling = YarnScaling.from_hf(params)
         elif rope_type == "default":
             scaling = None
         else:
             raise NotImplementedError(f"RoPE scaling {rope_type!r} is not modelled")
-        return cls(hidden_size=get("hidden_size"), num_heads=get("num_attention_heads"),
-                   num_kv_heads=get("num_key_value_heads", get("num_attention_heads")),
+        heads = get("num_attention_heads")
+        part = get("partial_rotary_factor")
+        part = params.get("partial_rotary_factor") if part is None else part
+        d = get("head_dim") or get("hidden_size") // heads
+        eps = get("rms_norm_eps")
+        return cls(hidden_size=get("hidden_size"), num_heads=heads,
+                   num_kv_heads=get("num_key_value_heads", heads),
                    head_dim=get("head_dim"), rope_theta=float(theta),
-                   max_position=get("max_position_embeddings", 4096), rope_scaling=scaling)
+                   max_position=get("max_position_embeddings", 4096), rope_scaling=scaling,
+                   rotary_dim=None if part is None else int(d * part),
+                   qk_norm_eps=1e-6 if eps is None else float(eps))
 
     @classmethod
     def tinyllama(cls) -> "ModelConfig":

@@ -190,6 +190,10 @@ struct insitu_cache {
     // prefill (insitu_attend_causal): scratch for a virtual batch of queries, their lengths
     ChunkScratch prefill_scr;
     int64_t *prefill_len = nullptr;
+    void *tree_scr = nullptr;             // insitu_attend_tree: spans' maxima and runs, one call's worth
+    size_t tree_bytes = 0;
+    uint8_t *keep_scr = nullptr;          // insitu_cache_keep: rows on their way, for long lists
+    size_t keep_bytes = 0;
     int32_t spin_limit = 1 << 20;         // insitu_cache_debug
     int32_t path = 0;                     // insitu_cache_debug: 0 auto, 1 scan, 2 chunked, 3 step kernel, 4 split
     int32_t prefill_path = 0;             // insitu_cache_debug: 0 auto, 1 virtual batch, 2 prefill kernel
@@ -237,6 +241,23 @@ int zero_stats(insitu_cache *c) {
     hipLaunchKernelGGL(zero_u64, dim3(1), dim3(64), 0, c->ctx->stream,
                        (unsigned long long *)c->stats, (int)(sizeof(DevStats) / 8));
     HIP_TRY(hipGetLastError(), "zero stats");
+    return INSITU_OK;
+}
+
+// A buffer of the cache, grown (the old one may still be in use by queued launches).
+template <class T>
+int grow(insitu_cache *k, T *&p, size_t &have, size_t need) {
+    if (have >= need) return INSITU_OK;
+    HIP_TRY(hipStreamSynchronize(k->ctx->stream), "sync");
+    if (p) HIP_TRY(hipFree(p), "hipFree");
+    p = nullptr;
+    have = 0;
+    void *q = nullptr;
+    const hipError_t e = hipMalloc(&q, need);
+    if (e == hipErrorOutOfMemory) return fail(INSITU_ENOMEM, "cache scratch");
+    HIP_TRY(e, "hipMalloc");
+    p = (T *)q;
+    have = need;
     return INSITU_OK;
 }
 
@@ -603,6 +624,8 @@ int insitu_cache_destroy(insitu_cache *k) {
     if (k->scr.p) hipFree(k->scr.p);
     if (k->prefill_scr.p) hipFree(k->prefill_scr.p);
     if (k->prefill_len) hipFree(k->prefill_len);
+    if (k->tree_scr) hipFree(k->tree_scr);
+    if (k->keep_scr) hipFree(k->keep_scr);
     delete k;
     return INSITU_OK;
 }
@@ -1074,6 +1097,168 @@ int insitu_attend_causal_static(insitu_cache *k, int32_t seq, int64_t base, int6
     }
     if (use_prefill_kernel(k, gv, base, n_q, mode)) return prefill_kernel_launch(k, gv, base, n_q, q, out, mode, false);
     return prefill_launches(k, gv, pl, ss.cs, ss.len, base, n_q, q, out, mode, false);
+}
+
+int insitu_attend_tree(insitu_cache *k, int32_t n, const int32_t *parents, int32_t per_sequence, const int32_t *q,
+                       int32_t *out, int32_t mode, insitu_stats *stats) {
+    if (!k) return fail(INSITU_EINVAL, "cache is NULL");
+    if (n < 1 || n > TREE_NODES) return fail(INSITU_EBADLEN, "a tree has 1 to 256 nodes");
+    if (!parents || !q || !out) return fail(INSITU_EINVAL, "null argument");
+    if (mode < INSITU_SEQUENTIAL || mode > INSITU_SERIAL) return fail(INSITU_EINVAL, "unknown mode");
+    int64_t longest = 0;
+    for (int b = 0; b < k->g.batch; ++b) {
+        if (k->len_host[b] < n) {
+            char buf[160];
+            snprintf(buf, sizeof buf, "sequence %d holds %lld rows, fewer than the tree's %d nodes", b,
+                     (long long)k->len_host[b], n);
+            return fail(INSITU_EBADLEN, buf);
+        }
+        longest = k->len_host[b] > longest ? k->len_host[b] : longest;
+    }
+    HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
+    int rc = stats ? zero_stats(k) : INSITU_OK;
+    if (rc) return rc;
+    const int64_t *len = k->len_dev[k->cur];
+    const int64_t pstride = per_sequence ? n : 0;
+    const int two_pass = mode == INSITU_TWO_PASS ? 1 : 0;
+    const bool fast = mode != INSITU_SERIAL && tree_supported(k->g);
+    if (fast) {
+        rc = grow(k, k->tree_scr, k->tree_bytes, tree_scratch_bytes(k->g, n, longest));
+        if (rc) return rc;
+    }
+    LaunchEv ev;
+    rc = timing_events(k->ctx, &ev);
+    if (rc) return rc;
+    if (fast)
+        HIP_TRY(launch_attend_tree(k->ctx->stream, k->g, k->tabs, q, out, len, parents, pstride, n, longest, two_pass,
+                                   stats != nullptr, k->tree_scr, k->tree_bytes, ev, k->stats),
+                "tree attend launch");
+    else
+        HIP_TRY(launch_attend_tree_serial(k->ctx->stream, k->g, k->tabs, q, out, len, parents, pstride, n, two_pass, ev,
+                                          k->stats),
+                "tree attend launch");
+    return copy_stats(k, stats);
+}
+
+int insitu_cache_fork(insitu_cache *k, int32_t n_copies, const int32_t *src, const int32_t *dst, int64_t n,
+                      const int32_t *rows, int64_t rows_stride, const int64_t *counts) {
+    if (!k || n_copies < 0 || (n_copies && (!src || !dst))) return fail(INSITU_EINVAL, "null argument");
+    if (n < 0 || n > 0x7fffffff || rows_stride < 0) return fail(INSITU_EBADLEN, "n in 0 .. 2^31 - 1, rows_stride >= 0");
+    if (n && !counts) return fail(INSITU_EINVAL, "counts are required with n");
+    const Geom &g = k->g;
+    for (int i = 0; i < n_copies; ++i) {
+        if (src[i] < 0 || src[i] >= g.batch || dst[i] < 0 || dst[i] >= g.batch)
+            return fail(INSITU_EINVAL, "no such sequence");
+        if (n > k->len_host[src[i]]) return fail(INSITU_EBADLEN, "the source holds fewer than n rows");
+        if (n && (counts[i] < 0 || counts[i] > n || (counts[i] && !rows)))
+            return fail(INSITU_EBADLEN, "0 .. n of the last n rows are kept, from rows_dev");
+        for (int j = 0; j < n_copies; ++j)
+            if (dst[i] == src[j] || (j < i && dst[i] == dst[j]))
+                return fail(INSITU_EINVAL, "a destination twice, or one that is a source");
+    }
+    if (!n_copies) return INSITU_OK;
+    HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
+    RowCopy c{};
+    c.rows = n ? rows : nullptr;
+    c.rows_stride = rows_stride;
+    c.n = n;
+    c.len = k->len_dev[k->cur];
+    // copies of one source that take the same rows are one group: its rows are read once
+    int groups = 0, at = 0;
+    auto flush = [&]() -> int {
+        if (!groups) return INSITU_OK;
+        HIP_TRY(launch_copy_rows(k->ctx->stream, g, g, c, groups), "fork launch");
+        groups = at = 0;
+        return INSITU_OK;
+    };
+    for (int i = 0; i < n_copies; ++i) {
+        const int64_t len = k->len_host[src[i]], head = len - n, count = n ? counts[i] : 0;
+        if (at == COPY_MAX) {
+            const int rc = flush();
+            if (rc) return rc;
+        }
+        const bool same = groups && c.src[groups - 1] == src[i] && (n == 0 || (rows_stride == 0 && c.end[groups - 1] == head + count));
+        if (!same) {
+            c.src[groups] = src[i];
+            c.first[groups] = at;
+            c.rows_at[groups] = i;
+            c.begin[groups] = 0;
+            c.head[groups] = c.add[groups] = head;
+            c.end[groups] = head + count;
+            ++groups;
+        }
+        c.dst[at++] = dst[i];
+        c.first[groups] = at;
+    }
+    const int rc = flush();
+    if (rc) return rc;
+    for (int i = 0; i < n_copies; ++i) k->len_host[dst[i]] = k->len_host[src[i]] - n + (n ? counts[i] : 0);
+    return INSITU_OK;
+}
+
+int insitu_cache_keep(insitu_cache *k, int64_t n, const int32_t *rows, int64_t rows_stride, const int64_t *counts) {
+    if (!k) return fail(INSITU_EINVAL, "cache is NULL");
+    const Geom &g = k->g;
+    if (n < 0 || n > 0x7fffffff || rows_stride < 0) return fail(INSITU_EBADLEN, "n in 0 .. 2^31 - 1, rows_stride >= 0");
+    int64_t most = 0;
+    for (int b = 0; b < g.batch; ++b) {
+        if (n > k->len_host[b]) return fail(INSITU_EBADLEN, "a sequence holds fewer than n rows");
+        const int64_t c = counts ? counts[b] : 0;
+        if (c < 0 || c > n || (c && !rows)) return fail(INSITU_EBADLEN, "0 .. n of the last n rows are kept, from rows_dev");
+        most = c > most ? c : most;
+    }
+    if (!n) return INSITU_OK;
+    HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
+    const hipStream_t s = k->ctx->stream;
+    int64_t *len = k->len_dev[k->cur];
+    if (most <= KEEP_ROWS) {
+        for (int b0 = 0; b0 < g.batch; b0 += KEEP_MAX) {
+            const int nb = g.batch - b0 < KEEP_MAX ? g.batch - b0 : KEEP_MAX;
+            RowKeep c{};
+            for (int i = 0; i < nb; ++i) {
+                c.base[i] = k->len_host[b0 + i] - n;
+                c.count[i] = counts ? (int32_t)counts[b0 + i] : 0;
+            }
+            c.rows = rows;
+            c.rows_stride = rows_stride;
+            c.n = (int32_t)n;
+            c.seq0 = b0;
+            c.len = len;
+            HIP_TRY(launch_keep_rows(s, g, c, nb, (int)most), "keep launch");
+        }
+    } else {
+        // through a buffer, a sequence at a time: rows collected, then back behind the context
+        Geom t = g;
+        t.span = (most * 16 + 255) / 256 * 256;
+        t.head_stride = g.n_planes * t.span;
+        t.seq_stride = 0;
+        const int rc = grow(k, k->keep_scr, k->keep_bytes, (size_t)(g.n_kv * t.head_stride));
+        if (rc) return rc;
+        t.base = k->keep_scr;
+        for (int b = 0; b < g.batch; ++b) {
+            const int64_t base = k->len_host[b] - n, count = counts ? counts[b] : 0;
+            RowCopy c{};
+            c.src[0] = b;
+            c.first[1] = 1;
+            c.rows_at[0] = b;
+            c.end[0] = count;
+            c.add[0] = base;
+            c.rows = rows;
+            c.rows_stride = rows_stride;
+            c.n = n;
+            HIP_TRY(launch_copy_rows(s, g, t, c, 1), "keep launch");
+            RowCopy d{};
+            d.dst[0] = b;
+            d.first[1] = 1;
+            d.begin[0] = d.head[0] = base;
+            d.end[0] = base + count;
+            d.len = len;
+            // (row r >= head of the cache is row r - head of the buffer)
+            HIP_TRY(launch_copy_rows(s, t, g, d, 1), "keep launch");
+        }
+    }
+    for (int b = 0; b < g.batch; ++b) k->len_host[b] += (counts ? counts[b] : 0) - n;
+    return INSITU_OK;
 }
 
 int insitu_step(insitu_cache *k, const int32_t *q, const int32_t *kw, const int32_t *vw,

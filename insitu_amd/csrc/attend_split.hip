@@ -86,50 +86,6 @@ struct Scratch {
     int32_t nblk, nwg;
 };
 
-// A lane's key codes of one tile: channels [grp d / 4, (grp + 1) d / 4) of token t.
-template <int D, int KB>
-struct Codes {
-    static constexpr int N = KB == 4 ? D / 32 : KB == 3 ? (D == 64 ? 2 : 3) : D / 64;
-    uint32_t w[N];
-    __device__ __forceinline__ void load(const uint8_t *hb, int64_t span, int64_t t, int grp) {
-        if constexpr (KB == 4 && D == 64) {
-            const uint2 v = *(const uint2 *)(hb + (grp >> 1) * span + t * 16 + (grp & 1) * 8);
-            w[0] = v.x;
-            w[1] = v.y;
-        } else if constexpr (KB == 4) {
-            const uint4 v = *(const uint4 *)(hb + grp * span + t * 16);
-            w[0] = v.x;
-            w[1] = v.y;
-            w[2] = v.z;
-            w[3] = v.w;
-        } else if constexpr (KB == 3) {
-            const int d0 = D == 64 ? (3 * grp) >> 1 : 3 * grp;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int dw = d0 + i, p = dw >> 2;              // d = 64: 6 words, the second plane 8 bytes wide
-                w[i] = *(const uint32_t *)(hb + p * span + t * (D == 64 && p == 1 ? 8 : 16) + (dw & 3) * 4);
-            }
-        } else if constexpr (D == 64) {
-            w[0] = *(const uint32_t *)(hb + t * 16 + grp * 4);
-        } else {
-            const uint2 v = *(const uint2 *)(hb + (grp >> 1) * span + t * 16 + (grp & 1) * 8);
-            w[0] = v.x;
-            w[1] = v.y;
-        }
-    }
-    // the 16 codes of block b
-    __device__ __forceinline__ uint64_t bits(int b, int grp) const {
-        if constexpr (KB == 4)
-            return (uint64_t)w[2 * b] | (uint64_t)w[2 * b + 1] << 32;
-        else if constexpr (KB == 3 && D == 64)
-            return ((uint64_t)w[0] | (uint64_t)w[1] << 32) >> (16 * (grp & 1));
-        else if constexpr (KB == 3)
-            return b == 0 ? (uint64_t)w[0] | (uint64_t)w[1] << 32 : ((uint64_t)w[1] | (uint64_t)w[2] << 32) >> 16;
-        else
-            return w[b];
-    }
-};
-
 // The query operand from rotated rows in LDS: row = (head 4 s + l / 4, digit l % 4).
 template <int D, int KB>
 __device__ __forceinline__ void query_operand(const int32_t (*qi)[D], int s, int lane, v4i (&a)[D / 64]) {

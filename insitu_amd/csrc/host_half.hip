@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "insitu_internal.h"
+#include "seam_heads.h"
 
 namespace insitu {
 
@@ -611,6 +612,33 @@ int insitu_seam_wire(insitu_ctx *c, const float *p, const float *bias, int64_t n
         hipLaunchKernelGGL(seam_wire_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, ctx_stream(c), p, n,
                            a);
         HIP_TRY(hipGetLastError(), "seam epilogue");
+    }
+    return seam_counts(c, counts_host);
+}
+
+int insitu_seam_heads(insitu_ctx *c, const insitu_seam_desc *s, const float *p, int64_t n, const int64_t *pos,
+                      int64_t pos0, int32_t *q, int32_t *k, int32_t *v, unsigned long long *counts_host) {
+    if (!c || !s || (n && (!p || !q || !k || !v || !s->cos_dev || !s->sin_dev))) return fail(INSITU_EINVAL, "null argument");
+    if (n < 0 || s->n_q <= 0 || s->n_kv <= 0 || s->max_pos <= 0) return fail(INSITU_EBADLEN, "bad seam shape");
+    if (s->n_q > 65536 || s->n_kv > 65536) return fail(INSITU_EBADLEN, "more than 65,536 heads");
+    if (s->d < 16 || s->d > 128 || (s->d & (s->d - 1)))
+        return fail(INSITU_EBADLEN, "head_dim is a power of two in 16..128 (rotate.py:146-147)");
+    if (s->rotary_dim < 2 || s->rotary_dim > s->d || s->rotary_dim % 2)
+        return fail(INSITU_EBADLEN, "rotary_dim is even, from 2 to head_dim");
+    if (s->frac < 0 || s->frac > 30) return fail(INSITU_EBADLEN, "frac is in 0..30");
+    if ((s->q_norm_dev || s->k_norm_dev) && !(s->norm_eps > 0.0)) return fail(INSITU_EINVAL, "norm_eps must be positive");
+    const int64_t heads = s->n_q + 2 * (int64_t)s->n_kv;
+    if (n > 0x7fffffff / heads) return fail(INSITU_EBADLEN, "tokens times heads must stay below 2^31");
+    HIP_TRY(hipSetDevice(ctx_device(c)), "hipSetDevice");
+    Blas &b = blas_of(c);
+    if (!b.counters) return fail(INSITU_EHIP, "counters");
+    if (counts_host) HIP_TRY(hipMemsetAsync(b.counters, 0, 2 * sizeof(unsigned long long), ctx_stream(c)), "memset");
+    if (n) {
+        const SeamHeads a{p, s->bias_dev, s->q_norm_dev, s->k_norm_dev, s->n_q, s->n_kv, s->d, s->rotary_dim, pos, pos0,
+                          s->cos_dev, s->sin_dev, s->max_pos, s->frac, s->interleaved, s->cast_after_rope,
+                          (uint32_t)(n * heads), 1.0 / (double)heads, s->attn_scale, s->norm_eps, q, k, v, b.counters,
+                          b.counters + 1};
+        HIP_TRY(launch_seam_heads(ctx_stream(c), a), "seam");
     }
     return seam_counts(c, counts_host);
 }

@@ -339,6 +339,46 @@ hipError_t launch_attend_serial(hipStream_t s, const Geom &g, const Tables *t, c
                                 int32_t *out, const int64_t *len, int two_pass, LaunchEv ev,
                                 DevStats *st);
 
+// Rows between sequences (cache_rows.hip), as group z of a launch: rows [begin, end) of the sequences
+// dst[first[z]] .. dst[first[z + 1] - 1] of one geometry from those of sequence src of another. Row r < head
+// comes from row r; row head + j from row add + j or, with rows, add + rows[rows_at * rows_stride + j] (a
+// device list of values below n). len (may be null) receives end for every dst.
+constexpr int COPY_MAX = 32;             // destinations a launch (the arguments travel by value)
+struct RowCopy {
+    int32_t src[COPY_MAX], first[COPY_MAX + 1], dst[COPY_MAX], rows_at[COPY_MAX];
+    int64_t begin[COPY_MAX], end[COPY_MAX], head[COPY_MAX], add[COPY_MAX];
+    const int32_t *rows;
+    int64_t rows_stride, n;
+    int64_t *len;
+};
+hipError_t launch_copy_rows(hipStream_t s, const Geom &src, const Geom &dst, const RowCopy &c, int groups);
+// Compaction in place: of the n rows behind base of sequence seq0 + z, those listed at rows + (seq0 + z) *
+// rows_stride, count of them and KEEP_ROWS at most, become the first; len receives base + count.
+constexpr int KEEP_MAX = 64;             // sequences a launch
+constexpr int KEEP_ROWS = 1024;
+struct RowKeep {
+    int64_t base[KEEP_MAX];
+    int32_t count[KEEP_MAX];
+    const int32_t *rows;
+    int64_t rows_stride;
+    int32_t n, seq0;
+    int64_t *len;
+};
+hipError_t launch_keep_rows(hipStream_t s, const Geom &g, const RowKeep &c, int seqs, int most);
+// The attend of a tree of drafted tokens (attend_tree.hip): node i of n, whose row is row len - n + i of its
+// sequence, over rows 0 .. len - n - 1 and those of its ancestors and itself. parents: pstride a sequence
+// (0: one list for all), -1 or an earlier node; longest: the longest sequence; count: gather statistics.
+constexpr int TREE_NODES = 256;
+bool tree_supported(const Geom &g);
+size_t tree_scratch_bytes(const Geom &g, int64_t n, int64_t longest);
+hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, const int32_t *q, int32_t *out,
+                              const int64_t *len, const int32_t *parents, int64_t pstride, int32_t n, int64_t longest,
+                              int two_pass, bool count, void *scratch, size_t scratch_bytes, LaunchEv ev, DevStats *st);
+// The same token by token, any format.
+hipError_t launch_attend_tree_serial(hipStream_t s, const Geom &g, const Tables *t, const int32_t *q, int32_t *out,
+                                     const int64_t *len, const int32_t *parents, int64_t pstride, int32_t n,
+                                     int two_pass, LaunchEv ev, DevStats *st);
+
 // Shared with the files that add entry points beside abi.hip: the error
 // message for insitu_last_error, and a context's device and stream.
 int set_last_error(int code, const char *msg);

@@ -42,16 +42,44 @@ __device__ __forceinline__ void stage_rows(const Geom &g, int b, int h, int64_t 
     }
 }
 
+// Every row of the context.
+struct AllRows {
+    __device__ __forceinline__ bool operator()(int64_t) const { return true; }
+};
+
+// The rows of a tree's node: those before the draft, and of the draft the ones whose bit is set.
+struct TreeRows {
+    const uint32_t *up;
+    int64_t base;
+    __device__ __forceinline__ bool operator()(int64_t t) const {
+        return t < base || ((up[(t - base) >> 5] >> ((t - base) & 31)) & 1u) != 0;
+    }
+};
+// The row of `up` of node i of n, by one wave (LDS): the node and its ancestors, a bit each. A parent that
+// is not an earlier node ends the path.
+__device__ __forceinline__ void tree_path(const int32_t *__restrict__ parents, int i, int n, uint32_t *up) {
+    const int lane = threadIdx.x & 63;
+    for (int k = lane; k < (n + 31) / 32; k += 64) up[k] = 0;
+    wave_sync();
+    for (int j = i, p; j >= 0; j = p) {
+        if (lane == 0) up[j >> 5] |= 1u << (j & 31);
+        p = parents[j];
+        if (p >= j) break;
+    }
+    wave_sync();
+}
+
+// rows: which of the first T rows the head attends.
 // kc/vc: the key/value centroids (int64) in LDS or global memory.
 // Writes out_row[0..d) and merges this head's statistics into `st`. Score
 // statistics are merged only when count_scores is set (the chunked kernel
 // has already counted them when it falls back here).
-template <int CPL, int RS>
+template <int CPL, int RS, class Rows = AllRows>
 __device__ __forceinline__ void serial_head(const Geom &g, const Tables *__restrict__ tabs,
                                             const int64_t *kc, const int64_t *vc,
                                             const int32_t *__restrict__ qrow, int b, int kvh, int64_t T,
                                             int two_pass, bool count_scores, SerialLds<RS> &L,
-                                            int32_t *out_row, DevStats *st) {
+                                            int32_t *out_row, DevStats *st, const Rows rows = Rows()) {
     const int lane = threadIdx.x & 63;
     const int d = g.d;
     const int score_shift = CENT_FRAC + g.norm_frac;                        // config.py:249-250
@@ -76,7 +104,7 @@ __device__ __forceinline__ void serial_head(const Geom &g, const Tables *__restr
             stage_rows<RS>(g, b, kvh, base, n, L.rows);
             wave_sync();
             int64_t s_mine = 0;
-            if (lane < n) {
+            if (lane < n && rows(base + lane)) {
                 int64_t dot = 0;
                 for (int c = 0; c < d; ++c)
                     dot = wadd(dot, wmul(L.qs[c], kc[code_at(L.rows[lane], c, g.kb)]));
@@ -94,6 +122,7 @@ __device__ __forceinline__ void serial_head(const Geom &g, const Tables *__restr
                 s_mine = s;
             }
             for (int j = 0; j < n; ++j) {
+                if (!rows(base + j)) continue;
                 const int64_t sj = readlane64(s_mine, j);
                 int64_t p;
                 if (!two_pass) {

@@ -54,9 +54,79 @@ class RopeScaling:
 
 
 @dataclass(frozen=True)
+class LinearScaling:
+    """Positions divided by a factor: every frequency is. Not in the reference."""
+
+    factor: float
+
+    def __post_init__(self) -> None:
+        if not self.factor > 0:
+            raise ValueError(f"factor={self.factor} must be positive")
+
+    def apply(self, inv_freq) -> np.ndarray:
+        return np.asarray(inv_freq, dtype=np.float64) / self.factor
+
+
+@dataclass(frozen=True)
+class YarnScaling:
+    """YaRN (Peng et al., arXiv:2309.00071): a frequency that turns more than beta_fast times over the
+    original context stays, one that turns less than beta_slow times is divided by factor, those
+    between change over linearly by their index; cos and sin are multiplied by attention_factor
+    (default 0.1 ln(factor) + 1). Not in the reference."""
+
+    factor: float
+    original_max_position: int
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention_factor: float | None = None
+    truncate: bool = True                # the indices between which they change over, as integers
+
+    def __post_init__(self) -> None:
+        if not self.factor > 0 or not self.original_max_position > 0:
+            raise ValueError(f"factor={self.factor} and original_max_position={self.original_max_position} "
+                             f"must be positive")
+        if not self.beta_fast > self.beta_slow > 0:
+            raise ValueError(f"beta_fast={self.beta_fast} must exceed beta_slow={self.beta_slow}, both positive")
+        if self.attention_factor is None:
+            object.__setattr__(self, "attention_factor", _yarn_mscale(self.factor))
+
+    @classmethod
+    def from_hf(cls, params: dict) -> "YarnScaling":
+        factor = float(params["factor"])
+        att = params.get("attention_factor")
+        if att is None and params.get("mscale") and params.get("mscale_all_dim"):
+            att = _yarn_mscale(factor, params["mscale"]) / _yarn_mscale(factor, params["mscale_all_dim"])
+        return cls(factor, int(params["original_max_position_embeddings"]),
+                   float(params.get("beta_fast") or 32.0), float(params.get("beta_slow") or 1.0),
+                   None if att is None else float(att), bool(params.get("truncate", True)))
+
+    def apply(self, inv_freq) -> np.ndarray:
+        f = np.asarray(inv_freq, dtype=np.float64)
+        if f.size < 2:                   # a single frequency, that of a turn each 2 pi tokens, stays
+            return f
+        step = -np.log(f[1] / f[0])      # ln(theta) 2 / d
+
+        def index(turns):                # of the frequency that turns so often over the original context
+            return np.log(self.original_max_position * f[0] / (2.0 * np.pi * turns)) / step
+        low, high = index(self.beta_fast), index(self.beta_slow)
+        if self.truncate:
+            low, high = np.floor(low), np.ceil(high)
+        low, high = max(low, 0.0), min(high, 2.0 * f.size - 1.0)
+        if high == low:
+            high += 0.001
+        ramp = np.clip((np.arange(f.size) - low) / (high - low), 0.0, 1.0)
+        return f / self.factor * ramp + f * (1.0 - ramp)
+
+
+def _yarn_mscale(factor: float, mscale: float = 1.0) -> float:
+    return 0.1 * mscale * float(np.log(factor)) + 1.0 if factor > 1.0 else 1.0
+
+
+@dataclass(frozen=True)
 class RoPE:
     """ops/rope.py:117-142: cos/sin for every reachable position, Q(32, frac), built
-    once in float64 (half to even); held on the device as int64 (max_position, d/2)."""
+    once in float64 (half to even); held on the device as int64 (max_position, d/2).
+    d is the channels that are rotated, all of a head or part of it."""
 
     cos: np.ndarray
     sin: np.ndarray
@@ -75,7 +145,8 @@ class RoPE:
 
         def q(a):
             return np.clip(np.rint(a * float(1 << frac)), -(1 << 31), (1 << 31) - 1).astype(np.int64)
-        return RoPE(q(np.cos(ang)), q(np.sin(ang)), frac)
+        amp = getattr(scaling, "attention_factor", 1.0)
+        return RoPE(q(np.cos(ang) * amp), q(np.sin(ang) * amp), frac)
 
 
 def fold_o_proj(o_proj, rotation_matrix: np.ndarray, num_heads: int) -> np.ndarray:
@@ -101,16 +172,108 @@ def _host_array(a):
     return np.asarray(a)
 
 
+def _norm_weight(w, d: int, ctx):
+    """(d,) weights of a head's norm, or None -> fp32 on the device."""
+    import torch
+    if w is None:
+        return None
+    if not isinstance(w, torch.Tensor):
+        w = np.asarray(w, dtype=np.float32)
+    if tuple(w.shape) != (d,):
+        raise ValueError(f"a head's norm has weights ({d},), got {tuple(w.shape)}")
+    return ctx.to_device(w.detach() if isinstance(w, torch.Tensor) else w, torch.float32)
+
+
+class Seam:
+    """The projections of q|k|v to the wire rows in front of the seam (kernel.py:209-249), with what
+    models have beside the reference's: RMS norms of query and key heads (q_norm, k_norm: weights
+    (head_dim,), eps model.qk_norm_eps), rotary positions over model.rotary_dim channels in half or
+    interleaved pairs (model.rope_interleaved), and any scaling of the frequencies that RoPE.build
+    takes. bias ((Hq + 2 Hkv) d) is added to the projections in fp32."""
+
+    def __init__(self, model, *, q_norm=None, k_norm=None, bias=None, cast_after_rope: bool = True, ctx=None,
+                 tables=None) -> None:
+        import torch
+        self.model = m = model
+        self.ctx = ctx or default_context()
+        dev = self.ctx.torch_device
+        self.q_norm, self.k_norm = (_norm_weight(a, m.head_dim, self.ctx) for a in (q_norm, k_norm))
+        self.width = m.q_out_features + 2 * m.kv_out_features
+        self.bias = None if bias is None else self.ctx.to_device(bias, torch.float32)
+        if self.bias is not None and tuple(self.bias.shape) != (self.width,):
+            raise ValueError(f"bias must be ({self.width},), got {tuple(self.bias.shape)}")
+        if tables is None:
+            rope = RoPE.build(m.rotary_dim, m.max_position, m.rope_theta, ROPE_FRAC, m.rope_scaling)
+            tables = (torch.from_numpy(rope.cos).to(dev), torch.from_numpy(rope.sin).to(dev))
+        self._cos, self._sin = tables
+        self.last_saturated = 0
+        dp = lambda t: None if t is None else t.data_ptr()
+        self._desc = _lib.SeamDesc(m.num_heads, m.num_kv_heads, m.head_dim, m.rotary_dim, int(m.rope_interleaved),
+                                   ROPE_FRAC, int(cast_after_rope), 1.0 / np.sqrt(m.head_dim), m.qk_norm_eps,
+                                   dp(self.bias), dp(self.q_norm), dp(self.k_norm), dp(self._cos), dp(self._sin),
+                                   m.max_position)
+
+    def wire(self, p, positions, *, counts: bool = True):
+        """p (n, (Hq + 2 Hkv) d) float32 projections -> the wire rows q (n, Hq, d), k and v
+        (n, Hkv, d), int32 Q8.16 on the device. positions: n values, any order; the first of
+        consecutive ones may be given alone as an int. Host positions are checked against the
+        table; a device tensor's are checked where counts is (which synchronises), and otherwise
+        the rows of positions beyond the table are left unwritten."""
+        import torch
+        m = self.model
+        p = self.ctx.to_device(p, torch.float32)
+        if p.dim() != 2 or p.shape[1] != self.width:
+            raise ValueError(f"p must be (n, {self.width}), got {tuple(p.shape)}")
+        n = int(p.shape[0])
+        pos, pos0 = None, 0
+        if isinstance(positions, torch.Tensor) and positions.is_cuda:
+            pos = self.ctx.to_device(positions, torch.int64)
+            if tuple(pos.shape) != (n,):
+                raise ValueError(f"expected {n} positions, got {tuple(pos.shape)}")
+        elif isinstance(positions, (int, np.integer)):
+            pos0 = int(positions)
+            _check_positions(pos0, pos0 + n - 1, m.max_position, n)
+        else:
+            host = np.asarray(positions, dtype=np.int64).reshape(-1)
+            if host.shape != (n,):
+                raise ValueError(f"expected {n} positions, got {host.shape}")
+            if n:
+                _check_positions(int(host.min()), int(host.max()), m.max_position, n)
+                pos0 = int(host[0])
+            if not np.all(np.diff(host) == 1):
+                pos = self.ctx.to_device(host, torch.int64)
+        dev = self.ctx.torch_device
+        q = torch.empty((n, m.num_heads, m.head_dim), dtype=torch.int32, device=dev)
+        k = torch.empty((n, m.num_kv_heads, m.head_dim), dtype=torch.int32, device=dev)
+        v = torch.empty_like(k)
+        cnt = (ctypes.c_uint64 * 2)() if counts else None
+        with self.ctx.ordered(p, pos, q, k, v):
+            _lib.check(self.ctx.lib.insitu_seam_heads(self.ctx.handle, ctypes.byref(self._desc), ptr(p), n,
+                                                      ptr(pos) if pos is not None else None, pos0, ptr(q), ptr(k),
+                                                      ptr(v), cnt))
+        if cnt is not None:
+            self.last_saturated = int(cnt[0])
+        self._keep = (p, pos)
+        return q, k, v
+
+
+def _check_positions(lo: int, hi: int, max_position: int, n: int) -> None:
+    if n and (lo < 0 or hi >= max_position):
+        raise _lib.FormatError(_lib.ERANGE, f"position {lo if lo < 0 else hi} beyond the RoPE table "
+                               f"(max_position {max_position})")
+
+
 class Weights:
     """weights.py:32-133: fp16 W_q | W_k | W_v stacked (the checkpoint's (out, in) layout),
     fp16 W_o' (R^-1 folded), fp32 biases; device-resident. rotation_matrix is the
     cache's Rotation or its dense matrix (R_last ... R_0)."""
 
     def __init__(self, q, k, v, o, model, rotation_matrix, *, q_bias=None, k_bias=None,
-                 v_bias=None, o_bias=None, ctx=None) -> None:
+                 v_bias=None, o_bias=None, q_norm=None, k_norm=None, ctx=None) -> None:
         import torch
         self.model = model
         self.ctx = ctx or default_context()
+        self.q_norm, self.k_norm = (_norm_weight(a, model.head_dim, self.ctx) for a in (q_norm, k_norm))
         q, k, v, o, q_bias, k_bias, v_bias, o_bias = (
             _host_array(a) for a in (q, k, v, o, q_bias, k_bias, v_bias, o_bias))
         shapes = {"q": (model.q_out_features, model.hidden_size),
@@ -139,7 +302,7 @@ class Weights:
 
     @staticmethod
     def random(model, rotation_matrix, seed: int = 0, scale: float | None = None, ctx=None) -> "Weights":
-        """weights.py:112-133: N(0, 1) float32 times 1/sqrt(hidden) (float64), in q, k, v, o order."""
+        """weights.py:112-133 (without norms of queries and keys): N(0, 1) float32 times 1/sqrt(hidden) (float64), in q, k, v, o order."""
         rng = np.random.default_rng(seed)
         s = scale if scale is not None else 1.0 / np.sqrt(model.hidden_size)
 
@@ -160,11 +323,17 @@ class HostHalf:
         self.weights = weights
         self.ctx = ctx or weights.ctx
         self.cast_after_rope = cast_after_rope
-        self.rope = RoPE.build(model.head_dim, model.max_position, model.rope_theta, ROPE_FRAC,
+        self.rope = RoPE.build(model.rotary_dim, model.max_position, model.rope_theta, ROPE_FRAC,
                                model.rope_scaling)
         dev = self.ctx.torch_device
         self._cos = torch.from_numpy(self.rope.cos).to(dev)
         self._sin = torch.from_numpy(self.rope.sin).to(dev)
+        # norms of queries and keys, or rotary positions other than the reference's
+        self.seam = None
+        if weights.q_norm is not None or weights.k_norm is not None or model.rope_interleaved or \
+                model.rotary_dim != model.head_dim:
+            self.seam = Seam(model, q_norm=weights.q_norm, k_norm=weights.k_norm, bias=weights.qkv_bias,
+                             cast_after_rope=cast_after_rope, ctx=self.ctx, tables=(self._cos, self._sin))
         self.attn_scale = 1.0 / np.sqrt(model.head_dim)           # kernel.py:103
         self.last_saturated = 0
 
@@ -193,6 +362,10 @@ class HostHalf:
             # rope.py:163-167; checked here so that counts=False needs no read-back
             raise _lib.FormatError(_lib.ERANGE, f"position {int(positions.max())} beyond the RoPE "
                                    f"table (max_position {m.max_position})")
+        if self.seam is not None:
+            rows = self.seam.wire(self.project_qkv(x), positions, counts=counts)
+            self.last_saturated = self.seam.last_saturated if counts else self.last_saturated
+            return rows
         # consecutive positions (a decode step, a prompt) go as their first value
         consecutive = n == 0 or bool(np.all(np.diff(positions) == 1))
         pos = None if consecutive else self.ctx.to_device(positions, torch.int64)

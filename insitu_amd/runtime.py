@@ -55,6 +55,15 @@ class Context:
         except Exception:
             pass
 
+    # -- streams --------------------------------------------------------------
+
+    def ordered(self, *tensors) -> "_Ordered":
+        """With this, library calls come after what the caller's current stream holds so far, and
+        what it gets later comes after them, where that stream is not the context's own; `tensors`
+        (used by the calls, perhaps from the other stream's pool) then stay in memory until they
+        are through. Nothing waits on the host."""
+        return _Ordered(self, tensors)
+
     # -- tensors --------------------------------------------------------------
 
     def to_device(self, a, dtype=None):
@@ -67,6 +76,24 @@ class Context:
         if dtype is not None:
             t = t.to(dtype)
         return t.contiguous()
+
+
+class _Ordered:
+    def __init__(self, ctx: Context, tensors) -> None:
+        self.ctx, self.tensors, self.other = ctx, tensors, None
+
+    def __enter__(self) -> None:
+        now = _torch().cuda.current_stream(self.ctx.device)
+        if now.cuda_stream != self.ctx.stream.cuda_stream:
+            self.other = now
+            self.ctx.stream.wait_stream(now)
+
+    def __exit__(self, *exc) -> None:
+        if self.other is not None:
+            self.other.wait_stream(self.ctx.stream)
+            for t in self.tensors:
+                if t is not None:
+                    t.record_stream(self.ctx.stream)
 
 
 def default_context(device: int = 0) -> Context:

@@ -1,0 +1,172 @@
+"""GPU: sequences that continue others (CompressedCache.fork) and the rows of a draft that stay
+(CompressedCache.keep), byte for byte against numpy on the planes, the bytes around them included."""
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+FORMATS = [(64, 4, 2, 8), (128, 3, 3, 2), (64, 3, 2, 3), (64, 1, 8, 1), (128, 5, 1, 2)]
+
+
+def _cache(ctx, fmt, batch, capacity, lens, seed=0):
+    """Random images (the rows behind a sequence's end as well) and lengths."""
+    from insitu_amd import QuantConfig
+    from insitu_amd.cache import CompressedCache
+    d, kb, vb, n_kv = fmt
+    c = CompressedCache(n_kv, d, capacity, QuantConfig(key_bits=kb, value_bits=vb), batch=batch, n_q_heads=n_kv, ctx=ctx)
+    rng = np.random.default_rng(seed)
+    imgs = rng.integers(0, 256, (batch, c.layout()["seq_stride"]), dtype=np.uint8)
+    for b in range(batch):
+        c.load_image(imgs[b], b)
+        c.set_length(lens[b], b)
+    return c, imgs
+
+
+def _take(lay, dst, at, src, rows, n_kv):
+    """Rows `rows` of image src become rows at, at + 1, .. of image dst, in every plane."""
+    rows = np.asarray(rows, dtype=np.int64)
+    old = src.copy()
+    off = 0
+    for h in range(n_kv):
+        for w, span in zip(lay["plane_width"], lay["plane_span"]):
+            for j, r in enumerate(rows):
+                dst[off + (at + j) * w:off + (at + j + 1) * w] = old[off + r * w:off + (r + 1) * w]
+            off += span
+
+
+def _same(c, imgs, lens):
+    assert c.lengths() == list(lens)
+    for b in range(len(lens)):
+        np.testing.assert_array_equal(c.image(b), imgs[b], err_msg=f"sequence {b}")
+
+
+def _device_lengths(c):
+    """An append on every sequence shows the lengths the device holds."""
+    d, n = c.head_dim, c.n_kv_heads
+    before = c.lengths()
+    one = np.full((c.batch, 1, n, d), 65536, dtype=np.int32)
+    c.append_rotated(one, one)
+    rows = [c.read_rows(0, n0, 1, b)[0] for b, n0 in enumerate(before)]
+    assert all(np.array_equal(r, rows[0]) for r in rows)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("length", [0, 1, 3, 16, 255, 1030])
+def test_whole_forks(ctx, fmt, length):
+    lens = [5, length, 9, 700, 2]
+    c, imgs = _cache(ctx, fmt, 5, 1100, lens)
+    c.fork(1, [0, 3, 4])
+    for b in (0, 3, 4):
+        _take(c.layout(), imgs[b], 0, imgs[1], np.arange(length), fmt[3])
+        lens[b] = length
+    _same(c, imgs, lens)
+    _device_lengths(c)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("length,n,kept", [(7, 7, 3), (40, 5, 0), (300, 64, 9), (1030, 1029, 517), (33, 1, 1)])
+def test_forks_with_a_selection(ctx, fmt, length, n, kept):
+    rng = np.random.default_rng(length)
+    lens = [4, length, 9]
+    c, imgs = _cache(ctx, fmt, 3, 1100, lens)
+    lists = [np.sort(rng.choice(n, kept, replace=False)), rng.integers(0, n, max(0, kept - 1))]
+    c.fork(1, [0, 2], n=n, rows=[list(map(int, x)) for x in lists])
+    for b, rows in zip((0, 2), lists):
+        idx = np.concatenate([np.arange(length - n), length - n + rows]).astype(np.int64)
+        _take(c.layout(), imgs[b], 0, imgs[1], idx, fmt[3])
+        lens[b] = len(idx)
+    _same(c, imgs, lens)
+    _device_lengths(c)
+
+
+def test_many_copies_of_several_sources(ctx):
+    fmt = FORMATS[0]
+    batch = 80
+    rng = np.random.default_rng(0)
+    lens = [int(x) for x in rng.integers(1, 60, batch)]
+    c, imgs = _cache(ctx, fmt, batch, 64, lens)
+    dst = [int(x) for x in rng.permutation(np.arange(3, batch))[:70]]
+    src = [int(x) for x in rng.integers(0, 3, 70)]
+    c.fork(src, dst)
+    for s, t in zip(src, dst):
+        _take(c.layout(), imgs[t], 0, imgs[s], np.arange(lens[s]), fmt[3])
+        lens[t] = lens[s]
+    _same(c, imgs, lens)
+
+
+def test_one_list_for_all_on_the_device(ctx):
+    import torch
+    fmt = FORMATS[1]
+    lens = [100, 0, 0]
+    c, imgs = _cache(ctx, fmt, 3, 128, lens)
+    rows = torch.tensor([1, 4, 90, -5, 1000], dtype=torch.int32, device=ctx.torch_device)   # the last two: 0 and 91
+    c.fork(0, [1, 2], n=92, rows=rows, counts=[5, 3])
+    for b, m in ((1, 5), (2, 3)):
+        _take(c.layout(), imgs[b], 0, imgs[0], np.concatenate([np.arange(8), 8 + np.array([1, 4, 90, 0, 91])[:m]]), fmt[3])
+        lens[b] = 8 + m
+    _same(c, imgs, lens)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("n,kept", [(1, 0), (1, 1), (64, 5), (13, 13), (300, 120), (1500, 1024), (1500, 1025), (2000, 1777)])
+def test_keep(ctx, fmt, n, kept):
+    rng = np.random.default_rng(n + kept)
+    lens = [n, n + 3, n + 70]
+    c, imgs = _cache(ctx, fmt, 3, n + 90, lens)
+    lists = [np.sort(rng.choice(n, kept, replace=False)) for _ in lens]
+    lists[1] = lists[1][:kept // 2]
+    lists[2] = rng.permutation(lists[2])
+    c.keep(n, [list(map(int, x)) for x in lists])
+    for b, rows in enumerate(lists):
+        base = lens[b] - n
+        _take(c.layout(), imgs[b], base, imgs[b], base + rows, fmt[3])
+        lens[b] = base + len(rows)
+    _same(c, imgs, lens)
+    _device_lengths(c)
+
+
+def test_keep_none_and_of_many_sequences(ctx):
+    fmt = FORMATS[0]
+    lens = [int(x) for x in np.random.default_rng(0).integers(8, 40, 70)]
+    c, imgs = _cache(ctx, fmt, 70, 48, lens)
+    c.keep(3)
+    lens = [x - 3 for x in lens]
+    _same(c, imgs, lens)
+    c.keep(5, [4, 1])
+    for b in range(70):
+        _take(c.layout(), imgs[b], lens[b] - 5, imgs[b], [lens[b] - 1, lens[b] - 4], fmt[3])
+    _same(c, imgs, [x - 3 for x in lens])
+    c.keep(0)
+    c.fork(0, [])
+    _same(c, imgs, [x - 3 for x in lens])
+
+
+def test_device_image_is_the_caches_memory(ctx):
+    import torch
+    fmt = FORMATS[0]
+    c, imgs = _cache(ctx, fmt, 2, 40, [20, 7])
+    img = c.device_image()
+    assert img.shape == imgs.shape and img.is_cuda and img.dtype == torch.uint8
+    np.testing.assert_array_equal(img.cpu().numpy(), imgs)
+    c.fork(0, [1])
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(img[1].cpu().numpy(), c.image(1))
+
+
+def test_refusals(ctx):
+    from insitu_amd import _lib
+    c, imgs = _cache(ctx, FORMATS[0], 4, 64, [10, 20, 30, 40])
+    bad = [dict(src=0, dst=[0]), dict(src=0, dst=[4]), dict(src=-1, dst=[1]), dict(src=0, dst=[1, 1]),
+           dict(src=[0, 1], dst=[2, 0]), dict(src=[0], dst=[1, 2]), dict(src=0, dst=[1], rows=[0]),
+           dict(src=0, dst=[1], n=11, rows=[0]), dict(src=0, dst=[1], n=5, rows=[5]), dict(src=0, dst=[1], n=5, rows=[-1]),
+           dict(src=0, dst=[1], n=5, rows=[0, 1], counts=[3]), dict(src=0, dst=[1, 2], n=5, rows=[[0], [1], [2]]),
+           dict(src=0, dst=[1], n=5, counts=[1])]
+    for kw in bad:
+        with pytest.raises((_lib.InsituError, ValueError)):
+            c.fork(kw.pop("src"), kw.pop("dst"), **kw)
+    for kw in (dict(n=11), dict(n=-1), dict(n=5, rows=[5]), dict(n=5, rows=[0], counts=[2, 0, 0, 0]),
+               dict(n=5, rows=[[0], [1]]), dict(n=5, counts=[1, 1, 1, 1])):
+        with pytest.raises((_lib.InsituError, ValueError)):
+            c.keep(kw.pop("n"), **kw)
+    _same(c, imgs, [10, 20, 30, 40])
