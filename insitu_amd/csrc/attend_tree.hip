@@ -279,7 +279,7 @@ struct Digits {
 };
 
 template <int D, int KB>
-__global__ void __launch_bounds__(W * 64) max_kernel(Job J) {
+__global__ void __launch_bounds__(W * 64, 4) max_kernel(Job J) {
     __shared__ Digits dgs;
     __shared__ uint32_t up[TREE_NODES][UPW];
     __shared__ int16_t at[TREE_NODES];
@@ -367,28 +367,34 @@ struct Values {
                     w[i][4 * p + 2] = v.z;
                     w[i][4 * p + 3] = v.w;
                 }
-            } else {
+            } else {                                   // 1-bit codes as 2-bit ones
 #pragma unroll
-                for (int k = 0; k < VW / 2; k += 2) {
-                    const uint2 v = *(const uint2 *)(vb0 + (t + i) * (D / 8) + 4 * k);
-                    w[i][k] = v.x;
-                    w[i][k + 1] = v.y;
+                for (int k = 0; k < VW; k += 4) {
+                    const uint2 v = *(const uint2 *)(vb0 + (t + i) * (D / 8) + 2 * k);
+                    w[i][k] = spread(v.x & 0xFFFFu);
+                    w[i][k + 1] = spread(v.x >> 16);
+                    w[i][k + 2] = spread(v.y & 0xFFFFu);
+                    w[i][k + 3] = spread(v.y >> 16);
                 }
             }
         }
     }
-    __device__ __forceinline__ void onehot(int c, int vb, v4i (&oh)[NC / 4]) const {
-        const int col = threadIdx.x & 15;
+    static __device__ __forceinline__ uint32_t spread(uint32_t x) {
+        x = (x | x << 8) & 0x00FF00FFu;
+        x = (x | x << 4) & 0x0F0F0F0Fu;
+        x = (x | x << 2) & 0x33333333u;
+        return (x | x << 1) & 0x55555555u;
+    }
+    __device__ __forceinline__ void onehot(int c, int col, v4i (&oh)[NC / 4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (NC == 4) {
-                const uint32_t x = vb == 2 ? w[i][c] >> (2 * col) & 3u : w[i][c >> 1] >> (16 * (c & 1) + col) & 1u;
-                oh[0][i] = (int)(1u << (8 * x));
+                oh[0][i] = (int)(1u << (8 * (w[i][c] >> (2 * col) & 3u)));
             } else {
                 // 16 channels are 48 bits, from bit 0 of word 3 c / 2 or bit 16 of the word before its end
                 const int w0 = 48 * c / 32, sh = 48 * c % 32 + 3 * col;
-                const uint64_t x = (uint64_t)w[i][w0] | (uint64_t)w[i][w0 + 1] << 32;
-                const uint64_t h = 1ull << (8 * ((uint32_t)(x >> sh) & 7u));
+                const uint32_t hi = w[i][w0 + 1], lo = sh < 32 ? w[i][w0] : hi;
+                const uint64_t h = 1ull << (8 * (__builtin_amdgcn_alignbit(hi, lo, sh & 31) & 7u));
                 oh[i >> 1][2 * (i & 1)] = (int)(uint32_t)h;
                 oh[i >> 1][2 * (i & 1) + 1] = (int)(uint32_t)(h >> 32);
             }
@@ -397,7 +403,7 @@ struct Values {
 };
 
 template <int D, int KB, int NC>
-__global__ void __launch_bounds__(W * 64) sum_kernel(Job J) {
+__global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel(Job J) {
     constexpr int CT = D / 16, PVK = NC / 4;
     __shared__ Digits dgs;
     __shared__ uint32_t up[TREE_NODES][UPW];
@@ -464,10 +470,14 @@ __global__ void __launch_bounds__(W * 64) sum_kernel(Job J) {
         return w < delta_max ? w : delta_max;
     };
     auto accumulate = [&](const v4i (&A)[3][PVK], const Values<D, NC> &V) __attribute__((always_inline)) {
+        // (opaque, so that the one-hot codes are made where they are used: kept over an events' loop they
+        // take 16 to 64 registers)
+        int ch = col;
+        asm volatile("" : "+v"(ch));
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
             v4i oh[PVK], t = {0, 0, 0, 0};
-            V.onehot(c, vb, oh);
+            V.onehot(c, ch, oh);
 #pragma unroll
             for (int k = 0; k < PVK; ++k) t = mma(oh[k], A[2][k], t);
             t = t << 8;
@@ -520,19 +530,23 @@ __global__ void __launch_bounds__(W * 64) sum_kernel(Job J) {
         const uint32_t nw[4] = {cur.norms.x, cur.norms.y, cur.norms.z, cur.norms.w};
         v4i A[3][PVK];
         uint32_t pw[4];
-        // p and the terms of every (token, code) as digit bytes. NC = 4: dword = token; NC = 8: block =
-        // token pair, dword = (token, half its codes)
-        auto terms = [&](const uint32_t (&dl)[4]) __attribute__((always_inline)) {
+        auto weights = [&](const uint32_t (&dl)[4]) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) pw[i] = lut(dl[i]);
             if (tail) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) pw[i] = in >> i & 1 ? pw[i] : 0u;
             }
+        };
+        // the terms of every (token, code) as digit bytes, of the tokens of segment `sg` (of seg). NC = 4: dword =
+        // token; NC = 8: block = token pair, dword = (token, half its codes)
+        auto terms = [&](uint32_t seg, uint32_t sg) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int32_t w = __mul24((int32_t)nw[i] >> 16, (int)pw[i]);
-                const uint32_t aw = w < 0 ? 0u - (uint32_t)w : (uint32_t)w;
+                const uint32_t pi = ((seg >> (8 * i)) & 0xFFu) == sg ? pw[i] : 0u;
+                lp += pi;
+                const int32_t w = __mul24((int32_t)nw[i] >> 16, (int)pi);
+            const uint32_t aw = w < 0 ? 0u - (uint32_t)w : (uint32_t)w;
                 wmax = aw > wmax ? aw : wmax;
                 bs += (float)aw;
                 const double wd = (double)w;
@@ -556,8 +570,8 @@ __global__ void __launch_bounds__(W * 64) sum_kernel(Job J) {
         };
         if (evl == 0) {
             const uint32_t dl[4] = {clip(m, s[0]), clip(m, s[1]), clip(m, s[2]), clip(m, s[3])};
-            terms(dl);
-            lp += (pw[0] + pw[1]) + (pw[2] + pw[3]);
+            weights(dl);
+            terms(0u, 0u);
             accumulate(A, V);
             continue;
         }
@@ -588,24 +602,10 @@ __global__ void __launch_bounds__(W * 64) sum_kernel(Job J) {
         const int row_ev = __shfl((int)(off + n), 48 + col);
         m = __shfl(e, 48 + col);
         n_ev += n;
-        terms(dl);
+        weights(dl);
         for (int sg = 0;; ++sg) {
-            v4i B[3][PVK];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool now = ((seg >> (8 * i)) & 0xFFu) == (uint32_t)sg;
-                lp += now ? pw[i] : 0u;
-#pragma unroll
-                for (int l = 0; l < 3; ++l) {
-                    if constexpr (NC == 4) {
-                        B[l][0][i] = now ? A[l][0][i] : 0;
-                    } else {
-                        B[l][i >> 1][2 * (i & 1)] = now ? A[l][i >> 1][2 * (i & 1)] : 0;
-                        B[l][i >> 1][2 * (i & 1) + 1] = now ? A[l][i >> 1][2 * (i & 1) + 1] : 0;
-                    }
-                }
-            }
-            accumulate(B, V);
+            terms(seg, (uint32_t)sg);
+            accumulate(A, V);
             const bool has = row_ev > sg;
             if (__ballot(has) == 0) break;
             // the event that opens segment sg + 1 of the row
