@@ -385,19 +385,18 @@ class CompressedCache(KVCache):
         those n: rows (m,) for all or (len(dst), m) numbers of 0 .. n - 1, counts of them each
         (default m). Lists of lists may differ in length. No destination is a source or comes
         twice. Rows behind a copy's end stay as they are. Stream-ordered."""
-        dst = [int(b) for b in np.atleast_1d(dst)]
-        srcs = [int(b) for b in np.broadcast_to(np.asarray(src, dtype=np.int64), (len(dst),))] if np.ndim(src) == 0 \
-            else [int(b) for b in src]
+        dst = [int(b) for b in dst]
+        srcs = [int(src)] * len(dst) if isinstance(src, (int, np.integer)) else [int(b) for b in src]
         if len(srcs) != len(dst):
             raise ValueError(f"{len(srcs)} sources for {len(dst)} destinations")
         if n == 0 and (rows is not None or counts is not None):
             raise ValueError("rows and counts select from the last n rows: n is 0")
         rows, stride, counts = self._kept(n, rows, len(dst), counts)
-        arr = lambda t, v: (t * max(1, len(v)))(*v)
+        many = ctypes.c_int32 * len(dst)
         with self.ctx.ordered(rows):
             _lib.check(self.ctx.lib.insitu_cache_fork(
-                self.handle, len(dst), arr(ctypes.c_int32, srcs), arr(ctypes.c_int32, dst), n,
-                ptr(rows) if rows is not None else None, stride, arr(ctypes.c_int64, counts) if n else None))
+                self.handle, len(dst), many(*srcs), many(*dst), n,
+                ptr(rows) if rows is not None else None, stride, (ctypes.c_int64 * len(dst))(*counts) if n else None))
         self._keep_rows = rows
 
     def keep(self, n: int, rows=None, *, counts=None) -> None:

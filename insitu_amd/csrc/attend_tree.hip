@@ -6,7 +6,7 @@
 // A row of this file is one (node, query head) of a KV head's group; a wave takes tiles of 16 rows by 16
 // tokens over one span of the context. Every span is walked at the same time, in three launches that
 // wait on nobody:
-//   max_kernel     each (row, span)'s largest score;
+//   max_kernel     each row's largest score in parts of the spans;
 //   sum_kernel     the walk, from the maximum of the spans before (online) or of all (two-pass): the terms
 //                  floor(v_norm p c / 2^23) of a run of rows between two events are only added, so a span
 //                  gives a run's sum S and denominator L without knowing what came before it. Where the
@@ -24,6 +24,7 @@
 // three digits, which the one-hot value codes of the tokens sum up, lane = (row, 4 channels).
 #include <algorithm>
 #include <cstdlib>
+#include <type_traits>
 
 #include "digits.h"
 #include "query.h"
@@ -34,9 +35,10 @@ namespace insitu {
 namespace tr {
 
 constexpr int W = 4;                                   // waves a workgroup of max_kernel and sum_kernel
-constexpr int CW = 8;                                  // and of combine_kernel, two rows each
+constexpr int CW = 8;                                  // and of combine_kernel, a row each
 constexpr int UPW = TREE_NODES / 32 + 3;               // words of a node's path: ones, the bits, two of zeros
-constexpr int EXTRA = 256;                             // runs a row tile holds beside its spans' first ones
+// runs a row tile holds beside its spans' first ones: 256, and up to 4,096 where few tiles leave room
+constexpr int EXTRA_MIN = 256, EXTRA_MAX = 4096;
 constexpr int SPAN_MAX = 32768;                        // tokens a span: its events fit 31 bits, its L 32
 constexpr uint32_t LUT_N = LUT_SPAN + 1;
 constexpr double TERM_MAGIC = 402653184.0 + 8421504.0; // 1.5 * 2^28 + 0x808080: ulp 2^-24
@@ -50,10 +52,10 @@ struct __attribute__((aligned(4))) u128 {              // 16 bytes of a 4-byte a
     uint32_t x, y, z, w;
 };
 
-// Per row tile: 16 nspan runs, the first of each (span, row), and EXTRA more.
+// Per row tile: 16 nspan runs, the first of each (span, row), and `extra` more.
 struct Scratch {
-    int32_t *top;          // [tile][span][16]: largest scores
-    uint32_t *over;        // [tile][span]: rows whose scores did not do, a bit each
+    int32_t *top;          // [tile][max_kernel's span][16]: largest scores
+    uint32_t *over;        // [tile][max_kernel's span]: rows whose scores did not do, a bit each
     uint32_t *ev;          // [tile][span][16]: events, BAD
     uint32_t *pool;        // [tile]: extra runs taken
     uint4 *meta;           // [tile][run]: L, f | USED, the next run of the span or -1, a bound of |terms| (float)
@@ -68,7 +70,8 @@ struct Job {
     const int64_t *len;
     const int32_t *parents;
     int64_t pstride;
-    int32_t n, rows, tiles, span, nspan, two, seq0, nseq, count;   // count: gather statistics
+    int32_t n, rows, tiles, span, nspan, mspan, nms;   // mspan, nms: max_kernel's spans, whole parts of the others
+    int32_t extra, two, seq0, nseq, count;             // count: gather statistics
     Scratch sc;
     DevStats *st;
 };
@@ -237,27 +240,27 @@ __device__ __forceinline__ bool scores(const v4i (&a)[D / 64][3], const v4i (&qd
 }
 
 // A workgroup's place: chains fastest (a KV head's rows then stay in one XCD's cache where there are 8),
-// then the row tiles, which read the same tokens, then the spans.
+// then the row tiles (or groups of them), which read the same tokens, then the spans.
 struct Place {
     int chain, b, kvh, tile, s;
     int64_t T, base, lo, hi;                           // the wave's span [lo, hi) of T rows
     bool tail;                                         // the workgroup's spans reach the tree's rows
-    __device__ __forceinline__ bool find(const Job &J) {
+    __device__ __forceinline__ bool find(const Job &J, int tiles, int span, int waves) {
         const int chains = J.nseq * J.g.n_kv;
         chain = (int)(blockIdx.x % (unsigned)chains);
         const int rest = (int)(blockIdx.x / (unsigned)chains);
-        tile = rest % J.tiles;
-        const int s0 = rest / J.tiles * W;
+        tile = rest % tiles;
+        const int s0 = rest / tiles * waves;
         s = s0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         b = J.seq0 + chain / J.g.n_kv;
         kvh = chain % J.g.n_kv;
         T = J.len[b];
         base = T - J.n;
-        const int64_t end = (int64_t)(s0 + W) * J.span;
+        const int64_t end = (int64_t)(s0 + waves) * span;
         tail = (end < T ? end : T) > base;
-        lo = (int64_t)s * J.span;
-        hi = lo + J.span < T ? lo + J.span : T;
-        return (int64_t)s0 * J.span < T;
+        lo = (int64_t)s * span;
+        hi = lo + span < T ? lo + span : T;
+        return (int64_t)s0 * span < T;
     }
 };
 
@@ -278,29 +281,39 @@ struct Digits {
     }
 };
 
-template <int D, int KB>
-__global__ void __launch_bounds__(W * 64, 4) max_kernel(Job J) {
+// RT row tiles a wave, which share the expanded keys.
+template <int D, int KB, int RT>
+__global__ void __launch_bounds__(W * 64, RT > 2 ? 3 : 4) max_kernel(Job J) {
     __shared__ Digits dgs;
     __shared__ uint32_t up[TREE_NODES][UPW];
     __shared__ int16_t at[TREE_NODES];
     Place p;
-    if (!p.find(J)) return;
-    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    if (!p.find(J, (J.tiles + RT - 1) / RT, J.mspan, W)) return;
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, tile0 = p.tile * RT;
+    const int nt = imin(RT, J.tiles - tile0);
     dgs.fill(J.tabs, J.g.kb);
     int none = 0;
     if (p.tail) none = tree_paths(J.parents + p.b * J.pstride, J.n, up, at);
     __syncthreads();
-    if (J.count && none && p.kvh == 0 && p.tile == 0 && p.T <= (int64_t)(p.s / W + 1) * W * J.span)
+    if (J.count && none && p.kvh == 0 && p.tile == 0 && p.T <= (int64_t)(p.s / W + 1) * W * J.mspan)
         atomicAdd(&J.st->range_errors, (unsigned long long)none);
     if (p.lo >= p.hi) return;
-    Query<D, KB> Q;
-    Q.load(J, p.b, p.kvh, p.tile, J.tabs->kc_absmax, J.count && p.s == 0 ? &J.st->range_errors : nullptr);
+    Query<D, KB> Q[RT];
+    const uint32_t *path[RT];
+    int32_t m[RT], lowest[RT];
+    bool over[RT];
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        const int tile = tile0 + imin(k, nt - 1);      // (a tile past the last one is not scored)
+        Q[k].load(J, p.b, p.kvh, tile, J.tabs->kc_absmax, J.count && p.s == 0 && k < nt ? &J.st->range_errors : nullptr);
+        path[k] = up[imin(tile * 16 + col, J.rows - 1) / J.g.G];
+        m[k] = NONE;
+        lowest[k] = 0;
+        over[k] = Q[k].bad;
+    }
     uint32_t dg[3][4];
     dgs.read(dg);
     const uint8_t *hb = plane_ptr(J.g, p.b, p.kvh, 0), *nb = hb + (J.g.n_planes - 1) * J.g.span;
-    const uint32_t *path = up[imin(p.tile * 16 + col, J.rows - 1) / J.g.G];
-    int32_t m = NONE, lowest = 0;
-    bool over = Q.bad;
     Keys<D, KB> next;
     next.load(hb, nb, J.g.span, p.lo);
     for (int64_t t0 = p.lo; t0 < p.hi; t0 += 16) {
@@ -308,34 +321,48 @@ __global__ void __launch_bounds__(W * 64, 4) max_kernel(Job J) {
         if (t0 + 16 < p.hi) next.load(hb, nb, J.g.span, t0 + 16);
         v4i a[D / 64][3];
         cur.expand(dg, a);
-        uint32_t in = 15u;
-        if (t0 + 16 > p.base) in = visible4(path, (int)(t0 - p.base) + 4 * grp);
-        int32_t s[4];
-        over |= scores<D>(a, Q.qd, cur.norms, Q.check, in, s);
+        const bool tail = t0 + 16 > p.base;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool on = in >> i & 1;
-            m = on && s[i] > m ? s[i] : m;
-            lowest = on && s[i] < lowest ? s[i] : lowest;
+        for (int k = 0; k < RT; ++k) {
+            if (k > 0 && k >= nt) break;
+            uint32_t in = 15u;
+            if (tail) in = visible4(path[k], (int)(t0 - p.base) + 4 * grp);
+            int32_t s[4];
+            over[k] |= scores<D>(a, Q[k].qd, cur.norms, Q[k].check, in, s);
+            if (tail) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool on = in >> i & 1;
+                    m[k] = on && s[i] > m[k] ? s[i] : m[k];
+                    lowest[k] = on && s[i] < lowest[k] ? s[i] : lowest[k];
+                }
+            } else {
+                m[k] = imax(m[k], imax(imax(s[0], s[1]), imax(s[2], s[3])));
+                lowest[k] = imin(lowest[k], imin(imin(s[0], s[1]), imin(s[2], s[3])));
+            }
         }
     }
-    const int64_t tl = (int64_t)p.chain * J.tiles + p.tile, at0 = tl * J.nspan + p.s;
-    m = row_max(m);
-    if (grp == 0) J.sc.top[at0 * 16 + col] = m;
-    const uint64_t bad = __ballot(over);
-    if (lane == 0) {
-        J.sc.over[at0] = (uint32_t)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu);
-        if (p.s == 0) J.sc.pool[tl] = 0;
-    }
-    if (J.count) {
-        const bool mine = !over && p.tile * 16 + col < J.rows;
-        const int64_t a = m == NONE ? 0 : m < 0 ? -(int64_t)m : m, c = -(int64_t)lowest;
-        const int64_t x = wave_max_i64(mine ? (a > c ? a : c) : 0);
-        if (lane == 0 && (unsigned long long)x > J.st->max_abs_score) atomicMax(&J.st->max_abs_score, (unsigned long long)x);
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        if (k >= nt) break;
+        const int64_t tl = (int64_t)p.chain * J.tiles + tile0 + k, at0 = tl * J.nms + p.s;
+        const int32_t top = row_max(m[k]);
+        if (grp == 0) J.sc.top[at0 * 16 + col] = top;
+        const uint64_t bad = __ballot(over[k]);
+        if (lane == 0) {
+            J.sc.over[at0] = (uint32_t)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu);
+            if (p.s == 0) J.sc.pool[tl] = 0;
+        }
+        if (J.count) {
+            const bool mine = !over[k] && (tile0 + k) * 16 + col < J.rows;
+            const int64_t a = top == NONE ? 0 : top < 0 ? -(int64_t)top : top, c = -(int64_t)lowest[k];
+            const int64_t x = wave_max_i64(mine ? (a > c ? a : c) : 0);
+            if (lane == 0 && (unsigned long long)x > J.st->max_abs_score) atomicMax(&J.st->max_abs_score, (unsigned long long)x);
+        }
     }
 }
 
-// A tile's value words, lane = tokens t0 + 4 grp .. + 3; then one-hot, lane = (channel 16 c + lane % 16, 4 tokens).
+// A tile's value words, lane = tokens t0 + 4 grp .. + 3.
 template <int D, int NC>
 struct Values {
     static constexpr int VW = D * (NC == 8 ? 3 : 2) / 32;
@@ -344,7 +371,7 @@ struct Values {
         const int64_t t = t0 + 4 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if constexpr (NC == 8) {
+            if (NC == 8 || vb == 2) {
 #pragma unroll
                 for (int p = 0; p < VW / 4; ++p) {
                     const uint4 v = *(const uint4 *)(vb0 + p * span + (t + i) * 16);
@@ -353,19 +380,10 @@ struct Values {
                     w[i][4 * p + 2] = v.z;
                     w[i][4 * p + 3] = v.w;
                 }
-                if constexpr (VW % 4) {
+                if constexpr (VW % 4 != 0) {
                     const uint2 v = *(const uint2 *)(vb0 + (VW / 4) * span + (t + i) * 8);
                     w[i][VW - 2] = v.x;
                     w[i][VW - 1] = v.y;
-                }
-            } else if (vb == 2) {
-#pragma unroll
-                for (int p = 0; p < VW / 4; ++p) {
-                    const uint4 v = *(const uint4 *)(vb0 + p * span + (t + i) * 16);
-                    w[i][4 * p] = v.x;
-                    w[i][4 * p + 1] = v.y;
-                    w[i][4 * p + 2] = v.z;
-                    w[i][4 * p + 3] = v.w;
                 }
             } else {                                   // 1-bit codes as 2-bit ones
 #pragma unroll
@@ -385,70 +403,55 @@ struct Values {
         x = (x | x << 2) & 0x33333333u;
         return (x | x << 1) & 0x55555555u;
     }
-    __device__ __forceinline__ void onehot(int c, int col, v4i (&oh)[NC / 4]) const {
+    // the codes of channel 16 c + col, a byte a token
+    __device__ __forceinline__ uint32_t codes(int c, int col) const {
+        if constexpr (NC == 4) {
+            const uint32_t b = (uint32_t)col >> 2, s = b | (4u + b) << 8;
+            const uint32_t x = perm(w[1][c], w[0][c], s | 0x0C0C0000u) | perm(w[3][c], w[2][c], s << 16 | 0x0C0Cu);
+            return x >> (2 * (col & 3)) & 0x03030303u;
+        } else {
+            // 16 channels are 48 bits, from bit 0 of word 3 c / 2 or bit 16 of the word before its end
+            const int w0 = 48 * c / 32, sh = 48 * c % 32 + 3 * col;
+            uint32_t x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (NC == 4) {
-                oh[0][i] = (int)(1u << (8 * (w[i][c] >> (2 * col) & 3u)));
-            } else {
-                // 16 channels are 48 bits, from bit 0 of word 3 c / 2 or bit 16 of the word before its end
-                const int w0 = 48 * c / 32, sh = 48 * c % 32 + 3 * col;
+            for (int i = 0; i < 4; ++i) {
                 const uint32_t hi = w[i][w0 + 1], lo = sh < 32 ? w[i][w0] : hi;
-                const uint64_t h = 1ull << (8 * (__builtin_amdgcn_alignbit(hi, lo, sh & 31) & 7u));
-                oh[i >> 1][2 * (i & 1)] = (int)(uint32_t)h;
-                oh[i >> 1][2 * (i & 1) + 1] = (int)(uint32_t)(h >> 32);
+                x[i] = __builtin_amdgcn_alignbit(hi, lo, sh & 31);
             }
+            return (perm(x[1], x[0], 0x0C0C0400u) | perm(x[3], x[2], 0x04000C0Cu)) & 0x07070707u;
         }
     }
 };
 
-template <int D, int KB, int NC>
-__global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel(Job J) {
-    constexpr int CT = D / 16, PVK = NC / 4;
-    __shared__ Digits dgs;
-    __shared__ uint32_t up[TREE_NODES][UPW];
-    __shared__ int16_t at[TREE_NODES];
-    __shared__ uint16_t lut_s[LUT_N + 7];
-    Place p;
-    if (!p.find(J)) return;
-    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
-    dgs.fill(J.tabs, J.g.kb);
-    {
-        const int32_t x = J.tabs->exp_table[tid];
-#pragma unroll
-        for (int i = 0; i < LUT_SPAN / 256; ++i) lut_s[256 * i + tid] = (uint16_t)(x >> i);
-        if (tid == 0) lut_s[LUT_SPAN] = 0;
-    }
-    if (p.tail) tree_paths(J.parents + p.b * J.pstride, J.n, up, at);
-    __syncthreads();
-    if (p.lo >= p.hi) return;
+// 1 where a code (bytes of 4) is m.
+__device__ __forceinline__ uint32_t is_code(int m, uint32_t codes) {
+    return m < 4 ? perm(0u, 1u << (8 * m), codes) : perm(1u << (8 * (m - 4)), 0u, codes);
+}
 
+// A wave's walk over its span, from the maximum m before it (or, two-pass, of all): its runs into the
+// scratch; returns the row's events, with BAD where it needs the serial path.
+template <int D, int KB, int NC>
+__device__ __forceinline__ uint32_t walk(const Job &J, const Place &p, const Query<D, KB> &Q, int32_t m, const Digits &dgs,
+                                     const uint32_t *path, const uint16_t *lut_s) {
+    constexpr int CT = D / 16, PVK = NC / 4;
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
     const int64_t tl = (int64_t)p.chain * J.tiles + p.tile;
-    // the maximum of the spans before, or of all
-    int32_t m = NONE;
-    {
-        const int end = J.two ? (int)((p.T + J.span - 1) / J.span) : p.s;
-        const int32_t *top = J.sc.top + tl * J.nspan * 16 + col;
-        for (int i = grp; i < end; i += 4) m = imax(m, top[i * 16]);
-        m = row_max(m);
-    }
-    Query<D, KB> Q;
-    Q.load(J, p.b, p.kvh, p.tile, J.tabs->kc_absmax, nullptr);
     uint32_t dg[3][4];
     dgs.read(dg);
+    const int vb = J.g.vb;
     double vcs[NC], vcmax = 0.0;                       // value centroids / 2^23
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        vcs[i] = __longlong_as_double(uni64(__double_as_longlong(i < (1 << J.g.vb) ? (double)J.tabs->vc[i] * 0x1p-23 : 0.0)));
+        vcs[i] = __longlong_as_double(uni64(__double_as_longlong(i < (1 << vb) ? (double)J.tabs->vc[i] * 0x1p-23 : 0.0)));
         vcmax = fmax(vcmax, fabs(vcs[i]));
     }
+    // |v_norm p| up to which a term is two balanced bytes
+    const uint32_t wide = (uint32_t)uni32((int)(uint32_t)(32639.0 / fmax(vcmax, 0x1p-16)));
     const uint32_t delta_max = (uint32_t)J.tabs->delta_max;
     const uint8_t *hb = plane_ptr(J.g, p.b, p.kvh, 0), *nb = hb + (J.g.n_planes - 1) * J.g.span;
     const uint8_t *vb0 = hb + (int64_t)((J.g.key_bytes + 15) / 16) * J.g.span;
-    const uint32_t *path = up[imin(p.tile * 16 + col, J.rows - 1) / J.g.G];
-    const int vb = J.g.vb;
-    const bool first = p.s == 0;                       // what the span finds is nothing: it scales in place
-    const int64_t run0 = tl * (16 * (int64_t)J.nspan + EXTRA);
+    bool first = p.s == 0;                             // what the span finds is nothing: it scales in place
+    const int64_t run0 = tl * (16 * (int64_t)J.nspan + J.extra);
 
     v4i acc[CT];                                       // lane = (row, 4 channels of each 16)
 #pragma unroll
@@ -456,7 +459,8 @@ __global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel
     uint32_t lp = 0;                                   // the lane's part of the denominator since the last event
     uint32_t l0 = 0;                                   // first span: the row's denominator up to there
     float bs = 0.0f;                                   // the lane's part of sum |v_norm p|
-    uint32_t wmax = 0;                                 // its largest
+    const float bs_max = 0x1p28f / (float)fmax(vcmax, 0x1p-23);          // (four lanes: terms below 2^30, and a tile's)
+    uint32_t wmax = 0;                                 // the largest |v_norm p|
     uint32_t n_ev = 0;                                 // the lane's events
     bool bad = Q.bad;
     int slot = p.s * 16 + col;                         // the row's open run, and its factor
@@ -468,26 +472,6 @@ __global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel
     auto clip = [&](int32_t hi, int32_t lo) __attribute__((always_inline)) -> uint32_t {
         const uint32_t w = (uint32_t)hi - (uint32_t)lo;
         return w < delta_max ? w : delta_max;
-    };
-    auto accumulate = [&](const v4i (&A)[3][PVK], const Values<D, NC> &V) __attribute__((always_inline)) {
-        // (opaque, so that the one-hot codes are made where they are used: kept over an events' loop they
-        // take 16 to 64 registers)
-        int ch = col;
-        asm volatile("" : "+v"(ch));
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            v4i oh[PVK], t = {0, 0, 0, 0};
-            V.onehot(c, ch, oh);
-#pragma unroll
-            for (int k = 0; k < PVK; ++k) t = mma(oh[k], A[2][k], t);
-            t = t << 8;
-#pragma unroll
-            for (int k = 0; k < PVK; ++k) t = mma(oh[k], A[1][k], t);
-            t = (t << 8) + acc[c];
-#pragma unroll
-            for (int k = 0; k < PVK; ++k) t = mma(oh[k], A[0][k], t);
-            acc[c] = t;
-        }
     };
     // the open run of the rows where `has`: into its record
     auto hand_over = [&](bool has, int next) __attribute__((always_inline)) {
@@ -505,21 +489,40 @@ __global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel
 #pragma unroll
         for (int c = 0; c < CT; ++c) *(v4i *)(to + 16 * c) = acc[c];
     };
+    // the run of the rows where `has` ends, and one with factor f begins
+    auto next_run = [&](bool has, uint32_t f) __attribute__((always_inline)) {
+        int to = 0;
+        if (has && grp == 0) to = (int)atomicAdd(J.sc.pool + tl, 1u);
+        to = __shfl(to, col);
+        bad = bad || (has && to >= J.extra);
+        to = 16 * J.nspan + imin(to, J.extra - 1);
+        hand_over(has, to);
+        if (has) {
+            slot = to;
+            fopen = f;
+            lp = 0;
+            bs = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) acc[c] = v4i{0, 0, 0, 0};
+        }
+    };
 
-    Keys<D, KB> nxt;
-    nxt.load(hb, nb, J.g.span, p.lo);
+    Keys<D, KB> next;
+    next.load(hb, nb, J.g.span, p.lo);
     for (int64_t t0 = p.lo; t0 < p.hi; t0 += 16) {
-        const Keys<D, KB> cur = nxt;
-        Values<D, NC> V;
+        const Keys<D, KB> cur = next;
+        Values<D, NC> V;                               // (loaded before it is known whether any counts)
         V.load(vb0, J.g.span, t0, vb);
-        if (t0 + 16 < p.hi) nxt.load(hb, nb, J.g.span, t0 + 16);
-        v4i a[D / 64][3];
-        cur.expand(dg, a);
+        if (t0 + 16 < p.hi) next.load(hb, nb, J.g.span, t0 + 16);
         const bool tail = t0 + 16 > p.base;
-        uint32_t in = 15u;
-        if (tail) in = visible4(path, (int)(t0 - p.base) + 4 * grp);
         int32_t s[4];
-        scores<D>(a, Q.qd, cur.norms, false, in, s);
+        uint32_t in = 15u;
+        {
+            v4i a[D / 64][3];
+            cur.expand(dg, a);
+            if (tail) in = visible4(path, (int)(t0 - p.base) + 4 * grp);
+            scores<D>(a, Q.qd, cur.norms, false, in, s);
+        }
         if (tail) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[i] = in >> i & 1 ? s[i] : NONE;
@@ -527,9 +530,17 @@ __global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel
         const int32_t mx = imax(imax(s[0], s[1]), imax(s[2], s[3]));
         const uint64_t evl = __ballot(mx > m);
         if (evl == 0 && __ballot((uint32_t)m - (uint32_t)mx < delta_max) == 0) continue;      // every p is 0
-        const uint32_t nw[4] = {cur.norms.x, cur.norms.y, cur.norms.z, cur.norms.w};
-        v4i A[3][PVK];
+        const int32_t vn[4] = {(int32_t)cur.norms.x >> 16, (int32_t)cur.norms.y >> 16, (int32_t)cur.norms.z >> 16,
+                               (int32_t)cur.norms.w >> 16};
+        if (__ballot(bs > bs_max) != 0) {              // acc may leave 32 bits: it becomes a run
+            first = false;
+            lp += grp == 0 ? l0 : 0u;
+            l0 = 0;
+            next_run(true, 1u << PROB_FRAC);
+        }
         uint32_t pw[4];
+        const float bs0 = bs;
+        v4i A[3][PVK];                     // the columns' digits
         auto weights = [&](const uint32_t (&dl)[4]) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) pw[i] = lut(dl[i]);
@@ -538,106 +549,167 @@ __global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel
                 for (int i = 0; i < 4; ++i) pw[i] = in >> i & 1 ? pw[i] : 0u;
             }
         };
-        // the terms of every (token, code) as digit bytes, of the tokens of segment `sg` (of seg). NC = 4: dword =
-        // token; NC = 8: block = token pair, dword = (token, half its codes)
-        auto terms = [&](uint32_t seg, uint32_t sg) __attribute__((always_inline)) {
+        // the terms for the weights; returns the largest |v_norm p|
+        auto terms = [&](const uint32_t (&pp)[4]) __attribute__((always_inline)) -> uint32_t {
+            uint32_t top = 0;
+            double wd[4];
+            uint32_t aw[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t pi = ((seg >> (8 * i)) & 0xFFu) == sg ? pw[i] : 0u;
-                lp += pi;
-                const int32_t w = __mul24((int32_t)nw[i] >> 16, (int)pi);
-            const uint32_t aw = w < 0 ? 0u - (uint32_t)w : (uint32_t)w;
-                wmax = aw > wmax ? aw : wmax;
-                bs += (float)aw;
-                const double wd = (double)w;
+                const int32_t w = __mul24(vn[i], (int)pp[i]);
+                aw[i] = w < 0 ? 0u - (uint32_t)w : (uint32_t)w;
+                top = aw[i] > top ? aw[i] : top;
+                bs += (float)aw[i];
+                wd[i] = (double)w;
+            }
 #pragma unroll
-                for (int k4 = 0; k4 < NC / 4; ++k4) {
-                    const int kbk = NC == 4 ? 0 : i >> 1, dw = NC == 4 ? i : 2 * (i & 1) + k4;
-                    uint32_t yl[4], yh[4];
+            for (int c = 0; c < NC; ++c) {
+                uint32_t yl[4], yh[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint64_t y = (uint64_t)__double_as_longlong(fma(wd, vcs[4 * k4 + k], TERM_MAGIC));
-                        yl[k] = (uint32_t)y;
-                        yh[k] = (uint32_t)(y >> 32);
+                for (int i = 0; i < 4; ++i) {
+                    const uint64_t y = (uint64_t)__double_as_longlong(fma(wd[i], vcs[c], TERM_MAGIC));
+                    yl[i] = (uint32_t)y;
+                    yh[i] = (uint32_t)(y >> 32);
+                }
+                const uint32_t l01 = perm(yl[1], yl[0], 0x0C0C0703u), l23 = perm(yl[3], yl[2], 0x07030C0Cu);
+                const uint32_t h01 = perm(yh[1], yh[0], 0x05010400u), h23 = perm(yh[3], yh[2], 0x05010400u);
+                A[0][c / 4][c % 4] = (int)((l01 | l23) ^ 0x80808080u);
+                A[1][c / 4][c % 4] = (int)(perm(h23, h01, 0x05040100u) ^ 0x80808080u);
+                A[2][c / 4][c % 4] = (int)(perm(h23, h01, 0x07060302u) ^ 0x80808080u);
+            }
+            return top;
+        };
+        // acc += the terms in A
+        auto accumulate = [&](auto three, const v4i (&A)[3][PVK]) __attribute__((always_inline)) {
+            // (opaque, so that the one-hot codes are made where they are used: kept over an events' loop they
+            // take 32 registers and more, but for 16 where there are 4 codes and 4 tiles)
+            int ch = col;
+            if constexpr (CT * NC > 16) asm volatile("" : "+v"(ch));
+            constexpr int GC = D == 64 ? 2 : 1;        // channel tiles at a time: registers
+#pragma unroll
+            for (int c0 = 0; c0 < CT; c0 += GC) {
+                v4i oh[GC][PVK];
+                v4i t[GC];
+#pragma unroll
+                for (int c = 0; c < GC; ++c) {
+                    const uint32_t x = V.codes(c0 + c, ch);
+#pragma unroll
+                    for (int k = 0; k < NC; ++k) oh[c][k / 4][k % 4] = (int)is_code(k, x);
+                    t[c] = v4i{0, 0, 0, 0};
+                    if constexpr (decltype(three)::value) {
+#pragma unroll
+                        for (int k = 0; k < PVK; ++k) t[c] = mma(oh[c][k], A[2][k], t[c]);
                     }
-                    const uint32_t l01 = perm(yl[1], yl[0], 0x0C0C0703u), l23 = perm(yl[3], yl[2], 0x07030C0Cu);
-                    const uint32_t h01 = perm(yh[1], yh[0], 0x05010400u), h23 = perm(yh[3], yh[2], 0x05010400u);
-                    A[0][kbk][dw] = (int)((l01 | l23) ^ 0x80808080u);
-                    A[1][kbk][dw] = (int)(perm(h23, h01, 0x05040100u) ^ 0x80808080u);
-                    A[2][kbk][dw] = (int)(perm(h23, h01, 0x07060302u) ^ 0x80808080u);
+                }
+#pragma unroll
+                for (int c = 0; c < GC; ++c) {
+                    if constexpr (decltype(three)::value) t[c] = t[c] << 8;
+#pragma unroll
+                    for (int k = 0; k < PVK; ++k) t[c] = mma(oh[c][k], A[1][k], t[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < GC; ++c) {
+                    t[c] = (t[c] << 8) + acc[c0 + c];
+#pragma unroll
+                    for (int k = 0; k < PVK; ++k) t[c] = mma(oh[c][k], A[0][k], t[c]);
+                    acc[c0 + c] = t[c];
                 }
             }
         };
         if (evl == 0) {
             const uint32_t dl[4] = {clip(m, s[0]), clip(m, s[1]), clip(m, s[2]), clip(m, s[3])};
             weights(dl);
-            terms(0u, 0u);
-            accumulate(A, V);
+            const uint32_t top = terms(pw);
+            wmax = top > wmax ? top : wmax;
+            lp += (pw[0] + pw[1]) + (pw[2] + pw[3]);
+            if (__ballot(top > wide) == 0)
+                accumulate(std::false_type{}, A);
+            else
+                accumulate(std::true_type{}, A);
             continue;
         }
-        // events: the row's tokens fall into segments, one more than its events (bits 8 i of seg the
-        // segment of token i)
-        int32_t e = m;                                 // the maximum before the lane's tokens
+        // events: the row's tokens fall into segments, one more than its events (bits 8 i of seg the segment of
+        // token i)
         {
-            const int32_t x = __shfl(mx, lane - 16), y = __shfl(mx, lane - 32), z = __shfl(mx, lane - 48);
-            if (grp > 0) e = imax(e, x);
-            if (grp > 1) e = imax(e, y);
-            if (grp > 2) e = imax(e, z);
-        }
-        uint32_t dl[4], fe[4], seg = 0, n = 0;
+            int32_t e = m;                             // the maximum before the lane's tokens
+            {
+                const int32_t x = __shfl(mx, lane - 16), y = __shfl(mx, lane - 32), z = __shfl(mx, lane - 48);
+                if (grp > 0) e = imax(e, x);
+                if (grp > 1) e = imax(e, y);
+                if (grp > 2) e = imax(e, z);
+            }
+            uint32_t dl[4], fe[4], seg = 0, n = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool ev = s[i] > e;
-            const uint32_t dd = clip(ev ? s[i] : e, ev ? e : s[i]);
-            fe[i] = ev ? dd + 1u : 0u;                 // an event's distance, + 1
-            dl[i] = ev ? 0u : dd;
-            e = ev ? s[i] : e;
-            n += ev ? 1 : 0;
-            seg |= n << (8 * i);
-        }
-        const uint32_t n1 = (uint32_t)__shfl((int)n, lane - 16), n2 = (uint32_t)__shfl((int)n, lane - 32),
-                       n3 = (uint32_t)__shfl((int)n, lane - 48);
-        const uint32_t off = (grp > 0 ? n1 : 0) + (grp > 1 ? n2 : 0) + (grp > 2 ? n3 : 0);
-        seg += off * 0x01010101u;                      // at most 16
-        const int row_ev = __shfl((int)(off + n), 48 + col);
-        m = __shfl(e, 48 + col);
-        n_ev += n;
-        weights(dl);
-        for (int sg = 0;; ++sg) {
-            terms(seg, (uint32_t)sg);
-            accumulate(A, V);
-            const bool has = row_ev > sg;
-            if (__ballot(has) == 0) break;
-            // the event that opens segment sg + 1 of the row
-            uint32_t fd = 0;
+            for (int i = 0; i < 4; ++i) {
+                const bool ev = s[i] > e;
+                const uint32_t dd = clip(ev ? s[i] : e, ev ? e : s[i]);
+                fe[i] = ev ? dd + 1u : 0u;             // an event's distance, + 1
+                dl[i] = ev ? 0u : dd;
+                e = ev ? s[i] : e;
+                n += ev ? 1 : 0;
+                seg |= n << (8 * i);
+            }
+            const uint32_t n1 = (uint32_t)__shfl((int)n, lane - 16), n2 = (uint32_t)__shfl((int)n, lane - 32),
+                           n3 = (uint32_t)__shfl((int)n, lane - 48);
+            const uint32_t off = (grp > 0 ? n1 : 0) + (grp > 1 ? n2 : 0) + (grp > 2 ? n3 : 0);
+            seg += off * 0x01010101u;                  // at most 16
+            const int row_ev = __shfl((int)(off + n), 48 + col);
+            m = __shfl(e, 48 + col);
+            n_ev += n;
+            weights(dl);
+            // a segment's terms are the tile's, masked, or made anew where the tile's would not fit beside them
+            constexpr bool KEEP = CT * NC <= 16;
+            uint32_t top = 0;
+            if constexpr (KEEP) top = terms(pw);
+            float bs_tile = bs - bs0;                  // (every run of the tile is bounded by all of it)
+            for (int sg = 0;; ++sg) {
+                uint32_t mask = 0, pp[4];              // the segment's tokens, a byte each
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fd = ((seg >> (8 * i)) & 0xFFu) == (uint32_t)(sg + 1) && fe[i] ? fe[i] : fd;
-            fd = row_or(fd);
-            const uint32_t f = has ? lut(fd - 1u) : 1u << PROB_FRAC;
-            if (first) {
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[c][i] = (int32_t)(((int64_t)acc[c][i] * (int32_t)f) >> PROB_FRAC);
-                const uint32_t l = l0 + row_sum(lp);
-                if (has) {
-                    l0 = (uint32_t)(((uint64_t)l * f) >> PROB_FRAC);
-                    lp = 0;
+                for (int i = 0; i < 4; ++i) {
+                    const bool now = ((seg >> (8 * i)) & 0xFFu) == (uint32_t)sg;
+                    mask |= now ? 0xFFu << (8 * i) : 0u;
+                    pp[i] = now ? pw[i] : 0u;
+                    lp += pp[i];
                 }
-            } else {
-                int to = 0;
-                if (has && grp == 0) to = (int)atomicAdd(J.sc.pool + tl, 1u);
-                to = __shfl(to, col);
-                bad = bad || (has && to >= EXTRA);
-                to = 16 * J.nspan + imin(to, EXTRA - 1);
-                hand_over(has, to);
-                if (has) {
-                    slot = to;
-                    fopen = f;
-                    lp = 0;
-                    bs = 0.0f;
+                if constexpr (KEEP) {
+                    v4i B[3][PVK];
 #pragma unroll
-                    for (int c = 0; c < CT; ++c) acc[c] = v4i{0, 0, 0, 0};
+                    for (int l = 0; l < 3; ++l)
+#pragma unroll
+                        for (int k = 0; k < PVK; ++k) B[l][k] = A[l][k] & (int)mask;
+                    accumulate(std::true_type{}, B);
+                } else {
+                    top = terms(pp);
+                    bs_tile = 0.0f;
+                    accumulate(std::true_type{}, A);
+                }
+                wmax = top > wmax ? top : wmax;
+                const bool has = row_ev > sg;
+                if (__ballot(has) == 0) break;
+                // the event that opens segment sg + 1 of the row
+                uint32_t fd = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) fd = ((seg >> (8 * i)) & 0xFFu) == (uint32_t)(sg + 1) && fe[i] ? fe[i] : fd;
+                fd = row_or(fd);
+                const uint32_t f = has ? lut(fd - 1u) : 1u << PROB_FRAC;
+                if (first) {
+                    const uint32_t l = l0 + row_sum(lp);
+                    if (has) {
+#pragma unroll
+                        for (int c = 0; c < CT; ++c) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                // floor(a f / 2^15) in halves of 16 bits: 2 hi f + floor(lo f / 2^15)
+                                const uint32_t lo = __umul24((uint32_t)acc[c][i] & 0xFFFFu, f) >> PROB_FRAC;
+                                acc[c][i] = __mul24(acc[c][i] >> 16, 2 * (int)f) + (int)lo;
+                            }
+                        }
+                        l0 = (uint32_t)(((uint64_t)l * f) >> PROB_FRAC);
+                        lp = 0;
+                    }
+                } else {
+                    next_run(has, f);
+                    bs = has ? bs_tile : bs;
                 }
             }
         }
@@ -648,133 +720,278 @@ __global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel
     bad = bad || !((double)wmax * vcmax + 2.0 <= TERM_LIMIT);
     const uint32_t events = row_sum(n_ev);
     const uint32_t any = row_or(bad ? BAD : 0u);
-    if (grp == 0) J.sc.ev[(tl * J.nspan + p.s) * 16 + col] = events | any;
+    return events | any;
+}
+
+// p by the integer part of its distance's table index, as lut_s[floor(d log2(e) / 2^24)] reads it (256 threads at least).
+__device__ __forceinline__ void fill_lut(const Tables *tabs, uint16_t *lut_s) {
+    if (threadIdx.x < 256) {
+        const int32_t x = tabs->exp_table[threadIdx.x];
+#pragma unroll
+        for (int i = 0; i < LUT_SPAN / 256; ++i) lut_s[256 * i + threadIdx.x] = (uint16_t)(x >> i);
+        if (threadIdx.x == 0) lut_s[LUT_SPAN] = 0;
+    }
+}
+
+template <int D, int KB, int NC>
+__global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel(Job J) {
+    __shared__ Digits dgs;
+    __shared__ uint32_t up[TREE_NODES][UPW];
+    __shared__ int16_t at[TREE_NODES];
+    __shared__ uint16_t lut_s[LUT_N + 7];
+    Place p;
+    if (!p.find(J, J.tiles, J.span, W)) return;
+    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+    dgs.fill(J.tabs, J.g.kb);
+    fill_lut(J.tabs, lut_s);
+    if (p.tail) tree_paths(J.parents + p.b * J.pstride, J.n, up, at);
+    __syncthreads();
+    if (p.lo >= p.hi) return;
+    // the maximum of the spans before, or of all
+    int32_t m = NONE;
+    {
+        const int end = J.two ? (int)((p.T + J.mspan - 1) / J.mspan) : p.s * (J.span / J.mspan);
+        const int32_t *top = J.sc.top + ((int64_t)p.chain * J.tiles + p.tile) * J.nms * 16 + col;
+        for (int i = grp; i < end; i += 4) m = imax(m, top[i * 16]);
+        m = row_max(m);
+    }
+    Query<D, KB> Q;
+    Q.load(J, p.b, p.kvh, p.tile, J.tabs->kc_absmax, nullptr);
+    const uint32_t ev = walk<D, KB, NC>(J, p, Q, m, dgs, up[imin(p.tile * 16 + col, J.rows - 1) / J.g.G], lut_s);
+    if (grp == 0) J.sc.ev[(((int64_t)p.chain * J.tiles + p.tile) * J.nspan + p.s) * 16 + col] = ev;
+}
+
+// What a workgroup's rows count.
+struct Tally {
+    unsigned long long events, bad, over, acc, score;
+    __device__ __forceinline__ void clear() { events = bad = over = acc = score = 0; }
+    __device__ __forceinline__ void post(const Job &J, bool first, int64_t T) const {
+        if (events) atomicAdd(&J.st->rescale_events, events);
+        if (bad) atomicAdd(&J.st->serial_fallbacks, bad);
+        if (over) atomicAdd(&J.st->acc_overflows, over);
+        if (acc > J.st->max_abs_acc) atomicMax(&J.st->max_abs_acc, acc);
+        if (score > J.st->max_abs_score) atomicMax(&J.st->max_abs_score, score);
+        if (first) atomicMax(&J.st->n_tokens, (unsigned long long)T);
+    }
+};
+
+// A wave puts row `col` of a tile together, lane = channel: its runs in order, then acc / l. bad: the row goes
+// token by token.
+template <int D>
+__device__ __forceinline__ void combine_row(const Job &J, const Place &p, int col, bool bad, uint32_t events,
+                                            SerialLds<D == 64 ? 60 : 116> &fb, uint32_t *up, Tally &tally) {
+    constexpr int CPL = D / 64;
+    const int lane = threadIdx.x & 63, r = p.tile * 16 + col, node = r / J.g.G;
+    const int64_t qrow = (((int64_t)p.b * J.n + node) * J.g.n_q + p.kvh * J.g.G + r % J.g.G) * D;
+    const int64_t run0 = ((int64_t)p.chain * J.tiles + p.tile) * (16 * (int64_t)J.nspan + J.extra);
+    const int ns = (int)((p.T + J.span - 1) / J.span);
+    int64_t acc[CPL], l = 0;
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) acc[k] = 0;
+    for (int i0 = 0; i0 < ns && !bad; i0 += 64) {
+        const uint4 mt = i0 + lane < ns ? J.sc.meta[run0 + (i0 + lane) * 16 + col] : make_uint4(0u, 0u, ~0u, 0u);
+        uint64_t todo = __ballot((mt.y & USED) != 0 || mt.z != ~0u);
+        constexpr int AHEAD = 16 / CPL;
+        int32_t v[AHEAD][CPL];
+        while (todo && !bad) {
+            int at[AHEAD];
+            uint64_t left = todo;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                at[j] = left ? __ffsll((long long)left) - 1 : -1;
+                left &= left - 1;
+                if (at[j] < 0) continue;
+                const int32_t *S = J.sc.S + (run0 + (i0 + at[j]) * 16 + col) * D;
+                const bool used = ((uint32_t)__builtin_amdgcn_readlane((int)mt.y, at[j]) & USED) != 0;
+#pragma unroll
+                for (int k = 0; k < CPL; ++k) v[j][k] = used ? S[lane + 64 * k] : 0;
+            }
+            todo = left;
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                if (at[j] < 0) continue;
+                uint32_t L = (uint32_t)__builtin_amdgcn_readlane((int)mt.x, at[j]);
+                uint32_t f = (uint32_t)__builtin_amdgcn_readlane((int)mt.y, at[j]);
+                int next = __builtin_amdgcn_readlane((int)mt.z, at[j]);
+                double bound = (double)__uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)mt.w, at[j]));
+                for (;;) {
+                    if (f & USED) {
+                        const int64_t ff = f & (USED - 1);
+#pragma unroll
+                        for (int k = 0; k < CPL; ++k) {
+                            acc[k] = (acc[k] * ff) >> PROB_FRAC;
+                            const int64_t m = acc[k] < 0 ? -acc[k] : acc[k];
+                            // two-pass clamps once, at the end: only the run's own sum must fit
+                            bad = bad || !((J.two ? 0.0 : (double)m) + bound <= 2147483647.0);
+                            acc[k] += v[j][k];
+                        }
+                        l = ((l * ff) >> PROB_FRAC) + L;
+                    }
+                    if (next < 0) break;
+                    const uint4 x = J.sc.meta[run0 + next];
+                    const int32_t *S = J.sc.S + (run0 + next) * D;
+                    L = x.x;
+                    f = x.y;
+                    bound = (double)__uint_as_float(x.w);
+#pragma unroll
+                    for (int k = 0; k < CPL; ++k) v[j][k] = f & USED ? S[lane + 64 * k] : 0;
+                    next = (int)x.z;
+                }
+            }
+            bad = __ballot(bad) != 0;
+        }
+    }
+    if (bad) {
+        tree_path(J.parents + p.b * J.pstride, node, J.n, up);
+        serial_head<CPL, (D == 64 ? 60 : 116)>(J.g, J.tabs, J.tabs->kc, J.tabs->vc, J.q + qrow, p.b, p.kvh, p.T, J.two, true, fb,
+                                               J.out + qrow, J.st, TreeRows{up, p.base});
+        if (lane == 0) atomicAdd(&tally.bad, 1ull);
+        return;
+    }
+    const Recip rc = reciprocal(l);
+    int64_t amax = 0, over = 0;
+#pragma unroll
+    for (int k = 0; k < CPL; ++k) {
+        if (acc[k] < ACC_LO || acc[k] > ACC_HI) {
+            ++over;
+            acc[k] = acc[k] < ACC_LO ? ACC_LO : ACC_HI;
+        }
+        J.out[qrow + lane + 64 * k] = (int32_t)(wmul(acc[k], rc.r) >> rc.shift);
+        const int64_t m = acc[k] < 0 ? -acc[k] : acc[k];
+        amax = m > amax ? m : amax;
+    }
+    if (J.count) {
+        const int64_t ev = wave_sum_i64((int64_t)events);
+        amax = wave_max_i64(amax);
+        over = wave_sum_i64(over);
+        if (lane == 0) {
+            if (ev && !J.two) atomicAdd(&tally.events, (unsigned long long)ev);
+            if (over) atomicAdd(&tally.over, (unsigned long long)over);
+            atomicMax(&tally.acc, (unsigned long long)amax);
+        }
+    }
 }
 
 template <int D>
 __global__ void __launch_bounds__(CW * 64) combine_kernel(Job J) {
-    constexpr int CPL = D / 64, RS = D == 64 ? 60 : 116;
-    __shared__ SerialLds<RS> fb[CW];
+    __shared__ SerialLds<D == 64 ? 60 : 116> fb[CW];
     __shared__ uint32_t up[CW][TREE_NODES / 32];
-    __shared__ unsigned long long s_ev, s_bad, s_ovf, s_acc;
+    __shared__ Tally tally;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int chains = J.nseq * J.g.n_kv;
-    const int chain = (int)(blockIdx.x % (unsigned)chains), tile = (int)(blockIdx.x / (unsigned)chains);
-    const int b = J.seq0 + chain / J.g.n_kv, kvh = chain % J.g.n_kv, G = J.g.G;
-    const int64_t T = J.len[b], base = T - J.n, tl = (int64_t)chain * J.tiles + tile;
-    const int ns = (int)((T + J.span - 1) / J.span);
-    const int64_t run0 = tl * (16 * (int64_t)J.nspan + EXTRA);
-    if (tid == 0) s_ev = s_bad = s_ovf = s_acc = 0;
+    const int part = (int)(blockIdx.x / (unsigned)chains);
+    Place p;
+    p.chain = (int)(blockIdx.x % (unsigned)chains);
+    p.tile = part / (16 / CW);
+    p.b = J.seq0 + p.chain / J.g.n_kv;
+    p.kvh = p.chain % J.g.n_kv;
+    p.T = J.len[p.b];
+    p.base = p.T - J.n;
+    if (tid == 0) tally.clear();
     __syncthreads();
-    for (int col = wv; col < 16; col += CW) {
-        const int r = tile * 16 + col;
-        if (r >= J.rows) break;
-        const int node = r / G;
-        const int64_t qrow = (((int64_t)b * J.n + node) * J.g.n_q + kvh * G + r % G) * D;
-        int64_t acc[CPL], l = 0;
-#pragma unroll
-        for (int k = 0; k < CPL; ++k) acc[k] = 0;
+    const int col = part % (16 / CW) * CW + wv;
+    if (p.tile * 16 + col < J.rows) {
+        const int64_t tl = (int64_t)p.chain * J.tiles + p.tile;
+        const int ns = (int)((p.T + J.span - 1) / J.span), nm = (int)((p.T + J.mspan - 1) / J.mspan);
         uint32_t events = 0;
         bool bad = false;
-        for (int i0 = 0; i0 < ns; i0 += 64) {
-            const bool in = i0 + lane < ns;
-            const uint32_t e = in ? J.sc.ev[(tl * J.nspan + i0 + lane) * 16 + col] : 0u;
-            const uint32_t o = in ? J.sc.over[tl * J.nspan + i0 + lane] : 0u;
+        for (int i = lane; i < ns; i += 64) {
+            const uint32_t e = J.sc.ev[(tl * J.nspan + i) * 16 + col];
             events += e & ~BAD;
-            bad = bad || __ballot((e & BAD) != 0 || (o >> col & 1) != 0) != 0;
+            bad = bad || (e & BAD) != 0;
         }
-        for (int i0 = 0; i0 < ns && !bad; i0 += 64) {
-            const uint4 mt = i0 + lane < ns ? J.sc.meta[run0 + (i0 + lane) * 16 + col] : make_uint4(0u, 0u, ~0u, 0u);
-            uint64_t todo = __ballot((mt.y & USED) != 0 || mt.z != ~0u);
-            constexpr int AHEAD = 4;
-            int32_t v[AHEAD][CPL];
-            while (todo && !bad) {
-                int at[AHEAD];
-                uint64_t left = todo;
-#pragma unroll
-                for (int j = 0; j < AHEAD; ++j) {
-                    at[j] = left ? __ffsll((long long)left) - 1 : -1;
-                    left &= left - 1;
-                    if (at[j] < 0) continue;
-                    const int32_t *S = J.sc.S + (run0 + (i0 + at[j]) * 16 + col) * D;
-                    const bool used = ((uint32_t)__builtin_amdgcn_readlane((int)mt.y, at[j]) & USED) != 0;
-#pragma unroll
-                    for (int k = 0; k < CPL; ++k) v[j][k] = used ? S[lane + 64 * k] : 0;
-                }
-                todo = left;
-#pragma unroll
-                for (int j = 0; j < AHEAD; ++j) {
-                    if (at[j] < 0) continue;
-                    uint32_t L = (uint32_t)__builtin_amdgcn_readlane((int)mt.x, at[j]);
-                    uint32_t f = (uint32_t)__builtin_amdgcn_readlane((int)mt.y, at[j]);
-                    int next = __builtin_amdgcn_readlane((int)mt.z, at[j]);
-                    double bound = (double)__uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)mt.w, at[j]));
-                    for (;;) {
-                        if (f & USED) {
-                            const int64_t ff = f & (USED - 1);
-#pragma unroll
-                            for (int k = 0; k < CPL; ++k) {
-                                acc[k] = (acc[k] * ff) >> PROB_FRAC;
-                                const int64_t m = acc[k] < 0 ? -acc[k] : acc[k];
-                                // two-pass clamps once, at the end: only the run's own sum must fit
-                                bad = bad || !((J.two ? 0.0 : (double)m) + bound <= 2147483647.0);
-                                acc[k] += v[j][k];
-                            }
-                            l = ((l * ff) >> PROB_FRAC) + L;
-                        }
-                        if (next < 0) break;
-                        const uint4 x = J.sc.meta[run0 + next];
-                        const int32_t *S = J.sc.S + (run0 + next) * D;
-                        L = x.x;
-                        f = x.y;
-                        bound = (double)__uint_as_float(x.w);
-#pragma unroll
-                        for (int k = 0; k < CPL; ++k) v[j][k] = f & USED ? S[lane + 64 * k] : 0;
-                        next = (int)x.z;
-                    }
-                }
-                bad = __ballot(bad) != 0;
-            }
-        }
-        if (bad) {
-            tree_path(J.parents + b * J.pstride, node, J.n, up[wv]);
-            serial_head<CPL, RS>(J.g, J.tabs, J.tabs->kc, J.tabs->vc, J.q + qrow, b, kvh, T, J.two, true, fb[wv], J.out + qrow,
-                                 J.st, TreeRows{up[wv], base});
-            if (lane == 0) atomicAdd(&s_bad, 1ull);
-            continue;
-        }
-        const Recip rc = reciprocal(l);
-        int64_t amax = 0, ovf = 0;
-#pragma unroll
-        for (int k = 0; k < CPL; ++k) {
-            if (acc[k] < ACC_LO || acc[k] > ACC_HI) {
-                ++ovf;
-                acc[k] = acc[k] < ACC_LO ? ACC_LO : ACC_HI;
-            }
-            J.out[qrow + lane + 64 * k] = (int32_t)(wmul(acc[k], rc.r) >> rc.shift);
-            const int64_t m = acc[k] < 0 ? -acc[k] : acc[k];
-            amax = m > amax ? m : amax;
-        }
-        if (J.count) {
-            const int64_t ev = wave_sum_i64((int64_t)events);
-            amax = wave_max_i64(amax);
-            ovf = wave_sum_i64(ovf);
-            if (lane == 0) {
-                if (ev && !J.two) atomicAdd(&s_ev, (unsigned long long)ev);
-                if (ovf) atomicAdd(&s_ovf, (unsigned long long)ovf);
-                atomicMax(&s_acc, (unsigned long long)amax);
-            }
-        }
+        for (int i = lane; i < nm; i += 64) bad = bad || (J.sc.over[tl * J.nms + i] >> col & 1) != 0;
+        combine_row<D>(J, p, col, __ballot(bad) != 0, events, fb[wv], up[wv], tally);
     }
     if (!J.count) return;
     __syncthreads();
+    if (tid == 0) tally.post(J, part == 0 && p.kvh == 0, p.T);
+}
+
+// All of it in one launch, where the spans are a workgroup's waves: short contexts, and many row tiles.
+constexpr int FW = 8;
+template <int D, int KB, int NC>
+__global__ void __launch_bounds__(FW * 64, 2) fused_kernel(Job J) {
+    __shared__ Digits dgs;
+    __shared__ uint32_t up[TREE_NODES][UPW];
+    __shared__ int16_t at[TREE_NODES];
+    __shared__ uint16_t lut_s[LUT_N + 7];
+    __shared__ int32_t top_s[FW][16];
+    __shared__ uint32_t over_s, ev_s[FW][16];
+    __shared__ SerialLds<D == 64 ? 60 : 116> fb[FW];
+    __shared__ uint32_t fup[FW][TREE_NODES / 32];
+    __shared__ Tally tally;
+    Place p;
+    p.find(J, J.tiles, J.span, FW);
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
+    const int64_t tl = (int64_t)p.chain * J.tiles + p.tile;
+    Query<D, KB> Q;
+    Q.load(J, p.b, p.kvh, p.tile, J.tabs->kc_absmax, J.count && p.s == 0 ? &J.st->range_errors : nullptr);
+    dgs.fill(J.tabs, J.g.kb);
+    fill_lut(J.tabs, lut_s);
     if (tid == 0) {
-        if (s_ev) atomicAdd(&J.st->rescale_events, s_ev);
-        if (s_bad) atomicAdd(&J.st->serial_fallbacks, s_bad);
-        if (s_ovf) atomicAdd(&J.st->acc_overflows, s_ovf);
-        if (s_acc > J.st->max_abs_acc) atomicMax(&J.st->max_abs_acc, s_acc);
-        if (tile == 0 && kvh == 0) atomicMax(&J.st->n_tokens, (unsigned long long)T);
+        over_s = 0;
+        tally.clear();
+        J.sc.pool[tl] = 0;
     }
+    const int none = tree_paths(J.parents + p.b * J.pstride, J.n, up, at);
+    if (J.count && none && p.kvh == 0 && p.tile == 0) atomicAdd(&J.st->range_errors, (unsigned long long)none);
+    __syncthreads();
+    const uint32_t *path = up[imin(p.tile * 16 + col, J.rows - 1) / J.g.G];
+    int32_t m = NONE;
+    if (p.lo < p.hi) {
+        int32_t lowest = 0;
+        bool over = Q.bad;
+        uint32_t dg[3][4];
+        dgs.read(dg);
+        const uint8_t *hb = plane_ptr(J.g, p.b, p.kvh, 0), *nb = hb + (J.g.n_planes - 1) * J.g.span;
+        Keys<D, KB> next;
+        next.load(hb, nb, J.g.span, p.lo);
+        for (int64_t t0 = p.lo; t0 < p.hi; t0 += 16) {
+            const Keys<D, KB> cur = next;
+            if (t0 + 16 < p.hi) next.load(hb, nb, J.g.span, t0 + 16);
+            v4i a[D / 64][3];
+            cur.expand(dg, a);
+            uint32_t in = 15u;
+            if (t0 + 16 > p.base) in = visible4(path, (int)(t0 - p.base) + 4 * grp);
+            int32_t s[4];
+            over |= scores<D>(a, Q.qd, cur.norms, Q.check, in, s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool on = in >> i & 1;
+                m = on && s[i] > m ? s[i] : m;
+                lowest = on && s[i] < lowest ? s[i] : lowest;
+            }
+        }
+        m = row_max(m);
+        const uint64_t bad = __ballot(over);
+        if (lane == 0 && bad) atomicOr(&over_s, (uint32_t)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu));
+        if (J.count) {
+            const bool mine = !over && p.tile * 16 + col < J.rows;
+            const int64_t x = m == NONE ? 0 : m < 0 ? -(int64_t)m : m, y = -(int64_t)lowest;
+            const int64_t z = wave_max_i64(mine ? (x > y ? x : y) : 0);
+            if (lane == 0) atomicMax(&tally.score, (unsigned long long)z);
+        }
+    }
+    if (grp == 0) top_s[p.s][col] = m;
+    __syncthreads();
+    if (p.lo < p.hi) {
+        m = NONE;
+        for (int i = 0; i < (J.two ? FW : p.s); ++i) m = imax(m, top_s[i][col]);
+        const uint32_t ev = walk<D, KB, NC>(J, p, Q, m, dgs, path, lut_s);
+        if (grp == 0) ev_s[p.s][col] = ev;
+    } else if (grp == 0) {
+        ev_s[p.s][col] = 0;
+    }
+    __syncthreads();
+    for (int c = p.s; c < 16; c += FW) {
+        if (p.tile * 16 + c >= J.rows) break;
+        const uint32_t e = lane < FW ? ev_s[lane][c] : 0u;
+        combine_row<D>(J, p, c, __ballot((e & BAD) != 0) != 0 || (over_s >> c & 1) != 0, e & ~BAD, fb[p.s], fup[p.s], tally);
+    }
+    if (!J.count) return;
+    __syncthreads();
+    if (tid == 0) tally.post(J, p.tile == 0 && p.kvh == 0, p.T);
 }
 
 // Any format, token by token: a wave a row.
@@ -804,18 +1021,24 @@ __global__ void __launch_bounds__(64) serial_kernel(Job J) {
                                 TreeRows{up, T - J.n});
 }
 
-// The scratch of a launch over nseq sequences, carved from p (null: only its size).
-size_t carve(const Geom &g, int64_t nseq, int64_t tiles, int64_t nspan, uint8_t *p, Scratch *sc) {
+// Sequences a launch takes, and the spans of the longest.
+struct Plan {
+    int64_t seqs, tiles, span, nspan, mspan, nms, rt, extra;
+    bool fused;
+};
+// The scratch of a launch, carved from p (null: only its size).
+size_t carve(const Geom &g, const Plan &pl, uint8_t *p, Scratch *sc) {
+    const int64_t nseq = pl.seqs, tiles = pl.tiles, nspan = pl.nspan, nms = pl.nms;
     size_t o = 0;
     auto take = [&](size_t n) {
         uint8_t *a = p ? p + o : nullptr;
         o += (n + 255) / 256 * 256;
         return a;
     };
-    const size_t all = (size_t)nseq * g.n_kv * tiles, runs = all * (16 * (size_t)nspan + EXTRA);
+    const size_t all = (size_t)nseq * g.n_kv * tiles, runs = all * (16 * (size_t)nspan + pl.extra);
     Scratch c{};
-    c.top = (int32_t *)take(all * nspan * 64);
-    c.over = (uint32_t *)take(all * nspan * 4);
+    c.top = (int32_t *)take(all * nms * 64);
+    c.over = (uint32_t *)take(all * nms * 4);
     c.ev = (uint32_t *)take(all * nspan * 64);
     c.pool = (uint32_t *)take(all * 4);
     c.meta = (uint4 *)take(runs * 16);
@@ -824,39 +1047,66 @@ size_t carve(const Geom &g, int64_t nseq, int64_t tiles, int64_t nspan, uint8_t 
     return o;
 }
 
-// Sequences a launch takes, and the spans of the longest.
-struct Plan {
-    int64_t seqs, tiles, span, nspan;
-};
 constexpr size_t BUDGET = (size_t)512 << 20;
+constexpr int64_t FUSED_MAX = 512;
 Plan plan(const Geom &g, int64_t n, int64_t longest, int64_t batch) {
     Plan p{};
     p.tiles = (n * g.G + 15) / 16;
     p.seqs = batch;
     for (;;) {
         const int64_t all = p.seqs * g.n_kv * p.tiles;
-        int64_t want = (4096 + all - 1) / all, most = (longest + 63) / 64;
-        const int64_t least = (longest + SPAN_MAX - 1) / SPAN_MAX;
-        want = want > most ? most : want;
-        want = want < least ? least : want;
-        p.span = ((longest + want - 1) / want + 15) / 16 * 16;
-        p.nspan = (longest + p.span - 1) / p.span;
-        if (p.seqs == 1 || carve(g, p.seqs, p.tiles, p.nspan, nullptr, nullptr) <= BUDGET) return p;
+        // row tiles a wave of max_kernel: as many as leave it 2,048 waves of 64 tokens
+        p.rt = g.d == 64 ? 4 : 2;
+        while (p.rt > 1 && (p.tiles <= p.rt / 2 || p.seqs * g.n_kv * ((p.tiles + p.rt - 1) / p.rt) * ((longest + 63) / 64) < 2048)) p.rt /= 2;
+        const int64_t most = (longest + 63) / 64, least = (longest + SPAN_MAX - 1) / SPAN_MAX;
+        // as many waves as the chip holds of sum_kernel, and twice that for long walks, whose ragged ends and first
+        // spans' events a second round evens out
+        int64_t want = 1024 * (g.d == 64 && g.vb <= 2 ? 3 : 2) / all;
+        if (longest > 512 * want) want *= 2;
+        want = std::max<int64_t>(std::min(want, most), std::max<int64_t>(least, 1));
+        static const int64_t FM = getenv("FM") ? atoll(getenv("FM")) : FUSED_MAX;
+        p.fused = longest <= FM;
+        if (p.fused) {
+            p.span = ((longest + FW - 1) / FW + 15) / 16 * 16;
+            p.nspan = FW;
+        } else {
+            // a multiple of 64 tokens, so that up to four of max_kernel's make one
+            p.span = ((longest + want - 1) / want + 63) / 64 * 64;
+            p.nspan = (longest + p.span - 1) / p.span;
+        }
+        p.mspan = p.span;
+        while (!p.fused && p.mspan % 32 == 0 && p.span / p.mspan < 4 &&
+               p.seqs * g.n_kv * ((p.tiles + p.rt - 1) / p.rt) * ((longest + p.mspan - 1) / p.mspan) < 4096)
+            p.mspan /= 2;
+        p.nms = (longest + p.mspan - 1) / p.mspan;
+        const int64_t room = (64 << 20) / (all * (g.d * 4 + 16));
+        p.extra = room < EXTRA_MIN ? EXTRA_MIN : room > EXTRA_MAX ? EXTRA_MAX : room;
+        if (p.seqs == 1 || carve(g, p, nullptr, nullptr) <= BUDGET) return p;
         p.seqs = (p.seqs + 1) / 2;
     }
 }
 
 template <int D, int KB, int NC>
-hipError_t launch(hipStream_t s, const Job &J, LaunchEv ev) {
+hipError_t launch(hipStream_t s, const Job &J, int rt, bool fused, LaunchEv ev) {
     const int64_t chains = (int64_t)J.nseq * J.g.n_kv;
+    if (fused) {
+        hipExtLaunchKernelGGL((fused_kernel<D, KB, NC>), dim3((unsigned)(chains * J.tiles)), dim3(FW * 64), 0, s, ev.start, ev.stop, 0, J);
+        return hipGetLastError();
+    }
     const dim3 grid((unsigned)(chains * J.tiles * ((J.nspan + W - 1) / W)));
-    hipExtLaunchKernelGGL((max_kernel<D, KB>), grid, dim3(W * 64), 0, s, ev.start, nullptr, 0, J);
+    const int64_t ms = (J.nms + W - 1) / W;
+    if (rt == 1)
+        hipExtLaunchKernelGGL((max_kernel<D, KB, 1>), dim3((unsigned)(chains * ms * J.tiles)), dim3(W * 64), 0, s, ev.start, nullptr, 0, J);
+    else if (D == 128 || rt == 2)
+        hipExtLaunchKernelGGL((max_kernel<D, KB, 2>), dim3((unsigned)(chains * ms * ((J.tiles + 1) / 2))), dim3(W * 64), 0, s, ev.start, nullptr, 0, J);
+    else
+        hipExtLaunchKernelGGL((max_kernel<D, KB, D == 128 ? 2 : 4>), dim3((unsigned)(chains * ms * ((J.tiles + 3) / 4))), dim3(W * 64), 0, s, ev.start, nullptr, 0, J);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipExtLaunchKernelGGL((sum_kernel<D, KB, NC>), grid, dim3(W * 64), 0, s, nullptr, nullptr, 0, J);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipExtLaunchKernelGGL((combine_kernel<D>), dim3((unsigned)(chains * J.tiles)), dim3(CW * 64), 0, s, nullptr, ev.stop, 0, J);
+    hipExtLaunchKernelGGL((combine_kernel<D>), dim3((unsigned)(chains * ((J.rows + CW - 1) / CW))), dim3(CW * 64), 0, s, nullptr, ev.stop, 0, J);
     return hipGetLastError();
 }
 
@@ -868,7 +1118,7 @@ bool tree_supported(const Geom &g) {
 
 size_t tree_scratch_bytes(const Geom &g, int64_t n, int64_t longest) {
     const tr::Plan p = tr::plan(g, n, longest, g.batch);
-    return tr::carve(g, p.seqs, p.tiles, p.nspan, nullptr, nullptr);
+    return tr::carve(g, p, nullptr, nullptr);
 }
 
 hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, const int32_t *q, int32_t *out,
@@ -877,7 +1127,7 @@ hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, con
     using namespace tr;
     const Plan p = plan(g, n, longest, g.batch);
     Job J{};
-    if (carve(g, p.seqs, p.tiles, p.nspan, (uint8_t *)scratch, &J.sc) > scratch_bytes) return hipErrorInvalidValue;
+    if (carve(g, p, (uint8_t *)scratch, &J.sc) > scratch_bytes) return hipErrorInvalidValue;
     J.g = g;
     J.tabs = t;
     J.q = q;
@@ -890,6 +1140,9 @@ hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, con
     J.tiles = (int32_t)p.tiles;
     J.span = (int32_t)p.span;
     J.nspan = (int32_t)p.nspan;
+    J.mspan = (int32_t)p.mspan;
+    J.nms = (int32_t)p.nms;
+    J.extra = (int32_t)p.extra;
     J.two = two_pass;
     J.count = count;
     J.st = st;
@@ -899,7 +1152,7 @@ hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, con
         const LaunchEv e{b == 0 ? ev.start : nullptr, b + p.seqs >= g.batch ? ev.stop : nullptr};
         hipError_t rc = hipErrorInvalidValue;
 #define INSITU_TREE_CASE(DD, KK, CC) \
-    if (g.d == DD && g.kb == KK && (g.vb <= 2 ? 4 : 8) == CC) rc = launch<DD, KK, CC>(s, J, e);
+    if (g.d == DD && g.kb == KK && (g.vb <= 2 ? 4 : 8) == CC) rc = launch<DD, KK, CC>(s, J, (int)p.rt, p.fused, e);
 #define INSITU_TREE_D(DD)                                                                              \
     INSITU_TREE_CASE(DD, 2, 4) INSITU_TREE_CASE(DD, 3, 4) INSITU_TREE_CASE(DD, 4, 4)                   \
     INSITU_TREE_CASE(DD, 2, 8) INSITU_TREE_CASE(DD, 3, 8) INSITU_TREE_CASE(DD, 4, 8)

@@ -36,6 +36,7 @@ class Context:
         with torch.cuda.device(device):
             s = stream if stream is not None else torch.cuda.current_stream(device)
         self.stream = s
+        self._raw = s.cuda_stream
         h = ctypes.c_void_p()
         _lib.check(self.lib.insitu_ctx_create(device, ctypes.c_void_p(s.cuda_stream),
                                               ctypes.byref(h)))
@@ -70,6 +71,8 @@ class Context:
         """numpy/torch -> contiguous torch tensor on this device (int32 by default)."""
         torch = _torch()
         if isinstance(a, torch.Tensor):
+            if a.device == self.torch_device and (dtype is None or a.dtype == dtype) and a.is_contiguous():
+                return a
             t = a.to(self.torch_device, non_blocking=False)
         else:
             t = torch.from_numpy(np.ascontiguousarray(a)).to(self.torch_device)
@@ -83,10 +86,9 @@ class _Ordered:
         self.ctx, self.tensors, self.other = ctx, tensors, None
 
     def __enter__(self) -> None:
-        now = _torch().cuda.current_stream(self.ctx.device)
-        if now.cuda_stream != self.ctx.stream.cuda_stream:
-            self.other = now
-            self.ctx.stream.wait_stream(now)
+        if _raw_stream(self.ctx.device) != self.ctx._raw:
+            self.other = _torch().cuda.current_stream(self.ctx.device)
+            self.ctx.stream.wait_stream(self.other)
 
     def __exit__(self, *exc) -> None:
         if self.other is not None:
@@ -94,6 +96,13 @@ class _Ordered:
             for t in self.tensors:
                 if t is not None:
                     t.record_stream(self.ctx.stream)
+
+
+def _raw_stream(device: int) -> int:
+    """The handle of torch's current stream (without the Stream object around it, 2 us, where torch gives it)."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def default_context(device: int = 0) -> Context:
