@@ -93,16 +93,36 @@ __device__ __forceinline__ uint32_t row_sum(uint32_t v) {
 }
 
 // The paths of all nodes: bit 32 + j of up[i] is set where j is i or an ancestor of it; the word before
-// is ones (the context's rows), those behind are zeros. Each round doubles how far a node has looked up.
-// Returns the number of parents that are none (this thread's).
-__device__ __forceinline__ int tree_paths(const int32_t *__restrict__ parents, int n, uint32_t (*up)[UPW], int16_t *at) {
+// is ones (the context's rows), those behind are zeros. Each round doubles how far a node has looked up. p: the
+// thread's node's parent, or -1. Returns the number of parents that are none (this thread's).
+__device__ __forceinline__ int tree_paths(int p, int n, uint32_t (*up)[UPW], int16_t *at) {
     const int i = threadIdx.x, words = (n + 31) / 32;
     int bad = 0;
-    int p = -1;
     if (i < n) {
-        p = parents[i];
         bad = p >= i || p < -1;
         p = bad ? -1 : p;
+    }
+    if (n <= 64) {                                     // one wave, in registers; the caller's barrier shows it
+        if (i < 64) {
+            uint32_t lo = i < 32 ? 1u << i : 0u, hi = i < 32 ? 0u : 1u << (i - 32);
+            while (__ballot(p >= 0) != 0) {
+                const int j = p >= 0 ? p : i;
+                const uint32_t l = (uint32_t)__shfl((int)lo, j), h = (uint32_t)__shfl((int)hi, j);
+                const int far = __shfl(p, j);
+                lo |= l;
+                hi |= h;
+                p = far;
+            }
+            if (i < n) {
+                up[i][0] = ~0u;
+                up[i][1] = lo;
+                up[i][2] = hi;
+                up[i][3] = up[i][4] = up[i][5] = 0u;
+            }
+        }
+        return bad;
+    }
+    if (i < n) {
         at[i] = (int16_t)p;
         for (int k = 0; k < UPW; ++k) up[i][k] = k == 0 ? ~0u : k - 1 == i >> 5 ? 1u << (i & 31) : 0u;
     }
@@ -133,16 +153,48 @@ __device__ __forceinline__ uint32_t visible4(const uint32_t *up, int rel) {
     return __builtin_amdgcn_alignbit(up[k + 1], up[k], rel & 31) & 15u;
 }
 
+// A workgroup's place: chains fastest (a KV head's rows then stay in one XCD's cache where there are 8),
+// then the row tiles (or groups of them), which read the same tokens, then the spans.
+struct Place {
+    int chain, b, kvh, tile, s;
+    int64_t T, base, lo, hi;                           // the wave's span [lo, hi) of T rows
+    bool tail;                                         // the workgroup's spans reach the tree's rows
+    __device__ __forceinline__ bool find(const Job &J, int tiles, int span, int waves) {
+        const int chains = J.nseq * J.g.n_kv;
+        chain = (int)(blockIdx.x % (unsigned)chains);
+        const int rest = (int)(blockIdx.x / (unsigned)chains);
+        tile = rest % tiles;
+        const int s0 = rest / tiles * waves;
+        s = s0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        b = J.seq0 + chain / J.g.n_kv;
+        kvh = chain % J.g.n_kv;
+        T = J.len[b];
+        base = T - J.n;
+        const int64_t end = (int64_t)(s0 + waves) * span;
+        tail = (end < T ? end : T) > base;
+        lo = (int64_t)s * span;
+        hi = lo + span < T ? lo + span : T;
+        return (int64_t)s0 * span < T;
+    }
+};
+
 // A row tile's queries: lane = (row, D / 4 channels from grp D / 4 on, in the order the codes expand in).
 template <int D, int KB>
 struct Query {
     v4i qd[3][D / 64];
     bool bad;                                          // the row needs the serial path
     bool check;                                        // scores of the tile may leave int32 (wave-uniform)
-    __device__ __forceinline__ void load(const Job &J, int b, int kvh, int tile, double cmax, unsigned long long *range) {
+    u128 raw[4 * (D / 64)];
+    // the loads, and then what is made of them
+    __device__ __forceinline__ void fetch(const Job &J, const Place &p, int tile) {
         const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
         const int r = imin(tile * 16 + col, J.rows - 1), G = J.g.G;
-        const int32_t *row = J.q + (((int64_t)b * J.n + r / G) * J.g.n_q + kvh * G + r % G) * D + grp * (D / 4);
+        const int32_t *row = J.q + (((int64_t)p.b * J.n + r / G) * J.g.n_q + p.kvh * G + r % G) * D + grp * (D / 4);
+#pragma unroll
+        for (int i = 0; i < 4 * (D / 64); ++i) raw[i] = *(const u128 *)(row + 4 * i);
+    }
+    __device__ __forceinline__ void digest(const Job &J, int tile, unsigned long long *range) {
+        const int col = threadIdx.x & 15;
         int64_t l1 = 0;
         uint32_t wide = 0, out = 0;
 #pragma unroll
@@ -150,7 +202,7 @@ struct Query {
             uint32_t z[16];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const u128 v = *(const u128 *)(row + 16 * k + 4 * i);
+                const u128 v = raw[4 * k + i];
                 const int32_t x[4] = {(int32_t)v.x, (int32_t)v.y, (int32_t)v.z, (int32_t)v.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -174,7 +226,7 @@ struct Query {
                 for (int i = 0; i < 3; ++i) qd[i][k][w] = (int)o[i];
             }
         }
-        double b1 = (double)l1 * cmax;
+        double b1 = (double)l1 * J.tabs->kc_absmax;
         b1 += __shfl_xor(b1, 16);
         b1 += __shfl_xor(b1, 32);
         bad = row_or(wide) != 0 || !(b1 < DOT_MAX);
@@ -239,36 +291,11 @@ __device__ __forceinline__ bool scores(const v4i (&a)[D / 64][3], const v4i (&qd
     return over;
 }
 
-// A workgroup's place: chains fastest (a KV head's rows then stay in one XCD's cache where there are 8),
-// then the row tiles (or groups of them), which read the same tokens, then the spans.
-struct Place {
-    int chain, b, kvh, tile, s;
-    int64_t T, base, lo, hi;                           // the wave's span [lo, hi) of T rows
-    bool tail;                                         // the workgroup's spans reach the tree's rows
-    __device__ __forceinline__ bool find(const Job &J, int tiles, int span, int waves) {
-        const int chains = J.nseq * J.g.n_kv;
-        chain = (int)(blockIdx.x % (unsigned)chains);
-        const int rest = (int)(blockIdx.x / (unsigned)chains);
-        tile = rest % tiles;
-        const int s0 = rest / tiles * waves;
-        s = s0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        b = J.seq0 + chain / J.g.n_kv;
-        kvh = chain % J.g.n_kv;
-        T = J.len[b];
-        base = T - J.n;
-        const int64_t end = (int64_t)(s0 + waves) * span;
-        tail = (end < T ? end : T) > base;
-        lo = (int64_t)s * span;
-        hi = lo + span < T ? lo + span : T;
-        return (int64_t)s0 * span < T;
-    }
-};
-
 struct Digits {
     alignas(16) uint32_t dig[3][4];
-    __device__ __forceinline__ void fill(const Tables *tabs, int kb) {
+    __device__ __forceinline__ void fill(int32_t c) {  // c: the thread's centroid, for 16 threads
         if (threadIdx.x < 16) {
-            const uint32_t z = balanced((int)threadIdx.x < (1 << kb) ? (int32_t)tabs->kc[threadIdx.x] : 0);
+            const uint32_t z = balanced(c);
 #pragma unroll
             for (int l = 0; l < 3; ++l) ((uint8_t *)dig[l])[threadIdx.x] = (uint8_t)(z >> (8 * l));
         }
@@ -278,6 +305,43 @@ struct Digits {
         for (int i = 0; i < 3; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) dg[i][j] = (uint32_t)uni32((int)dig[i][j]);
+    }
+};
+
+// What a workgroup's tables are made of, a value a thread, requested together at its start.
+struct Start {
+    int32_t c, x;
+    int parent;
+    __device__ __forceinline__ Start(const Job &J, const Place &p, bool paths) {
+        const int i = threadIdx.x;
+        c = i < (1 << J.g.kb) ? (int32_t)J.tabs->kc[i & 15] : 0;
+        x = J.tabs->exp_table[i & 255];
+        parent = paths && i < J.n ? J.parents[p.b * J.pstride + i] : -1;
+    }
+    // lut_s[floor(d log2(e) / 2^24)]: p by distance, the table an octave after the other (256 threads at least)
+    __device__ __forceinline__ void lut(uint16_t *lut_s) const {
+        if (threadIdx.x < 256) {
+#pragma unroll
+            for (int i = 0; i < LUT_SPAN / 256; ++i) lut_s[256 * i + threadIdx.x] = (uint16_t)(x >> i);
+            if (threadIdx.x == 0) lut_s[LUT_SPAN] = 0;
+        }
+    }
+};
+
+// The value side: centroids / 2^23 and what follows from them.
+template <int NC>
+struct ValueTable {
+    double vcs[NC], vcmax;
+    uint32_t wide, delta_max;                          // wide: |v_norm p| up to which a term is two balanced bytes
+    __device__ __forceinline__ explicit ValueTable(const Job &J) {
+        vcmax = 0.0;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            vcs[i] = __longlong_as_double(uni64(__double_as_longlong(i < (1 << J.g.vb) ? (double)J.tabs->vc[i] * 0x1p-23 : 0.0)));
+            vcmax = fmax(vcmax, fabs(vcs[i]));
+        }
+        wide = (uint32_t)uni32((int)(uint32_t)(32639.0 / fmax(vcmax, 0x1p-16)));
+        delta_max = (uint32_t)J.tabs->delta_max;
     }
 };
 
@@ -291,13 +355,7 @@ __global__ void __launch_bounds__(W * 64, RT > 2 ? 3 : 4) max_kernel(Job J) {
     if (!p.find(J, (J.tiles + RT - 1) / RT, J.mspan, W)) return;
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, tile0 = p.tile * RT;
     const int nt = imin(RT, J.tiles - tile0);
-    dgs.fill(J.tabs, J.g.kb);
-    int none = 0;
-    if (p.tail) none = tree_paths(J.parents + p.b * J.pstride, J.n, up, at);
-    __syncthreads();
-    if (J.count && none && p.kvh == 0 && p.tile == 0 && p.T <= (int64_t)(p.s / W + 1) * W * J.mspan)
-        atomicAdd(&J.st->range_errors, (unsigned long long)none);
-    if (p.lo >= p.hi) return;
+    const Start start(J, p, p.tail);
     Query<D, KB> Q[RT];
     const uint32_t *path[RT];
     int32_t m[RT], lowest[RT];
@@ -305,17 +363,25 @@ __global__ void __launch_bounds__(W * 64, RT > 2 ? 3 : 4) max_kernel(Job J) {
 #pragma unroll
     for (int k = 0; k < RT; ++k) {
         const int tile = tile0 + imin(k, nt - 1);      // (a tile past the last one is not scored)
-        Q[k].load(J, p.b, p.kvh, tile, J.tabs->kc_absmax, J.count && p.s == 0 && k < nt ? &J.st->range_errors : nullptr);
+        Q[k].fetch(J, p, tile);
+        Q[k].digest(J, tile, J.count && p.s == 0 && k < nt ? &J.st->range_errors : nullptr);
+        over[k] = Q[k].bad;
         path[k] = up[imin(tile * 16 + col, J.rows - 1) / J.g.G];
         m[k] = NONE;
         lowest[k] = 0;
-        over[k] = Q[k].bad;
     }
-    uint32_t dg[3][4];
-    dgs.read(dg);
     const uint8_t *hb = plane_ptr(J.g, p.b, p.kvh, 0), *nb = hb + (J.g.n_planes - 1) * J.g.span;
     Keys<D, KB> next;
-    next.load(hb, nb, J.g.span, p.lo);
+    if (p.lo < p.hi) next.load(hb, nb, J.g.span, p.lo);
+    dgs.fill(start.c);
+    int none = 0;
+    if (p.tail) none = tree_paths(start.parent, J.n, up, at);
+    __syncthreads();
+    if (J.count && none && p.kvh == 0 && p.tile == 0 && p.T <= (int64_t)(p.s / W + 1) * W * J.mspan)
+        atomicAdd(&J.st->range_errors, (unsigned long long)none);
+    if (p.lo >= p.hi) return;
+    uint32_t dg[3][4];
+    dgs.read(dg);
     for (int64_t t0 = p.lo; t0 < p.hi; t0 += 16) {
         const Keys<D, KB> cur = next;
         if (t0 + 16 < p.hi) next.load(hb, nb, J.g.span, t0 + 16);
@@ -428,30 +494,61 @@ __device__ __forceinline__ uint32_t is_code(int m, uint32_t codes) {
     return m < 4 ? perm(0u, 1u << (8 * m), codes) : perm(1u << (8 * (m - 4)), 0u, codes);
 }
 
+// A row tile's runs: 16 a span, the first of each row, and extra ones in order of demand. LDS: the first
+// `near` of them in the workgroup's memory.
+template <int D, bool LDS>
+struct Runs {
+    uint4 *meta, *meta_l;
+    int32_t *S, *S_l;
+    uint32_t *pool;
+    int near;
+    __device__ __forceinline__ Runs(const Job &J, const Place &p, uint4 *ml, int32_t *sl, int n) : meta_l(ml), S_l(sl), near(n) {
+        const int64_t tl = (int64_t)p.chain * J.tiles + p.tile, run0 = tl * (16 * (int64_t)J.nspan + J.extra);
+        meta = J.sc.meta + run0;
+        S = J.sc.S + run0 * D;
+        pool = J.sc.pool + tl;
+    }
+    // lane = (row, 4 channels of each 16), as the walk holds them
+    __device__ __forceinline__ void put(int slot, const uint4 &m, const v4i (&acc)[D / 16], bool used) const {
+        const int grp = (threadIdx.x & 63) >> 4;
+        if (LDS && slot < near) {
+            if (grp == 0) meta_l[slot] = m;
+            if (!used) return;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) *(v4i *)(S_l + slot * D + 16 * c + 4 * grp) = acc[c];
+        } else {
+            if (grp == 0) meta[slot] = m;
+            if (!used) return;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) *(v4i *)(S + (int64_t)slot * D + 16 * c + 4 * grp) = acc[c];
+        }
+    }
+    __device__ __forceinline__ uint4 info(int slot) const { return LDS && slot < near ? meta_l[slot] : meta[slot]; }
+    // of a wave-uniform run, lane = channel
+    __device__ __forceinline__ void sum(int slot, bool used, int32_t (&v)[D / 64]) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k)
+            v[k] = !used ? 0 : LDS && slot < near ? S_l[slot * D + lane + 64 * k] : S[(int64_t)slot * D + lane + 64 * k];
+    }
+};
+
 // A wave's walk over its span, from the maximum m before it (or, two-pass, of all): its runs into the
 // scratch; returns the row's events, with BAD where it needs the serial path.
-template <int D, int KB, int NC>
-__device__ __forceinline__ uint32_t walk(const Job &J, const Place &p, const Query<D, KB> &Q, int32_t m, const Digits &dgs,
-                                     const uint32_t *path, const uint16_t *lut_s) {
+template <int D, int KB, int NC, bool LDS>
+__device__ __forceinline__ uint32_t walk(const Job &J, const Place &p, const Query<D, KB> &Q, int32_t m,
+                                         const ValueTable<NC> &values, const Runs<D, LDS> &runs, const Digits &dgs,
+                                         const uint32_t *path, const uint16_t *lut_s) {
     constexpr int CT = D / 16, PVK = NC / 4;
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
-    const int64_t tl = (int64_t)p.chain * J.tiles + p.tile;
     uint32_t dg[3][4];
     dgs.read(dg);
     const int vb = J.g.vb;
-    double vcs[NC], vcmax = 0.0;                       // value centroids / 2^23
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        vcs[i] = __longlong_as_double(uni64(__double_as_longlong(i < (1 << vb) ? (double)J.tabs->vc[i] * 0x1p-23 : 0.0)));
-        vcmax = fmax(vcmax, fabs(vcs[i]));
-    }
-    // |v_norm p| up to which a term is two balanced bytes
-    const uint32_t wide = (uint32_t)uni32((int)(uint32_t)(32639.0 / fmax(vcmax, 0x1p-16)));
-    const uint32_t delta_max = (uint32_t)J.tabs->delta_max;
+    const double (&vcs)[NC] = values.vcs, vcmax = values.vcmax;
+    const uint32_t wide = values.wide, delta_max = values.delta_max;
     const uint8_t *hb = plane_ptr(J.g, p.b, p.kvh, 0), *nb = hb + (J.g.n_planes - 1) * J.g.span;
     const uint8_t *vb0 = hb + (int64_t)((J.g.key_bytes + 15) / 16) * J.g.span;
     bool first = p.s == 0;                             // what the span finds is nothing: it scales in place
-    const int64_t run0 = tl * (16 * (int64_t)J.nspan + J.extra);
 
     v4i acc[CT];                                       // lane = (row, 4 channels of each 16)
 #pragma unroll
@@ -481,18 +578,14 @@ __device__ __forceinline__ uint32_t walk(const Job &J, const Place &p, const Que
         b += __shfl_xor(b, 32);
         if (!has) return;
         const bool used = L != 0 || fopen != 1u << PROB_FRAC;
-        if (grp == 0)
-            J.sc.meta[run0 + slot] = make_uint4(L, fopen | (used ? USED : 0u), (uint32_t)next,
-                                                __float_as_uint(b * (float)vcmax * 1.001f + (float)J.span));
-        if (!used) return;
-        int32_t *to = J.sc.S + (run0 + slot) * D + 4 * grp;
-#pragma unroll
-        for (int c = 0; c < CT; ++c) *(v4i *)(to + 16 * c) = acc[c];
+        const uint4 mt = make_uint4(L, fopen | (used ? USED : 0u), (uint32_t)next,
+                                    __float_as_uint(b * (float)vcmax * 1.001f + (float)J.span));
+        runs.put(slot, mt, acc, used);
     };
     // the run of the rows where `has` ends, and one with factor f begins
     auto next_run = [&](bool has, uint32_t f) __attribute__((always_inline)) {
         int to = 0;
-        if (has && grp == 0) to = (int)atomicAdd(J.sc.pool + tl, 1u);
+        if (has && grp == 0) to = (int)atomicAdd(runs.pool, 1u);
         to = __shfl(to, col);
         bad = bad || (has && to >= J.extra);
         to = 16 * J.nspan + imin(to, J.extra - 1);
@@ -723,16 +816,6 @@ __device__ __forceinline__ uint32_t walk(const Job &J, const Place &p, const Que
     return events | any;
 }
 
-// p by the integer part of its distance's table index, as lut_s[floor(d log2(e) / 2^24)] reads it (256 threads at least).
-__device__ __forceinline__ void fill_lut(const Tables *tabs, uint16_t *lut_s) {
-    if (threadIdx.x < 256) {
-        const int32_t x = tabs->exp_table[threadIdx.x];
-#pragma unroll
-        for (int i = 0; i < LUT_SPAN / 256; ++i) lut_s[256 * i + threadIdx.x] = (uint16_t)(x >> i);
-        if (threadIdx.x == 0) lut_s[LUT_SPAN] = 0;
-    }
-}
-
 template <int D, int KB, int NC>
 __global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel(Job J) {
     __shared__ Digits dgs;
@@ -742,22 +825,26 @@ __global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel
     Place p;
     if (!p.find(J, J.tiles, J.span, W)) return;
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
-    dgs.fill(J.tabs, J.g.kb);
-    fill_lut(J.tabs, lut_s);
-    if (p.tail) tree_paths(J.parents + p.b * J.pstride, J.n, up, at);
-    __syncthreads();
-    if (p.lo >= p.hi) return;
+    const Start start(J, p, p.tail);
+    Query<D, KB> Q;
+    Q.fetch(J, p, p.tile);
+    Q.digest(J, p.tile, nullptr);
     // the maximum of the spans before, or of all
     int32_t m = NONE;
-    {
+    if (p.lo < p.hi) {
         const int end = J.two ? (int)((p.T + J.mspan - 1) / J.mspan) : p.s * (J.span / J.mspan);
         const int32_t *top = J.sc.top + ((int64_t)p.chain * J.tiles + p.tile) * J.nms * 16 + col;
         for (int i = grp; i < end; i += 4) m = imax(m, top[i * 16]);
         m = row_max(m);
     }
-    Query<D, KB> Q;
-    Q.load(J, p.b, p.kvh, p.tile, J.tabs->kc_absmax, nullptr);
-    const uint32_t ev = walk<D, KB, NC>(J, p, Q, m, dgs, up[imin(p.tile * 16 + col, J.rows - 1) / J.g.G], lut_s);
+    const ValueTable<NC> values(J);
+    dgs.fill(start.c);
+    start.lut(lut_s);
+    if (p.tail) tree_paths(start.parent, J.n, up, at);
+    __syncthreads();
+    if (p.lo >= p.hi) return;
+    const Runs<D, false> runs(J, p, nullptr, nullptr, 0);
+    const uint32_t ev = walk<D, KB, NC, false>(J, p, Q, m, values, runs, dgs, up[imin(p.tile * 16 + col, J.rows - 1) / J.g.G], lut_s);
     if (grp == 0) J.sc.ev[(((int64_t)p.chain * J.tiles + p.tile) * J.nspan + p.s) * 16 + col] = ev;
 }
 
@@ -775,80 +862,94 @@ struct Tally {
     }
 };
 
-// A wave puts row `col` of a tile together, lane = channel: its runs in order, then acc / l. bad: the row goes
-// token by token.
-template <int D>
-__device__ __forceinline__ void combine_row(const Job &J, const Place &p, int col, bool bad, uint32_t events,
-                                            SerialLds<D == 64 ? 60 : 116> &fb, uint32_t *up, Tally &tally) {
+// A wave puts row `col` of a tile together, lane = channel: its runs in order, then acc / l. False where the
+// row has to go token by token.
+template <int D, bool LDS>
+__device__ __forceinline__ bool combine_row(const Job &J, const Place &p, int col, uint32_t events, const Runs<D, LDS> &runs,
+                                            int32_t (*buf)[D], int32_t *list, Tally &tally) {
     constexpr int CPL = D / 64;
     const int lane = threadIdx.x & 63, r = p.tile * 16 + col, node = r / J.g.G;
     const int64_t qrow = (((int64_t)p.b * J.n + node) * J.g.n_q + p.kvh * J.g.G + r % J.g.G) * D;
-    const int64_t run0 = ((int64_t)p.chain * J.tiles + p.tile) * (16 * (int64_t)J.nspan + J.extra);
     const int ns = (int)((p.T + J.span - 1) / J.span);
-    int64_t acc[CPL], l = 0;
+    int64_t acc[CPL];                                  // (online: what 32 bits hold)
+    uint64_t l = 0;
 #pragma unroll
     for (int k = 0; k < CPL; ++k) acc[k] = 0;
-    for (int i0 = 0; i0 < ns && !bad; i0 += 64) {
-        const uint4 mt = i0 + lane < ns ? J.sc.meta[run0 + (i0 + lane) * 16 + col] : make_uint4(0u, 0u, ~0u, 0u);
+    bool bad = false;
+    // one run after another; the loop is not unrolled, since its instructions come from memory but once
+    auto apply = [&](uint32_t L, uint32_t f, float bound, const int32_t (&v)[CPL]) __attribute__((always_inline)) {
+        if (J.two) {                                   // (no factors; clamped once, at the end)
+#pragma unroll
+            for (int k = 0; k < CPL; ++k) acc[k] += v[k];
+            l += L;
+            return;
+        }
+        const int32_t ff = (int32_t)(f & (USED - 1));
+#pragma unroll
+        for (int k = 0; k < CPL; ++k) {
+            // floor(a f / 2^15) in halves of 16 bits, as in the walk
+            const int32_t x = (int32_t)acc[k];
+            const int32_t y = __mul24(x >> 16, 2 * ff) + (int32_t)(__umul24((uint32_t)x & 0xFFFFu, (uint32_t)ff) >> PROB_FRAC);
+            bad = bad || !(fabsf((float)y) + bound <= 2147483000.0f);
+            acc[k] = y + v[k];
+        }
+        l = ((l * (uint32_t)ff) >> PROB_FRAC) + L;
+    };
+    for (int i0 = 0; i0 < ns; i0 += 64) {
+        const uint4 mt = i0 + lane < ns ? runs.info((i0 + lane) * 16 + col) : make_uint4(0u, 0u, ~0u, 0u);
         uint64_t todo = __ballot((mt.y & USED) != 0 || mt.z != ~0u);
-        constexpr int AHEAD = 16 / CPL;
-        int32_t v[AHEAD][CPL];
-        while (todo && !bad) {
-            int at[AHEAD];
-            uint64_t left = todo;
+        while (todo) {
+            // (of the workgroup's memory they are read where they are; of the scratch, 16 at a time)
+            uint64_t now = todo;
+            if constexpr (!LDS) {
+                constexpr int LR = D / 4, PER = 64 / LR;       // lanes a sum, 16 bytes each; sums a load
+                const int rank = __popcll(todo & ((1ull << lane) - 1ull));
+                wave_sync();
+                if (todo >> lane & 1 && rank < 16) list[rank] = lane;
+                now = __ballot((todo >> lane & 1) != 0 && rank < 16);
+                wave_sync();
+                const int cnt = __popcll(now);
+                uint4 v[16 / PER];
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                at[j] = left ? __ffsll((long long)left) - 1 : -1;
-                left &= left - 1;
-                if (at[j] < 0) continue;
-                const int32_t *S = J.sc.S + (run0 + (i0 + at[j]) * 16 + col) * D;
-                const bool used = ((uint32_t)__builtin_amdgcn_readlane((int)mt.y, at[j]) & USED) != 0;
+                for (int j = 0; j < 16 / PER; ++j)
+                    v[j] = *(const uint4 *)(runs.S + ((int64_t)(i0 + list[imin(PER * j + lane / LR, cnt - 1)]) * 16 + col) * D + 4 * (lane % LR));
 #pragma unroll
-                for (int k = 0; k < CPL; ++k) v[j][k] = used ? S[lane + 64 * k] : 0;
+                for (int j = 0; j < 16 / PER; ++j) *(uint4 *)&buf[PER * j + lane / LR][4 * (lane % LR)] = v[j];
+                wave_sync();
             }
-            todo = left;
+            todo &= ~now;
+#pragma unroll 1
+            for (int j = 0; now; ++j) {
+                const int at = __ffsll((long long)now) - 1;
+                now &= now - 1;
+                uint32_t L = (uint32_t)__builtin_amdgcn_readlane((int)mt.x, at);
+                uint32_t f = (uint32_t)__builtin_amdgcn_readlane((int)mt.y, at);
+                int next = __builtin_amdgcn_readlane((int)mt.z, at);
+                uint32_t bound = (uint32_t)__builtin_amdgcn_readlane((int)mt.w, at);
+                int32_t v[CPL];
+                if constexpr (LDS) {
+                    runs.sum((i0 + at) * 16 + col, (f & USED) != 0, v);
+                } else {
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                if (at[j] < 0) continue;
-                uint32_t L = (uint32_t)__builtin_amdgcn_readlane((int)mt.x, at[j]);
-                uint32_t f = (uint32_t)__builtin_amdgcn_readlane((int)mt.y, at[j]);
-                int next = __builtin_amdgcn_readlane((int)mt.z, at[j]);
-                double bound = (double)__uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)mt.w, at[j]));
+                    for (int k = 0; k < CPL; ++k) v[k] = buf[j][lane + 64 * k];
+                }
+#pragma unroll 1
                 for (;;) {
-                    if (f & USED) {
-                        const int64_t ff = f & (USED - 1);
-#pragma unroll
-                        for (int k = 0; k < CPL; ++k) {
-                            acc[k] = (acc[k] * ff) >> PROB_FRAC;
-                            const int64_t m = acc[k] < 0 ? -acc[k] : acc[k];
-                            // two-pass clamps once, at the end: only the run's own sum must fit
-                            bad = bad || !((J.two ? 0.0 : (double)m) + bound <= 2147483647.0);
-                            acc[k] += v[j][k];
-                        }
-                        l = ((l * ff) >> PROB_FRAC) + L;
-                    }
+                    if (f & USED) apply(L, f, __uint_as_float(bound), v);
                     if (next < 0) break;
-                    const uint4 x = J.sc.meta[run0 + next];
-                    const int32_t *S = J.sc.S + (run0 + next) * D;
-                    L = x.x;
-                    f = x.y;
-                    bound = (double)__uint_as_float(x.w);
-#pragma unroll
-                    for (int k = 0; k < CPL; ++k) v[j][k] = f & USED ? S[lane + 64 * k] : 0;
-                    next = (int)x.z;
+                    const int slot = next;
+                    const uint4 x = runs.info(slot);
+                    L = (uint32_t)uni32((int)x.x);
+                    f = (uint32_t)uni32((int)x.y);
+                    next = uni32((int)x.z);
+                    bound = (uint32_t)uni32((int)x.w);
+                    runs.sum(slot, (f & USED) != 0, v);
                 }
             }
-            bad = __ballot(bad) != 0;
         }
     }
-    if (bad) {
-        tree_path(J.parents + p.b * J.pstride, node, J.n, up);
-        serial_head<CPL, (D == 64 ? 60 : 116)>(J.g, J.tabs, J.tabs->kc, J.tabs->vc, J.q + qrow, p.b, p.kvh, p.T, J.two, true, fb,
-                                               J.out + qrow, J.st, TreeRows{up, p.base});
-        if (lane == 0) atomicAdd(&tally.bad, 1ull);
-        return;
-    }
-    const Recip rc = reciprocal(l);
+    if (__ballot(bad) != 0) return false;
+    const Recip rc = reciprocal((int64_t)l);
     int64_t amax = 0, over = 0;
 #pragma unroll
     for (int k = 0; k < CPL; ++k) {
@@ -870,11 +971,28 @@ __device__ __forceinline__ void combine_row(const Job &J, const Place &p, int co
             atomicMax(&tally.acc, (unsigned long long)amax);
         }
     }
+    return true;
+}
+
+template <int D>
+using RowLds = SerialLds<D == 64 ? 60 : 116>;          // (the widest row: 4-bit keys, 3-bit values)
+template <int D>
+__device__ __forceinline__ void serial_row(const Job &J, const Place &p, int col, RowLds<D> &fb, uint32_t *up, Tally &tally) {
+    const int r = p.tile * 16 + col, node = r / J.g.G;
+    const int64_t qrow = (((int64_t)p.b * J.n + node) * J.g.n_q + p.kvh * J.g.G + r % J.g.G) * D;
+    tree_path(J.parents + p.b * J.pstride, node, J.n, up);
+    serial_head<D / 64, (D == 64 ? 60 : 116)>(J.g, J.tabs, J.tabs->kc, J.tabs->vc, J.q + qrow, p.b, p.kvh, p.T, J.two, true, fb,
+                                              J.out + qrow, J.st, TreeRows{up, p.base});
+    if ((threadIdx.x & 63) == 0) atomicAdd(&tally.bad, 1ull);
 }
 
 template <int D>
 __global__ void __launch_bounds__(CW * 64) combine_kernel(Job J) {
-    __shared__ SerialLds<D == 64 ? 60 : 116> fb[CW];
+    __shared__ union {
+        RowLds<D> fb;
+        alignas(16) int32_t buf[16][D];
+    } u[CW];
+    __shared__ int32_t list[CW][16];
     __shared__ uint32_t up[CW][TREE_NODES / 32];
     __shared__ Tally tally;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -901,7 +1019,9 @@ __global__ void __launch_bounds__(CW * 64) combine_kernel(Job J) {
             bad = bad || (e & BAD) != 0;
         }
         for (int i = lane; i < nm; i += 64) bad = bad || (J.sc.over[tl * J.nms + i] >> col & 1) != 0;
-        combine_row<D>(J, p, col, __ballot(bad) != 0, events, fb[wv], up[wv], tally);
+        const Runs<D, false> runs(J, p, nullptr, nullptr, 0);
+        if (__ballot(bad) != 0 || !combine_row<D, false>(J, p, col, events, runs, u[wv].buf, list[wv], tally))
+            serial_row<D>(J, p, col, u[wv].fb, up[wv], tally);
     }
     if (!J.count) return;
     __syncthreads();
@@ -917,24 +1037,39 @@ __global__ void __launch_bounds__(FW * 64, 2) fused_kernel(Job J) {
     __shared__ int16_t at[TREE_NODES];
     __shared__ uint16_t lut_s[LUT_N + 7];
     __shared__ int32_t top_s[FW][16];
-    __shared__ uint32_t over_s, ev_s[FW][16];
-    __shared__ SerialLds<D == 64 ? 60 : 116> fb[FW];
-    __shared__ uint32_t fup[FW][TREE_NODES / 32];
+    __shared__ uint32_t bad_s, ev_s[FW][16];
     __shared__ Tally tally;
+    constexpr int NEAR = D == 64 ? 192 : 160;
+    __shared__ union {
+        struct {
+            uint4 meta[NEAR];
+            int32_t S[NEAR][D];
+        } r;
+        struct {
+            RowLds<D> fb[FW];
+            uint32_t up[FW][TREE_NODES / 32];
+        } f;
+    } u;
     Place p;
     p.find(J, J.tiles, J.span, FW);
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
-    const int64_t tl = (int64_t)p.chain * J.tiles + p.tile;
     Query<D, KB> Q;
-    Q.load(J, p.b, p.kvh, p.tile, J.tabs->kc_absmax, J.count && p.s == 0 ? &J.st->range_errors : nullptr);
-    dgs.fill(J.tabs, J.g.kb);
-    fill_lut(J.tabs, lut_s);
+    Q.fetch(J, p, p.tile);
+    const Start start(J, p, true);
+    const uint8_t *hb = plane_ptr(J.g, p.b, p.kvh, 0), *nb = hb + (J.g.n_planes - 1) * J.g.span;
+    Keys<D, KB> next;
+    if (p.lo < p.hi) next.load(hb, nb, J.g.span, p.lo);
+    const ValueTable<NC> values(J);
+    Q.digest(J, p.tile, J.count && p.s == 0 ? &J.st->range_errors : nullptr);
+    const Runs<D, true> runs(J, p, u.r.meta, u.r.S[0], NEAR);
+    dgs.fill(start.c);
+    start.lut(lut_s);
     if (tid == 0) {
-        over_s = 0;
+        bad_s = 0;
         tally.clear();
-        J.sc.pool[tl] = 0;
+        *runs.pool = 0;
     }
-    const int none = tree_paths(J.parents + p.b * J.pstride, J.n, up, at);
+    const int none = tree_paths(start.parent, J.n, up, at);
     if (J.count && none && p.kvh == 0 && p.tile == 0) atomicAdd(&J.st->range_errors, (unsigned long long)none);
     __syncthreads();
     const uint32_t *path = up[imin(p.tile * 16 + col, J.rows - 1) / J.g.G];
@@ -944,9 +1079,6 @@ __global__ void __launch_bounds__(FW * 64, 2) fused_kernel(Job J) {
         bool over = Q.bad;
         uint32_t dg[3][4];
         dgs.read(dg);
-        const uint8_t *hb = plane_ptr(J.g, p.b, p.kvh, 0), *nb = hb + (J.g.n_planes - 1) * J.g.span;
-        Keys<D, KB> next;
-        next.load(hb, nb, J.g.span, p.lo);
         for (int64_t t0 = p.lo; t0 < p.hi; t0 += 16) {
             const Keys<D, KB> cur = next;
             if (t0 + 16 < p.hi) next.load(hb, nb, J.g.span, t0 + 16);
@@ -965,7 +1097,7 @@ __global__ void __launch_bounds__(FW * 64, 2) fused_kernel(Job J) {
         }
         m = row_max(m);
         const uint64_t bad = __ballot(over);
-        if (lane == 0 && bad) atomicOr(&over_s, (uint32_t)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu));
+        if (lane == 0 && bad) atomicOr(&bad_s, (uint32_t)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xFFFFu));
         if (J.count) {
             const bool mine = !over && p.tile * 16 + col < J.rows;
             const int64_t x = m == NONE ? 0 : m < 0 ? -(int64_t)m : m, y = -(int64_t)lowest;
@@ -978,7 +1110,7 @@ __global__ void __launch_bounds__(FW * 64, 2) fused_kernel(Job J) {
     if (p.lo < p.hi) {
         m = NONE;
         for (int i = 0; i < (J.two ? FW : p.s); ++i) m = imax(m, top_s[i][col]);
-        const uint32_t ev = walk<D, KB, NC>(J, p, Q, m, dgs, path, lut_s);
+        const uint32_t ev = walk<D, KB, NC, true>(J, p, Q, m, values, runs, dgs, path, lut_s);
         if (grp == 0) ev_s[p.s][col] = ev;
     } else if (grp == 0) {
         ev_s[p.s][col] = 0;
@@ -987,8 +1119,15 @@ __global__ void __launch_bounds__(FW * 64, 2) fused_kernel(Job J) {
     for (int c = p.s; c < 16; c += FW) {
         if (p.tile * 16 + c >= J.rows) break;
         const uint32_t e = lane < FW ? ev_s[lane][c] : 0u;
-        combine_row<D>(J, p, c, __ballot((e & BAD) != 0) != 0 || (over_s >> c & 1) != 0, e & ~BAD, fb[p.s], fup[p.s], tally);
+        const bool bad = __ballot((e & BAD) != 0) != 0 || (bad_s >> c & 1) != 0;
+        if (bad || !combine_row<D, true>(J, p, c, e & ~BAD, runs, nullptr, nullptr, tally)) {
+            if (lane == 0) atomicOr(&bad_s, 1u << (16 + c));
+        }
     }
+    __syncthreads();                                   // (the serial path's rows lie over the runs)
+    const uint32_t bad = (uint32_t)uni32((int)(bad_s >> 16));
+    for (int c = p.s; c < 16; c += FW)
+        if (bad >> c & 1) serial_row<D>(J, p, c, u.f.fb[p.s], u.f.up[p.s], tally);
     if (!J.count) return;
     __syncthreads();
     if (tid == 0) tally.post(J, p.tile == 0 && p.kvh == 0, p.T);
@@ -1048,7 +1187,7 @@ size_t carve(const Geom &g, const Plan &pl, uint8_t *p, Scratch *sc) {
 }
 
 constexpr size_t BUDGET = (size_t)512 << 20;
-constexpr int64_t FUSED_MAX = 512;
+constexpr int64_t FUSED_MAX = 1024;
 Plan plan(const Geom &g, int64_t n, int64_t longest, int64_t batch) {
     Plan p{};
     p.tiles = (n * g.G + 15) / 16;
@@ -1064,8 +1203,7 @@ Plan plan(const Geom &g, int64_t n, int64_t longest, int64_t batch) {
         int64_t want = 1024 * (g.d == 64 && g.vb <= 2 ? 3 : 2) / all;
         if (longest > 512 * want) want *= 2;
         want = std::max<int64_t>(std::min(want, most), std::max<int64_t>(least, 1));
-        static const int64_t FM = getenv("FM") ? atoll(getenv("FM")) : FUSED_MAX;
-        p.fused = longest <= FM;
+        p.fused = longest <= FUSED_MAX;
         if (p.fused) {
             p.span = ((longest + FW - 1) / FW + 15) / 16 * 16;
             p.nspan = FW;
