@@ -178,6 +178,8 @@ struct Place {
     }
 };
 
+__device__ __forceinline__ uint32_t magnitude(int32_t x) { return x < 0 ? 0u - (uint32_t)x : (uint32_t)x; }
+
 // A row tile's queries: lane = (row, D / 4 channels from grp D / 4 on, in the order the codes expand in).
 template <int D, int KB>
 struct Query {
@@ -185,18 +187,18 @@ struct Query {
     bool bad;                                          // the row needs the serial path
     bool check;                                        // scores of the tile may leave int32 (wave-uniform)
     u128 raw[4 * (D / 64)];
+    int64_t at;                                        // of the lane's channels
     // the loads, and then what is made of them
     __device__ __forceinline__ void fetch(const Job &J, const Place &p, int tile) {
         const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
         const int r = imin(tile * 16 + col, J.rows - 1), G = J.g.G;
-        const int32_t *row = J.q + (((int64_t)p.b * J.n + r / G) * J.g.n_q + p.kvh * G + r % G) * D + grp * (D / 4);
+        at = (((int64_t)p.b * J.n + r / G) * J.g.n_q + p.kvh * G + r % G) * D + grp * (D / 4);
 #pragma unroll
-        for (int i = 0; i < 4 * (D / 64); ++i) raw[i] = *(const u128 *)(row + 4 * i);
+        for (int i = 0; i < 4 * (D / 64); ++i) raw[i] = *(const u128 *)(J.q + at + 4 * i);
     }
     __device__ __forceinline__ void digest(const Job &J, int tile, unsigned long long *range) {
         const int col = threadIdx.x & 15;
-        int64_t l1 = 0;
-        uint32_t wide = 0, out = 0;
+        uint32_t l1 = 0, top = 0;                      // (l1: of a row that is not bad at most 32 x 2^23)
 #pragma unroll
         for (int k = 0; k < D / 64; ++k) {
             uint32_t z[16];
@@ -206,30 +208,35 @@ struct Query {
                 const int32_t x[4] = {(int32_t)v.x, (int32_t)v.y, (int32_t)v.z, (int32_t)v.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t a = x[j] < 0 ? 0u - (uint32_t)x[j] : (uint32_t)x[j];
+                    const uint32_t a = magnitude(x[j]);
                     l1 += a;
-                    out += a >= (uint32_t)Q_ROT_LIMIT ? 1 : 0;
-                    wide |= a > 0x7F7F7Fu ? 1u : 0u;
+                    top = a > top ? a : top;
                     z[4 * i + j] = balanced(x[j]);
                 }
             }
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t o[3] = {0, 0, 0};
+            for (int w = 0; w < 4; ++w) {              // four words' bytes to three digits' words
+                uint32_t y[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t y = z[channel_of(KB, 4 * w + j)];
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) o[i] |= ((y >> (8 * i)) & 0xFFu) << (8 * j);
-                }
-#pragma unroll
-                for (int i = 0; i < 3; ++i) qd[i][k][w] = (int)o[i];
+                for (int j = 0; j < 4; ++j) y[j] = z[channel_of(KB, 4 * w + j)];
+                const uint32_t e = perm(y[1], y[0], 0x05010400u), f = perm(y[3], y[2], 0x05010400u);
+                qd[0][k][w] = (int)perm(f, e, 0x05040100u);
+                qd[1][k][w] = (int)perm(f, e, 0x07060302u);
+                qd[2][k][w] = (int)perm(perm(y[3], y[2], 0x0C0C0602u), perm(y[1], y[0], 0x0C0C0602u), 0x05040100u);
+            }
+        }
+        uint32_t out = 0;
+        if (range && top >= (uint32_t)Q_ROT_LIMIT) {
+#pragma unroll 1
+            for (int i = 0; i < 4 * (D / 64); ++i) {
+                const u128 v = *(const u128 *)(J.q + at + 4 * i);
+                for (uint32_t x : {v.x, v.y, v.z, v.w}) out += magnitude((int32_t)x) >= (uint32_t)Q_ROT_LIMIT ? 1 : 0;
             }
         }
         double b1 = (double)l1 * J.tabs->kc_absmax;
         b1 += __shfl_xor(b1, 16);
         b1 += __shfl_xor(b1, 32);
-        bad = row_or(wide) != 0 || !(b1 < DOT_MAX);
+        bad = row_or(top > 0x7F7F7Fu ? 1u : 0u) != 0 || !(b1 < DOT_MAX);
         check = __ballot(!bad && !(b1 * 32768.0 < NARROW_LIMIT)) != 0;
         if (range && out && tile * 16 + col < J.rows) atomicAdd(range, (unsigned long long)out);
     }
@@ -1187,7 +1194,7 @@ size_t carve(const Geom &g, const Plan &pl, uint8_t *p, Scratch *sc) {
 }
 
 constexpr size_t BUDGET = (size_t)512 << 20;
-constexpr int64_t FUSED_MAX = 1024;
+constexpr int64_t FUSED_MAX = 512;
 Plan plan(const Geom &g, int64_t n, int64_t longest, int64_t batch) {
     Plan p{};
     p.tiles = (n * g.G + 15) / 16;
@@ -1212,10 +1219,12 @@ Plan plan(const Geom &g, int64_t n, int64_t longest, int64_t batch) {
             p.span = ((longest + want - 1) / want + 63) / 64 * 64;
             p.nspan = (longest + p.span - 1) / p.span;
         }
+        // max_kernel's waves: a round of them where each still walks 128 tokens, half a round else: what comes
+        // before a walk costs as much as some 50 tokens (26 nodes behind 32,768: 160 tokens a wave 42 us, 80 tokens
+        // 44; 9 nodes x 16 ragged sequences: 144 tokens 46 us, 288 tokens 50)
         p.mspan = p.span;
-        while (!p.fused && p.mspan % 32 == 0 && p.span / p.mspan < 4 &&
-               p.seqs * g.n_kv * ((p.tiles + p.rt - 1) / p.rt) * ((longest + p.mspan - 1) / p.mspan) < 4096)
-            p.mspan /= 2;
+        auto waves = [&] { return p.seqs * g.n_kv * ((p.tiles + p.rt - 1) / p.rt) * ((longest + p.mspan - 1) / p.mspan); };
+        while (!p.fused && p.mspan % 32 == 0 && p.span / p.mspan < 4 && waves() < (p.mspan >= 256 ? 4096 : 2048)) p.mspan /= 2;
         p.nms = (longest + p.mspan - 1) / p.mspan;
         const int64_t room = (64 << 20) / (all * (g.d * 4 + 16));
         p.extra = room < EXTRA_MIN ? EXTRA_MIN : room > EXTRA_MAX ? EXTRA_MAX : room;
