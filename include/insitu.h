@@ -204,7 +204,9 @@ int insitu_attend_causal_head(insitu_cache *cache, int32_t seq, int32_t kv_head,
  * other value counts as -1 and as a range error (statistics). q_rot_dev int32 (batch, n, n_q_heads,
  * d) rotated; out_dev int32, the same shape, Q16. EBADLEN when a sequence holds fewer than n rows.
  * stats_host may be NULL: then nothing synchronises, and once a call of the shape has allocated the
- * cache's scratch nothing allocates either. */
+ * cache's scratch nothing allocates either, so that such a call may be captured into a graph. Its
+ * replays are for the lengths of the capture (changed ones are cut to n .. the longest of these), and
+ * share the scratch: one at a time, in order with the cache's other calls. */
 int insitu_attend_tree(insitu_cache *cache, int32_t n, const int32_t *parents_dev, int32_t per_sequence,
                        const int32_t *q_rot_dev, int32_t *out_dev, int32_t mode, insitu_stats *stats_host);
 
@@ -311,7 +313,8 @@ int insitu_load_rows(insitu_cache *cache, int32_t seq, int32_t head, int64_t t0,
  * order given, counts_host[i] of those n, row rows_dev[i * rows_stride + j] as number j (0 .. n - 1;
  * a value outside is taken as the nearest one inside). rows_stride 0: one list for all. The
  * destinations are different sequences, none of them a source. Rows behind the new length stay as
- * they are. Stream-ordered; nothing synchronises. */
+ * they are. Stream-ordered; nothing synchronises. In a graph, this and insitu_cache_keep repeat what
+ * they did, with the lengths of the capture and what rows_dev holds by then. */
 int insitu_cache_fork(insitu_cache *cache, int32_t n_copies, const int32_t *src_host, const int32_t *dst_host,
                       int64_t n, const int32_t *rows_dev, int64_t rows_stride, const int64_t *counts_host);
 /* Of the last n rows of every sequence, the listed ones (as insitu_cache_fork's lists, a list a

@@ -4,11 +4,13 @@
 // power of two, GQA divisibility), config.py:178-207 (code widths, whole
 // bytes), quantize.py:150-156 (threshold_frac >= qk_frac), base.py:67-73
 // (capacity), ddr_layout.py:126-146 (beat-friendly planes).
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <atomic>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -194,6 +196,7 @@ struct insitu_cache {
     size_t tree_bytes = 0;
     uint8_t *keep_scr = nullptr;          // insitu_cache_keep: rows on their way, for long lists
     size_t keep_bytes = 0;
+    std::vector<void *> retired;          // both, before they grew
     int32_t spin_limit = 1 << 20;         // insitu_cache_debug
     int32_t path = 0;                     // insitu_cache_debug: 0 auto, 1 scan, 2 chunked, 3 step kernel, 4 split
     int32_t prefill_path = 0;             // insitu_cache_debug: 0 auto, 1 virtual batch, 2 prefill kernel
@@ -244,20 +247,35 @@ int zero_stats(insitu_cache *c) {
     return INSITU_OK;
 }
 
-// A buffer of the cache, grown (the old one may still be in use by queued launches).
+// A buffer of the cache, grown to twice its size at least. The old one stays allocated until the cache goes:
+// queued launches and captured graphs may still use it. A capture allocates nothing.
 template <class T>
 int grow(insitu_cache *k, T *&p, size_t &have, size_t need) {
     if (have >= need) return INSITU_OK;
-    HIP_TRY(hipStreamSynchronize(k->ctx->stream), "sync");
-    if (p) HIP_TRY(hipFree(p), "hipFree");
-    p = nullptr;
-    have = 0;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    HIP_TRY(hipStreamIsCapturing(k->ctx->stream, &st), "hipStreamIsCapturing");
+    if (st != hipStreamCaptureStatusNone)
+        return fail(INSITU_EINVAL, "the scratch of a captured call is allocated by such a call before the capture");
+    try {
+        k->retired.reserve(k->retired.size() + 1);
+    } catch (const std::bad_alloc &) {
+        return fail(INSITU_ENOMEM, "cache scratch");
+    }
     void *q = nullptr;
-    const hipError_t e = hipMalloc(&q, need);
-    if (e == hipErrorOutOfMemory) return fail(INSITU_ENOMEM, "cache scratch");
+    size_t n = std::max(need, 2 * have);
+    hipError_t e = hipMalloc(&q, n);
+    if (e == hipErrorOutOfMemory && n > need) {
+        (void)hipGetLastError();
+        e = hipMalloc(&q, n = need);
+    }
+    if (e == hipErrorOutOfMemory) {
+        (void)hipGetLastError();
+        return fail(INSITU_ENOMEM, "cache scratch");
+    }
     HIP_TRY(e, "hipMalloc");
+    if (p) k->retired.push_back(p);
     p = (T *)q;
-    have = need;
+    have = n;
     return INSITU_OK;
 }
 
@@ -626,6 +644,7 @@ int insitu_cache_destroy(insitu_cache *k) {
     if (k->prefill_len) hipFree(k->prefill_len);
     if (k->tree_scr) hipFree(k->tree_scr);
     if (k->keep_scr) hipFree(k->keep_scr);
+    for (void *p : k->retired) hipFree(p);
     delete k;
     return INSITU_OK;
 }
@@ -1134,7 +1153,7 @@ int insitu_attend_tree(insitu_cache *k, int32_t n, const int32_t *parents, int32
                                    stats != nullptr, k->tree_scr, k->tree_bytes, ev, k->stats),
                 "tree attend launch");
     else
-        HIP_TRY(launch_attend_tree_serial(k->ctx->stream, k->g, k->tabs, q, out, len, parents, pstride, n, two_pass, ev,
+        HIP_TRY(launch_attend_tree_serial(k->ctx->stream, k->g, k->tabs, q, out, len, parents, pstride, n, longest, two_pass, ev,
                                           k->stats),
                 "tree attend launch");
     return copy_stats(k, stats);

@@ -72,6 +72,7 @@ struct Job {
     int64_t pstride;
     int32_t n, rows, tiles, span, nspan, mspan, nms;   // mspan, nms: max_kernel's spans, whole parts of the others
     int32_t extra, two, seq0, nseq, count;             // count: gather statistics
+    int64_t longest;
     Scratch sc;
     DevStats *st;
 };
@@ -147,6 +148,12 @@ __device__ __forceinline__ int tree_paths(int p, int n, uint32_t (*up)[UPW], int
     return bad;
 }
 
+// A sequence's rows. A call replayed from a graph after the lengths changed stays within the spans it was
+// planned with.
+__device__ __forceinline__ int64_t rows_of(const Job &J, int b) {
+    const int64_t T = J.len[b] < J.longest ? J.len[b] : J.longest;
+    return T < J.n ? J.n : T;
+}
 // Which of tokens rel .. rel + 3 behind the context a row sees, a bit each (rel from -16 on).
 __device__ __forceinline__ uint32_t visible4(const uint32_t *up, int rel) {
     const int k = (rel + 32) >> 5;
@@ -168,7 +175,7 @@ struct Place {
         s = s0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         b = J.seq0 + chain / J.g.n_kv;
         kvh = chain % J.g.n_kv;
-        T = J.len[b];
+        T = rows_of(J, b);
         base = T - J.n;
         const int64_t end = (int64_t)(s0 + waves) * span;
         tail = (end < T ? end : T) > base;
@@ -1010,7 +1017,7 @@ __global__ void __launch_bounds__(CW * 64) combine_kernel(Job J) {
     p.tile = part / (16 / CW);
     p.b = J.seq0 + p.chain / J.g.n_kv;
     p.kvh = p.chain % J.g.n_kv;
-    p.T = J.len[p.b];
+    p.T = rows_of(J, p.b);
     p.base = p.T - J.n;
     if (tid == 0) tally.clear();
     __syncthreads();
@@ -1162,11 +1169,12 @@ __global__ void __launch_bounds__(64) serial_kernel(Job J) {
     if (qh == 0 && lane == 0 && (parents[node] >= node || parents[node] < -1)) atomicAdd(&J.st->range_errors, 1ull);
     __syncthreads();
     tree_path(parents, node, J.n, up);
-    const int64_t T = J.len[b];
+    const int64_t T = rows_of(J, b);
     serial_head<CPL, SERIAL_RS>(J.g, J.tabs, kc, vc, J.q + at, b, qh / J.g.G, T, J.two, true, L, J.out + at, J.st,
                                 TreeRows{up, T - J.n});
 }
 
+namespace {
 // Sequences a launch takes, and the spans of the longest.
 struct Plan {
     int64_t seqs, tiles, span, nspan, mspan, nms, rt, extra;
@@ -1233,6 +1241,8 @@ Plan plan(const Geom &g, int64_t n, int64_t longest, int64_t batch) {
     }
 }
 
+}  // namespace
+
 template <int D, int KB, int NC>
 hipError_t launch(hipStream_t s, const Job &J, int rt, bool fused, LaunchEv ev) {
     const int64_t chains = (int64_t)J.nseq * J.g.n_kv;
@@ -1292,6 +1302,7 @@ hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, con
     J.extra = (int32_t)p.extra;
     J.two = two_pass;
     J.count = count;
+    J.longest = longest;
     J.st = st;
     for (int64_t b = 0; b < g.batch; b += p.seqs) {
         J.seq0 = (int32_t)b;
@@ -1313,7 +1324,7 @@ hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, con
 }
 
 hipError_t launch_attend_tree_serial(hipStream_t s, const Geom &g, const Tables *t, const int32_t *q, int32_t *out,
-                                     const int64_t *len, const int32_t *parents, int64_t pstride, int32_t n,
+                                     const int64_t *len, const int32_t *parents, int64_t pstride, int32_t n, int64_t longest,
                                      int two_pass, LaunchEv ev, DevStats *st) {
     tr::Job J{};
     J.g = g;
@@ -1325,6 +1336,7 @@ hipError_t launch_attend_tree_serial(hipStream_t s, const Geom &g, const Tables 
     J.pstride = pstride;
     J.n = n;
     J.two = two_pass;
+    J.longest = longest;
     J.st = st;
     const int64_t blocks = (int64_t)g.batch * n * g.n_q;
     if (blocks > 0x7fffffff) return hipErrorInvalidValue;

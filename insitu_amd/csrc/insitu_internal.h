@@ -376,7 +376,7 @@ hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, con
                               int two_pass, bool count, void *scratch, size_t scratch_bytes, LaunchEv ev, DevStats *st);
 // The same token by token, any format.
 hipError_t launch_attend_tree_serial(hipStream_t s, const Geom &g, const Tables *t, const int32_t *q, int32_t *out,
-                                     const int64_t *len, const int32_t *parents, int64_t pstride, int32_t n,
+                                     const int64_t *len, const int32_t *parents, int64_t pstride, int32_t n, int64_t longest,
                                      int two_pass, LaunchEv ev, DevStats *st);
 
 // Shared with the files that add entry points beside abi.hip: the error

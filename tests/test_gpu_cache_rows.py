@@ -142,6 +142,83 @@ def test_keep_none_and_of_many_sequences(ctx):
     _same(c, imgs, [x - 3 for x in lens])
 
 
+def test_on_another_stream(ctx):
+    """Lists made late on a stream that is not the context's; the rows read there without a synchronisation."""
+    import torch
+    fmt = FORMATS[0]
+    lens = [1500, 10, 1400]
+    c, imgs = _cache(ctx, fmt, 3, 1600, lens)
+    kept = np.sort(np.random.default_rng(1).choice(1300, 1200, replace=False))
+    img = c.device_image()
+    side = torch.cuda.Stream(ctx.torch_device)
+    rows = torch.from_numpy(kept.astype(np.int32)).to(ctx.torch_device)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        big = torch.randn(2048, 2048, device=ctx.torch_device)
+        for _ in range(20):
+            big = big @ big * 1e-3
+        late = rows + (big[0, 0] * 0).to(torch.int32)
+        c.fork(0, [1], n=1300, rows=late)
+        first = img[1].clone()
+        c.set_length(1400, 0)
+        c.set_length(1400, 1)
+        late = rows.clone() + (big[0, 0] * 0).to(torch.int32)
+        c.keep(1300, late)
+        second = img.clone()
+        c.keep(3, torch.tensor([2, 0], dtype=torch.int32, device=ctx.torch_device))
+        third = img.clone()
+    side.synchronize()
+    lay = c.layout()
+    _take(lay, imgs[1], 0, imgs[0], np.concatenate([np.arange(200), 200 + kept]), fmt[3])
+    np.testing.assert_array_equal(first.cpu().numpy(), imgs[1])
+    for b in range(3):
+        _take(lay, imgs[b], 100, imgs[b], 100 + kept, fmt[3])
+    np.testing.assert_array_equal(second.cpu().numpy(), imgs)
+    for b in range(3):
+        _take(lay, imgs[b], 1297, imgs[b], [1299, 1297], fmt[3])
+    np.testing.assert_array_equal(third.cpu().numpy(), imgs)
+    assert c.lengths() == [1299] * 3
+
+
+@pytest.mark.parametrize("n,kept", [(40, 9), (1500, 1200)])
+def test_captured_and_replayed(ctx, n, kept):
+    """A fork and a compaction in one graph: replays read the lists anew and begin at the captured lengths."""
+    import torch
+    from insitu_amd.runtime import Context
+    fmt, T = FORMATS[1], 1600
+    side = torch.cuda.Stream(ctx.torch_device)
+    own = Context(ctx.device, stream=side)
+    rng = np.random.default_rng(2)
+    with torch.cuda.stream(side):
+        c, imgs = _cache(own, fmt, 2, 1700, [T, T])
+        start = imgs.copy()
+        rows = torch.zeros((2, kept), dtype=torch.int32, device=own.torch_device)
+        c.keep(n, rows)                                 # (the buffer is allocated before the capture)
+        for b in range(2):
+            c.set_length(T, b)
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            c.fork(0, [1], n=n, rows=rows[0], counts=[kept - 1])
+            c.keep(kept - 1, rows[:, :3].contiguous() % (kept - 1), counts=[3, 2])
+        for _ in range(3):
+            imgs = start.copy()
+            for b in range(2):
+                c.load_image(imgs[b], b)
+            new = rng.integers(0, n, (2, kept))
+            rows.copy_(torch.from_numpy(new.astype(np.int32)))
+            g.replay()
+            side.synchronize()
+            lay, cut = c.layout(), new[:, :3] % (kept - 1)
+            _take(lay, imgs[1], 0, imgs[0], np.concatenate([np.arange(T - n), T - n + new[0, :kept - 1]]), fmt[3])
+            for b, m, end in ((0, 3, T), (1, 2, T - n + kept - 1)):
+                base = end - (kept - 1)
+                _take(lay, imgs[b], base, imgs[b], base + cut[b, :m], fmt[3])
+            _same(c, imgs, [T - (kept - 1) + 3, T - n + 2])
+            for b in range(2):                          # (and eager work between the replays)
+                c.read_rows(0, 0, 5, b)
+
+
 def test_device_image_is_the_caches_memory(ctx):
     import torch
     fmt = FORMATS[0]

@@ -176,6 +176,43 @@ def test_every_row_an_event(ctx, T, serial):
 
 
 @pytest.mark.parametrize("mode", ["online", "two_pass"])
+@pytest.mark.parametrize("fmt", [FORMATS[0], FORMATS[4], FORMATS[5]])
+def test_around_the_longest_context_of_one_launch(ctx, fmt, mode):
+    """The longest sequence decides between one launch and three: 511 to 514 rows, with shorter ones beside."""
+    for rows in (511, 512, 513, 514):
+        _run(ctx, fmt, (rows - 5, 60, 0), 5, "random", mode, seed=rows)
+
+
+@pytest.mark.parametrize("fmt", [FORMATS[0], FORMATS[5]])
+def test_every_row_an_event_in_one_launch(ctx, fmt):
+    """A context of one launch whose events are more than shared memory and the scratch hold together."""
+    d, n, T = fmt[0], 5, 500
+    rng = np.random.default_rng(13)
+    k, u = _rising(d, T, 0.02)
+    q = np.rint(np.broadcast_to(u / 32, (1, n, N_KV * 4, d))).astype(np.int64)
+    v = _draw(rng, 65536, 1, T, N_KV, d)
+    _, st = _run(ctx, fmt, (T - n,), n, "chain", "online", serial=None, k=k, v=v, q=q)
+    assert st.serial_fallbacks > 0
+
+
+@pytest.mark.parametrize("mode", ["online", "two_pass"])
+@pytest.mark.parametrize("fmt", [FORMATS[1], FORMATS[5]])
+def test_long_runs_of_wide_values(ctx, fmt, mode):
+    """Flat weights over spans of hundreds of tokens, values of norm 40: a term is up to
+    20480 x 32768 x 70498 / 2^23 = 5.6 M, so that 384 of them could pass 2^31, and runs end before."""
+    d, _, _, G = fmt
+    _, st = _run(ctx, fmt, (5600, 3000), 256, "random", mode, q_scale=1 << 4, nodes=[0, 130, 255], serial=None,
+                 kv_scale=40 / d ** 0.5 * 65536)
+    assert st.serial_fallbacks == 0 and st.acc_overflows == 0
+
+
+@pytest.mark.parametrize("base", [40, 400])
+def test_batches_past_the_scratch(ctx, base):
+    """16 sequences of 256 nodes and 16 heads: their runs take several launches, a part of the batch each."""
+    _run(ctx, FORMATS[7], tuple(base + i for i in range(16)), 256, "random", "online", nodes=[0, 97, 255])
+
+
+@pytest.mark.parametrize("mode", ["online", "two_pass"])
 def test_queries_past_three_digits(ctx, mode):
     """Values of 2^23 and more, up to the seam's range and beyond it (range errors)."""
     fmt, n = FORMATS[0], 4
@@ -321,6 +358,83 @@ def test_captured_and_replayed(ctx):
             for x, p, o in zip(new, ps, got):
                 assert torch.equal(a.attend_tree(x, p, stats=False)[0], o), f"replay {r}"
             side.synchronize()
+
+
+def test_captured_before_the_scratch_grew(ctx):
+    """A graph keeps the scratch that it was captured with; and one captured without any is refused."""
+    import torch
+    from insitu_amd import _lib
+    from insitu_amd.attention import CompressedAttention
+    from insitu_amd.runtime import Context
+    fmt, T, n = FORMATS[0], 2600, 5
+    side = torch.cuda.Stream(ctx.torch_device)
+    own = Context(ctx.device, stream=side)
+    rng = np.random.default_rng(14)
+    dev = own.torch_device
+    with torch.cuda.stream(side):
+        c = _cache(own, fmt, [T])
+        _fill(c, fmt, [T], *(_draw(rng, 65536, 1, T, N_KV, 64) for _ in "kv"))
+        a = CompressedAttention(c)
+        q = torch.from_numpy(_draw(rng, 1 << 14, n, N_KV * 4, 64).astype(np.int32)).to(dev)
+        p = torch.from_numpy(_tree("random", n, rng).astype(np.int32)).to(dev)
+        out = torch.zeros_like(q)
+        side.synchronize()
+        with pytest.raises(_lib.InsituError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                a.attend_tree(q, p, out=out, stats=False)
+        a.attend_tree(q, p, out=out, stats=False)
+        side.synchronize()
+        want = out.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            a.attend_tree(q, p, out=out, stats=False)
+        big = torch.from_numpy(_draw(rng, 1 << 14, 256, N_KV * 4, 64).astype(np.int32)).to(dev)
+        large = a.attend_tree(big, np.arange(256) - 1, stats=False)[0].clone()
+        filler = [torch.full((1 << 22,), 77, dtype=torch.int32, device=dev) for _ in range(8)]
+        for _ in range(3):
+            out.zero_()
+            g.replay()
+            side.synchronize()
+            assert torch.equal(out, want)
+            assert torch.equal(a.attend_tree(big, np.arange(256) - 1, stats=False)[0], large)
+        assert all(bool((x == 77).all()) for x in filler)
+
+
+@pytest.mark.parametrize("T", [300, 2000])
+def test_replayed_after_the_lengths_changed(ctx, T):
+    """Shorter sequences are attended as they are, longer ones as far as the captured call's went."""
+    import torch
+    from insitu_amd.attention import CompressedAttention
+    from insitu_amd.runtime import Context
+    fmt, n = FORMATS[0], 6
+    side = torch.cuda.Stream(ctx.torch_device)
+    own = Context(ctx.device, stream=side)
+    rng = np.random.default_rng(15)
+    dev = own.torch_device
+    with torch.cuda.stream(side):
+        c = _cache(own, fmt, [2 * T])
+        _fill(c, fmt, [2 * T], *(_draw(rng, 65536, 1, 2 * T, N_KV, 64) for _ in "kv"))
+        a = CompressedAttention(c)
+        q = torch.from_numpy(_draw(rng, 1 << 14, n, N_KV * 4, 64).astype(np.int32)).to(dev)
+        p = torch.from_numpy(_tree("random", n, rng).astype(np.int32)).to(dev)
+        graphs, want = {}, {}
+        for mode in ("online", "two_pass", "serial"):
+            out = torch.zeros_like(q)
+            for m in (7, T // 2, T):
+                c.set_length(m, 0)
+                a.attend_tree(q, p, mode, out=out, stats=False)
+                side.synchronize()
+                want[mode, m] = out.clone()
+            graphs[mode] = torch.cuda.CUDAGraph(), out
+            with torch.cuda.graph(graphs[mode][0], stream=side):
+                a.attend_tree(q, p, mode, out=out, stats=False)
+        for now, as_if in ((7, 7), (T // 2, T // 2), (T, T), (T + 1, T), (2 * T, T)):
+            c.set_length(now, 0)
+            for mode, (g, out) in graphs.items():
+                out.zero_()
+                g.replay()
+                side.synchronize()
+                assert torch.equal(out, want[mode, as_if]), (mode, now)
 
 
 def test_refusals(ctx):
