@@ -189,7 +189,8 @@ class Seam:
     models have beside the reference's: RMS norms of query and key heads (q_norm, k_norm: weights
     (head_dim,), eps model.qk_norm_eps), rotary positions over model.rotary_dim channels in half or
     interleaved pairs (model.rope_interleaved), and any scaling of the frequencies that RoPE.build
-    takes. bias ((Hq + 2 Hkv) d) is added to the projections in fp32."""
+    takes. bias ((Hq + 2 Hkv) d) is added to the projections in fp32. tables: RoPE.build's (cos, sin)
+    where they are on the device already."""
 
     def __init__(self, model, *, q_norm=None, k_norm=None, bias=None, cast_after_rope: bool = True, ctx=None,
                  tables=None) -> None:
@@ -205,6 +206,11 @@ class Seam:
         if tables is None:
             rope = RoPE.build(m.rotary_dim, m.max_position, m.rope_theta, ROPE_FRAC, m.rope_scaling)
             tables = (torch.from_numpy(rope.cos).to(dev), torch.from_numpy(rope.sin).to(dev))
+        for t in tables:
+            if t.device != dev or t.dtype != torch.int64 or not t.is_contiguous() or \
+                    tuple(t.shape) != (m.max_position, m.rotary_dim // 2):
+                raise ValueError(f"tables: cos and sin, contiguous int64 ({m.max_position}, {m.rotary_dim // 2}) "
+                                 f"on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         self._cos, self._sin = tables
         self.last_saturated = 0
         dp = lambda t: None if t is None else t.data_ptr()
@@ -243,14 +249,14 @@ class Seam:
             if not np.all(np.diff(host) == 1):
                 pos = self.ctx.to_device(host, torch.int64)
         dev = self.ctx.torch_device
-        q = torch.empty((n, m.num_heads, m.head_dim), dtype=torch.int32, device=dev)
-        k = torch.empty((n, m.num_kv_heads, m.head_dim), dtype=torch.int32, device=dev)
+        q = torch.empty(n, m.num_heads, m.head_dim, dtype=torch.int32, device=dev)
+        k = torch.empty(n, m.num_kv_heads, m.head_dim, dtype=torch.int32, device=dev)
         v = torch.empty_like(k)
         cnt = (ctypes.c_uint64 * 2)() if counts else None
         with self.ctx.ordered(p, pos, q, k, v):
-            _lib.check(self.ctx.lib.insitu_seam_heads(self.ctx.handle, ctypes.byref(self._desc), ptr(p), n,
-                                                      ptr(pos) if pos is not None else None, pos0, ptr(q), ptr(k),
-                                                      ptr(v), cnt))
+            _lib.check(self.ctx.lib.insitu_seam_heads(self.ctx.handle, ctypes.byref(self._desc), p.data_ptr(), n,
+                                                      pos.data_ptr() if pos is not None else None, pos0,
+                                                      q.data_ptr(), k.data_ptr(), v.data_ptr(), cnt))
         if cnt is not None:
             self.last_saturated = int(cnt[0])
         self._keep = (p, pos)

@@ -210,3 +210,41 @@ def test_captured_and_replayed(ctx):
             for a, b in zip(got, s.wire(p, pos, counts=False)):
                 assert torch.equal(a, b)
             side.synchronize()
+
+
+def test_refuses_other_tables(ctx):
+    import torch
+    from insitu_amd import ModelConfig, Seam
+    from insitu_amd.host import RoPE
+    m = ModelConfig(hidden_size=256, num_heads=4, num_kv_heads=1, max_position=64, rotary_dim=32)
+    rope = RoPE.build(32, 64)
+    good = [torch.from_numpy(t).to(ctx.torch_device) for t in (rope.cos, rope.sin)]
+    assert Seam(m, ctx=ctx, tables=good).wire(np.zeros((2, 384), np.float32), 3)[0].shape == (2, 4, 64)
+    short = [t[:63].contiguous() for t in good]
+    wide = [torch.from_numpy(t).to(ctx.torch_device) for t in (RoPE.build(64, 64).cos, RoPE.build(64, 64).sin)]
+    for bad in (short, wide, (good[0], short[1]), [t.to(torch.int32) for t in good], [t.cpu() for t in good],
+                [t.t().contiguous().t() for t in good]):
+        with pytest.raises(ValueError, match="tables"):
+            Seam(m, ctx=ctx, tables=bad)
+
+
+def test_on_another_stream(ctx):
+    """Projections made late on a stream that is not the context's, rows used there without a synchronisation."""
+    import torch
+    from insitu_amd import ModelConfig, Seam
+    m = ModelConfig(hidden_size=256, num_heads=4, num_kv_heads=1, max_position=64)
+    s = Seam(m, q_norm=np.ones(64, np.float32), k_norm=np.ones(64, np.float32), ctx=ctx)
+    p = torch.randn((40, s.width), device=ctx.torch_device)
+    pos = torch.arange(40, device=ctx.torch_device)
+    want = [x.clone() for x in s.wire(p, pos, counts=False)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream(ctx.torch_device)
+    with torch.cuda.stream(side):
+        big = torch.randn(2048, 2048, device=ctx.torch_device)
+        for _ in range(20):
+            big = big @ big * 1e-3
+        late = p + (big[0, 0] * 0).nan_to_num()
+        got = [x + 0 for x in s.wire(late, pos, counts=False)]
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
