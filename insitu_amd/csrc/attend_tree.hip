@@ -73,6 +73,7 @@ struct Job {
     int32_t n, rows, tiles, span, nspan, mspan, nms;   // mspan, nms: max_kernel's spans, whole parts of the others
     int32_t extra, two, seq0, nseq, count;             // count: gather statistics
     int64_t longest;
+    double kc_absmax;
     Scratch sc;
     DevStats *st;
 };
@@ -240,7 +241,7 @@ struct Query {
                 for (uint32_t x : {v.x, v.y, v.z, v.w}) out += magnitude((int32_t)x) >= (uint32_t)Q_ROT_LIMIT ? 1 : 0;
             }
         }
-        double b1 = (double)l1 * J.tabs->kc_absmax;
+        double b1 = (double)l1 * J.kc_absmax;
         b1 += __shfl_xor(b1, 16);
         b1 += __shfl_xor(b1, 32);
         bad = row_or(top > 0x7F7F7Fu ? 1u : 0u) != 0 || !(b1 < DOT_MAX);
@@ -328,9 +329,10 @@ struct Start {
     int parent;
     __device__ __forceinline__ Start(const Job &J, const Place &p, bool paths) {
         const int i = threadIdx.x;
-        c = i < (1 << J.g.kb) ? (int32_t)J.tabs->kc[i & 15] : 0;
+        c = (int32_t)J.tabs->kc[i & 15];               // (no code names one behind the codebook's end)
         x = J.tabs->exp_table[i & 255];
-        parent = paths && i < J.n ? J.parents[p.b * J.pstride + i] : -1;
+        const int at = J.parents[p.b * J.pstride + imin(i, J.n - 1)];
+        parent = paths && i < J.n ? at : -1;
     }
     // lut_s[floor(d log2(e) / 2^24)]: p by distance, the table an octave after the other (256 threads at least)
     __device__ __forceinline__ void lut(uint16_t *lut_s) const {
@@ -378,11 +380,14 @@ __global__ void __launch_bounds__(W * 64, RT > 2 ? 3 : 4) max_kernel(Job J) {
     for (int k = 0; k < RT; ++k) {
         const int tile = tile0 + imin(k, nt - 1);      // (a tile past the last one is not scored)
         Q[k].fetch(J, p, tile);
-        Q[k].digest(J, tile, J.count && p.s == 0 && k < nt ? &J.st->range_errors : nullptr);
-        over[k] = Q[k].bad;
         path[k] = up[imin(tile * 16 + col, J.rows - 1) / J.g.G];
         m[k] = NONE;
         lowest[k] = 0;
+    }
+#pragma unroll
+    for (int k = 0; k < RT; ++k) {
+        Q[k].digest(J, tile0 + imin(k, nt - 1), J.count && p.s == 0 && k < nt ? &J.st->range_errors : nullptr);
+        over[k] = Q[k].bad;
     }
     const uint8_t *hb = plane_ptr(J.g, p.b, p.kvh, 0), *nb = hb + (J.g.n_planes - 1) * J.g.span;
     Keys<D, KB> next;
@@ -830,6 +835,39 @@ __device__ __forceinline__ uint32_t walk(const Job &J, const Place &p, const Que
     return events | any;
 }
 
+// Each row's largest of n spans' maxima (top: [span][16]), in the lanes of its column. A load takes 16 spans,
+// lane = (span, 4 rows), and four of them are in flight: one by one a late span's hundred would cost more
+// than its walk.
+__device__ __forceinline__ int32_t top_of(const int32_t *top, int n) {
+    const int lane = threadIdx.x & 63, col = lane & 15;
+    int32_t m[4] = {NONE, NONE, NONE, NONE};
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        int4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + 16 * j + (lane >> 2);
+            v[j] = make_int4(NONE, NONE, NONE, NONE);
+            if (i < n) v[j] = *(const int4 *)(top + (int64_t)i * 16 + 4 * (lane & 3));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            m[0] = imax(m[0], v[j].x);
+            m[1] = imax(m[1], v[j].y);
+            m[2] = imax(m[2], v[j].z);
+            m[3] = imax(m[3], v[j].w);
+        }
+    }
+    int32_t mine = NONE;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int x = 4; x < 64; x *= 2) m[k] = imax(m[k], __shfl_xor(m[k], x));
+        const int32_t y = __shfl(m[k], col >> 2);
+        mine = (col & 3) == k ? y : mine;
+    }
+    return mine;
+}
+
 template <int D, int KB, int NC>
 __global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel(Job J) {
     __shared__ Digits dgs;
@@ -842,15 +880,12 @@ __global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel
     const Start start(J, p, p.tail);
     Query<D, KB> Q;
     Q.fetch(J, p, p.tile);
-    Q.digest(J, p.tile, nullptr);
     // the maximum of the spans before, or of all
     int32_t m = NONE;
-    if (p.lo < p.hi) {
-        const int end = J.two ? (int)((p.T + J.mspan - 1) / J.mspan) : p.s * (J.span / J.mspan);
-        const int32_t *top = J.sc.top + ((int64_t)p.chain * J.tiles + p.tile) * J.nms * 16 + col;
-        for (int i = grp; i < end; i += 4) m = imax(m, top[i * 16]);
-        m = row_max(m);
-    }
+    if (p.lo < p.hi)
+        m = top_of(J.sc.top + ((int64_t)p.chain * J.tiles + p.tile) * J.nms * 16,
+                   J.two ? (int)((p.T + J.mspan - 1) / J.mspan) : p.s * (J.span / J.mspan));
+    Q.digest(J, p.tile, nullptr);
     const ValueTable<NC> values(J);
     dgs.fill(start.c);
     start.lut(lut_s);
@@ -1278,7 +1313,7 @@ size_t tree_scratch_bytes(const Geom &g, int64_t n, int64_t longest) {
     return tr::carve(g, p, nullptr, nullptr);
 }
 
-hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, const int32_t *q, int32_t *out,
+hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, double kc_absmax, const int32_t *q, int32_t *out,
                               const int64_t *len, const int32_t *parents, int64_t pstride, int32_t n, int64_t longest,
                               int two_pass, bool count, void *scratch, size_t scratch_bytes, LaunchEv ev, DevStats *st) {
     using namespace tr;
@@ -1303,6 +1338,7 @@ hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, con
     J.two = two_pass;
     J.count = count;
     J.longest = longest;
+    J.kc_absmax = kc_absmax;
     J.st = st;
     for (int64_t b = 0; b < g.batch; b += p.seqs) {
         J.seq0 = (int32_t)b;
