@@ -22,6 +22,19 @@
 // Matrix operands as in the prefill attend: scores from three balanced digits of q and of the centroids,
 // nine int8 products a 64 channels, lane = (row, 4 tokens); there p and the terms of all value codes, as
 // three digits, which the one-hot value codes of the tokens sum up, lane = (row, 4 channels).
+//
+// A context of up to 512 tokens takes one launch (fused_kernel): a workgroup's eight waves are the spans, and the
+// three steps follow each other behind barriers, the runs mostly in shared memory.
+//
+// What bounds it. Memory does not: 32 nodes of 4 heads behind 8 x 32,768 tokens read 218 MB, 46 us at the rate of a
+// copy, and take 1,850 us. The integers do: a token and row of d = 128 with 3-bit values costs 66 matrix
+// instructions a 16 x 16 tile (24 % of the walk's cycles) and 530 vector ones, which fill 64 % of the issue slots:
+// the keys' digits, the scores' carries in 64 bits, the terms in float64 for every value code (exact: 53 bits), their
+// digits' bytes and the one-hot codes. So the tile's terms use two digits where they fit, no tile is walked whose
+// weights are all zero, and max_kernel's row tiles share the expanded keys. Measured kernels: 26 nodes behind 32,768
+// tokens (4b/2b, 32 heads) 40 + 67 + 13 us, 64 nodes behind 4,097 two-pass 16 + 38 + 5 us; tried and slower: 32
+// tokens a step, storing the scores between the launches, one launch for long contexts, signed codebooks halved by
+// symmetry, two or four tokens' tiles sharing one-hot codes at d = 128 (registers), four waves a SIMD.
 #include <algorithm>
 #include <cstdlib>
 #include <type_traits>
@@ -868,8 +881,9 @@ __device__ __forceinline__ int32_t top_of(const int32_t *top, int n) {
     return mine;
 }
 
-template <int D, int KB, int NC>
-__global__ void __launch_bounds__(W * 64, D == 64 && NC == 4 ? 3 : 2) sum_kernel(Job J) {
+// OCC waves a SIMD.
+template <int D, int KB, int NC, int OCC>
+__global__ void __launch_bounds__(W * 64, OCC) sum_kernel(Job J) {
     __shared__ Digits dgs;
     __shared__ uint32_t up[TREE_NODES][UPW];
     __shared__ int16_t at[TREE_NODES];
@@ -1077,7 +1091,8 @@ __global__ void __launch_bounds__(CW * 64) combine_kernel(Job J) {
     if (tid == 0) tally.post(J, part == 0 && p.kvh == 0, p.T);
 }
 
-// All of it in one launch, where the spans are a workgroup's waves: short contexts, and many row tiles.
+// All of it in one launch, where the spans are a workgroup's waves (20 us for 5 nodes behind 100 tokens, a chain of
+// round trips: tables and queries 4, maxima 1, walk 6, runs 5; the rest launch and end).
 constexpr int FW = 8;
 template <int D, int KB, int NC>
 __global__ void __launch_bounds__(FW * 64, 2) fused_kernel(Job J) {
@@ -1213,7 +1228,7 @@ namespace {
 // Sequences a launch takes, and the spans of the longest.
 struct Plan {
     int64_t seqs, tiles, span, nspan, mspan, nms, rt, extra;
-    bool fused;
+    bool fused, longw;
 };
 // The scratch of a launch, carved from p (null: only its size).
 size_t carve(const Geom &g, const Plan &pl, uint8_t *p, Scratch *sc) {
@@ -1237,6 +1252,8 @@ size_t carve(const Geom &g, const Plan &pl, uint8_t *p, Scratch *sc) {
 }
 
 constexpr size_t BUDGET = (size_t)512 << 20;
+// Contexts up to here in one launch (5 nodes behind 100 tokens 20 us, in three 29; 26 behind 512: 31 and 32; behind
+// 1,024: 42 and 36; 26 x 8 sequences: 45 and 46, 59 and 58, 77 and 73).
 constexpr int64_t FUSED_MAX = 512;
 Plan plan(const Geom &g, int64_t n, int64_t longest, int64_t batch) {
     Plan p{};
@@ -1244,14 +1261,22 @@ Plan plan(const Geom &g, int64_t n, int64_t longest, int64_t batch) {
     p.seqs = batch;
     for (;;) {
         const int64_t all = p.seqs * g.n_kv * p.tiles;
-        // row tiles a wave of max_kernel: as many as leave it 2,048 waves of 64 tokens
+        // row tiles a wave of max_kernel: as many as leave it 4,096 waves of 64 tokens (64 nodes behind 4,097 tokens:
+        // two 57 us, four 61; 26 behind 8,192 x 8 sequences: four 193, two 200; 9 x 16 ragged: four 147, one 164)
         p.rt = g.d == 64 ? 4 : 2;
-        while (p.rt > 1 && (p.tiles <= p.rt / 2 || p.seqs * g.n_kv * ((p.tiles + p.rt - 1) / p.rt) * ((longest + 63) / 64) < 2048)) p.rt /= 2;
+        while (p.rt > 1 && (p.tiles <= p.rt / 2 || p.seqs * g.n_kv * ((p.tiles + p.rt - 1) / p.rt) * ((longest + 63) / 64) < 4096)) p.rt /= 2;
         const int64_t most = (longest + 63) / 64, least = (longest + SPAN_MAX - 1) / SPAN_MAX;
-        // as many waves as the chip holds of sum_kernel, and twice that for long walks, whose ragged ends and first
-        // spans' events a second round evens out
-        int64_t want = 1024 * (g.d == 64 && g.vb <= 2 ? 3 : 2) / all;
-        if (longest > 512 * want) want *= 2;
+        // spans: as many waves of sum_kernel as the chip holds at two a SIMD. Where they would walk more than 300 tokens
+        // each: with 4 value codes at d = 64 three a SIMD, for which some registers go to memory (13 nodes x 4 behind
+        // 2,047 tokens: two a SIMD 58 us, three 62; 26 behind 32,768: 120 and 110), and up to three rounds of them
+        // while that leaves 256 tokens, since later ones even out ragged ends and first spans' events (9 nodes x 16
+        // ragged: one 177, two 147, three 140; 5 x 3 behind 20,000, 105 tokens each in three: one 95, three 109)
+        int64_t want = 2048 / all;
+        p.longw = longest > 300 * want;
+        if (p.longw) {
+            const int64_t round = std::max<int64_t>(1024 * (g.d == 64 && g.vb <= 2 ? 3 : 2) / all, 1);
+            want = round * std::min<int64_t>(std::max<int64_t>(longest / (256 * round), 1), 3);
+        }
         want = std::max<int64_t>(std::min(want, most), std::max<int64_t>(least, 1));
         p.fused = longest <= FUSED_MAX;
         if (p.fused) {
@@ -1279,7 +1304,7 @@ Plan plan(const Geom &g, int64_t n, int64_t longest, int64_t batch) {
 }  // namespace
 
 template <int D, int KB, int NC>
-hipError_t launch(hipStream_t s, const Job &J, int rt, bool fused, LaunchEv ev) {
+hipError_t launch(hipStream_t s, const Job &J, int rt, bool fused, bool longw, LaunchEv ev) {
     const int64_t chains = (int64_t)J.nseq * J.g.n_kv;
     if (fused) {
         hipExtLaunchKernelGGL((fused_kernel<D, KB, NC>), dim3((unsigned)(chains * J.tiles)), dim3(FW * 64), 0, s, ev.start, ev.stop, 0, J);
@@ -1295,7 +1320,11 @@ hipError_t launch(hipStream_t s, const Job &J, int rt, bool fused, LaunchEv ev) 
         hipExtLaunchKernelGGL((max_kernel<D, KB, D == 128 ? 2 : 4>), dim3((unsigned)(chains * ms * ((J.tiles + 3) / 4))), dim3(W * 64), 0, s, ev.start, nullptr, 0, J);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipExtLaunchKernelGGL((sum_kernel<D, KB, NC>), grid, dim3(W * 64), 0, s, nullptr, nullptr, 0, J);
+    constexpr int OCC = D == 64 && NC == 4 ? 3 : 2;
+    if (longw)
+        hipExtLaunchKernelGGL((sum_kernel<D, KB, NC, OCC>), grid, dim3(W * 64), 0, s, nullptr, nullptr, 0, J);
+    else
+        hipExtLaunchKernelGGL((sum_kernel<D, KB, NC, 2>), grid, dim3(W * 64), 0, s, nullptr, nullptr, 0, J);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipExtLaunchKernelGGL((combine_kernel<D>), dim3((unsigned)(chains * ((J.rows + CW - 1) / CW))), dim3(CW * 64), 0, s, nullptr, ev.stop, 0, J);
@@ -1346,7 +1375,7 @@ hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, dou
         const LaunchEv e{b == 0 ? ev.start : nullptr, b + p.seqs >= g.batch ? ev.stop : nullptr};
         hipError_t rc = hipErrorInvalidValue;
 #define INSITU_TREE_CASE(DD, KK, CC) \
-    if (g.d == DD && g.kb == KK && (g.vb <= 2 ? 4 : 8) == CC) rc = launch<DD, KK, CC>(s, J, (int)p.rt, p.fused, e);
+    if (g.d == DD && g.kb == KK && (g.vb <= 2 ? 4 : 8) == CC) rc = launch<DD, KK, CC>(s, J, (int)p.rt, p.fused, p.longw, e);
 #define INSITU_TREE_D(DD)                                                                              \
     INSITU_TREE_CASE(DD, 2, 4) INSITU_TREE_CASE(DD, 3, 4) INSITU_TREE_CASE(DD, 4, 4)                   \
     INSITU_TREE_CASE(DD, 2, 8) INSITU_TREE_CASE(DD, 3, 8) INSITU_TREE_CASE(DD, 4, 8)

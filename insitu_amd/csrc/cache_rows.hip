@@ -6,6 +6,9 @@
 // Both are copies, bound by memory: every byte of a row is read once, and once for all copies of it. A
 // lane takes 16 bytes of a destination plane, which in the narrower planes (8 and 4 bytes a row) are
 // the pieces of 2 or 4 rows, one load where those lie together in the source and one a row where not.
+// Measured: 8 copies of 32,768 rows (8 heads, 4b/2b, 123 MB with what is read) 25 us, 4.9 TB/s, as a large
+// copy; 14,003 of the last 30,001 rows at d = 128 12 us for 27 MB (every other row kept: the lines of the
+// others are read with it); 3 copies of 100 rows 5 us, a launch.
 #include "insitu_internal.h"
 
 namespace insitu {
@@ -78,7 +81,8 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(Geom s, Geom t, RowCopy 
 }
 
 // Up to 1,024 kept rows of a sequence's last n: a workgroup a (plane, KV head, sequence) reads them
-// all before it writes one, so that it may write where it reads.
+// all before it writes one, so that it may write where it reads (1,024 rows 4 to 7 us; more go through a
+// buffer, two launches a sequence: 1,025 rows of one sequence 15 us, of 16 sequences 200).
 __global__ void __launch_bounds__(1024) keep_rows_kernel(Geom g, RowKeep c) {
     const int p = blockIdx.x, h = blockIdx.y, z = blockIdx.z, b = c.seq0 + z;
     const int j = threadIdx.x, count = c.count[z];

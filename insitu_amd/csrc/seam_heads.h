@@ -12,7 +12,9 @@
 // What bounds it: memory, 8 bytes a channel (205 MB for 4,096 tokens of 48 heads of 128). So a lane takes
 // 8 channels of one head, two groups of 4 consecutive ones that pair up (16-byte loads and stores), a
 // head of 64 takes 8 lanes, and a sum over a head is 3 or 4 DPP steps. Heads and tokens are numbered
-// through, so that no lane idles whatever the head count.
+// through, so that no lane idles whatever the head count. 4,096 tokens of 48 heads of 128 with norms: 43.5 us,
+// 4.7 TB/s, the rate of a large copy; 777 tokens of 64, half interleaved, 8.4 us; one token 4.3, a launch. Rows
+// that are not 16-byte aligned, or a rotary_dim that is no multiple of 8, take single words: 80 us and 12 us.
 #pragma once
 
 #include "insitu_internal.h"
