@@ -92,7 +92,7 @@ class CompressedAttention:
             if host.shape and (np.any(host >= np.arange(host.shape[-1])) or np.any(host < -1)):
                 raise ValueError("a node's parent is an earlier node, or -1")
             parents = host
-        par = self.ctx.to_device(parents, torch.int32)
+        par = self.ctx.numbers(parents, -1, n)
         if tuple(par.shape) not in ((n,), (self.cache.batch, n)):
             raise ValueError(f"parents must be ({n},) or ({self.cache.batch}, {n}), got {tuple(par.shape)}")
         return par

@@ -165,11 +165,12 @@ class AttentionBlock:
         k = self.ctx.to_device(ki, torch.int32).reshape(self.batch, n, m.num_kv_heads, m.head_dim)
         v = self.ctx.to_device(vi, torch.int32).reshape(self.batch, n, m.num_kv_heads, m.head_dim)
         parents = self.attn.check_parents(parents, n)       # before the rows are written
-        qr = self.rotation.apply(q, self.ctx)
-        if self.rotation.rounds:
-            self.cache.append_wire(k, v) if self.batch > 1 else self.cache.append_wire(k[0], v[0], seq=0)
-        else:
-            self.cache.append_rotated(k, v) if self.batch > 1 else self.cache.append_rotated(k[0], v[0], seq=0)
+        with self.ctx.ordered(q, k, v, parents):
+            qr = self.rotation.apply(q, self.ctx)
+            if self.rotation.rounds:
+                self.cache.append_wire(k, v) if self.batch > 1 else self.cache.append_wire(k[0], v[0], seq=0)
+            else:
+                self.cache.append_rotated(k, v) if self.batch > 1 else self.cache.append_rotated(k[0], v[0], seq=0)
         out, self.last_stats = self.attn.attend_tree(qr, parents, self.softmax, stats=stats)
         return out.reshape(self.batch, n, m.num_heads * m.head_dim)
 
@@ -199,7 +200,8 @@ class AttentionBlock:
                 depth[i] = depth[p] + 1
         base = self.cache.length
         host = self.host
-        qi, ki, vi = host.wire(x, base + depth, counts=stats)
+        with self.ctx.ordered(x):
+            qi, ki, vi = host.wire(x, base + depth, counts=stats)
         self.taps = {"wire.q": qi, "wire.k": ki, "wire.v": vi}
         out = self.step_tree(qi[None], ki[None], vi[None], parents_dev, stats=stats)[0]
         self.taps["out"] = out
@@ -207,7 +209,9 @@ class AttentionBlock:
         if stats:
             report.saturated = host.last_saturated
             report.conversions = n * (m.num_heads + 2 * m.num_kv_heads) * m.head_dim
-        return host.output(out), report
+        with self.ctx.ordered(out):
+            y = host.output(out)
+        return y, report
 
     def accept(self, n: int, rows=None, *, counts=None) -> None:
         """After a draft of n nodes: of every sequence's, the listed rows stay (the taken path's nodes

@@ -365,12 +365,14 @@ class CompressedCache(KVCache):
             if isinstance(rows, (list, tuple)) and rows and isinstance(rows[0], (list, tuple, np.ndarray)):
                 if counts is None:
                     counts = [len(r) for r in rows]
+                elif len(counts) != len(rows) or any(c > len(r) for c, r in zip(counts, rows)):
+                    raise ValueError(f"counts {list(counts)} for lists of {[len(r) for r in rows]}")
                 wide = max(len(r) for r in rows)
                 rows = np.array([list(r) + [0] * (wide - len(r)) for r in rows], dtype=np.int64).reshape(len(rows), wide)
             rows = np.asarray(rows, dtype=np.int64)
             if rows.size and (rows.min() < 0 or rows.max() >= n):
                 raise ValueError(f"rows are numbers of the last {n} rows, 0 .. {n - 1}")
-        rows = self.ctx.to_device(rows, torch.int32)
+        rows = self.ctx.numbers(rows, 0, n)
         if rows.dim() not in (1, 2) or (rows.dim() == 2 and rows.shape[0] != lists):
             raise ValueError(f"rows must be (m,) or ({lists}, m), got {tuple(rows.shape)}")
         m = int(rows.shape[-1])

@@ -12,6 +12,10 @@ import math
 from dataclasses import dataclass
 
 
+class _Whole(int):
+    """A head's width as rotary_dim, where none was given."""
+
+
 @dataclass(frozen=True)
 class ModelConfig:
     """config.py:33-76: the attention shape, and the RoPE settings the host half uses."""
@@ -39,7 +43,8 @@ class ModelConfig:
                              f"Walsh-Hadamard butterfly")
         if d % 2:
             raise ValueError(f"head_dim={d} must be even")
-        r = d if self.rotary_dim is None else self.rotary_dim
+        # (dataclasses.replace hands the resolved value back: all of a head stays all of it)
+        r = _Whole(d) if self.rotary_dim is None or isinstance(self.rotary_dim, _Whole) else self.rotary_dim
         object.__setattr__(self, "rotary_dim", r)
         if r % 2 or not 2 <= r <= d:
             raise ValueError(f"rotary_dim={r} must be even, from 2 to head_dim={d}")

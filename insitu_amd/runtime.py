@@ -80,6 +80,13 @@ class Context:
             t = t.to(dtype)
         return t.contiguous()
 
+    def numbers(self, a, lo: int, hi: int):
+        """to_device(a, int32) of numbers of lo .. hi, without making such a number of one that is not."""
+        torch = _torch()
+        if isinstance(a, torch.Tensor) and (a.dtype == torch.int64 or a.is_floating_point()):
+            a = a.clamp(lo - 1, hi + 1)
+        return self.to_device(a, torch.int32)
+
 
 class _Ordered:
     def __init__(self, ctx: Context, tensors) -> None:

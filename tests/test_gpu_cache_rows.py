@@ -247,3 +247,29 @@ def test_refusals(ctx):
         with pytest.raises((_lib.InsituError, ValueError)):
             c.keep(kw.pop("n"), **kw)
     _same(c, imgs, [10, 20, 30, 40])
+
+
+def test_lists_shorter_than_their_counts(ctx):
+    from insitu_amd import _lib
+    lens = [10, 20, 30, 40]
+    c, imgs = _cache(ctx, FORMATS[0], 4, 64, lens)
+    for counts in ([2, 2], [1], [2, 1, 1]):
+        with pytest.raises(ValueError, match="counts"):
+            c.fork(3, [0, 1], n=5, rows=[[1, 2], [3]], counts=counts)
+    with pytest.raises(ValueError, match="counts"):
+        c.keep(5, [[0], [1, 2], [3], []], counts=[1, 1, 1, 1])
+    _same(c, imgs, lens)
+    c.fork(3, [0, 1], n=5, rows=[[1, 2], [3]], counts=[1, 1])
+    for b, r in ((0, 1), (1, 3)):
+        _take(c.layout(), imgs[b], 0, imgs[3], list(range(35)) + [35 + r], 8)
+        lens[b] = 36
+    _same(c, imgs, lens)
+
+
+def test_rows_past_32_bits(ctx):
+    import torch
+    lens = [30, 5]
+    c, imgs = _cache(ctx, FORMATS[0], 2, 64, lens)
+    c.fork(0, [1], n=20, rows=torch.tensor([(1 << 32) + 3, -(1 << 33), 7], device=ctx.torch_device))
+    _take(c.layout(), imgs[1], 0, imgs[0], list(range(10)) + [29, 10, 17], 8)
+    _same(c, imgs, [30, 13])

@@ -103,6 +103,35 @@ def test_forward_tree(ctx, softmax, form):
     assert torch.equal(ya, yb) and ra.context == 24
 
 
+def test_a_draft_on_another_stream(ctx):
+    """Hidden states made late on a stream that is not the block's; the outputs used there."""
+    import torch
+    m = _model()
+    a, b = _block(ctx, m), _block(ctx, m)
+    rng = np.random.default_rng(6)
+    x = torch.from_numpy(rng.standard_normal((len(PARENTS), 256)).astype(np.float32)).to(ctx.torch_device)
+    prompt = rng.standard_normal((30, 256)).astype(np.float32)
+    for blk in (a, b):
+        blk.forward(prompt)
+    want = a.forward_tree(x, PARENTS, stats=False)[0]
+    rows = [_wire(rng, 1, len(PARENTS), h) for h in (8, 2, 2)]
+    rows = [torch.as_tensor(np.asarray(r), dtype=torch.int32).to(ctx.torch_device) for r in rows]
+    a.accept(len(PARENTS), PATH)
+    want_step = a.step_tree(*rows, PARENTS, stats=False)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream(ctx.torch_device)
+    with torch.cuda.stream(side):
+        big = torch.randn(2048, 2048, device=ctx.torch_device)
+        for _ in range(20):
+            big = big @ big * 1e-3
+        zero = (big[0, 0] * 0).nan_to_num()
+        got = b.forward_tree(x + zero, PARENTS, stats=False)[0] + 0
+        b.accept(len(PARENTS), PATH)
+        got_step = b.step_tree(*(r + zero.to(torch.int32) for r in rows), PARENTS, stats=False) + 0
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(got_step, want_step)
+
+
 def test_branches_become_sequences(ctx):
     """Two branches of a draft go on as sequences of their own, each as if only its path had been decoded."""
     m = _model()

@@ -284,6 +284,21 @@ def test_bad_parents_on_the_device_count_as_roots(ctx):
         assert st.range_errors == 3
 
 
+def test_bad_parents_past_32_bits(ctx):
+    """A device tensor of 64-bit numbers: 2^32 + 1 is no node 1."""
+    import torch
+    from insitu_amd.attention import CompressedAttention
+    fmt, T, n = FORMATS[0], 40, 4
+    rng = np.random.default_rng(16)
+    c = _cache(ctx, fmt, [T])
+    hosts, f = _fill(c, fmt, [T], *(_draw(rng, 65536, 1, T, N_KV, 64) for _ in "kv"))
+    q = _draw(rng, 1 << 14, 1, n, N_KV * 4, 64)
+    bad = torch.tensor([-1, 0, (1 << 32) + 1, -(1 << 32)], device=ctx.torch_device)
+    out, st = CompressedAttention(c).attend_tree(q, bad)
+    _check(out.cpu().numpy(), None, q, hosts, f, 4, [T], np.array([[-1, 0, -1, -1]]), n, "online")
+    assert st.range_errors == 2
+
+
 def test_repeated_and_other_shapes_between(ctx):
     """The scratch is shared by calls of all shapes: results do not depend on what ran before."""
     from insitu_amd.attention import CompressedAttention

@@ -99,3 +99,15 @@ def test_from_hf_reads_the_forms():
 def test_model_config_refuses(kw):
     with pytest.raises(ValueError):
         ModelConfig(hidden_size=256, num_heads=4, num_kv_heads=2, **kw)
+
+
+def test_a_replaced_head_is_rotated_whole():
+    import dataclasses
+    from insitu_amd import ModelConfig
+    m = ModelConfig(hidden_size=256, num_heads=4, num_kv_heads=2)
+    for d in (32, 128):
+        r = dataclasses.replace(m, head_dim=d)
+        assert r.rotary_dim == d and dataclasses.replace(r, head_dim=64).rotary_dim == 64
+    part = dataclasses.replace(m, rotary_dim=32)
+    assert dataclasses.replace(part, head_dim=128).rotary_dim == 32
+    assert dataclasses.replace(part, rotary_dim=None).rotary_dim == 64 and m == dataclasses.replace(m)
