@@ -534,11 +534,12 @@ struct Runs {
     int32_t *S, *S_l;
     uint32_t *pool;
     int near;
-    __device__ __forceinline__ Runs(const Job &J, const Place &p, uint4 *ml, int32_t *sl, int n) : meta_l(ml), S_l(sl), near(n) {
+    __device__ __forceinline__ Runs(const Job &J, const Place &p, uint4 *ml, int32_t *sl, int n, uint32_t *pl = nullptr)
+        : meta_l(ml), S_l(sl), near(n) {
         const int64_t tl = (int64_t)p.chain * J.tiles + p.tile, run0 = tl * (16 * (int64_t)J.nspan + J.extra);
         meta = J.sc.meta + run0;
         S = J.sc.S + run0 * D;
-        pool = J.sc.pool + tl;
+        pool = LDS ? pl : J.sc.pool + tl;
     }
     // lane = (row, 4 channels of each 16), as the walk holds them
     __device__ __forceinline__ void put(int slot, const uint4 &m, const v4i (&acc)[D / 16], bool used) const {
@@ -1101,7 +1102,7 @@ __global__ void __launch_bounds__(FW * 64, 2) fused_kernel(Job J) {
     __shared__ int16_t at[TREE_NODES];
     __shared__ uint16_t lut_s[LUT_N + 7];
     __shared__ int32_t top_s[FW][16];
-    __shared__ uint32_t bad_s, ev_s[FW][16];
+    __shared__ uint32_t bad_s, pool_s, ev_s[FW][16];
     __shared__ Tally tally;
     constexpr int NEAR = D == 64 ? 192 : 160;
     __shared__ union {
@@ -1125,13 +1126,13 @@ __global__ void __launch_bounds__(FW * 64, 2) fused_kernel(Job J) {
     if (p.lo < p.hi) next.load(hb, nb, J.g.span, p.lo);
     const ValueTable<NC> values(J);
     Q.digest(J, p.tile, J.count && p.s == 0 ? &J.st->range_errors : nullptr);
-    const Runs<D, true> runs(J, p, u.r.meta, u.r.S[0], NEAR);
+    const Runs<D, true> runs(J, p, u.r.meta, u.r.S[0], NEAR, &pool_s);
     dgs.fill(start.c);
     start.lut(lut_s);
     if (tid == 0) {
         bad_s = 0;
         tally.clear();
-        *runs.pool = 0;
+        pool_s = 0;
     }
     const int none = tree_paths(start.parent, J.n, up, at);
     if (J.count && none && p.kvh == 0 && p.tile == 0) atomicAdd(&J.st->range_errors, (unsigned long long)none);
