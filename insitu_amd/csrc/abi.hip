@@ -1149,7 +1149,7 @@ int insitu_attend_tree(insitu_cache *k, int32_t n, const int32_t *parents, int32
     rc = timing_events(k->ctx, &ev);
     if (rc) return rc;
     if (fast)
-        HIP_TRY(launch_attend_tree(k->ctx->stream, k->g, k->tabs, k->tabs_host.kc_absmax, q, out, len, parents, pstride, n, longest, two_pass,
+        HIP_TRY(launch_attend_tree(k->ctx->stream, k->g, k->tabs, k->tabs_host, q, out, len, parents, pstride, n, longest, two_pass,
                                    stats != nullptr, k->tree_scr, k->tree_bytes, ev, k->stats),
                 "tree attend launch");
     else

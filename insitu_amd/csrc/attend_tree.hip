@@ -36,7 +36,7 @@
 // tokens a step, storing the scores between the launches, one launch for long contexts, signed codebooks halved by
 // symmetry, two or four tokens' tiles sharing one-hot codes at d = 128 (registers), four waves a SIMD.
 #include <algorithm>
-#include <cstdlib>
+#include <cmath>
 #include <type_traits>
 
 #include "digits.h"
@@ -86,7 +86,8 @@ struct Job {
     int32_t n, rows, tiles, span, nspan, mspan, nms;   // mspan, nms: max_kernel's spans, whole parts of the others
     int32_t extra, two, seq0, nseq, count;             // count: gather statistics
     int64_t longest;
-    double kc_absmax;
+    double kc_absmax, vcs[8], vcmax;                   // ValueTable's, and its wide and delta_max
+    uint32_t wide, delta_max;
     Scratch sc;
     DevStats *st;
 };
@@ -362,15 +363,9 @@ template <int NC>
 struct ValueTable {
     double vcs[NC], vcmax;
     uint32_t wide, delta_max;                          // wide: |v_norm p| up to which a term is two balanced bytes
-    __device__ __forceinline__ explicit ValueTable(const Job &J) {
-        vcmax = 0.0;
+    __device__ __forceinline__ explicit ValueTable(const Job &J) : vcmax(J.vcmax), wide(J.wide), delta_max(J.delta_max) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            vcs[i] = __longlong_as_double(uni64(__double_as_longlong(i < (1 << J.g.vb) ? (double)J.tabs->vc[i] * 0x1p-23 : 0.0)));
-            vcmax = fmax(vcmax, fabs(vcs[i]));
-        }
-        wide = (uint32_t)uni32((int)(uint32_t)(32639.0 / fmax(vcmax, 0x1p-16)));
-        delta_max = (uint32_t)J.tabs->delta_max;
+        for (int i = 0; i < NC; ++i) vcs[i] = J.vcs[i];
     }
 };
 
@@ -1343,7 +1338,7 @@ size_t tree_scratch_bytes(const Geom &g, int64_t n, int64_t longest) {
     return tr::carve(g, p, nullptr, nullptr);
 }
 
-hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, double kc_absmax, const int32_t *q, int32_t *out,
+hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, const Tables &host, const int32_t *q, int32_t *out,
                               const int64_t *len, const int32_t *parents, int64_t pstride, int32_t n, int64_t longest,
                               int two_pass, bool count, void *scratch, size_t scratch_bytes, LaunchEv ev, DevStats *st) {
     using namespace tr;
@@ -1368,7 +1363,13 @@ hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, dou
     J.two = two_pass;
     J.count = count;
     J.longest = longest;
-    J.kc_absmax = kc_absmax;
+    J.kc_absmax = host.kc_absmax;
+    for (int i = 0; i < 1 << g.vb; ++i) {
+        J.vcs[i] = (double)host.vc[i] * 0x1p-23;
+        J.vcmax = std::fmax(J.vcmax, std::fabs(J.vcs[i]));
+    }
+    J.wide = (uint32_t)(32639.0 / std::fmax(J.vcmax, 0x1p-16));
+    J.delta_max = (uint32_t)host.delta_max;
     J.st = st;
     for (int64_t b = 0; b < g.batch; b += p.seqs) {
         J.seq0 = (int32_t)b;

@@ -371,7 +371,7 @@ hipError_t launch_keep_rows(hipStream_t s, const Geom &g, const RowKeep &c, int 
 constexpr int TREE_NODES = 256;
 bool tree_supported(const Geom &g);
 size_t tree_scratch_bytes(const Geom &g, int64_t n, int64_t longest);
-hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, double kc_absmax, const int32_t *q, int32_t *out,
+hipError_t launch_attend_tree(hipStream_t s, const Geom &g, const Tables *t, const Tables &host, const int32_t *q, int32_t *out,
                               const int64_t *len, const int32_t *parents, int64_t pstride, int32_t n, int64_t longest,
                               int two_pass, bool count, void *scratch, size_t scratch_bytes, LaunchEv ev, DevStats *st);
 // The same token by token, any format.
