@@ -27,12 +27,12 @@
 // three steps follow each other behind barriers, the runs mostly in shared memory.
 //
 // What bounds it. Memory does not: 32 nodes of 4 heads behind 8 x 32,768 tokens read 218 MB, 46 us at the rate of a
-// copy, and take 1,850 us. The integers do: a token and row of d = 128 with 3-bit values costs 66 matrix
-// instructions a 16 x 16 tile (24 % of the walk's cycles) and 530 vector ones, which fill 64 % of the issue slots:
+// copy, and take 1,770 us. The integers do: a tile of 16 x 16 at d = 128 with 3-bit values costs 66 matrix
+// instructions (24 % of the walk's cycles) and 510 vector ones, which fill 64 % of the issue slots:
 // the keys' digits, the scores' carries in 64 bits, the terms in float64 for every value code (exact: 53 bits), their
 // digits' bytes and the one-hot codes. So the tile's terms use two digits where they fit, no tile is walked whose
 // weights are all zero, and max_kernel's row tiles share the expanded keys. Measured kernels: 26 nodes behind 32,768
-// tokens (4b/2b, 32 heads) 40 + 67 + 13 us, 64 nodes behind 4,097 two-pass 16 + 38 + 5 us; tried and slower: 32
+// tokens (4b/2b, 32 heads) 39 + 66 + 13 us, 64 nodes behind 4,097 two-pass 16 + 38 + 6 us; tried and slower: 32
 // tokens a step, storing the scores between the launches, one launch for long contexts, signed codebooks halved by
 // symmetry, two or four tokens' tiles sharing one-hot codes at d = 128 (registers), four waves a SIMD.
 #include <algorithm>
@@ -1087,8 +1087,8 @@ __global__ void __launch_bounds__(CW * 64) combine_kernel(Job J) {
     if (tid == 0) tally.post(J, part == 0 && p.kvh == 0, p.T);
 }
 
-// All of it in one launch, where the spans are a workgroup's waves (20 us for 5 nodes behind 100 tokens, a chain of
-// round trips: tables and queries 4, maxima 1, walk 6, runs 5; the rest launch and end).
+// All of it in one launch, where the spans are a workgroup's waves (19 us for 5 nodes behind 100 tokens, a chain of
+// waits: tables and queries 4, maxima 1, walk 6, runs 5; the rest launch and end).
 constexpr int FW = 8;
 template <int D, int KB, int NC>
 __global__ void __launch_bounds__(FW * 64, 2) fused_kernel(Job J) {
