@@ -202,7 +202,8 @@ int insitu_attend_causal_head(insitu_cache *cache, int32_t seq, int32_t kv_head,
  * (SEQUENTIAL and SPLIT, or TWO_PASS; SERIAL token by token). n is 1 .. 256. parents_dev int32 (n),
  * or (batch, n) with per_sequence = 1: the parent's number, or -1 for a child of the context; any
  * other value counts as -1 and as a range error (statistics). q_rot_dev int32 (batch, n, n_q_heads,
- * d) rotated; out_dev int32, the same shape, Q16. EBADLEN when a sequence holds fewer than n rows.
+ * d) rotated; out_dev int32, the same shape, Q16 (q_rot_dev itself may be given). EBADLEN when a
+ * sequence holds fewer than n rows.
  * stats_host may be NULL: then nothing synchronises, and once a call of the shape has allocated the
  * cache's scratch nothing allocates either, so that such a call may be captured into a graph. Its
  * replays are for the lengths of the capture (changed ones are cut to n .. the longest of these), and

@@ -299,6 +299,31 @@ def test_bad_parents_past_32_bits(ctx):
     assert st.range_errors == 2
 
 
+@pytest.mark.parametrize("T", [90, 1300])
+def test_unaligned_tensors_and_in_place(ctx, T):
+    """Queries, parents and outputs 4 bytes behind a boundary; outputs over the queries."""
+    import torch
+    from insitu_amd.attention import CompressedAttention
+    fmt, n = FORMATS[5], 11
+    rng = np.random.default_rng(17)
+    c = _cache(ctx, fmt, [T, T - 30])
+    _fill(c, fmt, [T, T - 30], *(_draw(rng, 65536, 2, T, N_KV, 128) for _ in "kv"))
+    q = torch.from_numpy(_draw(rng, 1 << 14, 2, n, N_KV * 4, 128).astype(np.int32)).to(ctx.torch_device)
+    q[1, 3, 2, 5] = (1 << 23) + 9                       # (a row of the token-by-token path)
+    par = torch.from_numpy(_tree("random", n, rng).astype(np.int32)).to(ctx.torch_device)
+    a = CompressedAttention(c)
+
+    def behind(t):
+        b = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+        return b.copy_(t)
+    for mode in ("online", "two_pass", "serial"):
+        want = a.attend_tree(q, par, mode, stats=False)[0]
+        out = behind(torch.zeros_like(q))
+        assert a.attend_tree(behind(q), behind(par), mode, out=out, stats=False)[0] is out and torch.equal(out, want)
+        x = q.clone()
+        assert torch.equal(a.attend_tree(x, par, mode, out=x, stats=False)[0], want)
+
+
 def test_repeated_and_other_shapes_between(ctx):
     """The scratch is shared by calls of all shapes: results do not depend on what ran before."""
     from insitu_amd.attention import CompressedAttention
