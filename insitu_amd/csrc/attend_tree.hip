@@ -588,7 +588,7 @@ __device__ __forceinline__ uint32_t walk(const Job &J, const Place &p, const Que
     uint32_t wmax = 0;                                 // the largest |v_norm p|
     uint32_t n_ev = 0;                                 // the lane's events
     bool bad = Q.bad;
-    int slot = p.s * 16 + col;                         // the row's open run, and its factor
+    int slot = p.s * 16 + col;                         // the row's open run (-1: none was left), and its factor
     uint32_t fopen = 1u << PROB_FRAC;
 
     auto lut = [&](uint32_t d) __attribute__((always_inline)) -> uint32_t {
@@ -604,19 +604,21 @@ __device__ __forceinline__ uint32_t walk(const Job &J, const Place &p, const Que
         float b = bs;
         b += __shfl_xor(b, 16);
         b += __shfl_xor(b, 32);
-        if (!has) return;
+        if (!has || slot < 0) return;
         const bool used = L != 0 || fopen != 1u << PROB_FRAC;
         const uint4 mt = make_uint4(L, fopen | (used ? USED : 0u), (uint32_t)next,
                                     __float_as_uint(b * (float)vcmax * 1.001f + (float)J.span));
         runs.put(slot, mt, acc, used);
     };
-    // the run of the rows where `has` ends, and one with factor f begins
+    // the run of the rows where `has` ends, and one with factor f begins. A row for which none is left goes token
+    // by token and writes no more: every record is another row's, whose chain has to hold
     auto next_run = [&](bool has, uint32_t f) __attribute__((always_inline)) {
         int to = 0;
         if (has && grp == 0) to = (int)atomicAdd(runs.pool, 1u);
         to = __shfl(to, col);
-        bad = bad || (has && to >= J.extra);
-        to = 16 * J.nspan + imin(to, J.extra - 1);
+        const bool none = to >= J.extra;
+        bad = bad || (has && none);
+        to = none ? -1 : 16 * J.nspan + to;
         hand_over(has, to);
         if (has) {
             slot = to;
