@@ -152,7 +152,9 @@ int insitu_cache_set_length(insitu_cache *cache, int32_t seq, int64_t len);
 int insitu_cache_layout(const insitu_cache *cache, insitu_layout *out);
 
 /* append_rotated (compressed.py:64-86): encode, pack and write n_tok rows at
- * each sequence's length. k/v_rot_dev int32 (batch, n_tok, n_kv_heads, d). */
+ * each sequence's length. k/v_rot_dev int32 (batch, n_tok, n_kv_heads, d). Appends and steps are
+ * not for graph capture: the lengths they read lie in one of two arrays in turn, and a graph would
+ * keep the one of its capture. */
 int insitu_append(insitu_cache *cache, const int32_t *k_rot_dev, const int32_t *v_rot_dev,
                   int32_t n_tok);
 /* The same for one sequence: k/v_rot_dev int32 (n_tok, n_kv_heads, d). */
@@ -206,7 +208,7 @@ int insitu_attend_causal_head(insitu_cache *cache, int32_t seq, int32_t kv_head,
  * sequence holds fewer than n rows.
  * stats_host may be NULL: then nothing synchronises, and once a call of the shape has allocated the
  * cache's scratch nothing allocates either, so that such a call may be captured into a graph. Its
- * replays are for the lengths of the capture (changed ones are cut to n .. the longest of these), and
+ * replays attend the lengths that the cache has by then, cut to n .. the longest of the capture, and
  * share the scratch: one at a time, in order with the cache's other calls. */
 int insitu_attend_tree(insitu_cache *cache, int32_t n, const int32_t *parents_dev, int32_t per_sequence,
                        const int32_t *q_rot_dev, int32_t *out_dev, int32_t mode, insitu_stats *stats_host);
@@ -315,7 +317,10 @@ int insitu_load_rows(insitu_cache *cache, int32_t seq, int32_t head, int64_t t0,
  * a value outside is taken as the nearest one inside). rows_stride 0: one list for all. The
  * destinations are different sequences, none of them a source. Rows behind the new length stay as
  * they are. Stream-ordered; nothing synchronises. In a graph, this and insitu_cache_keep repeat what
- * they did, with the lengths of the capture and what rows_dev holds by then. */
+ * they did, with the lengths of the capture and what rows_dev holds by then: they begin at the lengths
+ * that the sequences had then, and every later call finds the ones they set. The host's copy
+ * (insitu_cache_length, and what calls check) follows the capture, no replay: where it differs,
+ * insitu_cache_set_length before the next call that is not a replay brings it in line. */
 int insitu_cache_fork(insitu_cache *cache, int32_t n_copies, const int32_t *src_host, const int32_t *dst_host,
                       int64_t n, const int32_t *rows_dev, int64_t rows_stride, const int64_t *counts_host);
 /* Of the last n rows of every sequence, the listed ones (as insitu_cache_fork's lists, a list a

@@ -175,6 +175,9 @@ struct insitu_cache {
     int64_t total_bytes = 0;
     int64_t *len_dev[2] = {nullptr, nullptr};
     int cur = 0;
+    // the lengths once more, always here: what a call that may be captured reads. (Appends and steps read one
+    // half of the double buffer and write the other, and which is which changes with each of them.)
+    int64_t *len_now = nullptr;
     std::vector<int64_t> len_host;
     DevStats *stats = nullptr;
     int32_t *wire_scratch = nullptr;      // insitu_step: the rotated queries
@@ -245,6 +248,14 @@ int zero_stats(insitu_cache *c) {
                        (unsigned long long *)c->stats, (int)(sizeof(DevStats) / 8));
     HIP_TRY(hipGetLastError(), "zero stats");
     return INSITU_OK;
+}
+
+// All of a cache's length arrays, for the calls that set lengths: a replay of one finds either half of the double
+// buffer current.
+void length_arrays(const insitu_cache *k, int64_t *(&len)[LEN_ARRAYS]) {
+    len[0] = k->len_dev[0];
+    len[1] = k->len_dev[1];
+    len[2] = k->len_now;
 }
 
 // A buffer of the cache, grown to twice its size at least. The old one stays allocated until the cache goes:
@@ -569,9 +580,9 @@ int insitu_cache_create(insitu_ctx *c, const insitu_cache_desc *desc, insitu_cac
     if (e == hipSuccess) e = hipMalloc(&k->tabs, sizeof(Tables));
     if (e == hipSuccess)
         e = hipMemcpyAsync(k->tabs, &t, sizeof(Tables), hipMemcpyHostToDevice, c->stream);
-    for (int i = 0; i < 2 && e == hipSuccess; ++i) {
-        e = hipMalloc(&k->len_dev[i], sizeof(int64_t) * g.batch);
-        if (e == hipSuccess) e = hipMemsetAsync(k->len_dev[i], 0, sizeof(int64_t) * g.batch, c->stream);
+    for (int64_t **p : {&k->len_dev[0], &k->len_dev[1], &k->len_now}) {
+        if (e == hipSuccess) e = hipMalloc(p, sizeof(int64_t) * g.batch);
+        if (e == hipSuccess) e = hipMemsetAsync(*p, 0, sizeof(int64_t) * g.batch, c->stream);
     }
     if (e == hipSuccess) e = hipMalloc(&k->stats, sizeof(DevStats));
     if (e == hipSuccess) e = hipMemsetAsync(k->stats, 0, sizeof(DevStats), c->stream);
@@ -635,7 +646,7 @@ int insitu_cache_destroy(insitu_cache *k) {
     hipStreamSynchronize(k->ctx->stream);
     if (k->base) hipFree(k->base);
     if (k->tabs) hipFree(k->tabs);
-    for (auto *p : k->len_dev)
+    for (auto *p : {k->len_dev[0], k->len_dev[1], k->len_now})
         if (p) hipFree(p);
     if (k->stats) hipFree(k->stats);
     if (k->wire_scratch) hipFree(k->wire_scratch);
@@ -652,7 +663,7 @@ int insitu_cache_destroy(insitu_cache *k) {
 int insitu_cache_reset(insitu_cache *k) {
     if (!k) return fail(INSITU_EINVAL, "cache is NULL");
     HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
-    for (auto *p : k->len_dev)
+    for (auto *p : {k->len_dev[0], k->len_dev[1], k->len_now})
         HIP_TRY(hipMemsetAsync(p, 0, sizeof(int64_t) * k->g.batch, k->ctx->stream), "reset");
     HIP_TRY(hipStreamSynchronize(k->ctx->stream), "sync");
     k->len_host.assign(k->g.batch, 0);
@@ -672,9 +683,9 @@ int insitu_cache_set_length(insitu_cache *k, int32_t seq, int64_t len) {
     if (len < 0 || len > k->g.capacity) return fail(INSITU_ECAPACITY, "length beyond capacity");
     HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
     k->len_host[seq] = len;
-    HIP_TRY(hipMemcpyAsync(k->len_dev[k->cur] + seq, &k->len_host[seq], sizeof(int64_t),
-                           hipMemcpyHostToDevice, k->ctx->stream),
-            "length upload");
+    for (auto *p : {k->len_dev[k->cur], k->len_now})
+        HIP_TRY(hipMemcpyAsync(p + seq, &k->len_host[seq], sizeof(int64_t), hipMemcpyHostToDevice, k->ctx->stream),
+                "length upload");
     HIP_TRY(hipStreamSynchronize(k->ctx->stream), "sync");
     return INSITU_OK;
 }
@@ -711,7 +722,7 @@ static int append_impl(insitu_cache *k, int seq_lo, int seq_hi, const int32_t *k
         }
     HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
     HIP_TRY(launch_append(k->ctx->stream, k->g, k->tabs, kr, vr, n_tok, seq_lo, seq_hi,
-                          k->len_dev[k->cur], k->len_dev[k->cur ^ 1], k->stats,
+                          k->len_dev[k->cur], k->len_dev[k->cur ^ 1], k->len_now, k->stats,
                           wire ? k->desc.fmt.rot_rounds : 0, wire ? k->desc.fmt.rot_signs : nullptr,
                           k->tabs_host, k->append_path),
             "append launch");
@@ -1137,7 +1148,7 @@ int insitu_attend_tree(insitu_cache *k, int32_t n, const int32_t *parents, int32
     HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
     int rc = stats ? zero_stats(k) : INSITU_OK;
     if (rc) return rc;
-    const int64_t *len = k->len_dev[k->cur];
+    const int64_t *len = k->len_now;
     const int64_t pstride = per_sequence ? n : 0;
     const int two_pass = mode == INSITU_TWO_PASS ? 1 : 0;
     const bool fast = mode != INSITU_SERIAL && tree_supported(k->g);
@@ -1181,7 +1192,7 @@ int insitu_cache_fork(insitu_cache *k, int32_t n_copies, const int32_t *src, con
     c.rows = n ? rows : nullptr;
     c.rows_stride = rows_stride;
     c.n = n;
-    c.len = k->len_dev[k->cur];
+    length_arrays(k, c.len);
     // copies of one source that take the same rows are one group: its rows are read once
     int groups = 0, at = 0;
     auto flush = [&]() -> int {
@@ -1229,7 +1240,6 @@ int insitu_cache_keep(insitu_cache *k, int64_t n, const int32_t *rows, int64_t r
     if (!n) return INSITU_OK;
     HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
     const hipStream_t s = k->ctx->stream;
-    int64_t *len = k->len_dev[k->cur];
     if (most <= KEEP_ROWS) {
         for (int b0 = 0; b0 < g.batch; b0 += KEEP_MAX) {
             const int nb = g.batch - b0 < KEEP_MAX ? g.batch - b0 : KEEP_MAX;
@@ -1242,7 +1252,7 @@ int insitu_cache_keep(insitu_cache *k, int64_t n, const int32_t *rows, int64_t r
             c.rows_stride = rows_stride;
             c.n = (int32_t)n;
             c.seq0 = b0;
-            c.len = len;
+            length_arrays(k, c.len);
             HIP_TRY(launch_keep_rows(s, g, c, nb, (int)most), "keep launch");
         }
     } else {
@@ -1271,7 +1281,7 @@ int insitu_cache_keep(insitu_cache *k, int64_t n, const int32_t *rows, int64_t r
             d.first[1] = 1;
             d.begin[0] = d.head[0] = base;
             d.end[0] = base + count;
-            d.len = len;
+            length_arrays(k, d.len);
             // (row r >= head of the cache is row r - head of the buffer)
             HIP_TRY(launch_copy_rows(s, t, g, d, 1), "keep launch");
         }
@@ -1314,6 +1324,7 @@ int insitu_step(insitu_cache *k, const int32_t *q, const int32_t *kw, const int3
         si.sg = rot_signs(k->desc.fmt.rot_rounds, k->desc.fmt.rot_signs);
         si.rounds = k->desc.fmt.rot_rounds;
         si.len_out = k->len_dev[k->cur ^ 1];
+        si.len_now = k->len_now;
         rc = attend_impl(k, qr, out, mode, false, &si);
         if (rc) return rc;
         k->cur ^= 1;
@@ -1333,7 +1344,7 @@ int insitu_step(insitu_cache *k, const int32_t *q, const int32_t *kw, const int3
     }
     HIP_TRY(launch_step_write(k->ctx->stream, g, k->tabs, q, kw, vw, k->desc.fmt.rot_rounds,
                               k->desc.fmt.rot_signs, qr, qd, qok, k->len_dev[k->cur],
-                              k->len_dev[k->cur ^ 1], k->stats),
+                              k->len_dev[k->cur ^ 1], k->len_now, k->stats),
             "step write launch");
     k->cur ^= 1;
     for (int b = 0; b < g.batch; ++b) k->len_host[b] += 1;

@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(CT, SEQ && D > 64 ? 4 : 2) chunk_kernel(Geom g
     const int64_t nch = T > 0 ? (T + CHUNK - 1) / CHUNK : 1;
     const bool has_work = chunk < nch;
     const bool new_row = STEP && chunk == nch - 1;     // this chunk holds the step's new token
-    if (STEP && chunk == 0 && kvh == 0 && tid == 0) si.len_out[b] = T;
+    if (STEP && chunk == 0 && kvh == 0 && tid == 0) si.len_out[b] = si.len_now[b] = T;
     const int nv = 1 << g.vb;
     const int acc_shift = CENT_FRAC + g.norm_frac + PROB_FRAC - ACC_FRAC;
     const int score_shift = CENT_FRAC + g.norm_frac;

@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(SC_NT, 1) scan_kernel(ScanArgs a) {
     // 0 .. G - 1) drain that counter: writes that are on no chain are made by the
     // last wave instead.
     const bool side = tid == SC_NT - 64;
-    if (STEP && chunk == 0 && kvh == 0 && side) a.si.len_out[b] = T;
+    if (STEP && chunk == 0 && kvh == 0 && side) a.si.len_out[b] = a.si.len_now[b] = T;
     const int64_t t0 = (int64_t)chunk * SC_CHUNK;
     const int64_t t = t0 + tid;
     const bool in = t < T;

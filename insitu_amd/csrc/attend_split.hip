@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(W * 64) score_max_kernel(Geom g, const Tables 
     const int nblk = (int)((T + BT - 1) / BT);
     if (x > 0 && 4 * r * x >= nblk) return;
     const bool owner = STEP && x == (nblk - 1) / (4 * r);        // this workgroup holds the new token
-    if (STEP && x == 0 && kvh == 0 && tid == 0) si.len_out[b] = T;
+    if (STEP && x == 0 && kvh == 0 && tid == 0) si.len_out[b] = si.len_now[b] = T;
 
     // -- the small loads, then the first block's rows -----------------------------------------
     const int64_t kc_t = tid < (1 << g.kb) ? tabs->kc[tid] : 0;

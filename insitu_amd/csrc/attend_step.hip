@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(NT, 1) step_kernel(Geom g, const Tables *__res
     // would only take issue slots from the waves that share its SIMD) and leaves neutral
     // entries in LDS; it still takes every barrier and its share of the walk.
     const bool wlive = t0 + 64 * wv < T;
-    if (own && kvh == 0 && tid == 0) si.len_out[b] = T;
+    if (own && kvh == 0 && tid == 0) si.len_out[b] = si.len_now[b] = T;
     // a KV head seen as several chains: every one encodes the new row and stores the same words, the
     // first one counts its range errors
     // (4-bit keys come in chains of their own: step_supported)

@@ -28,8 +28,8 @@ constexpr int UNITS = 4;       // 16-byte units a lane, their loads in flight to
 
 __global__ void __launch_bounds__(256) copy_rows_kernel(Geom s, Geom t, RowCopy c) {
     const int z = blockIdx.z, p = blockIdx.y % s.n_planes, h = blockIdx.y / s.n_planes;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && c.len && threadIdx.x < (unsigned)(c.first[z + 1] - c.first[z]))
-        c.len[c.dst[c.first[z] + threadIdx.x]] = c.end[z];
+    if (blockIdx.x == 0 && blockIdx.y == 0 && c.len[0] && threadIdx.x < (unsigned)(c.first[z + 1] - c.first[z]))
+        for (int64_t *len : c.len) len[c.dst[c.first[z] + threadIdx.x]] = c.end[z];
     const int w = s.plane_w[p], per = 16 / w;
     const int64_t begin = c.begin[z], end = c.end[z];
     const int64_t u0 = begin / per, u1 = (end + per - 1) / per;
@@ -87,7 +87,8 @@ __global__ void __launch_bounds__(1024) keep_rows_kernel(Geom g, RowKeep c) {
     const int p = blockIdx.x, h = blockIdx.y, z = blockIdx.z, b = c.seq0 + z;
     const int j = threadIdx.x, count = c.count[z];
     const int64_t base = c.base[z];
-    if (p == 0 && h == 0 && j == 0) c.len[b] = base + count;
+    if (p == 0 && h == 0 && j == 0)
+        for (int64_t *len : c.len) len[b] = base + count;
     const int w = g.plane_w[p];
     uint8_t *rows = plane_ptr(g, b, h, p) + base * w;
     int i = j < count ? c.rows[(int64_t)b * c.rows_stride + j] : 0;

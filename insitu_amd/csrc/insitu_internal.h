@@ -80,12 +80,12 @@ inline RotSigns rot_signs(int rounds, const uint64_t (*signs)[2]) {
 
 // The fused decode step's inputs to the chunked attend: the wire rows (batch,
 // heads, d) in Q8.16, the rotation, and the other half of the length double
-// buffer, which receives len + 1.
+// buffer, which receives len + 1, as len_now does.
 struct StepIn {
     const int32_t *qw, *kw, *vw;
     RotSigns sg;
     int32_t rounds;
-    int64_t *len_out;
+    int64_t *len_out, *len_now;
 };
 
 // Device statistics; merged with atomics (AttentionStats.merge semantics).
@@ -203,7 +203,7 @@ hipError_t launch_finalize(hipStream_t s, const int64_t *acc, const int64_t *l, 
 // the kernel, 0 automatic, 1 the lane-per-channel one, 2 lane = row where it handles the format.
 hipError_t launch_append(hipStream_t s, const Geom &g, const Tables *t, const int32_t *k,
                          const int32_t *v, int n_tok, int seq_lo, int seq_hi, const int64_t *len_in,
-                         int64_t *len_out, DevStats *st, int rounds, const uint64_t (*signs)[2],
+                         int64_t *len_out, int64_t *len_now, DevStats *st, int rounds, const uint64_t (*signs)[2],
                          const Tables &host_tabs, int path);
 bool chunked_supported(const Geom &g, int64_t capacity);
 int64_t chunked_max_chunks(int64_t capacity);
@@ -320,7 +320,7 @@ hipError_t launch_step(hipStream_t s, const Geom &g, const Tables *t, int32_t *o
 hipError_t launch_step_write(hipStream_t s, const Geom &g, const Tables *t, const int32_t *qw,
                              const int32_t *kw, const int32_t *vw, int rounds,
                              const uint64_t (*signs)[2], int32_t *qr, double *qd, int32_t *qok,
-                             const int64_t *len_in, int64_t *len_out, DevStats *st);
+                             const int64_t *len_in, int64_t *len_out, int64_t *len_now, DevStats *st);
 // The two-pass attend in two launches (attend_split.hip): one query a sequence, or with step the whole
 // decode step (len the lengths before it); longest: the longest sequence, the new token included.
 bool split_supported(const Geom &g, const Tables &host_tabs, int64_t capacity);
@@ -342,18 +342,19 @@ hipError_t launch_attend_serial(hipStream_t s, const Geom &g, const Tables *t, c
 // Rows between sequences (cache_rows.hip), as group z of a launch: rows [begin, end) of the sequences
 // dst[first[z]] .. dst[first[z + 1] - 1] of one geometry from those of sequence src of another. Row r < head
 // comes from row r; row head + j from row add + j or, with rows, add + rows[rows_at * rows_stride + j] (a
-// device list of values below n). len (may be null) receives end for every dst.
+// device list of values below n). The arrays len (the first null: none) receive end for every dst.
+constexpr int LEN_ARRAYS = 3;            // a cache's length arrays: the double buffer and len_now (abi.hip)
 constexpr int COPY_MAX = 32;             // destinations a launch (the arguments travel by value)
 struct RowCopy {
     int32_t src[COPY_MAX], first[COPY_MAX + 1], dst[COPY_MAX], rows_at[COPY_MAX];
     int64_t begin[COPY_MAX], end[COPY_MAX], head[COPY_MAX], add[COPY_MAX];
     const int32_t *rows;
     int64_t rows_stride, n;
-    int64_t *len;
+    int64_t *len[LEN_ARRAYS];
 };
 hipError_t launch_copy_rows(hipStream_t s, const Geom &src, const Geom &dst, const RowCopy &c, int groups);
 // Compaction in place: of the n rows behind base of sequence seq0 + z, those listed at rows + (seq0 + z) *
-// rows_stride, count of them and KEEP_ROWS at most, become the first; len receives base + count.
+// rows_stride, count of them and KEEP_ROWS at most, become the first; the arrays len receive base + count.
 constexpr int KEEP_MAX = 64;             // sequences a launch
 constexpr int KEEP_ROWS = 1024;
 struct RowKeep {
@@ -362,7 +363,7 @@ struct RowKeep {
     const int32_t *rows;
     int64_t rows_stride;
     int32_t n, seq0;
-    int64_t *len;
+    int64_t *len[LEN_ARRAYS];
 };
 hipError_t launch_keep_rows(hipStream_t s, const Geom &g, const RowKeep &c, int seqs, int most);
 // The attend of a tree of drafted tokens (attend_tree.hip): node i of n, whose row is row len - n + i of its

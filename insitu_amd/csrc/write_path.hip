@@ -120,7 +120,7 @@ constexpr int APPEND_WAVES = 4;
 template <int CPL, bool ROT>
 __global__ void __launch_bounds__(64 * APPEND_WAVES) append_kernel(
         Geom g, const Tables *__restrict__ tabs, const int32_t *__restrict__ k, const int32_t *__restrict__ v,
-        int n_tok, int seq_lo, const int64_t *__restrict__ len_in, int64_t *len_out, int seq_hi, int rounds,
+        int n_tok, int seq_lo, const int64_t *__restrict__ len_in, int64_t *len_out, int64_t *len_now, int seq_hi, int rounds,
         RotSigns sg, DevStats *st) {
     __shared__ uint8_t codes[APPEND_WAVES][2][MAX_D];
     __shared__ int64_t bnd[2][255];
@@ -129,10 +129,10 @@ __global__ void __launch_bounds__(64 * APPEND_WAVES) append_kernel(
     stage_bounds(tabs, g, bnd);
     // The length bookkeeping rides on workgroup 0: len_out = len_in + n_tok for the
     // sequences this call appends to, len_in elsewhere (double-buffered so no
-    // workgroup can observe a half-updated length).
+    // workgroup can observe a half-updated length); len_now the same.
     if (blockIdx.x == 0) {
         for (int i = threadIdx.x; i < g.batch; i += blockDim.x)
-            len_out[i] = len_in[i] + ((i >= seq_lo && i < seq_hi) ? n_tok : 0);
+            len_out[i] = len_now[i] = len_in[i] + ((i >= seq_lo && i < seq_hi) ? n_tok : 0);
     }
     const bool bisect = tabs->bnd_sorted != 0;
     const bool regpack = (32 % g.kb) == 0 && (32 % g.vb) == 0;   // widths 1, 2, 4, 8
@@ -496,7 +496,7 @@ hipError_t launch_rotate(hipStream_t s, const int32_t *x, int32_t *y, int64_t n_
 template <int KB, int VB, bool ROT>
 __global__ void __launch_bounds__(64 * AR_WAVES) append_rows_kernel(
         Geom g, const Tables *__restrict__ tabs, const int32_t *__restrict__ k, const int32_t *__restrict__ v,
-        int n_tok, int seq_lo, const int64_t *__restrict__ len_in, int64_t *len_out, int seq_hi, int rounds,
+        int n_tok, int seq_lo, const int64_t *__restrict__ len_in, int64_t *len_out, int64_t *len_now, int seq_hi, int rounds,
         RotSigns sg, DevStats *st, int rows) {
     static_assert(32 % KB == 0 && 32 % VB == 0 && KB <= 4 && VB <= 4, "code widths of 1, 2 or 4 bits");
     constexpr int NW = 2 * KB + 2 * VB + 1;            // the row's dwords: key codes, value codes, norms
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(64 * AR_WAVES) append_rows_kernel(
     // the length bookkeeping rides on workgroup 0 (as in append_kernel)
     if (blockIdx.x == 0) {
         for (int i = threadIdx.x; i < g.batch; i += blockDim.x)
-            len_out[i] = len_in[i] + ((i >= seq_lo && i < seq_hi) ? n_tok : 0);
+            len_out[i] = len_now[i] = len_in[i] + ((i >= seq_lo && i < seq_hi) ? n_tok : 0);
     }
     const int r0 = (blockIdx.x * AR_WAVES + wv) * 64;
     if (r0 >= rows) return;
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__((2 + MAX_G) * 64) step_write_kernel(
         Geom g, const Tables *__restrict__ tabs, const int32_t *__restrict__ qw,
         const int32_t *__restrict__ kw, const int32_t *__restrict__ vw, int rounds, RotSigns sg,
         int32_t *qr, double *qd, int32_t *qok, const int64_t *__restrict__ len_in, int64_t *len_out,
-        DevStats *st) {
+        int64_t *len_now, DevStats *st) {
     __shared__ uint8_t codes[2][MAX_D];
     __shared__ int64_t bnd[2][255];
     __shared__ int64_t norms[2];
@@ -620,7 +620,7 @@ __global__ void __launch_bounds__((2 + MAX_G) * 64) step_write_kernel(
     const int d = g.d;
 
     if (blockIdx.x == 0 && wv == 0) {
-        for (int i = lane; i < g.batch; i += 64) len_out[i] = len_in[i] + 1;
+        for (int i = lane; i < g.batch; i += 64) len_out[i] = len_now[i] = len_in[i] + 1;
     }
     if (threadIdx.x == 0) ok_s = 1;
     stage_bounds(tabs, g, bnd);
@@ -667,7 +667,7 @@ __global__ void __launch_bounds__((2 + MAX_G) * 64) step_write_kernel(
 hipError_t launch_step_write(hipStream_t s, const Geom &g, const Tables *t, const int32_t *qw,
                              const int32_t *kw, const int32_t *vw, int rounds,
                              const uint64_t (*signs)[2], int32_t *qr, double *qd, int32_t *qok,
-                             const int64_t *len_in, int64_t *len_out, DevStats *st) {
+                             const int64_t *len_in, int64_t *len_out, int64_t *len_now, DevStats *st) {
     const int64_t blocks = (int64_t)g.batch * g.n_kv;
     if (blocks <= 0) return hipSuccess;
     if (rounds > 2 || g.G > MAX_G || (qd && g.G != GF) || blocks > 0x7fffffff)
@@ -676,10 +676,10 @@ hipError_t launch_step_write(hipStream_t s, const Geom &g, const Tables *t, cons
     dim3 grid((unsigned)blocks), block((unsigned)((2 + g.G) * 64));
     if (g.d <= 64)
         hipLaunchKernelGGL(step_write_kernel<1>, grid, block, 0, s, g, t, qw, kw, vw, rounds, sg, qr,
-                           qd, qok, len_in, len_out, st);
+                           qd, qok, len_in, len_out, len_now, st);
     else
         hipLaunchKernelGGL(step_write_kernel<2>, grid, block, 0, s, g, t, qw, kw, vw, rounds, sg, qr,
-                           qd, qok, len_in, len_out, st);
+                           qd, qok, len_in, len_out, len_now, st);
     return hipGetLastError();
 }
 
@@ -709,7 +709,7 @@ bool append_rows_ok(const Geom &g, const Tables &th, const int32_t *k, const int
 
 hipError_t launch_append(hipStream_t s, const Geom &g, const Tables *t, const int32_t *k,
                          const int32_t *v, int n_tok, int seq_lo, int seq_hi, const int64_t *len_in,
-                         int64_t *len_out, DevStats *st, int rounds, const uint64_t (*signs)[2],
+                         int64_t *len_out, int64_t *len_now, DevStats *st, int rounds, const uint64_t (*signs)[2],
                          const Tables &host_tabs, int path) {
     const int64_t rows = (int64_t)(seq_hi - seq_lo) * n_tok * g.n_kv;
     if (rows <= 0) return hipSuccess;
@@ -721,7 +721,7 @@ hipError_t launch_append(hipStream_t s, const Geom &g, const Tables *t, const in
         const int nr = (int)rows;
 #define INSITU_AR(KB, VB, ROT)                                                                     \
     hipLaunchKernelGGL((append_rows_kernel<KB, VB, ROT>), grid, block, 0, s, g, t, k, v, n_tok, seq_lo, \
-                       len_in, len_out, seq_hi, rounds, sg, st, nr)
+                       len_in, len_out, len_now, seq_hi, rounds, sg, st, nr)
         if (g.kb == 4) {
             if (rounds) INSITU_AR(4, 2, true); else INSITU_AR(4, 2, false);
         } else {
@@ -741,17 +741,17 @@ hipError_t launch_append(hipStream_t s, const Geom &g, const Tables *t, const in
     if (g.d <= 64) {
         if (rot)
             hipLaunchKernelGGL((append_kernel<1, true>), grid, block, 0, s, g, t, k, v, n_tok, seq_lo, len_in,
-                               len_out, seq_hi, rounds, sg, st);
+                               len_out, len_now, seq_hi, rounds, sg, st);
         else
             hipLaunchKernelGGL((append_kernel<1, false>), grid, block, 0, s, g, t, k, v, n_tok, seq_lo, len_in,
-                               len_out, seq_hi, rounds, sg, st);
+                               len_out, len_now, seq_hi, rounds, sg, st);
     } else {
         if (rot)
             hipLaunchKernelGGL((append_kernel<2, true>), grid, block, 0, s, g, t, k, v, n_tok, seq_lo, len_in,
-                               len_out, seq_hi, rounds, sg, st);
+                               len_out, len_now, seq_hi, rounds, sg, st);
         else
             hipLaunchKernelGGL((append_kernel<2, false>), grid, block, 0, s, g, t, k, v, n_tok, seq_lo, len_in,
-                               len_out, seq_hi, rounds, sg, st);
+                               len_out, len_now, seq_hi, rounds, sg, st);
     }
     return hipGetLastError();
 }
