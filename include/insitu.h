@@ -102,7 +102,8 @@ typedef struct {
 } insitu_stats;
 
 /* --- context ------------------------------------------------------------- */
-/* Binds a device and a stream (NULL = the default stream); holds the exp LUT constants. */
+/* Binds a device and a stream (NULL = the default stream); holds the exp LUT constants. Destroyed
+ * before its caches, a context stays until the last of them is. */
 int insitu_ctx_create(int32_t device, void *hip_stream, insitu_ctx **out);
 int insitu_ctx_destroy(insitu_ctx *ctx);
 int insitu_ctx_sync(insitu_ctx *ctx);

@@ -99,6 +99,7 @@ struct insitu_ctx {
     std::vector<hipEvent_t> ev;           // 2 per attend: start, end
     size_t ev_used = 0;
     void *blas = nullptr;                 // the host half's rocBLAS state (host_half.hip)
+    std::atomic<int> holders{1};          // whoever created it, and its caches: a garbage collector may end it first
 };
 
 // The allocation-free prefill (insitu_attend_causal_static) keeps its chunk
@@ -337,8 +338,9 @@ int insitu_ctx_create(int32_t device, void *hip_stream, insitu_ctx **out) {
     return INSITU_OK;
 }
 
-int insitu_ctx_destroy(insitu_ctx *c) {
-    if (!c) return INSITU_OK;
+// One holder less; the last one's end is the context's.
+static void ctx_release(insitu_ctx *c) {
+    if (c->holders.fetch_sub(1) != 1) return;
     hipSetDevice(c->device);
     if (c->stream) hipStreamSynchronize(c->stream);
     for (hipEvent_t e : c->ev) hipEventDestroy(e);
@@ -348,6 +350,10 @@ int insitu_ctx_destroy(insitu_ctx *c) {
     blas_release(c);
     if (c->own_stream && c->stream) hipStreamDestroy(c->stream);
     delete c;
+}
+
+int insitu_ctx_destroy(insitu_ctx *c) {
+    if (c) ctx_release(c);
     return INSITU_OK;
 }
 
@@ -516,6 +522,7 @@ int insitu_cache_create(insitu_ctx *c, const insitu_cache_desc *desc, insitu_cac
     HIP_TRY(hipSetDevice(c->device), "hipSetDevice");
     auto *k = new insitu_cache();
     k->ctx = c;
+    c->holders.fetch_add(1);
     k->desc = *desc;
     k->desc.key_centroids_host = k->desc.key_bounds_host = nullptr;
     k->desc.value_centroids_host = k->desc.value_bounds_host = nullptr;
@@ -543,13 +550,13 @@ int insitu_cache_create(insitu_ctx *c, const insitu_cache_desc *desc, insitu_cac
         for (int a = fl[0]; a < fl[1];) {
             int bnd = a + 16 < fl[1] ? a + 16 : fl[1];
             if (g.n_planes >= MAX_PLANES) {
-                delete k;
+                insitu_cache_destroy(k);
                 return fail(INSITU_EINVAL, "row needs more than 16 planes");
             }
             g.plane_lo[g.n_planes] = a;
             g.plane_w[g.n_planes] = bnd - a;
             if (16 % (bnd - a)) {
-                delete k;
+                insitu_cache_destroy(k);
                 return fail(INSITU_EINVAL, "plane width does not divide the 16-byte beat "
                                            "(ddr_layout.py:140-146)");
             }
@@ -656,6 +663,7 @@ int insitu_cache_destroy(insitu_cache *k) {
     if (k->tree_scr) hipFree(k->tree_scr);
     if (k->keep_scr) hipFree(k->keep_scr);
     for (void *p : k->retired) hipFree(p);
+    ctx_release(k->ctx);
     delete k;
     return INSITU_OK;
 }
