@@ -30,7 +30,7 @@ class ModelConfig:
     # forms beside the reference's (insitu_amd.host.Seam):
     rotary_dim: int | None = None          # channels of a head that RoPE rotates; None: all of them
     rope_interleaved: bool = False         # channel pairs (2 j, 2 j + 1) instead of (j, j + rotary_dim / 2)
-    qk_norm_eps: float = 1e-6              # of the query and key norms, where the weights have them
+    qk_norm_eps: float | None = 1e-6       # of the query and key norms; None: no norm can be given
 
     def __post_init__(self) -> None:
         d = self.head_dim if self.head_dim is not None else self.hidden_size // self.num_heads
@@ -48,7 +48,7 @@ class ModelConfig:
         object.__setattr__(self, "rotary_dim", r)
         if r % 2 or not 2 <= r <= d:
             raise ValueError(f"rotary_dim={r} must be even, from 2 to head_dim={d}")
-        if not self.qk_norm_eps > 0:
+        if self.qk_norm_eps is not None and not self.qk_norm_eps > 0:
             raise ValueError(f"qk_norm_eps={self.qk_norm_eps} must be positive")
 
     @property
@@ -69,7 +69,8 @@ class ModelConfig:
         dict included). rope_theta is read top-level or from rope_parameters and
         never defaulted; "default", "llama3", "linear" and "yarn" RoPE (this one with
         its original_max_position_embeddings) are modelled, any other scaling type is
-        refused. partial_rotary_factor and rms_norm_eps are read where they are there."""
+        refused. partial_rotary_factor and rms_norm_eps are read where they are there: this one is for
+        the norms of queries and keys alone, and 0, as a model without them may have it, is none."""
         from .host import LinearScaling, RopeScaling, YarnScaling
         get = (lambda k, d=None: hf_config.get(k, d)) if isinstance(hf_config, dict) \
             else (lambda k, d=None: getattr(hf_config, k, d))
@@ -104,7 +105,7 @@ class ModelConfig:
                    head_dim=get("head_dim"), rope_theta=float(theta),
                    max_position=get("max_position_embeddings", 4096), rope_scaling=scaling,
                    rotary_dim=None if part is None else int(d * part),
-                   qk_norm_eps=1e-6 if eps is None else float(eps))
+                   qk_norm_eps=1e-6 if eps is None else float(eps) if float(eps) > 0 else None)
 
     @classmethod
     def tinyllama(cls) -> "ModelConfig":

@@ -199,6 +199,8 @@ class Seam:
         self.ctx = ctx or default_context()
         dev = self.ctx.torch_device
         self.q_norm, self.k_norm = (_norm_weight(a, m.head_dim, self.ctx) for a in (q_norm, k_norm))
+        if m.qk_norm_eps is None and (q_norm is not None or k_norm is not None):
+            raise ValueError("norms of queries and keys need the model's qk_norm_eps")
         self.width = m.q_out_features + 2 * m.kv_out_features
         self.bias = None if bias is None else self.ctx.to_device(bias, torch.float32)
         if self.bias is not None and tuple(self.bias.shape) != (self.width,):
@@ -215,7 +217,7 @@ class Seam:
         self.last_saturated = 0
         dp = lambda t: None if t is None else t.data_ptr()
         self._desc = _lib.SeamDesc(m.num_heads, m.num_kv_heads, m.head_dim, m.rotary_dim, int(m.rope_interleaved),
-                                   ROPE_FRAC, int(cast_after_rope), 1.0 / np.sqrt(m.head_dim), m.qk_norm_eps,
+                                   ROPE_FRAC, int(cast_after_rope), 1.0 / np.sqrt(m.head_dim), m.qk_norm_eps or 0.0,
                                    dp(self.bias), dp(self.q_norm), dp(self.k_norm), dp(self._cos), dp(self._sin),
                                    m.max_position)
 
