@@ -35,6 +35,7 @@ RMS norm of each head are refused with NotImplementedError rather than approxima
 from __future__ import annotations
 
 import dataclasses
+import sys
 
 import numpy as np
 import torch
@@ -129,14 +130,39 @@ def _head_norms(attn_module, m: ModelConfig):
     return weights[0], weights[1], eps[0] if eps else m.qk_norm_eps
 
 
+def _interleaved(attn_module, rotary_dim: int) -> bool:
+    """Whether the module's file turns channel 2 j with 2 j + 1 (else j with j + rotary_dim / 2), as its own
+    apply_rotary_pos_emb shows: a turn by a quarter (cos 0, sin 1, the same for every pair) takes channel 0 to its
+    partner. Half pairs where the file has no such function."""
+    turn = getattr(sys.modules.get(type(attn_module).__module__), "apply_rotary_pos_emb", None)
+    if turn is None:
+        return False
+    x = torch.zeros(1, 1, 1, rotary_dim)
+    x[..., 0] = 1.0
+    for width in (rotary_dim, rotary_dim // 2):       # (a channel's angle, or a pair's)
+        try:
+            y = turn(x, x, torch.zeros(1, 1, width), torch.ones(1, 1, width))[0].reshape(-1)
+        except Exception:
+            continue
+        at = torch.nonzero(y.abs() > 0.5).reshape(-1).tolist()
+        if at == [rotary_dim // 2]:
+            return False
+        if at == [1]:
+            return True
+    raise NotImplementedError(f"rotary positions of {type(attn_module).__name__}: which channels its "
+                              f"apply_rotary_pos_emb pairs up cannot be seen; give rope_interleaved")
+
+
 def build_from_layer(attn_module, model_config, *, quant: QuantConfig | None = None,
                      fmt: FixedFormat | None = None, hw=None, capacity: int = 4096,
                      compressed: bool = True, layer_idx: int = 0, softmax: str = "two_pass",
-                     ctx=None) -> KernelAttention:
+                     rope_interleaved: bool | None = None, ctx=None) -> KernelAttention:
     """torch_llama.py:172-203: a KernelAttention from an attention module's weights.
 
     softmax defaults to the reference AttentionKernel's default, "two_pass";
     "online" is the hardware's order and the single fused launch per decode step.
+    rope_interleaved: rotary pairs of channels (2 j, 2 j + 1) instead of (j, j + rotary_dim / 2);
+    None takes the module's own (_interleaved).
     """
     if not compressed:
         raise NotImplementedError("compressed=False is the reference's fp16 dense baseline; "
@@ -145,6 +171,8 @@ def build_from_layer(attn_module, model_config, *, quant: QuantConfig | None = N
         raise NotImplementedError("hw configures the reference's systolic-array model; the GPU "
                                   "block has no counterpart")
     m = ModelConfig.from_hf(model_config)
+    m = dataclasses.replace(m, rope_interleaved=_interleaved(attn_module, m.rotary_dim) if rope_interleaved is None
+                            else bool(rope_interleaved))
     q_norm, k_norm, eps = _head_norms(attn_module, m)
     m = dataclasses.replace(m, qk_norm_eps=eps)
     block = AttentionBlock(m, quant or QuantConfig(), fmt, capacity=capacity, softmax=softmax, ctx=ctx)

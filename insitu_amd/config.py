@@ -64,13 +64,14 @@ class ModelConfig:
         return self.num_kv_heads * self.head_dim
 
     @classmethod
-    def from_hf(cls, hf_config) -> "ModelConfig":
+    def from_hf(cls, hf_config, *, rope_interleaved: bool = False) -> "ModelConfig":
         """config.py:78-120: from a transformers config (or anything duck-typed, a
         dict included). rope_theta is read top-level or from rope_parameters and
         never defaulted; "default", "llama3", "linear" and "yarn" RoPE (this one with
         its original_max_position_embeddings) are modelled, any other scaling type is
         refused. partial_rotary_factor and rms_norm_eps are read where they are there: this one is for
-        the norms of queries and keys alone, and 0, as a model without them may have it, is none."""
+        the norms of queries and keys alone, and 0, as a model without them may have it, is none.
+        A configuration does not say which channels pair up: rope_interleaved does."""
         from .host import LinearScaling, RopeScaling, YarnScaling
         get = (lambda k, d=None: hf_config.get(k, d)) if isinstance(hf_config, dict) \
             else (lambda k, d=None: getattr(hf_config, k, d))
@@ -104,7 +105,7 @@ class ModelConfig:
                    num_kv_heads=get("num_key_value_heads", heads),
                    head_dim=get("head_dim"), rope_theta=float(theta),
                    max_position=get("max_position_embeddings", 4096), rope_scaling=scaling,
-                   rotary_dim=None if part is None else int(d * part),
+                   rotary_dim=None if part is None else int(d * part), rope_interleaved=rope_interleaved,
                    qk_norm_eps=1e-6 if eps is None else float(eps) if float(eps) > 0 else None)
 
     @classmethod
