@@ -69,7 +69,7 @@ class ModelConfig:
         dict included). rope_theta is read top-level or from rope_parameters and
         never defaulted; "default", "llama3", "linear" and "yarn" RoPE (this one with
         its original_max_position_embeddings) are modelled, any other scaling type is
-        refused. partial_rotary_factor and rms_norm_eps are read where they are there: this one is for
+        refused, and so is a part of a head that is no even number of channels. partial_rotary_factor and rms_norm_eps are read where they are there: this one is for
         the norms of queries and keys alone, and 0, as a model without them may have it, is none.
         A configuration does not say which channels pair up: rope_interleaved does."""
         from .host import LinearScaling, RopeScaling, YarnScaling
@@ -100,12 +100,16 @@ class ModelConfig:
         part = get("partial_rotary_factor")
         part = params.get("partial_rotary_factor") if part is None else part
         d = get("head_dim") or get("hidden_size") // heads
+        rotary = None if part is None else int(d * part)
+        if rotary is not None and (rotary % 2 or not 2 <= rotary <= d):
+            # (an odd width's frequencies go by it, and its pairs by an even one beside it)
+            raise NotImplementedError(f"rotary positions over {rotary} of a head's {d} channels are not modelled")
         eps = get("rms_norm_eps")
         return cls(hidden_size=get("hidden_size"), num_heads=heads,
                    num_kv_heads=get("num_key_value_heads", heads),
                    head_dim=get("head_dim"), rope_theta=float(theta),
                    max_position=get("max_position_embeddings", 4096), rope_scaling=scaling,
-                   rotary_dim=None if part is None else int(d * part), rope_interleaved=rope_interleaved,
+                   rotary_dim=rotary, rope_interleaved=rope_interleaved,
                    qk_norm_eps=1e-6 if eps is None else float(eps) if float(eps) > 0 else None)
 
     @classmethod
