@@ -210,7 +210,9 @@ int insitu_attend_causal_head(insitu_cache *cache, int32_t seq, int32_t kv_head,
  * stats_host may be NULL: then nothing synchronises, and once a call of the shape has allocated the
  * cache's scratch nothing allocates either, so that such a call may be captured into a graph. Its
  * replays attend the lengths that the cache has by then, cut to n .. the longest of the capture, and
- * share the scratch: one at a time, in order with the cache's other calls. */
+ * share the scratch: one at a time, in order with the cache's other calls. The scratch is the
+ * cache's, up to 512 MiB for most shapes; where a call needs more than there is, a buffer twice as
+ * large at least takes its place, and the ones before it, which graphs may hold, go with the cache. */
 int insitu_attend_tree(insitu_cache *cache, int32_t n, const int32_t *parents_dev, int32_t per_sequence,
                        const int32_t *q_rot_dev, int32_t *out_dev, int32_t mode, insitu_stats *stats_host);
 
@@ -327,7 +329,8 @@ int insitu_cache_fork(insitu_cache *cache, int32_t n_copies, const int32_t *src_
 /* Of the last n rows of every sequence, the listed ones (as insitu_cache_fork's lists, a list a
  * sequence, in any order) become the first, in place, and the sequence ends behind them: the accepted
  * path of a draft. counts_host (batch), or NULL: none is kept and rows_dev is not read. More than
- * 1,024 rows of a sequence go through a buffer of the cache, which the first such call allocates. */
+ * 1,024 rows of a sequence go through a buffer of the cache (16 bytes a row, plane and KV head of one
+ * sequence), which the first such call allocates and grows as the scratch of insitu_attend_tree does. */
 int insitu_cache_keep(insitu_cache *cache, int64_t n, const int32_t *rows_dev, int64_t rows_stride,
                       const int64_t *counts_host);
 
