@@ -162,8 +162,10 @@ class AttentionBlock:
             raise ValueError(f"qi must be ({self.batch}, n, {m.num_heads}, {m.head_dim}), got {tuple(q.shape)}")
         if not 1 <= n <= _lib.TREE_NODES:
             raise ValueError(f"a tree has 1 to {_lib.TREE_NODES} nodes, got {n}")
-        k = self.ctx.to_device(ki, torch.int32).reshape(self.batch, n, m.num_kv_heads, m.head_dim)
-        v = self.ctx.to_device(vi, torch.int32).reshape(self.batch, n, m.num_kv_heads, m.head_dim)
+        k, v = self.ctx.to_device(ki, torch.int32), self.ctx.to_device(vi, torch.int32)
+        for name, t in (("ki", k), ("vi", v)):
+            if tuple(t.shape) != (self.batch, n, m.num_kv_heads, m.head_dim):
+                raise ValueError(f"{name} must be ({self.batch}, {n}, {m.num_kv_heads}, {m.head_dim}), got {tuple(t.shape)}")
         parents = self.attn.check_parents(parents, n)       # before the rows are written
         with self.ctx.ordered(q, k, v, parents):
             qr = self.rotation.apply(q, self.ctx)
