@@ -27,14 +27,17 @@
 // three steps follow each other behind barriers, the runs mostly in shared memory.
 //
 // What bounds it. Memory does not: 32 nodes of 4 heads behind 8 x 32,768 tokens read 218 MB, 46 us at the rate of a
-// copy, and take 1,770 us. The integers do: a tile of 16 x 16 at d = 128 with 3-bit values costs 66 matrix
-// instructions (24 % of the walk's cycles) and 510 vector ones, which fill 64 % of the issue slots:
-// the keys' digits, the scores' carries in 64 bits, the terms in float64 for every value code (exact: 53 bits), their
-// digits' bytes and the one-hot codes. So the tile's terms use two digits where they fit, no tile is walked whose
-// weights are all zero, and max_kernel's row tiles share the expanded keys. Measured kernels: 26 nodes behind 32,768
-// tokens (4b/2b, 32 heads) 39 + 66 + 13 us, 64 nodes behind 4,097 two-pass 16 + 38 + 6 us; tried and slower: 32
-// tokens a step, storing the scores between the launches, one launch for long contexts, signed codebooks halved by
-// symmetry, two or four tokens' tiles sharing one-hot codes at d = 128 (registers), four waves a SIMD.
+// copy, and take 1,770 us. The integers do, though no one unit is full: a tile of 16 x 16 at d = 128 with 3-bit values
+// costs 580 vector instructions, 54 of them matrix ones, which fill 69 % of the issue slots (the matrix cores are busy
+// for 26 %), and two waves a SIMD do not cover the rest, the latency of their chains: the keys' digits, the scores'
+// carries in 64 bits, the terms in float64 for every value code (exact: 53 bits), their digits' bytes and the one-hot
+// codes. So the tile's terms use two digits where they fit, no tile is walked whose weights are all zero (scored it is,
+// once more), and max_kernel's row tiles share the expanded keys. Registers: the walk takes 201 to 256, and at d = 128
+// with 3-bit values spills 11 (17 in one launch); three waves a SIMD at d = 64 spill 21 to 33, still the faster way.
+// Measured kernels: 26 nodes behind 32,768 tokens (4b/2b, 32 heads) 40 + 66 + 13 us, 64 nodes behind 4,097 two-pass
+// 16 + 38 + 6 us; tried and slower: 32 tokens a step, storing the scores between the launches, one launch for long
+// contexts, signed codebooks halved by symmetry, two or four tokens' tiles sharing one-hot codes at d = 128
+// (registers), four waves a SIMD.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -1250,8 +1253,11 @@ size_t carve(const Geom &g, const Plan &pl, uint8_t *p, Scratch *sc) {
 }
 
 constexpr size_t BUDGET = (size_t)512 << 20;
-// Contexts up to here in one launch (5 nodes behind 100 tokens 20 us, in three 29; 26 behind 512: 31 and 32; behind
-// 1,024: 42 and 36; 26 x 8 sequences: 45 and 46, 59 and 58, 77 and 73).
+// Contexts up to here in one launch (4b/2b, 32 heads of 64 over 8, online, call to call: 5 nodes behind 100 tokens 18.6
+// us, in three launches 27.0; 26 behind 486: 29.2 and 30.4; behind 1,000: 42.6 and 33.8; 26 x 8 sequences behind 100,
+// 486 and 1,000: 35.7 and 36.8, 55.6 and 53.0, 82.0 and 84.9). Of many row tiles three would be the faster way at any
+// length, since its registers leave a CU one workgroup: 64 nodes x 8 sequences behind 100: 77.7 and 59.8, x 32: 298 and
+// 169; 256 x 8: 389 and 225.
 constexpr int64_t FUSED_MAX = 512;
 Plan plan(const Geom &g, int64_t n, int64_t longest, int64_t batch) {
     Plan p{};

@@ -226,7 +226,7 @@ class Seam:
         (n, Hkv, d), int32 Q8.16 on the device. positions: n values, any order; the first of
         consecutive ones may be given alone as an int. Host positions are checked against the
         table; a device tensor's are checked where counts is (which synchronises), and otherwise
-        the rows of positions beyond the table are left unwritten."""
+        the q and k rows of positions beyond the table are left unwritten."""
         import torch
         m = self.model
         p = self.ctx.to_device(p, torch.float32)
