@@ -206,3 +206,39 @@ def test_a_step_after_a_replayed_keep(ctx):
                 s.c.set_length(T - 4, b)
             s.rows(4)
             assert s.c.lengths() == [T] * 2
+
+
+def test_captured_on_the_callers_stream(ctx):
+    """A tree and a compaction of a block whose stream is not the capturing one: both are in the graph."""
+    import torch
+    s = Serving(ctx, "append_rotated")
+    dev = s.own.torch_device
+    mine = torch.cuda.Stream(dev)
+    q = torch.from_numpy(_draw(s.rng, 2, N, s.heads, 64)).to(dev)
+    p = torch.tensor([-1, 0, 1], dtype=torch.int32, device=dev)
+    rows = torch.tensor([0, 2], dtype=torch.int32, device=dev)
+    out = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(mine):
+        s.blk.attn.attend_tree(q, p, out=out, stats=False)
+        mine.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=mine):
+            s.blk.attn.attend_tree(q, p, out=out, stats=False)
+            s.c.keep(N, rows)
+            out += 1
+    for turn in range(3):
+        if turn:
+            s.rows(1)
+            assert s.c.lengths() == [T] * 2
+        with torch.cuda.stream(s.side):
+            want = s.like([T, T]).attend_tree(q, p, stats=False)[0]
+        s.side.synchronize()
+        with torch.cuda.stream(mine):
+            g.replay()
+            mine.synchronize()
+        assert torch.equal(out, want + 1)
+        with torch.cuda.stream(s.side):
+            s.lengths_are([T - 1] * 2)
+        for b in (0, 1):
+            s.c.set_length(T - 1, b)
