@@ -169,6 +169,34 @@ int insitu_append_seq(insitu_cache *cache, int32_t seq, const int32_t *k_rot_dev
 int insitu_append_wire(insitu_cache *cache, int32_t seq, const int32_t *k_wire_dev,
                        const int32_t *v_wire_dev, int32_t n_tok);
 
+/* Floating keys or values, a dense cache's for example: rows of (sequence, token, KV head) at
+ * dev + seq * seq_stride + tok * tok_stride + head * head_stride elements, a head's d channels
+ * together. */
+enum { INSITU_F32 = 0, INSITU_F16 = 1, INSITU_BF16 = 2 };
+typedef struct {
+    void *dev;
+    int64_t seq_stride, tok_stride, head_stride;
+} insitu_float_rows;
+/* n_tok post-RoPE rows of keys and values in floating point: cast to Q8.16 as the seam casts them
+ * (to_fixed, ops/convert.py:44-57: half to even, the ends of 24 bits where a value lies beyond
+ * them; NaN is 0), rotated with the cache format's rotation (none to two rounds) and appended, in
+ * one pass. seq = -1: every sequence; else that one, and k/v->seq_stride is not used. type:
+ * INSITU_F32 .. INSITU_BF16, both. Elements lie on their own size's boundary; rows on 16 bytes
+ * (address and strides) are read faster. saturated_host may be NULL: then nothing synchronises;
+ * otherwise it receives the number of values that did not fit. Like insitu_append not for graph
+ * capture. */
+int insitu_append_float(insitu_cache *cache, int32_t seq, const insitu_float_rows *k, const insitu_float_rows *v,
+                        int32_t type, int32_t n_tok, unsigned long long *saturated_host);
+/* Rows t0 .. t0 + n - 1 of a sequence (of every one for seq = -1) as floating keys and values:
+ * centroid times norm, turned back by the inverse of the cache format's rotation (none to two
+ * rounds), or with rotated = 1 as they are held. seq = -1: row t0 + i of sequence b goes to
+ * (b, i, head); rows behind a sequence's end leave the output as it was. A single sequence's rows
+ * have to be there (EBADLEN). k, v: outputs, no two elements in one place. Stream-ordered; replayed from a
+ * graph, seq = -1 goes by the lengths of the replay, and so does a single sequence (rows behind its end by then
+ * are left out). */
+int insitu_read_float(insitu_cache *cache, int32_t seq, int64_t t0, int64_t n, int32_t rotated,
+                      const insitu_float_rows *k, const insitu_float_rows *v, int32_t type);
+
 /* attend_online / attend_two_pass over every sequence's cache (kernel.py:337-345,
  * attention.py:429-513). q_rot_dev int32 (batch, n_q_heads, d) rotated;
  * out_dev int32 (batch, n_q_heads, d) Q16. stats_host may be NULL: then nothing
@@ -215,6 +243,21 @@ int insitu_attend_causal_head(insitu_cache *cache, int32_t seq, int32_t kv_head,
  * large at least takes its place, and the ones before it, which graphs may hold, go with the cache. */
 int insitu_attend_tree(insitu_cache *cache, int32_t n, const int32_t *parents_dev, int32_t per_sequence,
                        const int32_t *q_rot_dev, int32_t *out_dev, int32_t mode, insitu_stats *stats_host);
+
+/* Queries of layers with a sliding window, for every sequence at once (seq = -1) or one (no
+ * counterpart in the reference, which attends all of a context). The last n rows of the sequence
+ * are the queries' own, appended before: the query at row p attends, in row order, the rows t <= p
+ * with t < sinks or t > p - window (its own among them: window is at least 1), exactly as
+ * insitu_attend would in a cache that held those rows alone. A decode step is n = 1, a prompt its
+ * n tokens, a chunk of one the chunk's. q_rot_dev int32 (batch, n, n_q_heads, d) rotated, or (n,
+ * n_q_heads, d) for one sequence; out_dev int32, the same shape, Q16 (q_rot_dev itself may be
+ * given). EBADLEN when a sequence holds fewer than n rows. stats_host may be NULL: then nothing
+ * synchronises, and once a call of the shape has allocated the cache's scratch nothing allocates
+ * either, so that such a call may be captured into a graph. Its replays attend the lengths that the
+ * cache has by then (n at least), share the scratch with insitu_attend_tree and with each other, and run one at a time,
+ * in order with the cache's other calls. */
+int insitu_attend_window(insitu_cache *cache, int32_t seq, int64_t n, int64_t window, int64_t sinks,
+                         const int32_t *q_rot_dev, int32_t *out_dev, int32_t mode, insitu_stats *stats_host);
 
 /* insitu_attend_causal without allocating: no counterpart in the reference; for callers
  * that cannot call hipMalloc (tight serving loops, harnesses that forbid it). The same

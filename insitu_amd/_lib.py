@@ -7,6 +7,7 @@ entry point raises. The numpy model is never used to produce a product value.
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -30,7 +31,7 @@ EXPORTS = (
     "insitu_rotate", "insitu_encode", "insitu_qtab", "insitu_exp_lut", "insitu_finalize",
     "insitu_cache_create", "insitu_cache_destroy", "insitu_cache_reset", "insitu_cache_length",
     "insitu_cache_set_length", "insitu_cache_layout", "insitu_append", "insitu_append_seq",
-    "insitu_append_wire", "insitu_attend", "insitu_attend_causal", "insitu_attend_causal_head", "insitu_attend_causal_static", "insitu_step", "insitu_project", "insitu_seam_wire",
+    "insitu_append_wire", "insitu_append_float", "insitu_read_float", "insitu_attend_window", "insitu_attend", "insitu_attend_causal", "insitu_attend_causal_head", "insitu_attend_causal_static", "insitu_step", "insitu_project", "insitu_seam_wire",
     "insitu_project_seam", "insitu_seam_heads", "insitu_attend_tree", "insitu_cache_fork", "insitu_cache_keep",
     "insitu_output_projection", "insitu_read_rows", "insitu_load_rows", "insitu_read_image",
     "insitu_load_image", "insitu_probe_read", "insitu_probe_empty", "insitu_cache_debug",
@@ -92,6 +93,11 @@ class SeamDesc(ctypes.Structure):
         [("max_pos", ctypes.c_int64)]
 
 
+class FloatRows(ctypes.Structure):
+    _fields_ = [("dev", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("seq_stride", "tok_stride", "head_stride")]
+
+
+F32, F16, BF16 = range(3)
 TREE_NODES = 256         # nodes of a tree of drafted tokens, at most
 
 _lib = None
@@ -131,6 +137,9 @@ def load(path: str | None = None):
         "insitu_append": (i32, [vp, vp, vp, i32]),
         "insitu_append_seq": (i32, [vp, i32, vp, vp, i32]),
         "insitu_append_wire": (i32, [vp, i32, vp, vp, i32]),
+        "insitu_append_float": (i32, [vp, i32, P(FloatRows), P(FloatRows), i32, i32, P(ctypes.c_uint64)]),
+        "insitu_read_float": (i32, [vp, i32, i64, i64, i32, P(FloatRows), P(FloatRows), i32]),
+        "insitu_attend_window": (i32, [vp, i32, i64, i64, i64, vp, vp, i32, P(Stats)]),
         "insitu_attend": (i32, [vp, vp, vp, i32, P(Stats)]),
         "insitu_attend_causal": (i32, [vp, i32, i64, i64, vp, vp, i32, P(Stats)]),
         "insitu_attend_causal_head": (i32, [vp, i32, i32, i64, i64, vp, vp, i32, P(Stats)]),
@@ -164,6 +173,14 @@ def load(path: str | None = None):
         f.argtypes = args
     _lib = lib
     return lib
+
+
+def int64(x, name: str) -> int:
+    """A whole number that 64 bits hold (a call through ctypes would cut it off)."""
+    n = operator.index(x)
+    if not -(1 << 63) <= n < 1 << 63:
+        raise ValueError(f"{name}={n} is not a 64-bit number")
+    return n
 
 
 def check(status: int) -> None:

@@ -131,6 +131,41 @@ class CompressedAttention:
             out = out[0]
         return out, (AttentionStats.from_c(st) if st is not None else None)
 
+    # -- a sliding window and first rows that stay visible ------------------------
+
+    def attend_window(self, q_rot, window: int, sinks: int = 0, mode: str = "online", *, seq: int | None = None,
+                      out=None, stats: bool = True):
+        """Queries of a layer with a sliding window, whose own rows are the last n of every sequence
+        (or of sequence `seq`): q_rot (batch, n, n_q_heads, d) rotated, or (n, n_q_heads, d) of one
+        sequence (seq, or a batch of one). The query at row p attends the rows t <= p with t < sinks or
+        t > p - window, in row order: the integers that `attend` gives in a cache of those rows alone,
+        in every mode. n = 1 is a decode step. Returns (out torch int32 of q_rot's shape,
+        AttentionStats or None). With stats=False nothing synchronises."""
+        import torch
+        c = self.cache
+        q = self.ctx.to_device(q_rot, torch.int32)
+        lone = seq is not None or (q.dim() == 3 and c.batch == 1)
+        heads = (c.n_q_heads, c.head_dim)
+        if lone and (q.dim() != 3 or tuple(q.shape[1:]) != heads):
+            raise ValueError(f"q_rot must be (n, {c.n_q_heads}, {c.head_dim}), got {tuple(q.shape)}")
+        if not lone and (q.dim() != 4 or q.shape[0] != c.batch or tuple(q.shape[2:]) != heads):
+            raise ValueError(f"q_rot must be ({c.batch}, n, {c.n_q_heads}, {c.head_dim}), got {tuple(q.shape)}")
+        if out is None:
+            out = torch.empty_like(q)
+        elif tuple(out.shape) != tuple(q.shape) or out.dtype != torch.int32 or not out.is_contiguous() or \
+                out.device != q.device:
+            raise ValueError(f"out must be a contiguous int32 tensor {tuple(q.shape)} on {q.device}")
+        if seq is not None and not 0 <= seq < c.batch:
+            raise ValueError(f"sequence {seq} of {c.batch}")
+        st = _lib.Stats() if stats else None
+        with self.ctx.ordered(q, out):
+            _lib.check(self.ctx.lib.insitu_attend_window(c.handle, -1 if seq is None else seq, int(q.shape[-3]),
+                                                         _lib.int64(window, "window"), _lib.int64(sinks, "sinks"), ptr(q),
+                                                         ptr(out), _lib.MODES[mode],
+                                                         ctypes.byref(st) if st is not None else None))
+        self._keep = q
+        return out, (AttentionStats.from_c(st) if st is not None else None)
+
     # -- one KV head: the reference's call forms (kernel.py:317-331, 385-392) --------
 
     score_mode = "fused"     # attention.py:323: scores on the codes (architecture B)

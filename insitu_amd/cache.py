@@ -179,6 +179,34 @@ def unpack_rows(buf: np.ndarray, d: int, key_bits: int, value_bits: int,
     return CompressedKV(k_idx, k_norm, v_idx, v_norm)
 
 
+def _float_type(dtype) -> int:
+    import torch
+    types = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+    if dtype not in types:
+        raise TypeError(f"floating rows are float32, float16 or bfloat16, not {dtype}")
+    return types[dtype]
+
+
+def _float_rows(x) -> "_lib.FloatRows":
+    """(tokens, heads, d) or (batch, tokens, heads, d) as the library takes it."""
+    s = x.stride()
+    return _lib.FloatRows(x.data_ptr() or None, s[0] if x.dim() == 4 else 0, s[-3], s[-2])
+
+
+def _overlaps(x) -> bool:
+    """Whether a tensor's last dimension has a stride, or two of its elements may lie in one place."""
+    if x.numel() == 0:
+        return False
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        return True
+    reach = 0
+    for stride, size in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+        if stride <= reach:
+            return True
+        reach += stride * (size - 1)
+    return False
+
+
 class _Memory:
     """Device bytes as torch.as_tensor takes them."""
 
@@ -348,6 +376,94 @@ class CompressedCache(KVCache):
         _lib.check(self.ctx.lib.insitu_append_wire(self.handle, -1 if seq is None else seq,
                                                    ptr(k), ptr(v), n))
         self._keep = (k, v)     # keep inputs alive until the stream has consumed them
+
+    # -- floating rows: a dense cache's, taken over and handed back ---------------
+
+    def append_float(self, k, v, *, seq: int | None = None, counts: bool = False):
+        """Post-RoPE keys and values in floating point (torch tensors or arrays, both float32, float16 or
+        bfloat16) behind each sequence: cast to Q8.16 as the seam casts them, rotated, encoded and packed
+        in one pass. Shapes as append_wire's: (tokens, n_kv_heads, d) for a batch of one or `seq`,
+        (batch, tokens, n_kv_heads, d) otherwise; any strides but a head's channels', so that a dense
+        cache's (batch, n_kv_heads, tokens, d) goes as x.transpose(1, 2). With counts the number of
+        values beyond Q8.16 (which take its ends; NaN is 0) is returned, which synchronises. Raises
+        ValueError past capacity."""
+        k, v = self._floats(k, "k"), self._floats(v, "v")
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype} differ")
+        if seq is None and self.batch == 1 and k.dim() == 3:
+            seq = 0
+        want = ("tokens", self.n_kv_heads, self.head_dim) if seq is not None else \
+            (self.batch, "tokens", self.n_kv_heads, self.head_dim)
+        if k.dim() != len(want) or any(a != b for a, b in zip(k.shape, want) if b != "tokens"):
+            raise ValueError(f"expected {want}, got {tuple(k.shape)}")
+        lost = ctypes.c_uint64() if counts else None
+        if k.numel() == 0:
+            return 0 if counts else None
+        with self.ctx.ordered(k, v):
+            _lib.check(self.ctx.lib.insitu_append_float(
+                self.handle, -1 if seq is None else self._seq(seq), ctypes.byref(_float_rows(k)), ctypes.byref(_float_rows(v)),
+                _float_type(k.dtype), int(k.shape[-3]), ctypes.byref(lost) if counts else None))
+        self._keep = (k, v)
+        return int(lost.value) if counts else None
+
+    def read_float(self, t0: int = 0, n: int | None = None, *, seq: int | None = None, dtype=None, rotated: bool = False,
+                   out=None):
+        """Rows t0 .. t0 + n - 1 (by default those from t0 on) as floating keys and values (k, v), torch
+        tensors (batch, n, n_kv_heads, d), or (n, n_kv_heads, d) with `seq`: centroid times norm,
+        turned back into the model's basis, or with `rotated` as the cache holds them. Their memory
+        is a dense cache's, (batch, n_kv_heads, n, d), which k.transpose(1, 2) is again. Rows behind
+        a shorter sequence's end are zeros, or left as they were in `out`, two tensors of these shapes
+        and one dtype (float32, the default, float16 or bfloat16) with any strides but a head's
+        channels'. Stream-ordered."""
+        import torch
+        lens = self.lengths()
+        seq = None if seq is None else self._seq(seq)
+        end = max(lens) if seq is None else lens[seq]
+        t0 = _lib.int64(t0, "t0")
+        n = max(0, end - t0) if n is None else _lib.int64(n, "n")
+        if t0 < 0 or n < 0 or t0 + n > (self.capacity if seq is None else end):
+            raise ValueError(f"rows {t0} .. {t0 + n - 1} of {end}")
+        shape = ((self.batch,) if seq is None else ()) + (n, self.n_kv_heads, self.head_dim)
+        if out is None:
+            dtype = torch.float32 if dtype is None else dtype
+            _float_type(dtype)
+            make = torch.empty if seq is not None or t0 + n <= min(lens) else torch.zeros
+            lead = shape[:-3] + (self.n_kv_heads, n, self.head_dim)
+            out = tuple(make(lead, dtype=dtype, device=self.ctx.torch_device).transpose(-3, -2) for _ in range(2))
+        else:
+            out = tuple(out)
+            if len(out) != 2 or dtype not in (None, out[0].dtype) or out[0].dtype != out[1].dtype:
+                raise ValueError("out is two tensors of one dtype")
+            _float_type(out[0].dtype)
+            for x in out:
+                if tuple(x.shape) != shape or x.device != self.ctx.torch_device or _overlaps(x):
+                    raise ValueError(f"out must be two tensors {shape} on {self.ctx.torch_device}, a head's channels "
+                                     f"together and no two elements in one place")
+        if n == 0:
+            return out
+        with self.ctx.ordered(*out):
+            _lib.check(self.ctx.lib.insitu_read_float(
+                self.handle, -1 if seq is None else seq, t0, n, 1 if rotated else 0, ctypes.byref(_float_rows(out[0])),
+                ctypes.byref(_float_rows(out[1])), _float_type(out[0].dtype)))
+        return out
+
+    def _seq(self, seq) -> int:
+        seq = int(seq)
+        if not 0 <= seq < self.batch:
+            raise ValueError(f"sequence {seq} of {self.batch}")
+        return seq
+
+    def _floats(self, x, name: str):
+        """A floating tensor on this device whose heads' channels lie together."""
+        import torch
+        if not isinstance(x, torch.Tensor):
+            x = torch.from_numpy(np.ascontiguousarray(x))
+        _float_type(x.dtype)
+        if x.dim() not in (3, 4):
+            raise ValueError(f"{name} must be (tokens, {self.n_kv_heads}, {self.head_dim}) or (batch, tokens, "
+                             f"{self.n_kv_heads}, {self.head_dim}), got {tuple(x.shape)}")
+        x = x.detach().to(self.ctx.torch_device)
+        return x if x.stride(-1) == 1 else x.contiguous()
 
     # -- sequences that continue others, and drafts ------------------------------
 

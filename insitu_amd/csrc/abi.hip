@@ -751,6 +751,72 @@ int insitu_append_seq(insitu_cache *k, int32_t seq, const int32_t *kr, const int
     return append_impl(k, seq, seq + 1, kr, vr, n_tok);
 }
 
+static int float_rows_ok(const insitu_cache *k, int32_t seq, const insitu_float_rows *kr, const insitu_float_rows *vr, int32_t type) {
+    if (!k) return fail(INSITU_EINVAL, "cache is NULL");
+    if (seq < -1 || seq >= k->g.batch) return fail(INSITU_EINVAL, "no such sequence");
+    if (!kr || !vr || !kr->dev || !vr->dev) return fail(INSITU_EINVAL, "null argument");
+    if (type < INSITU_F32 || type > INSITU_BF16) return fail(INSITU_EINVAL, "unknown floating type");
+    const uintptr_t mask = type == INSITU_F32 ? 3 : 1;
+    if (((uintptr_t)kr->dev | (uintptr_t)vr->dev) & mask) return fail(INSITU_EINVAL, "floating rows off their elements' boundary");
+    if (k->desc.fmt.rot_rounds > 2) return fail(INSITU_EINVAL, "the cache's format rotates more than two rounds");
+    return INSITU_OK;
+}
+static FloatRows float_rows(const insitu_float_rows *r, bool one) {
+    return FloatRows{r->dev, one ? 0 : r->seq_stride, r->tok_stride, r->head_stride};
+}
+
+int insitu_append_float(insitu_cache *k, int32_t seq, const insitu_float_rows *kr, const insitu_float_rows *vr, int32_t type,
+                        int32_t n_tok, unsigned long long *saturated) {
+    int rc = float_rows_ok(k, seq, kr, vr, type);
+    if (rc) return rc;
+    if (n_tok < 0) return fail(INSITU_EBADLEN, "n_tok < 0");
+    if (saturated) *saturated = 0;
+    if (n_tok == 0) return INSITU_OK;
+    const int lo = seq < 0 ? 0 : seq, hi = seq < 0 ? k->g.batch : seq + 1;
+    for (int b = lo; b < hi; ++b)
+        if (k->len_host[b] + n_tok > k->g.capacity) {
+            char buf[200];
+            snprintf(buf, sizeof buf, "cache holds %lld of %lld tokens; cannot append %d (base.py:67-73)",
+                     (long long)k->len_host[b], (long long)k->g.capacity, n_tok);
+            return fail(INSITU_ECAPACITY, buf);
+        }
+    HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
+    if (saturated) {
+        rc = zero_stats(k);
+        if (rc) return rc;
+    }
+    HIP_TRY(launch_append_float(k->ctx->stream, k->g, k->tabs, float_rows(kr, seq >= 0), float_rows(vr, seq >= 0), type, n_tok, lo, hi,
+                                k->len_dev[k->cur], k->len_dev[k->cur ^ 1], k->len_now, k->desc.fmt.rot_rounds,
+                                k->desc.fmt.rot_signs, saturated != nullptr, k->stats),
+            "append launch");
+    k->cur ^= 1;
+    for (int b = lo; b < hi; ++b) k->len_host[b] += n_tok;
+    if (!saturated) return INSITU_OK;
+    insitu_stats st;
+    rc = copy_stats(k, &st);
+    if (rc) return rc;
+    *saturated = (unsigned long long)st.range_errors;
+    return INSITU_OK;
+}
+
+int insitu_read_float(insitu_cache *k, int32_t seq, int64_t t0, int64_t n, int32_t rotated, const insitu_float_rows *kr,
+                      const insitu_float_rows *vr, int32_t type) {
+    const int rc = float_rows_ok(k, seq, kr, vr, type);
+    if (rc) return rc;
+    if (t0 < 0 || n < 0 || t0 > k->g.capacity || n > k->g.capacity - t0) return fail(INSITU_EBADLEN, "rows beyond the capacity");
+    if (seq >= 0 && t0 + n > k->len_host[seq]) return fail(INSITU_EBADLEN, "rows behind the sequence's end");
+    const int lo = seq < 0 ? 0 : seq, hi = seq < 0 ? k->g.batch : seq + 1;
+    if (n == 0) return INSITU_OK;
+    for (const insitu_float_rows *r : {kr, vr})
+        if ((n > 1 && !r->tok_stride) || (k->g.n_kv > 1 && !r->head_stride) || (hi - lo > 1 && !r->seq_stride))
+            return fail(INSITU_EINVAL, "outputs in one place");
+    HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
+    HIP_TRY(launch_read_float(k->ctx->stream, k->g, k->tabs, float_rows(kr, seq >= 0), float_rows(vr, seq >= 0), type, t0, n, lo, hi,
+                              k->len_now, rotated ? 0 : k->desc.fmt.rot_rounds, k->desc.fmt.rot_signs),
+            "read launch");
+    return INSITU_OK;
+}
+
 int insitu_append_wire(insitu_cache *k, int32_t seq, const int32_t *kw, const int32_t *vw, int32_t n_tok) {
     if (!k) return fail(INSITU_EINVAL, "cache is NULL");
     if (seq < -1 || seq >= k->g.batch) return fail(INSITU_EINVAL, "no such sequence");
@@ -1175,6 +1241,43 @@ int insitu_attend_tree(insitu_cache *k, int32_t n, const int32_t *parents, int32
         HIP_TRY(launch_attend_tree_serial(k->ctx->stream, k->g, k->tabs, q, out, len, parents, pstride, n, longest, two_pass, ev,
                                           k->stats),
                 "tree attend launch");
+    return copy_stats(k, stats);
+}
+
+int insitu_attend_window(insitu_cache *k, int32_t seq, int64_t n, int64_t window, int64_t sinks, const int32_t *q, int32_t *out,
+                         int32_t mode, insitu_stats *stats) {
+    if (!k) return fail(INSITU_EINVAL, "cache is NULL");
+    if (seq < -1 || seq >= k->g.batch) return fail(INSITU_EINVAL, "no such sequence");
+    if (n < 1) return fail(INSITU_EBADLEN, "a window attend has 1 query at least");
+    if (window < 1 || sinks < 0) return fail(INSITU_EINVAL, "a window holds 1 row at least, sinks are 0 or more");
+    if (!q || !out) return fail(INSITU_EINVAL, "null argument");
+    if (mode < INSITU_SEQUENTIAL || mode > INSITU_SERIAL) return fail(INSITU_EINVAL, "unknown mode");
+    WindowJob w{};
+    w.seq_lo = seq < 0 ? 0 : seq;
+    w.nseq = seq < 0 ? k->g.batch : 1;
+    for (int b = w.seq_lo; b < w.seq_lo + w.nseq; ++b)
+        if (k->len_host[b] < n) {
+            char buf[160];
+            snprintf(buf, sizeof buf, "sequence %d holds %lld rows, fewer than the %lld queries' own", b,
+                     (long long)k->len_host[b], (long long)n);
+            return fail(INSITU_EBADLEN, buf);
+        }
+    if (n * w.nseq > 0x7fffffff / k->g.n_q) return fail(INSITU_EBADLEN, "more than 2^31 - 1 query heads");
+    w.q = q;
+    w.out = out;
+    w.len = k->len_now;
+    w.n = n;
+    // (no row is as far as the capacity)
+    w.window = std::min(window, k->g.capacity);
+    w.sinks = std::min(sinks, k->g.capacity);
+    w.two_pass = mode == INSITU_TWO_PASS ? 1 : 0;
+    HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
+    int rc = stats ? zero_stats(k) : INSITU_OK;
+    if (rc) return rc;
+    LaunchEv ev;
+    rc = timing_events(k->ctx, &ev);
+    if (rc) return rc;
+    HIP_TRY(launch_attend_window_serial(k->ctx->stream, k->g, k->tabs, w, ev, k->stats), "window attend launch");
     return copy_stats(k, stats);
 }
 

@@ -380,6 +380,33 @@ hipError_t launch_attend_tree_serial(hipStream_t s, const Geom &g, const Tables 
                                      const int64_t *len, const int32_t *parents, int64_t pstride, int32_t n, int64_t longest,
                                      int two_pass, LaunchEv ev, DevStats *st);
 
+// The attend of queries that see a sliding window and the first rows (attend_window.hip): the last n rows of
+// each of sequences seq_lo .. seq_lo + nseq - 1 are the queries' own, and the query at row p sees rows t <= p
+// with t < sinks or t > p - window. q, out: (nseq, n, g.n_q, d). Token by token, any format.
+struct WindowJob {
+    const int32_t *q;
+    int32_t *out;
+    const int64_t *len;
+    int64_t n, window, sinks;
+    int32_t seq_lo, nseq, two_pass;
+};
+hipError_t launch_attend_window_serial(hipStream_t s, const Geom &g, const Tables *t, const WindowJob &w, LaunchEv ev,
+                                       DevStats *st);
+
+// Floating rows of (sequence, token, KV head), strides in elements, a head's channels together
+// (float_rows.hip): cast to Q8.16, rotated and appended; or rows of a cache read back. type: INSITU_F32 ..
+struct FloatRows {
+    void *p;
+    int64_t seq, tok, head;
+};
+hipError_t launch_append_float(hipStream_t s, const Geom &g, const Tables *t, const FloatRows &k, const FloatRows &v, int type,
+                               int n_tok, int seq_lo, int seq_hi, const int64_t *len_in, int64_t *len_out, int64_t *len_now,
+                               int rounds, const uint64_t (*signs)[2], bool count, DevStats *st);
+// Rows t0 .. t0 + n - 1 (those below a sequence's length) in the basis before `rounds` rounds of rotation.
+hipError_t launch_read_float(hipStream_t s, const Geom &g, const Tables *t, const FloatRows &k, const FloatRows &v, int type,
+                             int64_t t0, int64_t n, int seq_lo, int seq_hi, const int64_t *len, int rounds,
+                             const uint64_t (*signs)[2]);
+
 // Shared with the files that add entry points beside abi.hip: the error
 // message for insitu_last_error, and a context's device and stream.
 int set_last_error(int code, const char *msg);

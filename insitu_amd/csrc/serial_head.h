@@ -42,9 +42,23 @@ __device__ __forceinline__ void stage_rows(const Geom &g, int b, int h, int64_t 
     }
 }
 
+// Which rows a head attends: whether row t; from where on, of t and the multiples of 64 behind it; and
+// how many of T.
 // Every row of the context.
 struct AllRows {
     __device__ __forceinline__ bool operator()(int64_t) const { return true; }
+    __device__ __forceinline__ int64_t from(int64_t t) const { return t; }
+    __device__ __forceinline__ int64_t count(int64_t T) const { return T; }
+};
+
+// The first rows (`sinks` of them) and those from lo on.
+struct WindowRows {
+    int64_t sinks, lo;
+    __device__ __forceinline__ bool operator()(int64_t t) const { return t < sinks || t >= lo; }
+    __device__ __forceinline__ int64_t from(int64_t t) const {
+        return t >= sinks && t + 64 <= lo ? lo / 64 * 64 : t;
+    }
+    __device__ __forceinline__ int64_t count(int64_t T) const { return T - (lo > sinks ? lo - sinks : 0); }
 };
 
 // The rows of a tree's node: those before the draft, and of the draft the ones whose bit is set.
@@ -54,6 +68,8 @@ struct TreeRows {
     __device__ __forceinline__ bool operator()(int64_t t) const {
         return t < base || ((up[(t - base) >> 5] >> ((t - base) & 31)) & 1u) != 0;
     }
+    __device__ __forceinline__ int64_t from(int64_t t) const { return t; }
+    __device__ __forceinline__ int64_t count(int64_t T) const { return T; }
 };
 // The row of `up` of node i of n, by one wave (LDS): the node and its ancestors, a bit each. A parent that
 // is not an earlier node ends the path.
@@ -98,7 +114,7 @@ __device__ __forceinline__ void serial_head(const Geom &g, const Tables *__restr
 
     const int passes = two_pass ? 2 : 1;
     for (int pass = 0; pass < passes; ++pass) {
-        for (int64_t base = 0; base < T; base += 64) {
+        for (int64_t base = rows.from(0); base < T; base = rows.from(base + 64)) {
             const int n = (int)((T - base) < 64 ? (T - base) : 64);
             wave_sync();
             stage_rows<RS>(g, b, kvh, base, n, L.rows);
@@ -187,7 +203,7 @@ __device__ __forceinline__ void serial_head(const Geom &g, const Tables *__restr
     sovf = (unsigned long long)wave_sum_i64((int64_t)sovf);
     aovf = (unsigned long long)wave_sum_i64((int64_t)aovf);
     if (lane == 0) {
-        atomicMax(&st->n_tokens, (unsigned long long)T);
+        atomicMax(&st->n_tokens, (unsigned long long)rows.count(T));
         atomicAdd(&st->rescale_events, events);
         atomicAdd(&st->acc_overflows, aovf);
         atomicMax(&st->max_abs_acc, (unsigned long long)amax);
