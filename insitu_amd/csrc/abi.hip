@@ -1277,7 +1277,10 @@ int insitu_attend_window(insitu_cache *k, int32_t seq, int64_t n, int64_t window
     LaunchEv ev;
     rc = timing_events(k->ctx, &ev);
     if (rc) return rc;
-    HIP_TRY(launch_attend_window_serial(k->ctx->stream, k->g, k->tabs, w, ev, k->stats), "window attend launch");
+    if (mode != INSITU_SERIAL && prefill_supported(k->g) && k->g.capacity <= PREFILL_MAX_ROWS)
+        HIP_TRY(launch_attend_window_prompt(k->ctx->stream, k->g, k->tabs, w, ev, k->stats), "window attend launch");
+    else
+        HIP_TRY(launch_attend_window_serial(k->ctx->stream, k->g, k->tabs, w, ev, k->stats), "window attend launch");
     return copy_stats(k, stats);
 }
 

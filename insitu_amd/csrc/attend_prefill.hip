@@ -134,10 +134,12 @@ struct Lds {
 // A workgroup's walk over its tokens, and its rows' outputs. Narrow scores: returns true when
 // they did not do (workgroup-uniform; nothing is written then). WIDE: int64 scores and a fourth
 // digit of q.
-template <int D, int NC, int W, int ST, bool TWO_PASS, bool WIDE>
+// WIN: the queries of w, several sequences of them, over a window and the first rows each. The workgroup's
+// tokens are then the stages of the first rows and those from its first row's window on, numbered on end.
+template <int D, int NC, int W, int ST, bool TWO_PASS, bool WIDE, bool WIN>
 __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__restrict__ tabs,
                                              const int32_t *__restrict__ q, int32_t *out, int64_t base, int64_t n_q,
-                                             DevStats *st, Lds<D, NC, W, ST> &S) {
+                                             DevStats *st, Lds<D, NC, W, ST> &S, const WindowJob *w) {
     using C = Shape<D, NC, W, ST>;
     using SC = typename std::conditional<WIDE, int64_t, int32_t>::type;
     constexpr int NQ = WIDE ? 4 : 3;                   // digits of q
@@ -148,13 +150,31 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
     // the longest contexts first; a KV head's workgroups a multiple of n_kv apart
     const int64_t rows = n_q * G;
     const int64_t nblk = (rows + W * 16 - 1) / (W * 16);
-    const int64_t blk = nblk - 1 - (int64_t)(blockIdx.x / (unsigned)g.n_kv);
     const int kvh = (int)(blockIdx.x % (unsigned)g.n_kv);
-    const uint8_t *hb = plane_ptr(g, 0, kvh, 0);
+    unsigned rest = blockIdx.x / (unsigned)g.n_kv;
+    int seq = 0;
+    if constexpr (WIN) {
+        seq = w->seq_lo + (int)(rest % (unsigned)w->nseq);
+        q += (int64_t)(rest % (unsigned)w->nseq) * n_q * g.n_q * D;
+        out += (int64_t)(rest % (unsigned)w->nseq) * n_q * g.n_q * D;
+        rest /= (unsigned)w->nseq;
+        const int64_t T = w->len[seq];
+        base = (T > n_q ? T : n_q) - n_q;
+    }
+    const int64_t blk = nblk - 1 - (int64_t)rest;
+    const uint8_t *hb = plane_ptr(g, seq, kvh, 0);
     const int64_t row0 = (blk * W + wv) * 16;          // this wave's first row
     const int64_t t_all = base + n_q;                  // rows the sequence holds for the last query
     const int64_t last_row = (blk + 1) * (W * 16) < rows ? (blk + 1) * (W * 16) - 1 : rows - 1;
     const int64_t tmax = base + last_row / G + 1;      // the workgroup's longest context
+    // WIN: the first rows, where stages skip from (a multiple of ST) and how far
+    const int sinks = WIN ? (int)w->sinks : 0;
+    int skip_at = 0, skip = 0;
+    if constexpr (WIN) {
+        const int64_t lo = base + blk * (W * 16) / G + 1 - w->window;
+        skip_at = (sinks + ST - 1) / ST * ST;
+        skip = lo > skip_at ? (int)(lo / ST * ST) - skip_at : 0;
+    }
 
     // -- tables, and each row's query digits -------------------------------------------------
     if (tid == 0) {
@@ -188,6 +208,7 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
     const bool valid = row0 + col < rows;
     const int64_t rowc = valid ? row0 + col : rows - 1;
     const int32_t limit = (int32_t)(base + rowc / G + 1);      // the row's context length
+    const int32_t wlo = WIN ? (int32_t)(limit - w->window) : 0;      // and where its window begins
     bool bad;                                          // its arithmetic is not proven: serial path
     double bq;                                         // largest ||q||_1 max|c| of the wave's rows
     bool over = false;                                 // narrow scores: a value too large
@@ -241,6 +262,9 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
         for (int o = 1; o < 16; o <<= 1) bq = fmax(bq, __shfl_xor(bq, o));
     }
     const int32_t wmin = (int32_t)(base + (row0 < rows ? row0 : rows - 1) / G + 1);       // the wave's contexts
+    // (WIN: the first and the last of the wave's windows)
+    const int32_t first_lo = WIN ? (int32_t)(wmin - w->window) : 0;
+    const int32_t last_lo = WIN ? (int32_t)(base + (row0 + 16 < rows ? row0 + 15 : rows - 1) / G + 1 - w->window) : 0;
     const int32_t wmax = row0 < rows ? (int32_t)(base + ((row0 + 16 < rows ? row0 + 16 : rows) - 1) / G + 1) : 0;
 
     // -- staging -------------------------------------------------------------------------
@@ -261,7 +285,8 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
     auto load_raw = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < C::UNITS; ++u) {
-            const int t = s * C::ST + (tid + u * C::THREADS) % C::ST;
+            int t = s * C::ST + (tid + u * C::THREADS) % C::ST;
+            if constexpr (WIN) t += s * C::ST >= skip_at ? skip : 0;
             if (width[u]) rg[u] = *(const u128 *)(src[u] + (int64_t)((t < (int)t_all ? t : (int)t_all - 1) * width[u]));
         }
     };
@@ -497,10 +522,13 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
             }
         }
         const int32_t tg = t0 + grp * 4;               // this lane's first token
+        auto seen = [&](int i) __attribute__((always_inline)) {
+            return tg + i < limit && (!WIN || tg + i >= wlo || tg + i < sinks);
+        };
         if (diag) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool in = tg + i < limit;
+                const bool in = seen(i);
                 if (P != FIXEDMAX) smin = in && s[i] < smin ? s[i] : smin;
                 s[i] = in ? s[i] : LO;
             }
@@ -523,7 +551,7 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
             for (int i = 0; i < 4; ++i) p[i] = lut(dl[i]);
             if (mask) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = tg + i < limit ? p[i] : 0u;
+                for (int i = 0; i < 4; ++i) p[i] = seen(i) ? p[i] : 0u;
             }
             const int4 vn4 = *(const int4 *)&S.vn[bf][tl * 16 + grp * 4];
             const int32_t w[4] = {__mul24(vn4.x, (int)p[0]), __mul24(vn4.y, (int)p[1]), __mul24(vn4.z, (int)p[2]),
@@ -583,9 +611,9 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
                 if (__ballot((uint32_t)m - (uint32_t)mx < delta_max) == 0) return;   // every p is 0
             }
         }
-        if (P != ONLINE || (plain && !diag)) {
+        if (P != ONLINE || (plain && (WIN || !diag))) {
             const uint32_t dl[4] = {clip(m, s[0]), clip(m, s[1]), clip(m, s[2]), clip(m, s[3])};
-            terms(P != ONLINE && diag, dl);
+            terms((WIN || P != ONLINE) && diag, dl);
             lp += (p[0] + p[1]) + (p[2] + p[3]);
             accumulate(A, bf, tl);
             return;
@@ -684,7 +712,7 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
 
     auto sweep = [&](auto passc) __attribute__((always_inline)) {
         constexpr Pass P = decltype(passc)::value;
-        const int nst = (int)((tmax + C::ST - 1) / C::ST);
+        const int nst = (int)((tmax - skip + C::ST - 1) / C::ST);
         load_raw(0);
         store_raw(0);
         __syncthreads();
@@ -713,9 +741,17 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
                     tight = uni32(!(bsum <= ACC_BOUND));
                 }
             }
-            const int32_t ts = s * C::ST;
-            for (int tl = 0; tl < C::NT && ts + tl * 16 < wmax; ++tl)
-                tile(passc, bf, tl, ts + tl * 16, ts + tl * 16 + 16 > wmin, check, tight);
+            int32_t ts = s * C::ST;
+            if constexpr (WIN) ts += ts >= skip_at ? skip : 0;
+            for (int tl = 0; tl < C::NT && ts + tl * 16 < wmax; ++tl) {
+                const int32_t t0 = ts + tl * 16;
+                bool diag = t0 + 16 > wmin;
+                if constexpr (WIN) {
+                    if (t0 >= sinks && t0 + 16 <= first_lo) continue;
+                    diag = diag || (t0 < last_lo && t0 + 16 > sinks);
+                }
+                tile(passc, bf, tl, t0, diag, check, tight);
+            }
             // a stage adds at most 16 tokens of 2^15 to a lane's 32 bits
             if (P != MAXONLY && (s & 4095) == 4095) {
                 l64 = denominator();
@@ -775,8 +811,13 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
             if (!(bads >> c & 1)) continue;
             const int64_t row = row0 + c, at = ((row / G) * g.n_q + (int64_t)kvh * G + row % G) * D;
             if (lane == 0) atomicAdd(&S.fallbacks, 1ull);
-            serial_head<D / 64, C::RS>(g, tabs, tabs->kc, tabs->vc, q + at, 0, kvh, base + row / G + 1, TWO_PASS ? 1 : 0,
-                                       true, S.u.fb[wv], out + at, st);
+            const int64_t T = base + row / G + 1;
+            if constexpr (WIN)
+                serial_head<D / 64, C::RS>(g, tabs, tabs->kc, tabs->vc, q + at, seq, kvh, T, TWO_PASS ? 1 : 0, true, S.u.fb[wv],
+                                           out + at, st, WindowRows{w->sinks, T - w->window});
+            else
+                serial_head<D / 64, C::RS>(g, tabs, tabs->kc, tabs->vc, q + at, 0, kvh, T, TWO_PASS ? 1 : 0, true, S.u.fb[wv],
+                                           out + at, st);
         }
     }
     __syncthreads();
@@ -788,16 +829,21 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
         if (S.fallbacks) atomicAdd(&st->serial_fallbacks, S.fallbacks);
         if (S.mabs > st->max_abs_score) atomicMax(&st->max_abs_score, S.mabs);
         if (S.macc > st->max_abs_acc) atomicMax(&st->max_abs_acc, S.macc);
-        if (blk == nblk - 1 && kvh == 0) atomicMax(&st->n_tokens, (unsigned long long)t_all);
+        if (blk == nblk - 1 && kvh == 0) {
+            int64_t most = t_all;
+            if constexpr (WIN) most = WindowRows{w->sinks, t_all - w->window}.count(t_all);
+            atomicMax(&st->n_tokens, (unsigned long long)most);
+        }
     }
     return false;
 }
 
 // Not inlined, so that its registers are its own: it is entered when narrow scores did not do.
-template <int D, int NC, int W, int ST, bool TWO_PASS>
+template <int D, int NC, int W, int ST, bool TWO_PASS, bool WIN = false>
 __device__ __attribute__((noinline)) void prefill_rows_wide(const Geom *g, const Tables *tabs, const int32_t *q, int32_t *out,
-                                                            int64_t base, int64_t n_q, DevStats *st, Lds<D, NC, W, ST> *S) {
-    prefill_rows<D, NC, W, ST, TWO_PASS, true>(*g, tabs, q, out, base, n_q, st, *S);
+                                                            int64_t base, int64_t n_q, DevStats *st, Lds<D, NC, W, ST> *S,
+                                                            const WindowJob *w = nullptr) {
+    prefill_rows<D, NC, W, ST, TWO_PASS, true, WIN>(*g, tabs, q, out, base, n_q, st, *S, w);
 }
 
 template <int D, int NC, int W, int ST, bool TWO_PASS>
@@ -805,8 +851,17 @@ __global__ void __launch_bounds__(W * 64, D == 64 && ST == 32 && NC == 4 ? 3 : 2
                                                            const int32_t *__restrict__ q, int32_t *out,
                                                            int64_t base, int64_t n_q, DevStats *st) {
     __shared__ Lds<D, NC, W, ST> S;
-    if (prefill_rows<D, NC, W, ST, TWO_PASS, false>(g, tabs, q, out, base, n_q, st, S))
+    if (prefill_rows<D, NC, W, ST, TWO_PASS, false, false>(g, tabs, q, out, base, n_q, st, S, nullptr))
         prefill_rows_wide<D, NC, W, ST, TWO_PASS>(&g, tabs, q, out, base, n_q, st, &S);
+}
+
+// The same for queries that see a window and the first rows.
+template <int D, int NC, int W, int ST, bool TWO_PASS>
+__global__ void __launch_bounds__(W * 64, D == 64 && ST == 32 && NC == 4 ? 3 : 2) window_kernel(Geom g, const Tables *__restrict__ tabs,
+                                                                                                WindowJob w, DevStats *st) {
+    __shared__ Lds<D, NC, W, ST> S;
+    if (prefill_rows<D, NC, W, ST, TWO_PASS, false, true>(g, tabs, w.q, w.out, 0, w.n, st, S, &w))
+        prefill_rows_wide<D, NC, W, ST, TWO_PASS, true>(&g, tabs, w.q, w.out, 0, w.n, st, &S, &w);
 }
 
 template <int D, int NC, int W, int ST>
@@ -819,6 +874,19 @@ hipError_t launch(hipStream_t s, const Geom &g, const Tables *t, const int32_t *
     else
         hipExtLaunchKernelGGL((prefill_kernel<D, NC, W, ST, false>), dim3((unsigned)blocks), dim3(W * 64), 0, s, ev.start,
                               ev.stop, 0, g, t, q, out, base, n_q, st);
+    return hipGetLastError();
+}
+
+template <int D, int NC, int W, int ST>
+hipError_t launch_window(hipStream_t s, const Geom &g, const Tables *t, const WindowJob &w, LaunchEv ev, DevStats *st) {
+    const int64_t blocks = (w.n * g.G + W * 16 - 1) / (W * 16) * w.nseq * g.n_kv;
+    if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+    if (w.two_pass)
+        hipExtLaunchKernelGGL((window_kernel<D, NC, W, ST, true>), dim3((unsigned)blocks), dim3(W * 64), 0, s, ev.start, ev.stop, 0,
+                              g, t, w, st);
+    else
+        hipExtLaunchKernelGGL((window_kernel<D, NC, W, ST, false>), dim3((unsigned)blocks), dim3(W * 64), 0, s, ev.start, ev.stop,
+                              0, g, t, w, st);
     return hipGetLastError();
 }
 
@@ -844,6 +912,18 @@ hipError_t launch_attend_prefill(hipStream_t s, const Geom &g, const Tables *t, 
     }
     if (g.vb <= 2) return pf::launch<128, 4, 8, 32>(s, g, t, q, out, base, n_q, two_pass, ev, st);
     return pf::launch<128, 8, 8, 32>(s, g, t, q, out, base, n_q, two_pass, ev, st);
+}
+
+hipError_t launch_attend_window_prompt(hipStream_t s, const Geom &g, const Tables *t, const WindowJob &w, LaunchEv ev, DevStats *st) {
+    if (g.capacity > PREFILL_MAX_ROWS) return hipErrorInvalidValue;
+    if (g.d == 64) {
+        const bool few = w.n * w.nseq * g.G * g.n_kv < 32768;          // (as a prompt's)
+        if (g.vb <= 2)
+            return few ? pf::launch_window<64, 4, 4, 64>(s, g, t, w, ev, st) : pf::launch_window<64, 4, 4, 32>(s, g, t, w, ev, st);
+        return pf::launch_window<64, 8, 4, 32>(s, g, t, w, ev, st);
+    }
+    if (g.vb <= 2) return pf::launch_window<128, 4, 8, 32>(s, g, t, w, ev, st);
+    return pf::launch_window<128, 8, 8, 32>(s, g, t, w, ev, st);
 }
 
 }  // namespace insitu

@@ -390,6 +390,8 @@ struct WindowJob {
     int64_t n, window, sinks;
     int32_t seq_lo, nseq, two_pass;
 };
+// On the prefill kernel (attend_prefill.hip), where prefill_supported and up to PREFILL_MAX_ROWS of capacity.
+hipError_t launch_attend_window_prompt(hipStream_t s, const Geom &g, const Tables *t, const WindowJob &w, LaunchEv ev, DevStats *st);
 hipError_t launch_attend_window_serial(hipStream_t s, const Geom &g, const Tables *t, const WindowJob &w, LaunchEv ev,
                                        DevStats *st);
 
