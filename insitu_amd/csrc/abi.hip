@@ -196,7 +196,7 @@ struct insitu_cache {
     // prefill (insitu_attend_causal): scratch for a virtual batch of queries, their lengths
     ChunkScratch prefill_scr;
     int64_t *prefill_len = nullptr;
-    void *tree_scr = nullptr;             // insitu_attend_tree: spans' maxima and runs, one call's worth
+    void *tree_scr = nullptr;             // insitu_attend_tree, insitu_attend_window: spans' maxima and runs, one call's worth
     size_t tree_bytes = 0;
     uint8_t *keep_scr = nullptr;          // insitu_cache_keep: rows on their way, for long lists
     size_t keep_bytes = 0;
@@ -1274,10 +1274,20 @@ int insitu_attend_window(insitu_cache *k, int32_t seq, int64_t n, int64_t window
     HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
     int rc = stats ? zero_stats(k) : INSITU_OK;
     if (rc) return rc;
+    const bool fast = mode != INSITU_SERIAL && prefill_supported(k->g);
+    const bool spans = fast && (n * k->g.G <= 512 || k->g.capacity > PREFILL_MAX_ROWS);
+    if (spans) {
+        rc = grow(k, k->tree_scr, k->tree_bytes, window_scratch_bytes(k->g, n, w.nseq));
+        if (rc) return rc;
+    }
     LaunchEv ev;
     rc = timing_events(k->ctx, &ev);
     if (rc) return rc;
-    if (mode != INSITU_SERIAL && prefill_supported(k->g) && k->g.capacity <= PREFILL_MAX_ROWS)
+    if (spans)
+        HIP_TRY(launch_attend_window_spans(k->ctx->stream, k->g, k->tabs, k->tabs_host, w, stats != nullptr, k->tree_scr, k->tree_bytes,
+                                           ev, k->stats),
+                "window attend launch");
+    else if (fast)
         HIP_TRY(launch_attend_window_prompt(k->ctx->stream, k->g, k->tabs, w, ev, k->stats), "window attend launch");
     else
         HIP_TRY(launch_attend_window_serial(k->ctx->stream, k->g, k->tabs, w, ev, k->stats), "window attend launch");

@@ -361,6 +361,37 @@ def test_captured_and_replayed(ctx):
                 assert torch.equal(x, y), f"replay {r} call {shapes[i]}"
 
 
+def test_captured_without_scratch(ctx):
+    """A capture allocates nothing: a call whose scratch is not there yet says so."""
+    import torch
+    from insitu_amd import _lib
+    from insitu_amd.attention import CompressedAttention
+    from insitu_amd.runtime import Context
+    side = torch.cuda.Stream(ctx.torch_device)
+    own = Context(ctx.device, stream=side)
+    rng = np.random.default_rng(14)
+    with torch.cuda.stream(side):
+        c = _cache(own, FORMATS[0], [900])
+        _fill(c, FORMATS[0], [900], *(_draw(rng, 65536, 1, 900, N_KV, 64) for _ in "kv"))
+        a = CompressedAttention(c)
+        q = torch.from_numpy(_draw(rng, 1 << 14, 3, N_KV * 4, 64).astype(np.int32)).to(own.torch_device)
+        out = torch.zeros_like(q)
+        side.synchronize()
+        with pytest.raises(_lib.InsituError, match="before the capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                a.attend_window(q, 700, 4, out=out, stats=False)
+        want = a.attend_window(q, 700, 4, stats=False)[0]
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            a.attend_window(q, 700, 4, out=out, stats=False)
+        for _ in range(3):
+            out.zero_()
+            g.replay()
+            side.synchronize()
+            assert torch.equal(out, want)
+
+
 def test_refusals(ctx):
     import torch
     from insitu_amd import _lib
