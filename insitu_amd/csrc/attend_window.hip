@@ -45,7 +45,8 @@ __device__ __forceinline__ WindowRows rows_of(const WindowJob &w, int64_t end) {
     return WindowRows{w.sinks, end > w.window ? end - w.window : 0};
 }
 
-constexpr int FW = 8;                                  // waves a workgroup
+constexpr int LATE = 16;                               // tiles by which the first span is shorter, online
+constexpr int DPP_ROW_ROR4 = 0x124, DPP_ROW_ROR12 = 0x12C;       // lane i <- lane (i - 4), (i + 4) mod 16 of its row
 constexpr int RUN_MAX = 32768;                         // tokens of a run, so that its L fits 32 bits
 constexpr uint32_t LUT_N = LUT_SPAN + 1;
 constexpr double TERM_MAGIC = 402653184.0 + 8421504.0; // 1.5 * 2^28 + 0x808080: ulp 2^-24
@@ -63,7 +64,7 @@ struct Job {
     Geom g;
     const Tables *tabs;
     WindowJob w;
-    int64_t rows;                                      // n G, of a (sequence, KV head)
+    int32_t rows;                                      // n G, of a (sequence, KV head)
     int32_t chains, extra, count;                      // extra: runs a workgroup has in the scratch; count: statistics
     double kc_absmax, vcs[8], vcmax;                   // vcs: value centroids / 2^23
     uint32_t wide, delta_max;                          // wide: |v_norm p| up to which a term is two balanced bytes
@@ -76,6 +77,22 @@ __device__ __forceinline__ int32_t imax(int32_t a, int32_t b) { return a > b ? a
 __device__ __forceinline__ int32_t imin(int32_t a, int32_t b) { return a < b ? a : b; }
 __device__ __forceinline__ uint32_t magnitude(int32_t x) { return x < 0 ? 0u - (uint32_t)x : (uint32_t)x; }
 
+// A barrier for what LDS holds: loads and stores of memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+// The value of the lane R j columns on, in turn: tokens' group j in the place of the first.
+template <int R>
+__device__ __forceinline__ uint32_t group_of(int j, uint32_t v) {
+    if constexpr (R == 16) return v;
+    // (every lane has a source; the compiler then takes the move into the instruction that uses it)
+    if (j == 0) return v;
+    if (R == 8 || j == 2) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, DPP_ROW_ROR8, 0xF, 0xF, true);
+    if (j == 1) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, DPP_ROW_ROR12, 0xF, 0xF, true);
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, DPP_ROW_ROR4, 0xF, 0xF, true);
+}
 // Over the lanes of a row: its column of every group of tokens (R apart), four times 16 lanes.
 template <int R, class F>
 __device__ __forceinline__ uint32_t row_all(uint32_t v, F f) {
@@ -103,26 +120,36 @@ __device__ __forceinline__ uint32_t row_sum(uint32_t v) {
 template <int R>
 struct Place {
     int b, seq, kvh;                                   // sequence of the call, of the cache
-    int64_t row0;                                      // the tile's first row
+    int row0;                                          // the tile's first row
+    int64_t len;                                       // (requested first, used last)
     int64_t base, U;                                   // the first query's own row; what the tile sees
     int64_t skip_at, skip;                             // where numbers and rows part, and how far
     int64_t first_end, last_lo;                        // the first row's end, where the last row's window begins
     __device__ __forceinline__ explicit Place(const Job &J) {
-        const int chain = (int)(blockIdx.x % (unsigned)J.chains);
-        row0 = (int64_t)(blockIdx.x / (unsigned)J.chains) * R;
-        b = chain / J.g.n_kv;
-        kvh = chain % J.g.n_kv;
+        const uint32_t chain = blockIdx.x % (uint32_t)J.chains;
+        row0 = (int)(blockIdx.x / (uint32_t)J.chains) * R;
+        b = (int)(chain / (uint32_t)J.g.n_kv);
+        kvh = (int)(chain % (uint32_t)J.g.n_kv);
         seq = J.w.seq_lo + b;
-        base = end_of(J.w, seq, 0) - 1;
-        const int64_t last = (row0 + R < J.rows ? row0 + R : J.rows) - 1;
-        first_end = base + row0 / J.g.G + 1;
-        const int64_t end = base + last / J.g.G + 1, lo = first_end - J.w.window;
+        len = J.w.len[seq];
+    }
+    __device__ __forceinline__ void find(const Job &J) {
+        base = (len > J.w.n ? len : J.w.n) - J.w.n;
+        const int last = (row0 + R < J.rows ? row0 + R : J.rows) - 1;
+        first_end = base + (uint32_t)row0 / (uint32_t)J.g.G + 1;
+        const int64_t end = base + (uint32_t)last / (uint32_t)J.g.G + 1, lo = first_end - J.w.window;
         last_lo = end - J.w.window;
-        skip_at = (J.w.sinks + 15) / 16 * 16;
-        skip = lo > skip_at ? lo / 16 * 16 - skip_at : 0;
+        skip_at = (J.w.sinks + 15) & ~(int64_t)15;
+        skip = lo > skip_at ? (lo & ~(int64_t)15) - skip_at : 0;
         U = end - skip;
     }
     __device__ __forceinline__ int64_t at(int64_t u) const { return u < skip_at ? u : u + skip; }      // u a multiple of 16
+    // of row r of the KV head: its query's place among the queries, and its own row's end
+    __device__ __forceinline__ int64_t query(const Job &J, int r) const {
+        const uint32_t G = (uint32_t)J.g.G, i = (uint32_t)r / G;
+        return ((int64_t)b * J.w.n + i) * J.g.n_q + kvh * G + ((uint32_t)r - i * G);
+    }
+    __device__ __forceinline__ int64_t end(const Job &J, int r) const { return base + (uint32_t)r / (uint32_t)J.g.G + 1; }
 };
 
 // A row's queries, lane = (row, D / 4 channels from grp D / 4 on, in the order the codes expand in), as digits.
@@ -131,12 +158,13 @@ struct Query {
     v4i qd[3][D / 64];
     bool bad, check;                                   // needs the serial path; scores may leave int32
     uint32_t out;                                      // values out of range
-    __device__ __forceinline__ void make(const int32_t *q, double kc_absmax) {
-        u128 raw[4 * (D / 64)];
+    u128 raw[4 * (D / 64)];
+    __device__ __forceinline__ void fetch(const int32_t *q) {
 #pragma unroll
         for (int i = 0; i < 4 * (D / 64); ++i) raw[i] = *(const u128 *)(q + 4 * i);
-        uint64_t l1 = 0;
-        uint32_t top = 0;
+    }
+    __device__ __forceinline__ void make(double kc_absmax) {
+        uint32_t l1 = 0, top = 0;                      // (l1: of a row that is not bad at most 32 x 2^23)
         out = 0;
 #pragma unroll
         for (int k = 0; k < D / 64; ++k) {
@@ -179,11 +207,10 @@ struct Keys {
     static constexpr int J = 16 / R;
     Codes<D, KB> c[J];
     uint4 norms;                                       // (k, v) int16 each
-    // Tiles past the last of U rows are that one again (what lies there is masked). Rows up to a tile's end are
+    // Tiles past the span's last are that one again (and are not looked at). Rows up to a tile's end are
     // read whatever the sequence's length: a plane holds a multiple of 256.
-    __device__ __forceinline__ void load(const Place<R> &p, const uint8_t *hb, const uint8_t *nb, int64_t span, int64_t u) {
+    __device__ __forceinline__ void load(const Place<R> &p, const uint8_t *hb, const uint8_t *nb, int64_t span, int64_t u, int64_t last) {
         const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
-        const int64_t last = (p.U - 1) & ~(int64_t)15;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int64_t v = u + 16 * j < last ? u + 16 * j : last;
@@ -194,10 +221,10 @@ struct Keys {
     }
 };
 
-template <int D, int NC, int R>
+template <int D, int NC, int R, int FW>
 struct Lds {
     static constexpr int J = 16 / R, RS = D == 64 ? 60 : 116;       // (the widest row: 4-bit keys, 3-bit values)
-    static constexpr int SCORED = D == 128 && R == 16 ? 8 : 10;      // steps of a wave whose scores are kept
+    static constexpr int SCORED = FW > 8 ? 7 : D == 128 && R == 16 ? 8 : 10;      // steps of a wave whose scores are kept
     static constexpr int FIRST = FW * R;               // runs: the first of each (span, row), and others
     static constexpr int NEAR = FIRST + (D == 64 ? (R == 16 ? 32 : 96) : (R == 16 ? 8 : R == 8 ? 24 : 48));
     alignas(16) v4i q[J][3][D / 64][64];
@@ -211,37 +238,44 @@ struct Lds {
     uint16_t lut[LUT_N + 7];
     int32_t top[FW][R];
     uint32_t ev[FW][R];
+    float bound[FW][R];                                // of the sum of |terms| of a span
     uint32_t qbad, over, check, pool, fail;            // rows as bits; runs taken
     unsigned long long events, bad, ovf, acc, score_max, range;
 };
 
-template <int D, int KB, int NC, int R>
-__global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
-    using L = Lds<D, NC, R>;
+// FW: waves a workgroup.
+template <int D, int KB, int NC, int R, int FW>
+__global__ void __launch_bounds__(FW * 64, FW / 4) span_kernel(Job J) {
+    using L = Lds<D, NC, R, FW>;
     constexpr int JT = L::J, ST = 16 * JT, CT = D / 16, PVK = NC / 4;
     __shared__ L S;
-    const Place<R> p(J);
+    Place<R> p(J);
     const Geom &g = J.g;
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, grp = lane >> 4, mine = col / R, r = col % R;
-    const uint8_t *hb = plane_ptr(g, p.seq, p.kvh, 0), *nb = hb + (g.n_planes - 1) * g.span;
-    // the wave's span
-    const int64_t span = (p.U + FW * ST - 1) / (FW * ST) * ST;
-    const int64_t lo = wv * span, hi = lo + span < p.U ? lo + span : p.U;
-    Keys<D, KB, R> next;
-    if (lo < hi) next.load(p, hb, nb, g.span, lo);
-    const int32_t kc = (int32_t)J.tabs->kc[tid & 15], ex = J.tabs->exp_table[tid & 255];
-    // the lane's row
-    const int64_t row = p.row0 + r < J.rows ? p.row0 + r : J.rows - 1;
-    const int64_t qrow = (((int64_t)p.b * J.w.n + row / g.G) * g.n_q + p.kvh * g.G + row % g.G) * D;
-    const int64_t end = p.base + row / g.G + 1, wlo = end - J.w.window;
+    // the lane's row, and what the tables are made of: requested together
+    const int row = p.row0 + r < J.rows ? p.row0 + r : J.rows - 1;
     Query<D, KB> Q;
-    if (wv < JT) Q.make(J.w.q + qrow + grp * (D / 4), J.kc_absmax);
+    if (wv < JT) Q.fetch(J.w.q + p.query(J, row) * D + grp * (D / 4));
+    const int32_t kc = (int32_t)J.tabs->kc[tid & 15], ex = J.tabs->exp_table[tid & 255];
+    p.find(J);
+    const uint8_t *hb = plane_ptr(g, p.seq, p.kvh, 0), *nb = hb + (g.n_planes - 1) * g.span;
+    // the wave's span, in tiles of 16: the first one's, which has most of the events, is shorter by what they cost
+    const int nt = (int)((p.U + 15) >> 4), late = J.w.two_pass ? 0 : LATE;
+    int t0 = (int)((uint32_t)(nt + late + FW - 1) / FW) - late;
+    t0 = t0 < 1 ? 1 : t0;
+    const int per = (int)((uint32_t)(nt - t0 + FW - 2) / (FW - 1));
+    const int64_t lo = wv == 0 ? 0 : 16 * (int64_t)(t0 + (wv - 1) * per);
+    const int64_t stop = 16 * (int64_t)(t0 + wv * per), hi = stop < p.U ? stop : p.U, last = (hi - 1) & ~(int64_t)15;
+    Keys<D, KB, R> next;
+    if (lo < hi) next.load(p, hb, nb, g.span, lo, last);
+    const int64_t end = p.end(J, row), wlo = end - J.w.window;
+    if (wv < JT) Q.make(J.kc_absmax);
 
     // -- tables ------------------------------------------------------------------------------
     if (tid == 0) {
-        S.qbad = S.over = S.check = S.pool = S.fail = 0;
-        S.events = S.bad = S.ovf = S.acc = S.score_max = S.range = 0;
+        S.over = S.pool = S.fail = 0;
+        S.events = S.bad = S.ovf = S.acc = S.score_max = 0;
     }
     if (tid < 256) {
 #pragma unroll
@@ -259,19 +293,23 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
 #pragma unroll
             for (int b = 0; b < D / 64; ++b) S.q[wv][l][b][lane] = mine == wv ? Q.qd[l][b] : v4i{0, 0, 0, 0};
     }
-    __syncthreads();
-    if (wv == 0 && p.row0 + r < J.rows && mine == 0) {
-        if (Q.bad && grp == 0) atomicOr(&S.qbad, 1u << r);
-        if (Q.check && grp == 0) atomicOr(&S.check, 1u);
-        if (J.count && Q.out) atomicAdd(&S.range, (unsigned long long)Q.out);
+    if (wv == 0) {
+        const bool there = p.row0 + r < J.rows;
+        const uint32_t bad = (uint32_t)__ballot(there && Q.bad), check = __ballot(there && Q.check) != 0;
+        const int64_t out = J.count ? wave_sum_i64(there && mine == 0 ? Q.out : 0) : 0;
+        if (lane == 0) {
+            S.qbad = bad & ((1u << R) - 1u);
+            S.check = check;
+            S.range = (unsigned long long)out;
+        }
     }
+    __syncthreads();
     uint32_t dg[3][4];
 #pragma unroll
     for (int i = 0; i < 3; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) dg[i][j] = (uint32_t)uni32((int)S.dig[i][j]);
 
-    __syncthreads();
     const bool check = uni32((int)S.check) != 0;
     const uint32_t qbad = (uint32_t)uni32((int)S.qbad);      // (such a row is taken to see nothing)
     // which of the lane's 4 tokens of the step its row sees, a bit each
@@ -281,20 +319,21 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
             const int64_t k = e - t;
             return k <= 0 ? 0u : k >= 4 ? 15u : (1u << (int)k) - 1u;
         };
-        return (qbad >> r & 1u) != 0 ? 0u : (~bits(wlo) | bits(J.w.sinks)) & bits(end);
+        return (qbad >> r & 1u) != 0 || u + 16 * mine >= hi ? 0u : (~bits(wlo) | bits(J.w.sinks)) & bits(end);
     };
     // whether a row may not see all of a step
     auto edge = [&](int64_t u) __attribute__((always_inline)) {
         const int64_t t = p.at(u), e = p.at(u + ST - 16) + 16;
-        return qbad != 0 || u + ST > p.U || e > p.first_end || (t < p.last_lo && e > J.w.sinks);
+        return qbad != 0 || u + ST > hi || e > p.first_end || (t < p.last_lo && e > J.w.sinks);
     };
     // floor(dot k_norm / 2^24) of the lane's row and 4 tokens: dot = 2^16 H + L. Returns whether a visible one left int32
-    auto scores = [&](const Keys<D, KB, R> &k, bool check, uint32_t in, int32_t (&s)[4]) __attribute__((always_inline)) {
+    auto scores = [&](const Keys<D, KB, R> &k, int64_t u, bool check, uint32_t in, int32_t (&s)[4]) __attribute__((always_inline)) {
         v4i T[5];
 #pragma unroll
         for (int i = 0; i < 5; ++i) T[i] = v4i{0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < JT; ++j) {
+            if (j > 0 && u + 16 * j >= hi) break;
 #pragma unroll
             for (int b = 0; b < D / 64; ++b) {
                 v4i a[3], q[3];
@@ -329,12 +368,12 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
         int step = 0;
         for (int64_t u = lo; u < hi; u += ST, ++step) {
             const Keys<D, KB, R> cur = next;
-            if (u + ST < hi) next.load(p, hb, nb, g.span, u + ST);
+            if (u + ST < hi) next.load(p, hb, nb, g.span, u + ST, last);
             int32_t s[4];
             uint32_t in = 15u;
             const bool e = edge(u);
             if (e) in = visible(u);
-            over |= scores(cur, check, in, s);
+            over |= scores(cur, u, check, in, s);
             if (e) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -356,7 +395,30 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
             atomicMax(&S.score_max, (unsigned long long)(a > c ? a : c));
         }
     }
-    __syncthreads();
+    // the lane's value words: CT codes together, of the field's words w0 and, over its end, w0 + 1
+    const int bit = col * CT * g.vb, w0 = bit >> 5, sh = bit & 31;
+    const int w1 = imin(w0 + 1, g.value_bytes / 4 - 1);
+    const int pv = (g.key_bytes + 15) / 16;
+    const uint8_t *const va0 = hb + (pv + w0 / 4) * g.span + (w0 % 4) * 4, *const va1 = hb + (pv + w1 / 4) * g.span + (w1 % 4) * 4;
+    const int vw0 = imin(16, g.value_bytes - w0 / 4 * 16), vw1 = imin(16, g.value_bytes - w1 / 4 * 16);
+    uint32_t vw[JT][4][NC == 8 ? 2 : 1];
+    uint4 vnorm;
+    auto values = [&](int64_t u) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+            const int64_t t = p.at(u + 16 * j < last ? u + 16 * j : last) + 4 * grp;
+            const uint8_t *const x = va0 + t * vw0, *const y = va1 + t * vw1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                vw[j][i][0] = *(const uint32_t *)(x + i * vw0);
+                if constexpr (NC == 8) vw[j][i][NC / 8] = *(const uint32_t *)(y + i * vw1);
+            }
+        }
+        const int64_t t = u + 16 * mine < last ? u + 16 * mine : last;
+        vnorm = *(const uint4 *)(nb + (p.at(t) + 4 * grp) * 4);
+    };
+    if (lo < hi) values(lo);                           // (in flight past the barrier)
+    lds_barrier();
 
     // -- the walk ------------------------------------------------------------------------------
     const int64_t wg = blockIdx.x;
@@ -370,15 +432,10 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
         for (int i = 0; i < NC; ++i) vcs[i] = J.vcs[i];
         const double vcmax = J.vcmax;
         const uint32_t delta_max = J.delta_max, wide = J.wide;
-        // the lane's value words: CT codes together, of the field's words w0 and, over its end, w0 + 1
-        const int bit = col * CT * g.vb, w0 = bit >> 5, sh = bit & 31;
-        const int w1 = imin(w0 + 1, g.value_bytes / 4 - 1);
-        const int pv = (g.key_bytes + 15) / 16;
-        const uint8_t *const va0 = hb + (pv + w0 / 4) * g.span + (w0 % 4) * 4, *const va1 = hb + (pv + w1 / 4) * g.span + (w1 % 4) * 4;
-        const int vw0 = imin(16, g.value_bytes - w0 / 4 * 16), vw1 = imin(16, g.value_bytes - w1 / 4 * 16);
-
         bool first = wv == 0;                          // what the span finds is nothing: it scales in place
-        v4i T[CT][3];                                  // the run's digit sums: lane = (row of its tokens, 4 channels a product)
+        // the run's digit sums, lane = (row, 4 channels a product) in the columns of the first group of tokens (the others'
+        // take another group's terms with these codes, and are not read)
+        v4i T[CT][3];
 #pragma unroll
         for (int c = 0; c < CT; ++c)
 #pragma unroll
@@ -399,29 +456,18 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
             const uint32_t w = (uint32_t)a - (uint32_t)b;
             return w < delta_max ? w : delta_max;
         };
-        // the rows' sums of the run, in all their lanes: T[c][0] takes them
+        // the run's sums: T[c][0] takes them
         auto gather = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int c = 0; c < CT; ++c)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    uint32_t x = (((uint32_t)T[c][2][i] << 8) + (uint32_t)T[c][1][i]) * 256u + (uint32_t)T[c][0][i];
-                    if constexpr (R <= 4) x += xor_lane32<4>(x, lane);
-                    if constexpr (R <= 8) x += xor_lane32<8>(x, lane);
-                    T[c][0][i] = (int)x;
+                    T[c][0][i] = (int)((((uint32_t)T[c][2][i] << 8) + (uint32_t)T[c][1][i]) * 256u + (uint32_t)T[c][0][i]);
                     T[c][1][i] = T[c][2][i] = 0;
                 }
         };
-        // (behind gather) one lane of a row's goes on with its sums, those of the rows where `clear` with none
-        auto spread = [&](bool clear) __attribute__((always_inline)) {
-            const bool keep = !clear && mine == 0;
-#pragma unroll
-            for (int c = 0; c < CT; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) T[c][0][i] = keep ? T[c][0][i] : 0;
-        };
-        // (behind gather) the open run of the rows where `has`: into its record. A lane writes 4 / J of its row's
-        // four times CT channels.
+        // (behind gather) the open run of the rows where `has`: into its record
+        float bs_all = 0.0f;                           // a bound of the row's sums |terms| so far
         auto hand_over = [&](bool has, int to) __attribute__((always_inline)) {
             const uint32_t Ls = row_sum<R>(lp + (grp == 0 && mine == 0 ? l0 : 0u));
             float b = bs;
@@ -429,10 +475,11 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
             if constexpr (R <= 8) b += __uint_as_float(xor_lane32<8>(__float_as_uint(b), lane));
             b += __uint_as_float(xor_lane32<16>(__float_as_uint(b), lane));
             b += __uint_as_float(xor_lane32<32>(__float_as_uint(b), lane));
+            b = b * (float)vcmax * 1.001f + (float)(RUN_MAX + ST);
+            bs_all += has ? b : 0.0f;
             if (!has || slot < 0) return;
             const bool used = Ls != 0 || fopen != 1u << PROB_FRAC;
-            const uint4 mt = make_uint4(Ls, fopen | (used ? USED : 0u), (uint32_t)to,
-                                        __float_as_uint(b * (float)vcmax * 1.001f + (float)(RUN_MAX + ST)));
+            const uint4 mt = make_uint4(Ls, fopen | (used ? USED : 0u), (uint32_t)to, __float_as_uint(b));
             const bool near = slot < L::NEAR;
             if (grp == 0 && mine == 0) {
                 if (near)
@@ -440,78 +487,37 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
                 else
                     far_meta[slot - L::NEAR] = mt;
             }
-            if (!used) return;
+            if (!used || mine != 0) return;
             int32_t *const dst = near ? &S.S[slot][0] : far_S + (int64_t)(slot - L::NEAR) * D;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (i / (4 / JT) != mine) continue;
 #pragma unroll
                 for (int c = 0; c < CT; c += 4)
                     *(v4i *)(dst + (4 * grp + i) * CT + c) = v4i{T[c][0][i], T[c + 1][0][i], T[c + 2][0][i], T[c + 3][0][i]};
             }
         };
-        // the run of the rows where `has` ends, and one with factor f begins. A row for which none is left goes
-        // token by token and writes no more.
-        auto next_run = [&](bool has, uint32_t f) __attribute__((always_inline)) {
-            int to = 0;
-            if (has && grp == 0 && mine == 0) to = (int)atomicAdd(&S.pool, 1u);
-            to = __shfl(to, r);
-            const bool none = L::FIRST + to >= L::NEAR + J.extra;
-            bad = bad || (has && none);
-            to = none ? -1 : L::FIRST + to;
-            gather();
-            hand_over(has, to);
-            if (has) {
-                slot = to;
-                fopen = f;
-                lp = 0;
-                l0 = 0;
-                bs = 0.0f;
-            }
-            spread(has);
-        };
-
         int step = 0;
         for (int64_t u = lo; u < hi; u += ST, ++step) {
-            // the values' words and norms, before it is known whether any counts
-            const int64_t last = (p.U - 1) & ~(int64_t)15;
-            uint32_t vw[JT][4][NC == 8 ? 2 : 1];
-#pragma unroll
-            for (int j = 0; j < JT; ++j) {
-                const int64_t t = p.at(u + 16 * j < last ? u + 16 * j : last) + 4 * grp;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    vw[j][i][0] = *(const uint32_t *)(va0 + (t + i) * vw0);
-                    if constexpr (NC == 8) vw[j][i][NC / 8] = *(const uint32_t *)(va1 + (t + i) * vw1);
-                }
-            }
-            int32_t s[4], vn[4];
+            int32_t s[4];
             if (step < L::SCORED) {
-                const int64_t t = u + 16 * mine < last ? u + 16 * mine : last;
-                const uint4 nw = *(const uint4 *)(nb + (p.at(t) + 4 * grp) * 4);
                 const int4 x = S.u.score[wv][step][lane];
                 s[0] = x.x, s[1] = x.y, s[2] = x.z, s[3] = x.w;
-                vn[0] = (int32_t)nw.x >> 16, vn[1] = (int32_t)nw.y >> 16, vn[2] = (int32_t)nw.z >> 16, vn[3] = (int32_t)nw.w >> 16;
             } else {
                 Keys<D, KB, R> k;
-                k.load(p, hb, nb, g.span, u);
-                scores(k, false, 0, s);
+                k.load(p, hb, nb, g.span, u, last);
+                scores(k, u, false, 0, s);
                 if (edge(u)) {
                     const uint32_t in = visible(u);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[i] = in >> i & 1 ? s[i] : NONE;
                 }
-                const uint4 nw = k.norms;
-                vn[0] = (int32_t)nw.x >> 16, vn[1] = (int32_t)nw.y >> 16, vn[2] = (int32_t)nw.z >> 16, vn[3] = (int32_t)nw.w >> 16;
             }
+            const int32_t vn[4] = {(int32_t)vnorm.x >> 16, (int32_t)vnorm.y >> 16, (int32_t)vnorm.z >> 16, (int32_t)vnorm.w >> 16};
             const int32_t mx = imax(imax(s[0], s[1]), imax(s[2], s[3]));
             const uint64_t evl = __ballot(mx > m);
-            if (evl == 0 && __ballot((uint32_t)m - (uint32_t)mx < delta_max) == 0) continue;      // every p is 0
-            if (run >= RUN_MAX || __ballot(bs > bs_max) != 0) {      // L or acc may leave 32 bits: they become a run
-                first = false;
-                next_run(true, 1u << PROB_FRAC);
-                run = 0;
-            }
+            const bool ends = u + ST >= hi;
+            // (else every p is 0; the last step's run ends there all the same)
+            if (ends || evl != 0 || __ballot((uint32_t)m - (uint32_t)mx < delta_max) != 0) {
             run += ST;
             const float bs0 = bs;
             uint32_t pw[4];
@@ -549,17 +555,19 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
                 }
                 return top;
             };
-            // T += the terms in A where `mask` (bytes: tokens), in the column groups that have any
+            // T += the terms in A, those of a group of tokens turned into the first group's columns
             auto accumulate = [&](bool three, uint32_t mask) __attribute__((always_inline)) {
 #pragma unroll
                 for (int j = 0; j < JT; ++j) {
-                    const uint32_t on = JT == 1 || mine == j ? mask : 0u;
-                    if (JT > 1 && __ballot(on != 0) == 0) continue;
+                    if (JT > 1 && __ballot(mine == j && mask != 0) == 0) continue;
                     v4i B[3][PVK];
+                    const uint32_t on = group_of<R>(j, mask);
 #pragma unroll
                     for (int l = 0; l < 3; ++l)
 #pragma unroll
-                        for (int k = 0; k < PVK; ++k) B[l][k] = A[l][k] & (int)on;
+                        for (int k = 0; k < PVK; ++k)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) B[l][k][i] = (int)(group_of<R>(j, (uint32_t)A[l][k][i]) & on);
                     // the lane's codes of 4 tokens, in bytes or halves (the shift is opaque, so that the one-hot codes are
                     // made where they are used: kept over the segments' loop they take all registers there are)
                     int sh_ = sh;
@@ -613,6 +621,7 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
             };
             // events: the row's tokens, in the order (group of tokens, lane group, token), fall into segments, one more
             // than its events (bits 8 i of seg the segment of token i)
+            const uint32_t there = u + 16 * mine < hi ? ~0u : 0u;      // (the lane's tokens are the span's)
             uint32_t dl[4], fe[4] = {0, 0, 0, 0}, seg = 0;
             int row_ev = 0;
             if (evl == 0) {
@@ -655,25 +664,36 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
             const bool three = __ballot(top > wide) != 0;
             const float bs_step = bs - bs0;            // (every run of the step is bounded by all of it)
             for (int sg = 0;; ++sg) {
-                uint32_t mask = 0;                     // the segment's tokens, a byte each
+                uint32_t mask = there;
+                if (evl == 0) {
+                    lp += (pw[0] + pw[1]) + (pw[2] + pw[3]);
+                } else {                               // the segment's tokens, a byte each
+                    mask = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool now = ((seg >> (8 * i)) & 0xFFu) == (uint32_t)sg;
-                    mask |= now ? 0xFFu << (8 * i) : 0u;
-                    lp += now ? pw[i] : 0u;
+                    for (int i = 0; i < 4; ++i) {
+                        const bool now = ((seg >> (8 * i)) & 0xFFu) == (uint32_t)sg;
+                        mask |= now ? 0xFFu << (8 * i) : 0u;
+                        lp += now ? pw[i] : 0u;
+                    }
+                    mask &= there;
                 }
                 accumulate(three, mask);
-                const bool has = row_ev > sg;
-                if (__ballot(has) == 0) break;
-                // the event that opens segment sg + 1 of the row
+                // the rows whose run ends: with an event, or all with the span, or before L or acc could leave 32 bits
+                bool has = row_ev > sg;
+                const bool event = __ballot(has) != 0;
+                if (!event) {
+                    if (!ends && run < RUN_MAX && __ballot(bs > bs_max) == 0) break;
+                    has = true;
+                }
+                // the event opens segment sg + 1 of the row
                 uint32_t fd = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) fd = ((seg >> (8 * i)) & 0xFFu) == (uint32_t)(sg + 1) && fe[i] ? fe[i] : fd;
                 fd = row_or<R>(fd);
-                const uint32_t f = has ? lut(fd - 1u) : 1u << PROB_FRAC;
-                if (first) {
+                const uint32_t f = has && event ? lut(fd - 1u) : 1u << PROB_FRAC;
+                gather();
+                if (event && first) {
                     const uint32_t l = l0 + row_sum<R>(lp);
-                    gather();
                     if (has) {
 #pragma unroll
                         for (int c = 0; c < CT; ++c) {
@@ -688,64 +708,149 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
                         l0 = (uint32_t)(((uint64_t)l * f) >> PROB_FRAC);
                         lp = 0;
                     }
-                    spread(false);
-                } else {
-                    next_run(has, f);
-                    bs = has ? bs_step : bs;
+                    continue;
+                }
+                // a row for which no run is left goes token by token and writes no more
+                first = false;
+                int to = -1;
+                if (event || !ends) {
+                    if (has && grp == 0 && mine == 0) to = (int)atomicAdd(&S.pool, 1u);
+                    to = __shfl(to, r);
+                    const bool none = L::FIRST + to >= L::NEAR + J.extra;
+                    bad = bad || (has && none);
+                    to = none ? -1 : L::FIRST + to;
+                }
+                hand_over(has, to);
+                if (has) {
+                    slot = to;
+                    fopen = f;
+                    lp = 0;
+                    l0 = 0;
+                    bs = event ? bs_step : 0.0f;
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) T[c][0] = v4i{0, 0, 0, 0};
+                }
+                if (!event) {
+                    run = 0;
+                    break;
                 }
             }
+            }
+            if (u + ST < hi) values(u + ST);           // the next step's values are requested
         }
-        gather();
-        hand_over(true, -1);
         bad = bad || !((double)wmax * vcmax + 2.0 <= TERM_LIMIT);
         const uint32_t events = row_sum<R>(n_ev), any = row_or<R>(bad ? BAD : 0u);
-        if (grp == 0 && mine == 0) S.ev[wv][r] = events | any;
+        if (grp == 0 && mine == 0) {
+            S.ev[wv][r] = events | any;
+            S.bound[wv][r] = bs_all;
+        }
     }
     __syncthreads();
 
     // -- the runs: a wave a row, lane = channel ----------------------------------------------------
-    const int ns = (int)((p.U + span - 1) / span);
+    const int ns = per ? 1 + (int)((uint32_t)(nt - t0 + per - 1) / (uint32_t)per) : 1;      // spans that hold any
     for (int rr = wv; rr < R && p.row0 + rr < J.rows; rr += FW) {
         constexpr int CPL = D / 64;
         const uint32_t e = lane < ns ? S.ev[lane][rr] : 0u;
+        const uint4 mine_ = S.meta[(lane < ns ? lane : 0) * R + rr];   // lane i: the first run of span i
         bool wrong = __ballot((e & BAD) != 0) != 0 || ((qbad | S.over) >> rr & 1u) != 0;
         int64_t acc[CPL];                              // (online: what 32 bits hold)
         uint64_t l = 0;
 #pragma unroll
         for (int k = 0; k < CPL; ++k) acc[k] = 0;
-        for (int i = 0; i < ns && !wrong; ++i) {
-            for (int slot = i * R + rr; slot >= 0;) {
-                const bool near = slot < L::NEAR;
-                const uint4 mt = near ? S.meta[slot] : far_meta[slot - L::NEAR];
-                const uint32_t Lr = (uint32_t)uni32((int)mt.x), fr = (uint32_t)uni32((int)mt.y);
-                const float bound = __uint_as_float((uint32_t)uni32((int)mt.w));
-                const int32_t *const src = near ? &S.S[slot][0] : far_S + (int64_t)(slot - L::NEAR) * D;
-                slot = uni32((int)mt.z);
-                if (!(fr & USED)) continue;
-                if (J.w.two_pass) {                    // (no factors; clamped once, at the end)
+        // of a run that is not in LDS' first ones, or follows one of them
+        uint4 mt;
+        int32_t v[CPL];
+        auto follow = [&](int slot) __attribute__((always_inline)) {
+            if (slot < L::NEAR) {
+                mt = S.meta[slot];
 #pragma unroll
-                    for (int k = 0; k < CPL; ++k) acc[k] += src[lane + 64 * k];
-                    l += Lr;
-                    continue;
-                }
-                const int32_t ff = (int32_t)(fr & (USED - 1));
+                for (int k = 0; k < CPL; ++k) v[k] = S.S[slot][lane + 64 * k];
+            } else {
+                mt = far_meta[slot - L::NEAR];
+#pragma unroll
+                for (int k = 0; k < CPL; ++k) v[k] = far_S[(int64_t)(slot - L::NEAR) * D + lane + 64 * k];
+            }
+        };
+        auto scaled = [&](int32_t x, int32_t f) __attribute__((always_inline)) {       // floor(x f / 2^15)
+            return __mul24(x >> 16, 2 * f) + (int32_t)(__umul24((uint32_t)x & 0xFFFFu, (uint32_t)f) >> PROB_FRAC);
+        };
+        float all = lane < ns ? S.bound[lane][rr] : 0.0f;
+#pragma unroll
+        for (int o = 1; o < 16; o *= 2) all += __shfl_xor(all, o);
+        if (wrong) {
+        } else if (uni32(all <= 2147483000.0f)) {
+            // no |acc| on the way passes the sum of all |terms|: 32 bits, no clamp
+            int32_t a32[CPL], v2[CPL];
+#pragma unroll
+            for (int k = 0; k < CPL; ++k) {
+                a32[k] = 0;
+                v2[k] = S.S[rr][lane + 64 * k];
+            }
+            // (the loops are not unrolled: their instructions come from memory but once)
+#pragma unroll 1
+            for (int i = 0; i < ns; ++i) {
+                const int after = i + 1 < ns ? i + 1 : i;
 #pragma unroll
                 for (int k = 0; k < CPL; ++k) {
-                    const int32_t x = (int32_t)acc[k];
-                    const int32_t y = __mul24(x >> 16, 2 * ff) + (int32_t)(__umul24((uint32_t)x & 0xFFFFu, (uint32_t)ff) >> PROB_FRAC);
-                    wrong = wrong || !(fabsf((float)y) + bound <= 2147483000.0f);
-                    acc[k] = y + src[lane + 64 * k];
+                    v[k] = v2[k];
+                    v2[k] = S.S[after * R + rr][lane + 64 * k];
                 }
-                wrong = __ballot(wrong) != 0;
-                l = ((l * (uint32_t)ff) >> PROB_FRAC) + Lr;
+                uint32_t Lr = (uint32_t)__builtin_amdgcn_readlane((int)mine_.x, i), fr = (uint32_t)__builtin_amdgcn_readlane((int)mine_.y, i);
+                int slot = __builtin_amdgcn_readlane((int)mine_.z, i);
+#pragma unroll 1
+                for (;;) {
+                    if (fr & USED) {
+                        const int32_t ff = (int32_t)(fr & (USED - 1));
+                        if (ff != 1 << PROB_FRAC) {
+#pragma unroll
+                            for (int k = 0; k < CPL; ++k) a32[k] = scaled(a32[k], ff);
+                            l = (l * (uint32_t)ff) >> PROB_FRAC;
+                        }
+#pragma unroll
+                        for (int k = 0; k < CPL; ++k) a32[k] += v[k];
+                        l += Lr;
+                    }
+                    if (slot < 0) break;
+                    follow(slot);
+                    Lr = (uint32_t)uni32((int)mt.x);
+                    fr = (uint32_t)uni32((int)mt.y);
+                    slot = uni32((int)mt.z);
+                }
             }
+#pragma unroll
+            for (int k = 0; k < CPL; ++k) acc[k] = a32[k];
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < ns; ++i) {
+#pragma unroll 1
+                for (int slot = i * R + rr; slot >= 0;) {
+                    follow(slot);
+                    const uint32_t Lr = (uint32_t)uni32((int)mt.x), fr = (uint32_t)uni32((int)mt.y);
+                    const float bound = __uint_as_float((uint32_t)uni32((int)mt.w));
+                    slot = uni32((int)mt.z);
+                    if (!(fr & USED)) continue;
+                    const int32_t ff = (int32_t)(fr & (USED - 1));
+#pragma unroll
+                    for (int k = 0; k < CPL; ++k) {
+                        if (!J.w.two_pass) {           // (two-pass: no factors; clamped once, at the end)
+                            const int32_t y = scaled((int32_t)acc[k], ff);
+                            wrong = wrong || !(fabsf((float)y) + bound <= 2147483000.0f);
+                            acc[k] = y;
+                        }
+                        acc[k] += v[k];
+                    }
+                    l = (J.w.two_pass ? l : (l * (uint32_t)ff) >> PROB_FRAC) + Lr;
+                }
+            }
+            wrong = __ballot(wrong) != 0;
         }
         if (wrong) {
             if (lane == 0) atomicOr(&S.fail, 1u << rr);
             continue;
         }
         const Recip rc = reciprocal((int64_t)l);
-        const int64_t row_ = p.row0 + rr, at = (((int64_t)p.b * J.w.n + row_ / g.G) * g.n_q + p.kvh * g.G + row_ % g.G) * D;
+        const int64_t at = p.query(J, p.row0 + rr) * D;
         int64_t amax = 0, over = 0;
 #pragma unroll
         for (int k = 0; k < CPL; ++k) {
@@ -772,8 +877,7 @@ __global__ void __launch_bounds__(FW * 64, 2) span_kernel(Job J) {
     const uint32_t fail = (uint32_t)uni32((int)S.fail);
     for (int rr = wv; rr < R; rr += FW) {
         if (!(fail >> rr & 1u)) continue;
-        const int64_t row_ = p.row0 + rr, at = (((int64_t)p.b * J.w.n + row_ / g.G) * g.n_q + p.kvh * g.G + row_ % g.G) * D;
-        const int64_t T_ = p.base + row_ / g.G + 1;
+        const int64_t at = p.query(J, p.row0 + rr) * D, T_ = p.end(J, p.row0 + rr);
         serial_head<D / 64, L::RS>(g, J.tabs, J.tabs->kc, J.tabs->vc, J.w.q + at, p.seq, p.kvh, T_, J.w.two_pass, true, S.u.fb[wv],
                                    J.w.out + at, J.st, rows_of(J.w, T_));
         if (lane == 0) atomicAdd(&S.bad, 1ull);
@@ -834,12 +938,13 @@ int64_t extra_runs(const Geom &g, int64_t wgs) {
 template <int D, int KB, int NC>
 hipError_t launch(hipStream_t s, const Job &J, unsigned blocks, LaunchEv ev) {
     const int R = tile_rows(J.rows);
+    constexpr int FW = D == 64 && NC == 4 ? 12 : 8;
     if (R == 4)
-        hipExtLaunchKernelGGL((span_kernel<D, KB, NC, 4>), dim3(blocks), dim3(FW * 64), 0, s, ev.start, ev.stop, 0, J);
+        hipExtLaunchKernelGGL((span_kernel<D, KB, NC, 4, FW>), dim3(blocks), dim3(FW * 64), 0, s, ev.start, ev.stop, 0, J);
     else if (R == 8)
-        hipExtLaunchKernelGGL((span_kernel<D, KB, NC, 8>), dim3(blocks), dim3(FW * 64), 0, s, ev.start, ev.stop, 0, J);
+        hipExtLaunchKernelGGL((span_kernel<D, KB, NC, 8, FW>), dim3(blocks), dim3(FW * 64), 0, s, ev.start, ev.stop, 0, J);
     else
-        hipExtLaunchKernelGGL((span_kernel<D, KB, NC, 16>), dim3(blocks), dim3(FW * 64), 0, s, ev.start, ev.stop, 0, J);
+        hipExtLaunchKernelGGL((span_kernel<D, KB, NC, 16, FW>), dim3(blocks), dim3(FW * 64), 0, s, ev.start, ev.stop, 0, J);
     return hipGetLastError();
 }
 
@@ -859,7 +964,7 @@ hipError_t launch_attend_window_spans(hipStream_t s, const Geom &g, const Tables
     J.g = g;
     J.tabs = t;
     J.w = w;
-    J.rows = w.n * g.G;
+    J.rows = (int32_t)(w.n * g.G);
     J.chains = w.nseq * g.n_kv;
     J.extra = (int32_t)extra_runs(g, wgs);
     J.count = count ? 1 : 0;
