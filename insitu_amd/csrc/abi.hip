@@ -787,7 +787,7 @@ int insitu_append_float(insitu_cache *k, int32_t seq, const insitu_float_rows *k
     }
     HIP_TRY(launch_append_float(k->ctx->stream, k->g, k->tabs, float_rows(kr, seq >= 0), float_rows(vr, seq >= 0), type, n_tok, lo, hi,
                                 k->len_dev[k->cur], k->len_dev[k->cur ^ 1], k->len_now, k->desc.fmt.rot_rounds,
-                                k->desc.fmt.rot_signs, saturated != nullptr, k->stats),
+                                k->desc.fmt.rot_signs, k->tabs_host, saturated != nullptr, k->stats),
             "append launch");
     k->cur ^= 1;
     for (int b = lo; b < hi; ++b) k->len_host[b] += n_tok;

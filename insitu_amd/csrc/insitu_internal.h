@@ -407,7 +407,7 @@ struct FloatRows {
 };
 hipError_t launch_append_float(hipStream_t s, const Geom &g, const Tables *t, const FloatRows &k, const FloatRows &v, int type,
                                int n_tok, int seq_lo, int seq_hi, const int64_t *len_in, int64_t *len_out, int64_t *len_now,
-                               int rounds, const uint64_t (*signs)[2], bool count, DevStats *st);
+                               int rounds, const uint64_t (*signs)[2], const Tables &host, bool count, DevStats *st);
 // Rows t0 .. t0 + n - 1 (those below a sequence's length) in the basis before `rounds` rounds of rotation.
 hipError_t launch_read_float(hipStream_t s, const Geom &g, const Tables *t, const FloatRows &k, const FloatRows &v, int type,
                              int64_t t0, int64_t n, int seq_lo, int seq_hi, const int64_t *len, int rounds,
