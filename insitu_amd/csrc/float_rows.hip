@@ -23,11 +23,18 @@ template <class T>
 __device__ __forceinline__ float to_f32(T x) {
     return (float)x;
 }
-// Q8.16, half to even, at the 24 bits' ends where it lies beyond them; NaN is 0. sat: whether it did not fit
-__device__ __forceinline__ int32_t to_q16(float f, bool &sat) {
+// Q8.16, half to even, at the 24 bits' ends where it lies beyond them; NaN is 0 (as the conversion to 32 bits gives
+// it, which takes their ends beyond them).
+__device__ __forceinline__ int32_t to_q16(float f) {
     const float r = rintf(f * 65536.0f);
-    sat = !(r >= -8388608.0f && r <= 8388607.0f);
-    return r != r ? 0 : (int32_t)fminf(fmaxf(r, -8388608.0f), 8388607.0f);
+    int32_t x;
+    asm("v_cvt_i32_f32 %0, %1" : "=v"(x) : "v"(r));
+    return x < -(1 << 23) ? -(1 << 23) : x > (1 << 23) - 1 ? (1 << 23) - 1 : x;
+}
+// Whether it did not fit.
+__device__ __forceinline__ bool lost_q16(float f) {
+    const float r = rintf(f * 65536.0f);
+    return !(r >= -8388608.0f && r <= 8388607.0f);
 }
 
 constexpr int WAVES = 4;
@@ -63,9 +70,9 @@ __global__ void __launch_bounds__(64 * WAVES) append_kernel(Geom g, const Tables
 #pragma unroll
             for (int j = 0; j < CPL; ++j) {
                 const int ch = lane + 64 * j;
-                bool sat = false;
-                x[j] = ch < g.d ? to_q16(to_f32(p[ch]), sat) : 0;
-                lost += sat ? 1 : 0;
+                const float y = ch < g.d ? to_f32(p[ch]) : 0.0f;
+                x[j] = to_q16(y);
+                lost += lost_q16(y) ? 1 : 0;
             }
             rotate_loaded<CPL>(x, g.d, rounds, sg, y, nullptr);
             int64_t z[CPL];
@@ -171,7 +178,7 @@ struct Tiles {
     const int64_t *len_in;
     int64_t *len_out, *len_now;                        // (append: null otherwise)
     int64_t t0, n;                                     // rows of a sequence
-    int64_t tiles;                                     // of all
+    uint32_t tiles;                                    // of all
     int32_t per;                                       // of a (sequence, KV head)
     int32_t seq_lo, seq_hi, type, count;               // count: values that do not fit
     uint64_t sa, sb;                                   // the rotation's signs of channels 0 .. 63 and 64 .. 127
@@ -179,15 +186,21 @@ struct Tiles {
     DevStats *st;
 };
 
-// The products' left operand: lane = (output m, 16 inputs from D / 4 grp + 16 b on), +-1 bytes. Output m = 4 a + i of product
-// c is channel D / 4 a + 4 c + i, which leaves a lane of the result D / 4 channels from D / 4 grp on. Of input j and
+// The channel that output m = 4 a + i of product c is, lane group a of the result holding it. SIDE: D / 4 channels side by
+// side a lane, for codes to be packed; otherwise a row's four lanes side by side, 16 bytes each, for stores: 4 channels of
+// 32 bits (LANES4) or, of two products, 8 of 16 (LANES8).
+enum Order { SIDE, LANES4, LANES8 };
+__device__ __forceinline__ int channel(Order how, int D, int c, int a, int i) {
+    return how == SIDE ? D / 4 * a + 4 * c + i : how == LANES4 ? 16 * c + 4 * a + i : 32 * (c / 2) + 8 * a + 4 * (c % 2) + i;
+}
+// The products' left operand: lane = (output m, 16 inputs from D / 4 grp + 16 b on), +-1 bytes. Of input j and
 // output o the sign is the parity of o & j times that of the rotation's diagonal, at the input (forward) or at the
-// output (inverse). IDENTITY: 1 where they are the same. KB: the order that 16 codes of KB bits expand in.
+// output (inverse). IDENTITY: 1 where they are the same.
 enum Turn { FORWARD, INVERSE, IDENTITY };
-template <int D, int KB>
-__device__ __forceinline__ void turn_row(Turn how, uint64_t sa, uint64_t sb, int c, v4i (&A)[D / 64]) {
+template <int D>
+__device__ __forceinline__ void turn_row(Turn how, Order order, uint64_t sa, uint64_t sb, int c, v4i (&A)[D / 64]) {
     const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
-    const uint32_t o = (uint32_t)(D / 4 * (col >> 2) + 4 * c + (col & 3));
+    const uint32_t o = (uint32_t)channel(order, D, c, col >> 2, col & 3);
     // bit j: the parity of o & j, j < 16
     const uint32_t w = ((o & 1) ? 0xAAAAu : 0u) ^ ((o & 2) ? 0xCCCCu : 0u) ^ ((o & 4) ? 0xF0F0u : 0u) ^ ((o & 8) ? 0xFF00u : 0u);
     const uint32_t so = (uint32_t)((o < 64 ? sa : sb) >> (o & 63)) & 1u;
@@ -200,12 +213,22 @@ __device__ __forceinline__ void turn_row(Turn how, uint64_t sa, uint64_t sb, int
         const uint32_t same = o >> 4 == j0 >> 4 ? 1u << (o & 15) : 0u;
         if (how == IDENTITY) x = same;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            uint32_t y = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y |= ((x >> channel_of(KB, 4 * d + i)) & 1u) << (8 * i);
+        for (int d = 0; d < 4; ++d) {                  // four bits to four bytes
+            const uint32_t y = ((x >> (4 * d) & 15u) * 0x00204081u) & 0x01010101u;
             A[b][d] = (int)(how == IDENTITY ? y : 0x01010101u + 0xFEu * y);        // 0: 1, 1: -1
         }
+    }
+}
+// All of them into LDS, a wave the c's of its number; the caller synchronises.
+template <int D>
+__device__ __forceinline__ void turn_rows(Turn how, Order order, uint64_t sa, uint64_t sb, v4i (*A)[D / 64][64]) {
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int c = 0; c < D / 16; c += WAVES) {
+        v4i a[D / 64];
+        turn_row<D>(how, order, sa, sb, c + wv, a);
+#pragma unroll
+        for (int b = 0; b < D / 64; ++b) A[c + wv][b][lane] = a[b];
     }
 }
 
@@ -213,8 +236,8 @@ __device__ __forceinline__ void turn_row(Turn how, uint64_t sa, uint64_t sb, int
 struct Tile {
     int b, h, t;                                       // sequence of the call; KV head; the lane's row, of n
     bool there;                                        // (a lane past the end holds the last row again)
-    __device__ __forceinline__ Tile(const Tiles &J, int64_t i) {
-        const uint32_t chain = (uint32_t)((uint64_t)i / (uint32_t)J.per), first = (uint32_t)(i - (int64_t)chain * J.per) * 16;
+    __device__ __forceinline__ Tile(const Tiles &J, uint32_t i) {
+        const uint32_t chain = i / (uint32_t)J.per, first = (i - chain * (uint32_t)J.per) * 16;
         b = (int)(chain / (uint32_t)J.g.n_kv);
         h = (int)(chain - (uint32_t)b * (uint32_t)J.g.n_kv);
         t = (int)first + (int)(threadIdx.x & 15);
@@ -322,10 +345,10 @@ __device__ __forceinline__ int32_t append_field(const Tiles &J, const double *bn
         else
             f.get(b, INSITU_F16, x);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            bool sat = false;
-            z[i] = balanced(to_q16(x[i], sat));
-            lost += sat ? 1 : 0;
+        for (int i = 0; i < 16; ++i) z[i] = balanced(to_q16(x[i]));
+        if (J.count) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) lost += lost_q16(x[i]) ? 1 : 0;
         }
 #pragma unroll
         for (int d = 0; d < 4; ++d) {                  // four words' bytes to three digits' words
@@ -344,72 +367,81 @@ __device__ __forceinline__ int32_t append_field(const Tiles &J, const double *bn
     asm volatile("" : "+v"(ln));
     int32_t y[D / 4];                                  // the lane's channels: at most 2^30 before the scale, 2^27 behind it
     int64_t sq = 0;
+    auto turn = [&](auto wide) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-        v4i a[D / 64], T = {0, 0, 0, 0};
+        for (int c = 0; c < D / 16; ++c) {
+            v4i T = {0, 0, 0, 0};
 #pragma unroll
-        for (int b = 0; b < D / 64; ++b) a[b] = A[c][b][ln];
-        if (four) {
+            for (int l = decltype(wide)::value ? 3 : 2; l >= 0; --l) {
+                if (l < (decltype(wide)::value ? 3 : 2)) T = T << 8;
 #pragma unroll
-            for (int b = 0; b < D / 64; ++b) T = mma(a[b], xd[3][b], T);
-        }
-#pragma unroll
-        for (int l = 2; l >= 0; --l) {
-            T = T << 8;
-#pragma unroll
-            for (int b = 0; b < D / 64; ++b) T = mma(a[b], xd[l][b], T);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
+                for (int b = 0; b < D / 64; ++b) T = mma(A[c][b][ln], xd[l][b], T);
+            }
             // 1 / sqrt d, floored: a shift, or (v 2896) >> 15
-            y[4 * c + i] = D == 64 ? T[i] >> 3 : __mulhi(T[i], 2896 << 17);
-            sq += (int64_t)y[4 * c + i] * y[4 * c + i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[4 * c + i] = D == 64 ? T[i] >> 3 : __mulhi(T[i], 2896 << 17);
         }
-    }
+    };
+    if (four)
+        turn(std::true_type{});
+    else
+        turn(std::false_type{});
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) sq += (int64_t)y[i] * y[i];
     sq += xor_lane64<16>(sq, threadIdx.x & 63);
     sq += xor_lane64<32>(sq, threadIdx.x & 63);
     int64_t n64 = rshift_even(isqrt64(sq >> (D == 64 ? 6 : 7)), QK_FRAC - 9);
     const int32_t norm = n64 > 32767 ? 32767 : (int32_t)n64;
-    // y 2^8 > norm b is y > floor(norm b / 2^8), below 2^31 as the boundaries are below 2^24
+    // y 2^8 > norm b is y > floor(norm b / 2^8), below 2^30 as the boundaries are below 2^23
     constexpr int NB = (1 << BITS) - 1;
     int32_t t[NB];
     const double nd = (double)norm;
 #pragma unroll
     for (int i = 0; i < NB; ++i) t[i] = (int32_t)floor(nd * bnd[i]);
+    // the codes by bisection (the boundaries do not decrease) on the signs of t - y, which do not overflow: a sign goes
+    // into the word by one instruction (the last code's lowest bit comes last), chooses by another two, and comparisons,
+    // whose results are scalars, would have to be waited for
+    int left = D / 4 * BITS;                           // bits to come
+    uint32_t x = 0;
+    auto push = [&](int32_t d) __attribute__((always_inline)) {
+        x = __builtin_amdgcn_alignbit(x, (uint32_t)d, 31);
+        if (--left % 32 == 0) w[left / 32] = x;
+    };
+    auto pick = [](int32_t d, int32_t a, int32_t b) __attribute__((always_inline)) {       // a where d is negative
+        const int32_t m = d >> 31;
+        return (m & a) | (~m & b);
+    };
 #pragma unroll
-    for (int i = 0; i < (D / 4 * BITS + 31) / 32; ++i) w[i] = 0;
-#pragma unroll
-    for (int i = 0; i < D / 4; ++i) {
-        uint32_t code;
-        if constexpr (BITS == 4) {                     // (the boundaries do not decrease)
-            const bool c3 = y[i] > t[7];
-            const bool c2 = y[i] > (c3 ? t[11] : t[3]);
-            const int32_t u = c3 ? t[9] : t[1], v = c3 ? t[13] : t[5];
-            const bool c1 = y[i] > (c2 ? v : u);
-            const int32_t p = c3 ? t[8] : t[0], q = c3 ? t[10] : t[2], r = c3 ? t[12] : t[4], s = c3 ? t[14] : t[6];
-            const int32_t pq = c1 ? q : p, rs = c1 ? s : r;
-            const bool c0 = y[i] > (c2 ? rs : pq);
-            code = (c3 ? 8u : 0u) + (c2 ? 4u : 0u) + (c1 ? 2u : 0u) + (c0 ? 1u : 0u);
+    for (int i = D / 4 - 1; i >= 0; --i) {
+        if constexpr (BITS == 4) {
+            const int32_t d3 = t[7] - y[i];
+            const int32_t d2 = pick(d3, t[11], t[3]) - y[i];
+            const int32_t d1 = pick(d2, pick(d3, t[13], t[5]), pick(d3, t[9], t[1])) - y[i];
+            const int32_t pr = pick(d2, pick(d3, t[12], t[4]), pick(d3, t[8], t[0]));
+            const int32_t qs = pick(d2, pick(d3, t[14], t[6]), pick(d3, t[10], t[2]));
+            push(d3);
+            push(d2);
+            push(d1);
+            push(pick(d1, qs, pr) - y[i]);
         } else if constexpr (BITS == 3) {
-            const bool c2 = y[i] > t[3];
-            const bool c1 = y[i] > (c2 ? t[5] : t[1]);
-            const int32_t p = c2 ? t[4] : t[0], q = c2 ? t[6] : t[2];
-            const bool c0 = y[i] > (c1 ? q : p);
-            code = (c2 ? 4u : 0u) + (c1 ? 2u : 0u) + (c0 ? 1u : 0u);
+            const int32_t d2 = t[3] - y[i];
+            const int32_t d1 = pick(d2, t[5], t[1]) - y[i];
+            push(d2);
+            push(d1);
+            push(pick(d1, pick(d2, t[6], t[2]), pick(d2, t[4], t[0])) - y[i]);
+        } else if constexpr (BITS == 2) {
+            const int32_t d1 = t[1] - y[i];
+            push(d1);
+            push(pick(d1, t[2], t[0]) - y[i]);
         } else {
-            code = 0;
-#pragma unroll
-            for (int k = 0; k < NB; ++k) code += y[i] > t[k] ? 1 : 0;
+            push(t[0] - y[i]);
         }
-        const int at = i * BITS;
-        w[at / 32] |= code << (at % 32);
-        if (at % 32 + BITS > 32) w[at / 32 + 1] |= code >> (32 - at % 32);
     }
     return norm;
 }
 
 template <int D, int KB, int VB>
-__global__ void __launch_bounds__(64 * WAVES, D == 64 ? 3 : 2) append_tiles_kernel(Tiles J) {
+__global__ void __launch_bounds__(64 * WAVES, D == 64 ? 4 : 2) append_tiles_kernel(Tiles J) {
     const Geom &g = J.g;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (blockIdx.x == 0) {                             // the lengths, as an append of wire rows leaves them
@@ -418,21 +450,15 @@ __global__ void __launch_bounds__(64 * WAVES, D == 64 ? 3 : 2) append_tiles_kern
     }
     // the left operands in LDS: 16 registers at d = 64, but 64 at 128
     __shared__ v4i A[D / 16][D / 64][64];
-    int64_t i = (int64_t)blockIdx.x * WAVES + wv;
-    const int64_t step = (int64_t)gridDim.x * WAVES;
+    uint32_t i = blockIdx.x * WAVES + (uint32_t)wv;
+    const uint32_t step = gridDim.x * WAVES;
     Floats<D> fk, fv;
     if (i < J.tiles) {
         const Tile T(J, i);
         fk.load(J.k.p, T.at(J.k), J.type);
         fv.load(J.v.p, T.at(J.v), J.type);
     }
-#pragma unroll
-    for (int c = 0; c < D / 16; c += WAVES) {
-        v4i a[D / 64];
-        turn_row<D, 2>(FORWARD, J.sa, J.sb, c + wv, a);
-#pragma unroll
-        for (int b = 0; b < D / 64; ++b) A[c + wv][b][lane] = a[b];
-    }
+    turn_rows<D>(FORWARD, SIDE, J.sa, J.sb, A);
     __syncthreads();
     uint32_t lost = 0;
     for (; i < J.tiles; i += step) {
@@ -480,7 +506,17 @@ struct Field {
             w = *(const uint32_t *)(base + t * 16 + 4 * grp);
     }
     __device__ __forceinline__ void digits(int b, const uint32_t (&dg)[3][4], v4i (&o)[3]) const {
-        if constexpr (BITS > 1) {
+        if constexpr (BITS == 4) {                     // (they come out as the even and the odd codes of each 8 in turn)
+            v4i x[3];
+            expand16<4>(c.bits(b, (threadIdx.x & 63) >> 4), dg, x);
+#pragma unroll
+            for (int l = 0; l < 3; ++l)
+#pragma unroll
+                for (int d = 0; d < 4; d += 2) {
+                    o[l][d] = (int)perm((uint32_t)x[l][d + 1], (uint32_t)x[l][d], 0x05010400u);
+                    o[l][d + 1] = (int)perm((uint32_t)x[l][d + 1], (uint32_t)x[l][d], 0x07030602u);
+                }
+        } else if constexpr (BITS > 1) {
             expand16<BITS>(c.bits(b, (threadIdx.x & 63) >> 4), dg, o);
         } else {
 #pragma unroll
@@ -500,7 +536,7 @@ __device__ __forceinline__ void read_field(const Field<D, BITS> &f, const uint32
     v4i x[D / 64][3];
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) f.digits(b, dg, x[b]);
-    const int64_t to = at + D / 4 * ((threadIdx.x & 63) >> 4);
+    const int grp = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int c0 = 0; c0 < D / 16; c0 += 2) {           // 8 channels at a time
         float y[8];
@@ -518,15 +554,16 @@ __device__ __forceinline__ void read_field(const Field<D, BITS> &f, const uint32
         }
         if (!there) continue;
         if (type == INSITU_F32) {
-            *(float4 *)((float *)dst + to + 4 * c0) = make_float4(y[0], y[1], y[2], y[3]);
-            *(float4 *)((float *)dst + to + 4 * c0 + 4) = make_float4(y[4], y[5], y[6], y[7]);
+            float *const to = (float *)dst + at + 16 * c0 + 4 * grp;
+            *(float4 *)to = make_float4(y[0], y[1], y[2], y[3]);
+            *(float4 *)(to + 16) = make_float4(y[4], y[5], y[6], y[7]);
         } else {
             uint32_t h[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 h[i] = type == INSITU_F16 ? (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)y[i])
                                           : (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)y[i]);
-            *(uint4 *)((uint16_t *)dst + to + 4 * c0) = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+            *(uint4 *)((uint16_t *)dst + at + 16 * c0 + 8 * grp) = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
         }
     }
 }
@@ -534,6 +571,7 @@ __device__ __forceinline__ void read_field(const Field<D, BITS> &f, const uint32
 template <int D, int KB, int VB>
 __global__ void __launch_bounds__(64 * WAVES, D == 64 ? 3 : 2) read_tiles_kernel(Tiles J, const Tables *__restrict__ tabs, int turned) {
     __shared__ uint32_t dig[2][3][4];
+    __shared__ v4i A_s[D / 16][D / 64][64];
     const Geom &g = J.g;
     const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (tid < 32) {                                    // (no code names a centroid behind the codebook's end)
@@ -541,7 +579,27 @@ __global__ void __launch_bounds__(64 * WAVES, D == 64 ? 3 : 2) read_tiles_kernel
 #pragma unroll
         for (int l = 0; l < 3; ++l) ((uint8_t *)dig[tid >> 4][l])[tid & 15] = (uint8_t)(z >> (8 * l));
     }
+    const int pv = (g.key_bytes + 15) / 16;
+    const uint32_t step = gridDim.x * WAVES;
+    uint32_t i = blockIdx.x * WAVES + (uint32_t)wv;
+    Field<D, KB> fk;                                   // (rows behind the end are the cache's own memory still)
+    Field<D, VB> fv;
+    uint32_t norms = 0;
+    auto fetch = [&](uint32_t i) __attribute__((always_inline)) {
+        const Tile T(J, i);
+        const uint8_t *const head = plane_ptr(g, J.seq_lo + T.b, T.h, 0);
+        fk.load(head, g.span, J.t0 + T.t);
+        fv.load(head + pv * g.span, g.span, J.t0 + T.t);
+        norms = *(const uint32_t *)(head + (g.n_planes - 1) * g.span + (J.t0 + T.t) * 4);
+    };
+    if (i < J.tiles) fetch(i);
+    turn_rows<D>(turned ? INVERSE : IDENTITY, J.type == INSITU_F32 ? LANES4 : LANES8, J.sa, J.sb, A_s);
     __syncthreads();
+    v4i A[D / 16][D / 64];
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int b = 0; b < D / 64; ++b) A[c][b] = A_s[c][b][tid & 63];
     uint32_t dk[3][4], dv[3][4];
 #pragma unroll
     for (int l = 0; l < 3; ++l)
@@ -550,32 +608,17 @@ __global__ void __launch_bounds__(64 * WAVES, D == 64 ? 3 : 2) read_tiles_kernel
             dk[l][j] = (uint32_t)uni32((int)dig[0][l][j]);
             dv[l][j] = (uint32_t)uni32((int)dig[1][l][j]);
         }
-    const Turn how = turned ? INVERSE : IDENTITY;
-    v4i A[D / 16][D / 64], Av[D / 16][D / 64];
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-        turn_row<D, KB>(how, J.sa, J.sb, c, A[c]);
-        if constexpr (KB == 4) turn_row<D, VB>(how, J.sa, J.sb, c, Av[c]);         // (4-bit codes expand in another order)
-    }
     const float unit = unit_of(D, turned ? 1 : 0);
-    const int pv = (g.key_bytes + 15) / 16;
-    const int64_t step = (int64_t)gridDim.x * WAVES;
-    for (int64_t i = (int64_t)blockIdx.x * WAVES + wv; i < J.tiles; i += step) {
+    for (; i < J.tiles; i += step) {
         const Tile T(J, i);
-        const int64_t len = J.len_in[J.seq_lo + T.b], pos = J.t0 + T.t;
-        const bool there = T.there && pos < len;
+        const bool there = T.there && J.t0 + T.t < J.len_in[J.seq_lo + T.b];
+        const Field<D, KB> k = fk;
+        const Field<D, VB> v = fv;
+        const uint32_t n = norms;
+        if (i + step < J.tiles) fetch(i + step);
         if (__ballot(there) == 0) continue;
-        const uint8_t *const head = plane_ptr(g, J.seq_lo + T.b, T.h, 0);
-        Field<D, KB> fk;                               // (rows behind the end are the cache's own memory still)
-        Field<D, VB> fv;
-        fk.load(head, g.span, pos);
-        fv.load(head + pv * g.span, g.span, pos);
-        const uint32_t norms = *(const uint32_t *)(head + (g.n_planes - 1) * g.span + pos * 4);
-        read_field<D, KB>(fk, dk, A, (float)(int16_t)(uint16_t)norms * unit, J.k.p, T.at(J.k), J.type, there);
-        if constexpr (KB == 4)
-            read_field<D, VB>(fv, dv, Av, (float)((int32_t)norms >> 16) * unit, J.v.p, T.at(J.v), J.type, there);
-        else
-            read_field<D, VB>(fv, dv, A, (float)((int32_t)norms >> 16) * unit, J.v.p, T.at(J.v), J.type, there);
+        read_field<D, KB>(k, dk, A, (float)(int16_t)(uint16_t)n * unit, J.k.p, T.at(J.k), J.type, there);
+        read_field<D, VB>(v, dv, A, (float)((int32_t)n >> 16) * unit, J.v.p, T.at(J.v), J.type, there);
     }
 }
 
@@ -620,7 +663,7 @@ Tiles tiles_of(const Geom &g, const FloatRows &k, const FloatRows &v, int type, 
     J.type = type;
     J.n = n;
     J.per = (int32_t)((n + 15) / 16);
-    J.tiles = (int64_t)J.per * (seq_hi - seq_lo) * g.n_kv;
+    J.tiles = (uint32_t)J.per * (uint32_t)(seq_hi - seq_lo) * (uint32_t)g.n_kv;
     J.seq_lo = seq_lo;
     J.seq_hi = seq_hi;
     J.len_in = len;
@@ -658,9 +701,9 @@ hipError_t launch_append_float(hipStream_t s, const Geom &g, const Tables *t, co
     if (rows <= 0) return hipSuccess;
     if (rounds < 0 || rounds > 2) return hipErrorInvalidValue;
     const RotSigns sg = rounds ? rot_signs(rounds, signs) : RotSigns{};
-    bool tiles = rounds == 1 && fr::tiles_ok(g, k, v, type, rounds) && host.bnd_sorted;
-    for (int i = 0; i + 1 < 1 << g.kb; ++i) tiles = tiles && std::abs(host.kbnd[i]) < 1 << 24;
-    for (int i = 0; i + 1 < 1 << g.vb; ++i) tiles = tiles && std::abs(host.vbnd[i]) < 1 << 24;
+    bool tiles = rounds == 1 && rows < int64_t(1) << 31 && fr::tiles_ok(g, k, v, type, rounds) && host.bnd_sorted;
+    for (int i = 0; i + 1 < 1 << g.kb; ++i) tiles = tiles && std::abs(host.kbnd[i]) < 1 << 23;
+    for (int i = 0; i + 1 < 1 << g.vb; ++i) tiles = tiles && std::abs(host.vbnd[i]) < 1 << 23;
     if (tiles) {
         fr::Tiles J = fr::tiles_of(g, k, v, type, n_tok, seq_lo, seq_hi, len_in, sg);
         J.len_out = len_out;
@@ -671,7 +714,7 @@ hipError_t launch_append_float(hipStream_t s, const Geom &g, const Tables *t, co
         for (int i = 0; i + 1 < 1 << g.vb; ++i) J.bnd[1][i] = (double)host.vbnd[i] * 0x1p-8;
         fr::by_format(g, [&](auto d, auto kb, auto vb) {
             constexpr int D = decltype(d)::value, KB = decltype(kb)::value, VB = decltype(vb)::value;
-            hipLaunchKernelGGL((fr::append_tiles_kernel<D, KB, VB>), dim3(fr::tiles_grid(J.tiles, D == 64 ? 3 : 2)), dim3(64 * fr::WAVES), 0, s, J);
+            hipLaunchKernelGGL((fr::append_tiles_kernel<D, KB, VB>), dim3(fr::tiles_grid(J.tiles, D == 64 ? 4 : 2)), dim3(64 * fr::WAVES), 0, s, J);
         });
         return hipGetLastError();
     }
@@ -693,7 +736,7 @@ hipError_t launch_read_float(hipStream_t s, const Geom &g, const Tables *t, cons
     if (rows <= 0) return hipSuccess;
     if (rounds < 0 || rounds > 2) return hipErrorInvalidValue;
     const RotSigns sg = rounds ? rot_signs(rounds, signs) : RotSigns{};
-    if (fr::tiles_ok(g, k, v, type, rounds) && n < 0x7fffffff) {
+    if (rows < int64_t(1) << 31 && fr::tiles_ok(g, k, v, type, rounds)) {
         fr::Tiles J = fr::tiles_of(g, k, v, type, n, seq_lo, seq_hi, len, sg);
         J.t0 = t0;
         fr::by_format(g, [&](auto d, auto kb, auto vb) {
