@@ -259,6 +259,12 @@ int insitu_attend_tree(insitu_cache *cache, int32_t n, const int32_t *parents_de
 int insitu_attend_window(insitu_cache *cache, int32_t seq, int64_t n, int64_t window, int64_t sinks,
                          const int32_t *q_rot_dev, int32_t *out_dev, int32_t mode, insitu_stats *stats_host);
 
+/* insitu_step of such a layer: q/k/v_dev int32 Q8.16 (batch, heads, d) -> rotate -> append -> each
+ * sequence's query over its window and first rows. While no sequence has rows that its window has left,
+ * it is insitu_step. Not for graph capture, as that is not. */
+int insitu_step_window(insitu_cache *cache, const int32_t *q_dev, const int32_t *k_dev, const int32_t *v_dev,
+                       int32_t *out_dev, int64_t window, int64_t sinks, int32_t mode, insitu_stats *stats_host);
+
 /* insitu_attend_causal without allocating: no counterpart in the reference; for callers
  * that cannot call hipMalloc (tight serving loops, harnesses that forbid it). The same
  * launches and results as insitu_attend_causal, but the chunk scratch and the lengths of

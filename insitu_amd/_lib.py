@@ -31,7 +31,7 @@ EXPORTS = (
     "insitu_rotate", "insitu_encode", "insitu_qtab", "insitu_exp_lut", "insitu_finalize",
     "insitu_cache_create", "insitu_cache_destroy", "insitu_cache_reset", "insitu_cache_length",
     "insitu_cache_set_length", "insitu_cache_layout", "insitu_append", "insitu_append_seq",
-    "insitu_append_wire", "insitu_append_float", "insitu_read_float", "insitu_attend_window", "insitu_attend", "insitu_attend_causal", "insitu_attend_causal_head", "insitu_attend_causal_static", "insitu_step", "insitu_project", "insitu_seam_wire",
+    "insitu_append_wire", "insitu_append_float", "insitu_read_float", "insitu_attend_window", "insitu_step_window", "insitu_attend", "insitu_attend_causal", "insitu_attend_causal_head", "insitu_attend_causal_static", "insitu_step", "insitu_project", "insitu_seam_wire",
     "insitu_project_seam", "insitu_seam_heads", "insitu_attend_tree", "insitu_cache_fork", "insitu_cache_keep",
     "insitu_output_projection", "insitu_read_rows", "insitu_load_rows", "insitu_read_image",
     "insitu_load_image", "insitu_probe_read", "insitu_probe_empty", "insitu_cache_debug",
@@ -140,6 +140,7 @@ def load(path: str | None = None):
         "insitu_append_float": (i32, [vp, i32, P(FloatRows), P(FloatRows), i32, i32, P(ctypes.c_uint64)]),
         "insitu_read_float": (i32, [vp, i32, i64, i64, i32, P(FloatRows), P(FloatRows), i32]),
         "insitu_attend_window": (i32, [vp, i32, i64, i64, i64, vp, vp, i32, P(Stats)]),
+        "insitu_step_window": (i32, [vp, vp, vp, vp, vp, i64, i64, i32, P(Stats)]),
         "insitu_attend": (i32, [vp, vp, vp, i32, P(Stats)]),
         "insitu_attend_causal": (i32, [vp, i32, i64, i64, vp, vp, i32, P(Stats)]),
         "insitu_attend_causal_head": (i32, [vp, i32, i32, i64, i64, vp, vp, i32, P(Stats)]),

@@ -20,6 +20,9 @@ the reference keeps it:
   * `past_key_values` is advanced with zero K/V of the right shape, so the
     model's own length bookkeeping stays right; it is never read back: the
     compressed cache is the block's own.
+  * a sequence that has begun can change sides: graft(..., past_key_values=cache) takes a dense cache's rows
+    into the blocks' own, ungraft(..., past_key_values=cache) writes the blocks' rows where the zeros are. A
+    layer with a sliding window is grafted as one with window="layer"; by default the block attends every row.
   * `attention_mask` and `position_embeddings` are ignored: the block is causal
     by construction and applies RoPE itself. A batch of more than one sequence
     is refused rather than attended across.
@@ -97,8 +100,78 @@ class KernelAttention(nn.Module):
                 f"{self.layer_idx}; positions after the first token would be wrong. Pass "
                 f"past_key_values=None, or update this shim.") from e
 
+    def take(self, past_key_values) -> int:
+        """The rows that a dense cache holds of this layer into the block's own, which is empty: a graft in
+        the middle of a sequence goes on where the model was. Returns their number. A cache that keeps
+        a window's rows alone is taken over with those."""
+        k, v = _dense(past_key_values, self.layer_idx)
+        if k is None:
+            return 0
+        if k.shape[0] != 1:
+            raise NotImplementedError(f"batch of {k.shape[0]}: this adapter holds one sequence's cache")
+        if self.kernel.cache.length:
+            raise ValueError(f"the block's cache holds {self.kernel.cache.length} rows already")
+        n = int(k.shape[2])
+        first = int(past_key_values.get_seq_length(self.layer_idx)) - n
+        if first < 0:
+            raise NotImplementedError(f"{type(past_key_values).__name__}: room for {n} rows, {n + first} of them written")
+        self.kernel.take(k[0].detach().transpose(0, 1), v[0].detach().transpose(0, 1), first=first)
+        return n
+
+    def give(self, past_key_values) -> int:
+        """The block's rows into a dense cache, in the place of the last it holds of this layer (which
+        _advance_hf_cache filled with zeros): the model goes on without the graft. Returns their number."""
+        k, v = _dense(past_key_values, self.layer_idx)
+        n = 0 if k is None else min(int(k.shape[2]), self.kernel.cache.length)
+        if not n:
+            return 0
+        if k.shape[0] != 1 or int(past_key_values.get_seq_length(self.layer_idx)) != self.kernel.first + self.kernel.cache.length:
+            raise ValueError(f"past_key_values is not of the block's sequence of {self.kernel.cache.length} rows")
+        types = (torch.float32, torch.float16, torch.bfloat16)
+        rows = self.kernel.cache.read_float(self.kernel.cache.length - n, n, seq=0,
+                                            dtype=k.dtype if k.dtype in types else torch.float32)
+        with torch.no_grad():
+            for dense, x in zip((k, v), rows):
+                dense[0, :, -n:].copy_(x.transpose(0, 1))
+        return n
+
     def reset(self) -> None:
         self.kernel.reset()
+
+
+def _dense(past_key_values, layer_idx: int):
+    """A transformers cache's (keys, values) of a layer, each (batch, n_kv_heads, tokens, d), or Nones where it holds
+    none yet."""
+    layers = getattr(past_key_values, "layers", None)
+    if layers is not None:
+        if layer_idx >= len(layers):
+            return None, None
+        k, v = getattr(layers[layer_idx], "keys", None), getattr(layers[layer_idx], "values", None)
+    elif hasattr(past_key_values, "key_cache"):           # the older spelling
+        if layer_idx >= len(past_key_values.key_cache):
+            return None, None
+        k, v = past_key_values.key_cache[layer_idx], past_key_values.value_cache[layer_idx]
+    else:
+        raise TypeError(f"{type(past_key_values).__name__} is no cache whose layers hold keys and values")
+    if not isinstance(k, torch.Tensor) or k.dim() != 4 or not k.numel():
+        return None, None
+    return k, v
+
+
+def _window(attn_module, model_config, layer_idx: int):
+    """The layer's sliding window, or None: the module's own `sliding_window`, else the configuration's where its
+    layer_types (if there are any) say so of this layer."""
+    get = (lambda k: model_config.get(k)) if isinstance(model_config, dict) else (lambda k: getattr(model_config, k, None))
+    if hasattr(attn_module, "sliding_window"):
+        w = attn_module.sliding_window
+    else:
+        kinds = get("layer_types")
+        w = get("sliding_window")
+        if kinds is not None and layer_idx < len(kinds) and kinds[layer_idx] != "sliding_attention":
+            w = None
+        if get("use_sliding_window") is False:
+            w = None
+    return None if w is None or int(w) < 1 else int(w)
 
 
 def _head_norms(attn_module, m: ModelConfig):
@@ -156,13 +229,16 @@ def _interleaved(attn_module, rotary_dim: int) -> bool:
 def build_from_layer(attn_module, model_config, *, quant: QuantConfig | None = None,
                      fmt: FixedFormat | None = None, hw=None, capacity: int = 4096,
                      compressed: bool = True, layer_idx: int = 0, softmax: str = "two_pass",
-                     rope_interleaved: bool | None = None, ctx=None) -> KernelAttention:
+                     rope_interleaved: bool | None = None, window: int | str | None = None, sinks: int = 0,
+                     ctx=None) -> KernelAttention:
     """torch_llama.py:172-203: a KernelAttention from an attention module's weights.
 
     softmax defaults to the reference AttentionKernel's default, "two_pass";
     "online" is the hardware's order and the single fused launch per decode step.
     rope_interleaved: rotary pairs of channels (2 j, 2 j + 1) instead of (j, j + rotary_dim / 2);
-    None takes the module's own (_interleaved).
+    None takes the module's own (_interleaved). window: rows that a query sees, its own the last,
+    and sinks: first rows that stay visible beside them; None is all rows, whatever the layer did, and "layer"
+    the layer's own sliding_window.
     """
     if not compressed:
         raise NotImplementedError("compressed=False is the reference's fp16 dense baseline; "
@@ -175,7 +251,10 @@ def build_from_layer(attn_module, model_config, *, quant: QuantConfig | None = N
                             else bool(rope_interleaved))
     q_norm, k_norm, eps = _head_norms(attn_module, m)
     m = dataclasses.replace(m, qk_norm_eps=eps)
-    block = AttentionBlock(m, quant or QuantConfig(), fmt, capacity=capacity, softmax=softmax, ctx=ctx)
+    if window == "layer":
+        window = _window(attn_module, model_config, layer_idx)
+    block = AttentionBlock(m, quant or QuantConfig(), fmt, capacity=capacity, softmax=softmax, window=window, sinks=sinks,
+                           ctx=ctx)
 
     def w(name):
         return getattr(attn_module, f"{name}_proj").weight
@@ -189,19 +268,27 @@ def build_from_layer(attn_module, model_config, *, quant: QuantConfig | None = N
     return KernelAttention(block, layer_idx=layer_idx)
 
 
-def graft(model, layers, **kw) -> dict:
+def graft(model, layers, *, past_key_values=None, **kw) -> dict:
     """torch_llama.py:206-219: replace model.model.layers[i].self_attn for each i;
-    returns the replaced modules, so the graft can be undone."""
+    returns the replaced modules, so the graft can be undone. past_key_values: a dense cache of a
+    sequence that has begun, whose rows the blocks take over."""
     original = {}
     for i in layers:
         layer = model.model.layers[i]
+        block = build_from_layer(layer.self_attn, model.config, layer_idx=i, **kw)
+        if past_key_values is not None:
+            block.take(past_key_values)
         original[i] = layer.self_attn
-        layer.self_attn = build_from_layer(layer.self_attn, model.config, layer_idx=i, **kw)
+        layer.self_attn = block
     return original
 
 
-def ungraft(model, original: dict) -> None:
+def ungraft(model, original: dict, *, past_key_values=None) -> None:
+    """past_key_values: the sequence's dense cache, which receives the blocks' rows for the model to go on with."""
     for i, module in original.items():
+        block = model.model.layers[i].self_attn
+        if past_key_values is not None and isinstance(block, KernelAttention):
+            block.give(past_key_values)
         model.model.layers[i].self_attn = module
 
 

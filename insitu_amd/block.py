@@ -15,7 +15,9 @@ It is one fused C call per decode step (insitu_step), the counterpart of
 the FPGA's CMD_STEP (host/attn_proto.py:65-72). A prompt of several tokens
 (kernel.py:316-332) rotates and appends all its rows, then attends every
 query at once (insitu_attend_causal: attend_online_batch in online mode,
-attend_causal_batch in two-pass mode), bit-identical to the token loop.
+attend_causal_batch in two-pass mode), bit-identical to the token loop. With
+window (and sinks) each query attends the last `window` rows and the first
+`sinks` alone (insitu_step_window, insitu_attend_window), steps and prompts alike.
 """
 
 from __future__ import annotations
@@ -77,8 +79,15 @@ class AttentionBlock:
     def __init__(self, model: ModelConfig, quant: QuantConfig | None = None,
                  fmt: FixedFormat | None = None, *, capacity: int = 2048, batch: int = 1,
                  softmax: str = "online", weights=None, cast_after_rope: bool = True,
-                 chunk_tokens: int | None = None, ctx=None) -> None:
+                 chunk_tokens: int | None = None, window: int | None = None, sinks: int = 0,
+                 ctx=None) -> None:
         self.model = model
+        # a layer with a sliding window (CompressedAttention.attend_window), or None: every row
+        self.window = None if window is None else _lib.int64(window, "window")
+        self.sinks = _lib.int64(sinks, "sinks")
+        if (self.window is not None and self.window < 1) or self.sinks < 0:
+            raise ValueError(f"window={window}, sinks={sinks}: a window holds 1 row at least, sinks are 0 or more")
+        self.first = 0                    # position of the cache's row 0 (take)
         self.quant = quant or QuantConfig()
         self.fmt = fmt or FixedFormat()
         self.ctx = ctx or default_context()
@@ -119,9 +128,13 @@ class AttentionBlock:
         v = self.ctx.to_device(vi, torch.int32).reshape(self.batch, m.num_kv_heads, m.head_dim)
         out = torch.empty_like(q)
         st = _lib.Stats() if stats else None
-        _lib.check(self.ctx.lib.insitu_step(self.cache.handle, ptr(q), ptr(k), ptr(v), ptr(out),
-                                            _lib.MODES[self.softmax],
-                                            ctypes.byref(st) if st is not None else None))
+        stp = ctypes.byref(st) if st is not None else None
+        if self.window is None:
+            _lib.check(self.ctx.lib.insitu_step(self.cache.handle, ptr(q), ptr(k), ptr(v), ptr(out),
+                                                _lib.MODES[self.softmax], stp))
+        else:
+            _lib.check(self.ctx.lib.insitu_step_window(self.cache.handle, ptr(q), ptr(k), ptr(v), ptr(out), self.window,
+                                                       self.sinks, _lib.MODES[self.softmax], stp))
         self._keep = (q, k, v)
         self.last_stats = AttentionStats.from_c(st) if st is not None else None
         return out.reshape(self.batch, m.num_heads * m.head_dim)
@@ -143,9 +156,27 @@ class AttentionBlock:
         base = self.cache.length
         qr = self.rotation.apply(q, self.ctx)
         self.cache.append_wire(k, v)            # rotate and append in one launch
-        out, st = self.attn.attend_prefill(qr, base, self.softmax, stats=stats)
+        if self._hides(base + n):
+            out, st = self.attn.attend_window(qr, self.window, self.sinks, self.softmax, stats=stats)
+        else:
+            out, st = self.attn.attend_prefill(qr, base, self.softmax, stats=stats)
         self.last_stats = st
         return out.reshape(n, m.num_heads * m.head_dim)
+
+    def _hides(self, length: int) -> bool:
+        """Whether a sequence of that length has rows that its last query does not see."""
+        return self.window is not None and length - 1 - self.sinks >= self.window
+
+    def take(self, k, v, *, first: int = 0, seq: int | None = None) -> None:
+        """A dense cache's post-RoPE keys and values behind what the block's cache holds
+        (CompressedCache.append_float), the first of them at position `first` of an empty cache: forward
+        goes on behind them."""
+        if first < 0 or (first and any(self.cache.lengths())):
+            raise ValueError("first is the position of an empty cache's first row")
+        if first and self.sinks:
+            raise ValueError(f"rows from position {first} on do not hold the {self.sinks} first ones that stay visible")
+        self.cache.append_float(k, v, seq=seq)
+        self.first = self.first or int(first)
 
     def step_tree(self, qi, ki, vi, parents, *, stats: bool = True):
         """A draft of n nodes for every sequence: qi (batch, n, num_heads, d), ki/vi (batch, n,
@@ -166,6 +197,8 @@ class AttentionBlock:
         for name, t in (("ki", k), ("vi", v)):
             if tuple(t.shape) != (self.batch, n, m.num_kv_heads, m.head_dim):
                 raise ValueError(f"{name} must be ({self.batch}, {n}, {m.num_kv_heads}, {m.head_dim}), got {tuple(t.shape)}")
+        if self._hides(max(self.cache.lengths()) + n):
+            raise NotImplementedError("a tree of drafted tokens behind a sliding window that has left rows")
         parents = self.attn.check_parents(parents, n)       # before the rows are written
         with self.ctx.ordered(q, k, v, parents):
             qr = self.rotation.apply(q, self.ctx)
@@ -203,7 +236,7 @@ class AttentionBlock:
         base = self.cache.length
         host = self.host
         with self.ctx.ordered(x):
-            qi, ki, vi = host.wire(x, base + depth, counts=stats)
+            qi, ki, vi = host.wire(x, self.first + base + depth, counts=stats)
         self.taps = {"wire.q": qi, "wire.k": ki, "wire.v": vi}
         out = self.step_tree(qi[None], ki[None], vi[None], parents_dev, stats=stats)[0]
         self.taps["out"] = out
@@ -250,7 +283,7 @@ class AttentionBlock:
         """kernel.py:177-357, batch == 1: (tokens, hidden) float32 in, (tokens,
         hidden) float32 out (a torch tensor on the device), and a StepReport.
 
-        positions default to cache.length .. cache.length + tokens - 1. The
+        positions default to cache.length .. cache.length + tokens - 1 (behind `first`, take). The
         wire rows and the Q16 `out` rows are kept in self.taps ("wire.q",
         "wire.k", "wire.v", "out"), the reference's tap points. stats=False
         leaves the report's counters empty and the step stream-ordered (the
@@ -268,7 +301,7 @@ class AttentionBlock:
         n = int(x.shape[0])
         base = self.cache.length
         if positions is None:
-            positions = np.arange(base, base + n)
+            positions = np.arange(self.first + base, self.first + base + n)
         positions = np.asarray(positions, dtype=np.int64)
         if positions.shape != (n,):
             raise ValueError(f"expected {n} positions, got {positions.shape}")
@@ -297,3 +330,4 @@ class AttentionBlock:
     def reset(self) -> None:
         """kernel.py:454-456: a new sequence; tables survive."""
         self.cache.reset()
+        self.first = 0

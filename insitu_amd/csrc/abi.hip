@@ -1244,25 +1244,16 @@ int insitu_attend_tree(insitu_cache *k, int32_t n, const int32_t *parents, int32
     return copy_stats(k, stats);
 }
 
-int insitu_attend_window(insitu_cache *k, int32_t seq, int64_t n, int64_t window, int64_t sinks, const int32_t *q, int32_t *out,
-                         int32_t mode, insitu_stats *stats) {
-    if (!k) return fail(INSITU_EINVAL, "cache is NULL");
-    if (seq < -1 || seq >= k->g.batch) return fail(INSITU_EINVAL, "no such sequence");
-    if (n < 1) return fail(INSITU_EBADLEN, "a window attend has 1 query at least");
-    if (window < 1 || sinks < 0) return fail(INSITU_EINVAL, "a window holds 1 row at least, sinks are 0 or more");
-    if (!q || !out) return fail(INSITU_EINVAL, "null argument");
-    if (mode < INSITU_SEQUENTIAL || mode > INSITU_SERIAL) return fail(INSITU_EINVAL, "unknown mode");
+static int window_ok(int64_t window, int64_t sinks) {
+    return window < 1 || sinks < 0 ? fail(INSITU_EINVAL, "a window holds 1 row at least, sinks are 0 or more") : INSITU_OK;
+}
+
+// The launches of insitu_attend_window, its arguments checked (but for the lengths).
+static int window_launch(insitu_cache *k, int32_t seq, int64_t n, int64_t window, int64_t sinks, const int32_t *q, int32_t *out,
+                         int32_t mode, bool count) {
     WindowJob w{};
     w.seq_lo = seq < 0 ? 0 : seq;
     w.nseq = seq < 0 ? k->g.batch : 1;
-    for (int b = w.seq_lo; b < w.seq_lo + w.nseq; ++b)
-        if (k->len_host[b] < n) {
-            char buf[160];
-            snprintf(buf, sizeof buf, "sequence %d holds %lld rows, fewer than the %lld queries' own", b,
-                     (long long)k->len_host[b], (long long)n);
-            return fail(INSITU_EBADLEN, buf);
-        }
-    if (n * w.nseq > 0x7fffffff / k->g.n_q) return fail(INSITU_EBADLEN, "more than 2^31 - 1 query heads");
     w.q = q;
     w.out = out;
     w.len = k->len_now;
@@ -1271,9 +1262,7 @@ int insitu_attend_window(insitu_cache *k, int32_t seq, int64_t n, int64_t window
     w.window = std::min(window, k->g.capacity);
     w.sinks = std::min(sinks, k->g.capacity);
     w.two_pass = mode == INSITU_TWO_PASS ? 1 : 0;
-    HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
-    int rc = stats ? zero_stats(k) : INSITU_OK;
-    if (rc) return rc;
+    int rc;
     const bool fast = mode != INSITU_SERIAL && prefill_supported(k->g);
     const bool spans = fast && (n * k->g.G <= 512 || k->g.capacity > PREFILL_MAX_ROWS);
     if (spans) {
@@ -1284,14 +1273,71 @@ int insitu_attend_window(insitu_cache *k, int32_t seq, int64_t n, int64_t window
     rc = timing_events(k->ctx, &ev);
     if (rc) return rc;
     if (spans)
-        HIP_TRY(launch_attend_window_spans(k->ctx->stream, k->g, k->tabs, k->tabs_host, w, stats != nullptr, k->tree_scr, k->tree_bytes,
-                                           ev, k->stats),
+        HIP_TRY(launch_attend_window_spans(k->ctx->stream, k->g, k->tabs, k->tabs_host, w, count, k->tree_scr, k->tree_bytes, ev,
+                                           k->stats),
                 "window attend launch");
     else if (fast)
         HIP_TRY(launch_attend_window_prompt(k->ctx->stream, k->g, k->tabs, w, ev, k->stats), "window attend launch");
     else
         HIP_TRY(launch_attend_window_serial(k->ctx->stream, k->g, k->tabs, w, ev, k->stats), "window attend launch");
-    return copy_stats(k, stats);
+    return INSITU_OK;
+}
+
+int insitu_attend_window(insitu_cache *k, int32_t seq, int64_t n, int64_t window, int64_t sinks, const int32_t *q, int32_t *out,
+                         int32_t mode, insitu_stats *stats) {
+    if (!k) return fail(INSITU_EINVAL, "cache is NULL");
+    if (seq < -1 || seq >= k->g.batch) return fail(INSITU_EINVAL, "no such sequence");
+    if (n < 1) return fail(INSITU_EBADLEN, "a window attend has 1 query at least");
+    int rc = window_ok(window, sinks);
+    if (rc) return rc;
+    if (!q || !out) return fail(INSITU_EINVAL, "null argument");
+    if (mode < INSITU_SEQUENTIAL || mode > INSITU_SERIAL) return fail(INSITU_EINVAL, "unknown mode");
+    const int lo = seq < 0 ? 0 : seq, hi = seq < 0 ? k->g.batch : seq + 1;
+    for (int b = lo; b < hi; ++b)
+        if (k->len_host[b] < n) {
+            char buf[160];
+            snprintf(buf, sizeof buf, "sequence %d holds %lld rows, fewer than the %lld queries' own", b,
+                     (long long)k->len_host[b], (long long)n);
+            return fail(INSITU_EBADLEN, buf);
+        }
+    if (n > 0x7fffffff / k->g.n_q / (hi - lo)) return fail(INSITU_EBADLEN, "more than 2^31 - 1 query heads");
+    HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
+    rc = stats ? zero_stats(k) : INSITU_OK;
+    if (!rc) rc = window_launch(k, seq, n, window, sinks, q, out, mode, stats != nullptr);
+    return rc ? rc : copy_stats(k, stats);
+}
+
+int insitu_step_window(insitu_cache *k, const int32_t *q, const int32_t *kw, const int32_t *vw, int32_t *out, int64_t window,
+                       int64_t sinks, int32_t mode, insitu_stats *stats) {
+    if (!k || !q || !kw || !vw || !out) return fail(INSITU_EINVAL, "null argument");
+    int rc = window_ok(window, sinks);
+    if (rc) return rc;
+    if (mode < INSITU_SEQUENTIAL || mode > INSITU_SERIAL) return fail(INSITU_EINVAL, "unknown mode");
+    const Geom &g = k->g;
+    int64_t longest = 0;
+    for (int b = 0; b < g.batch; ++b) longest = std::max(longest, k->len_host[b]);
+    // a row that the window has left, and that is none of the first ones
+    if (longest - sinks < window) return insitu_step(k, q, kw, vw, out, mode, stats);
+    if (longest + 1 > g.capacity) {
+        char buf[200];
+        snprintf(buf, sizeof buf, "cache holds %lld of %lld tokens; cannot append (base.py:67-73)", (long long)longest,
+                 (long long)g.capacity);
+        return fail(INSITU_ECAPACITY, buf);
+    }
+    HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
+    if (mode != INSITU_SERIAL && prefill_supported(g)) {               // (before the row is written)
+        rc = grow(k, k->tree_scr, k->tree_bytes, window_scratch_bytes(g, 1, g.batch));
+        if (rc) return rc;
+    }
+    rc = stats ? zero_stats(k) : INSITU_OK;
+    if (rc) return rc;
+    HIP_TRY(launch_step_write(k->ctx->stream, g, k->tabs, q, kw, vw, k->desc.fmt.rot_rounds, k->desc.fmt.rot_signs, k->wire_scratch,
+                              nullptr, nullptr, k->len_dev[k->cur], k->len_dev[k->cur ^ 1], k->len_now, k->stats),
+            "step write launch");
+    k->cur ^= 1;
+    for (int b = 0; b < g.batch; ++b) k->len_host[b] += 1;
+    rc = window_launch(k, -1, 1, window, sinks, k->wire_scratch, out, mode, stats != nullptr);
+    return rc ? rc : copy_stats(k, stats);
 }
 
 int insitu_cache_fork(insitu_cache *k, int32_t n_copies, const int32_t *src, const int32_t *dst, int64_t n,

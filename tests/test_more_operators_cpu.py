@@ -43,3 +43,26 @@ def test_outputs_in_one_place(make, bad):
     import torch
     from insitu_amd.cache import _overlaps
     assert _overlaps(make(torch)) is bad
+
+
+class _Names:
+    def __init__(self, **kw):
+        self.__dict__.update(kw)
+
+
+@pytest.mark.parametrize("module,config,want", [
+    (dict(), dict(), None),
+    (dict(), dict(sliding_window=4096), 4096),
+    (dict(), dict(sliding_window=None), None),
+    (dict(), dict(sliding_window=512, use_sliding_window=False), None),
+    (dict(), dict(sliding_window=512, layer_types=["full_attention", "sliding_attention"]), 512),
+    (dict(), dict(sliding_window=512, layer_types=["sliding_attention", "full_attention"]), None),
+    (dict(sliding_window=None), dict(sliding_window=512), None),
+    (dict(sliding_window=128), dict(), 128),
+    (dict(sliding_window=-1), dict(), None),
+])
+def test_a_layers_own_window(module, config, want):
+    """Of layer 1: the module's word before the configuration's, given as attributes or as a dictionary."""
+    from insitu_amd.adapters.torch_llama import _window
+    assert _window(_Names(**module), _Names(**config), 1) == want
+    assert _window(_Names(**module), config, 1) == want
