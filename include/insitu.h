@@ -420,6 +420,10 @@ enum {
                                         or 2/2-bit codes), 1 the lane-per-channel kernel for every
                                         format, 2 lane = row however few the rows, where it
                                         handles the format                                      */
+    INSITU_DEBUG_WINDOW = 7,         /* the window attends' kernel: 0 automatic (the few queries' one
+                                        while its tiles of 16 rows fill the chip a few times at most,
+                                        else the prompts'), 1 the few queries', 2 the prompts';
+                                        INSITU_EINVAL if it does not handle the cache           */
     INSITU_DEBUG_PREFILL = 6         /* the causal attends' kernel: 0 automatic (the prefill kernel
                                         where it handles the format and the queries fill it), 1 the
                                         decode attends over a virtual batch, 2 the prefill kernel

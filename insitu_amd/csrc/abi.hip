@@ -204,6 +204,7 @@ struct insitu_cache {
     int32_t spin_limit = 1 << 20;         // insitu_cache_debug
     int32_t path = 0;                     // insitu_cache_debug: 0 auto, 1 scan, 2 chunked, 3 step kernel, 4 split
     int32_t prefill_path = 0;             // insitu_cache_debug: 0 auto, 1 virtual batch, 2 prefill kernel
+    int32_t window_path = 0;              // insitu_cache_debug: 0 auto, 1 spans, 2 prompts
     int32_t append_path = 0;              // insitu_cache_debug: 0 auto, 1 the lane-per-channel kernel, 2 lane = row
 };
 
@@ -1248,6 +1249,20 @@ static int window_ok(int64_t window, int64_t sinks) {
     return window < 1 || sinks < 0 ? fail(INSITU_EINVAL, "a window holds 1 row at least, sinks are 0 or more") : INSITU_OK;
 }
 
+// Whether a window attend takes the few queries' kernel (workgroups of one tile of up to 16 rows, that run one a CU) or
+// the prompts' (waves of 16 rows). Few rows leave most of a prompt workgroup's 64 or 128 empty: a decode token of 160
+// sequences, 8 KV heads, window 1,024, takes 133 us against 356, of 4 tokens each 192 against 425. Else the spans win by a
+// factor 2 to 5 while two rounds of tiles fill the chip (512 tiles, window 1,024: 78 us against 144 at d = 64, 123 against
+// 245 at d = 128; window 128: 37 against 46 and 64 against 73), to about four rounds where a row sees more (1,024 tiles,
+// window 4,096: 382 against 411 and 578 against 704, window 1,024 148 against 147 and 230 against 246, window 128 70
+// against 52 and 113 against 77), and lose from there on (2,048 tiles, window 1,024: 300 against 235 and 430 against 255).
+static bool window_spans(const insitu_cache *k, int64_t n, int64_t nseq, int64_t window) {
+    const Geom &g = k->g;
+    if (k->window_path) return k->window_path == 1;
+    const int64_t tiles = window_tiles(g, n, nseq);
+    return n * g.G <= 16 || tiles <= 512 || (tiles <= 1024 && std::min(window, g.capacity) >= 1024) || g.capacity > PREFILL_MAX_ROWS;
+}
+
 // The launches of insitu_attend_window, its arguments checked (but for the lengths).
 static int window_launch(insitu_cache *k, int32_t seq, int64_t n, int64_t window, int64_t sinks, const int32_t *q, int32_t *out,
                          int32_t mode, bool count) {
@@ -1264,7 +1279,7 @@ static int window_launch(insitu_cache *k, int32_t seq, int64_t n, int64_t window
     w.two_pass = mode == INSITU_TWO_PASS ? 1 : 0;
     int rc;
     const bool fast = mode != INSITU_SERIAL && prefill_supported(k->g);
-    const bool spans = fast && (n * k->g.G <= 512 || k->g.capacity > PREFILL_MAX_ROWS);
+    const bool spans = fast && window_spans(k, n, w.nseq, window);
     if (spans) {
         rc = grow(k, k->tree_scr, k->tree_bytes, window_scratch_bytes(k->g, n, w.nseq));
         if (rc) return rc;
@@ -1325,7 +1340,7 @@ int insitu_step_window(insitu_cache *k, const int32_t *q, const int32_t *kw, con
         return fail(INSITU_ECAPACITY, buf);
     }
     HIP_TRY(hipSetDevice(k->ctx->device), "hipSetDevice");
-    if (mode != INSITU_SERIAL && prefill_supported(g)) {               // (before the row is written)
+    if (mode != INSITU_SERIAL && prefill_supported(g) && window_spans(k, 1, g.batch, window)) {     // (before the row is written)
         rc = grow(k, k->tree_scr, k->tree_bytes, window_scratch_bytes(g, 1, g.batch));
         if (rc) return rc;
     }
@@ -1587,6 +1602,12 @@ int insitu_cache_debug(insitu_cache *k, int32_t what, int64_t value) {
         if (value < 0 || value > 4)
             return fail(INSITU_EINVAL, "path is 0 (auto), 1 (scan), 2 (chunked), 3 (step kernel) or 4 (split)");
         k->path = (int32_t)value;
+        return INSITU_OK;
+    case INSITU_DEBUG_WINDOW:
+        if (value < 0 || value > 2) return fail(INSITU_EINVAL, "window is 0 (auto), 1 (few queries) or 2 (prompts)");
+        if (value && !prefill_supported(k->g)) return fail(INSITU_EINVAL, "neither kernel handles this cache");
+        if (value == 2 && k->g.capacity > PREFILL_MAX_ROWS) return fail(INSITU_EINVAL, "more rows than the prompts' kernel counts");
+        k->window_path = (int32_t)value;
         return INSITU_OK;
     case INSITU_DEBUG_PREFILL:
         if (value < 0 || value > 2) return fail(INSITU_EINVAL, "prefill is 0 (auto), 1 (virtual batch) or 2 (prefill kernel)");

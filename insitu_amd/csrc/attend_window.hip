@@ -45,7 +45,7 @@ __device__ __forceinline__ WindowRows rows_of(const WindowJob &w, int64_t end) {
     return WindowRows{w.sinks, end > w.window ? end - w.window : 0};
 }
 
-constexpr int LATE = 16;                               // tiles by which the first span is shorter, online
+constexpr float EVENTS = 8.0f, EVENTS_FROM = 5.0f;     // of span_start, in tiles
 constexpr int DPP_ROW_ROR4 = 0x124, DPP_ROW_ROR12 = 0x12C;       // lane i <- lane (i - 4), (i + 4) mod 16 of its row
 constexpr int RUN_MAX = 32768;                         // tokens of a run, so that its L fits 32 bits
 constexpr uint32_t LUT_N = LUT_SPAN + 1;
@@ -65,6 +65,7 @@ struct Job {
     const Tables *tabs;
     WindowJob w;
     int32_t rows;                                      // n G, of a (sequence, KV head)
+    uint32_t first;                                    // the launch's first workgroup of all
     int32_t chains, extra, count;                      // extra: runs a workgroup has in the scratch; count: statistics
     double kc_absmax, vcs[8], vcmax;                   // vcs: value centroids / 2^23
     uint32_t wide, delta_max;                          // wide: |v_norm p| up to which a term is two balanced bytes
@@ -115,6 +116,25 @@ __device__ __forceinline__ uint32_t row_sum(uint32_t v) {
     return row_all<R>(v, [](uint32_t a, uint32_t b) { return a + b; });
 }
 
+// Lane i <= FW: the tile that span i of FW begins with (of nt; span FW is the end). Events thin out as 1 / x along what
+// a tile of rows sees, so that its first x tiles take about x + a ln(1 + x / EVENTS_FROM) times a tile without any: the
+// spans share that out evenly (Newton; its start is behind the cut, and the steps after the first stay before it).
+template <int FW>
+__device__ __forceinline__ int span_start(int nt, float a) {
+    const int i = threadIdx.x & 63;
+    if (nt <= FW) return imin(i, nt);
+    const float rate = 1.0f / EVENTS_FROM, al = a * 0.693147181f, n = (float)nt;
+    const float goal = (n + al * __builtin_amdgcn_logf(1.0f + n * rate)) * ((float)i / FW);
+    float x = n * ((float)i / FW);
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+        const float y = 1.0f + x * rate, c = x + al * __builtin_amdgcn_logf(y);
+        x = fmaxf(x + (goal - c) * __builtin_amdgcn_rcpf(1.0f + a * rate * __builtin_amdgcn_rcpf(y)), 0.0f);
+    }
+    const int t = (int)(x + 0.5f);
+    return i <= 0 ? 0 : i >= FW ? nt : imin(imax(t, 1), nt);
+}
+
 // A workgroup's tile of rows and the rows of the cache that it sees: the 16-row tiles of the first rows and those
 // from the first row's window on, U rows numbered on end.
 template <int R>
@@ -126,8 +146,8 @@ struct Place {
     int64_t skip_at, skip;                             // where numbers and rows part, and how far
     int64_t first_end, last_lo;                        // the first row's end, where the last row's window begins
     __device__ __forceinline__ explicit Place(const Job &J) {
-        const uint32_t chain = blockIdx.x % (uint32_t)J.chains;
-        row0 = (int)(blockIdx.x / (uint32_t)J.chains) * R;
+        const uint32_t wg = J.first + blockIdx.x, chain = wg % (uint32_t)J.chains;
+        row0 = (int)(wg / (uint32_t)J.chains) * R;
         b = (int)(chain / (uint32_t)J.g.n_kv);
         kvh = (int)(chain % (uint32_t)J.g.n_kv);
         seq = J.w.seq_lo + b;
@@ -260,13 +280,10 @@ __global__ void __launch_bounds__(FW * 64, FW / 4) span_kernel(Job J) {
     const int32_t kc = (int32_t)J.tabs->kc[tid & 15], ex = J.tabs->exp_table[tid & 255];
     p.find(J);
     const uint8_t *hb = plane_ptr(g, p.seq, p.kvh, 0), *nb = hb + (g.n_planes - 1) * g.span;
-    // the wave's span, in tiles of 16: the first one's, which has most of the events, is shorter by what they cost
-    const int nt = (int)((p.U + 15) >> 4), late = J.w.two_pass ? 0 : LATE;
-    int t0 = (int)((uint32_t)(nt + late + FW - 1) / FW) - late;
-    t0 = t0 < 1 ? 1 : t0;
-    const int per = (int)((uint32_t)(nt - t0 + FW - 2) / (FW - 1));
-    const int64_t lo = wv == 0 ? 0 : 16 * (int64_t)(t0 + (wv - 1) * per);
-    const int64_t stop = 16 * (int64_t)(t0 + wv * per), hi = stop < p.U ? stop : p.U, last = (hi - 1) & ~(int64_t)15;
+    // the wave's span, in tiles of 16
+    const int nt = (int)((p.U + 15) >> 4), cut = span_start<FW>(nt, J.w.two_pass ? 0.0f : EVENTS);
+    const int64_t lo = 16 * (int64_t)__builtin_amdgcn_readlane(cut, wv), stop = 16 * (int64_t)__builtin_amdgcn_readlane(cut, wv + 1);
+    const int64_t hi = stop < p.U ? stop : p.U, last = (hi - 1) & ~(int64_t)15;
     Keys<D, KB, R> next;
     if (lo < hi) next.load(p, hb, nb, g.span, lo, last);
     const int64_t end = p.end(J, row), wlo = end - J.w.window;
@@ -744,11 +761,15 @@ __global__ void __launch_bounds__(FW * 64, FW / 4) span_kernel(Job J) {
             S.ev[wv][r] = events | any;
             S.bound[wv][r] = bs_all;
         }
+    } else if (grp == 0 && mine == 0) {                // (a span without tokens)
+        S.meta[wv * R + r] = make_uint4(0, 1u << PROB_FRAC, ~0u, 0);
+        S.ev[wv][r] = 0;
+        S.bound[wv][r] = 0.0f;
     }
     __syncthreads();
 
     // -- the runs: a wave a row, lane = channel ----------------------------------------------------
-    const int ns = per ? 1 + (int)((uint32_t)(nt - t0 + per - 1) / (uint32_t)per) : 1;      // spans that hold any
+    const int ns = imin(nt, FW);
     for (int rr = wv; rr < R && p.row0 + rr < J.rows; rr += FW) {
         constexpr int CPL = D / 64;
         const uint32_t e = lane < ns ? S.ev[lane][rr] : 0u;
@@ -929,9 +950,10 @@ int64_t workgroups(const Geom &g, int64_t n, int64_t nseq) {
     const int64_t rows = n * g.G, R = tile_rows(rows);
     return nseq * g.n_kv * ((rows + R - 1) / R);
 }
-// runs a workgroup has in the scratch beside those in LDS: up to 1,024, and 16 MiB in all
+constexpr int64_t LAUNCH = 1024;                       // workgroups a launch, which bounds the scratch
+// runs a workgroup has in the scratch beside those in LDS: up to 1,024 in 16 MiB, but 192 at least
 int64_t extra_runs(const Geom &g, int64_t wgs) {
-    return std::max<int64_t>(16, std::min<int64_t>(1024, ((int64_t)16 << 20) / (wgs * (g.d * 4 + 16))));
+    return std::max<int64_t>(192, std::min<int64_t>(1024, ((int64_t)16 << 20) / (wgs * (g.d * 4 + 16))));
 }
 }  // namespace
 
@@ -950,8 +972,10 @@ hipError_t launch(hipStream_t s, const Job &J, unsigned blocks, LaunchEv ev) {
 
 }  // namespace wn
 
+int64_t window_tiles(const Geom &g, int64_t n, int64_t nseq) { return wn::workgroups(g, n, nseq); }
+
 size_t window_scratch_bytes(const Geom &g, int64_t n, int64_t nseq) {
-    const int64_t wgs = wn::workgroups(g, n, nseq), runs = wgs * wn::extra_runs(g, wgs);
+    const int64_t wgs = std::min(wn::workgroups(g, n, nseq), wn::LAUNCH), runs = wgs * wn::extra_runs(g, wgs);
     return (size_t)runs * (16 + g.d * 4) + 256;
 }
 
@@ -959,8 +983,8 @@ hipError_t launch_attend_window_spans(hipStream_t s, const Geom &g, const Tables
                                       void *scratch, size_t scratch_bytes, LaunchEv ev, DevStats *st) {
     using namespace wn;
     Job J{};
-    const int64_t wgs = workgroups(g, w.n, w.nseq);
-    if (wgs > 0x7fffffff || window_scratch_bytes(g, w.n, w.nseq) > scratch_bytes) return hipErrorInvalidValue;
+    const int64_t all = workgroups(g, w.n, w.nseq), wgs = std::min(all, LAUNCH);
+    if (all > 0x7fffffff || window_scratch_bytes(g, w.n, w.nseq) > scratch_bytes) return hipErrorInvalidValue;
     J.g = g;
     J.tabs = t;
     J.w = w;
@@ -978,9 +1002,9 @@ hipError_t launch_attend_window_spans(hipStream_t s, const Geom &g, const Tables
     J.meta = (uint4 *)scratch;
     J.S = (int32_t *)((uint8_t *)scratch + (wgs * J.extra * 16 + 255) / 256 * 256);
     J.st = st;
-    hipError_t rc = hipErrorInvalidValue;
+    hipError_t (*run)(hipStream_t, const Job &, unsigned, LaunchEv) = nullptr;
 #define INSITU_WINDOW_CASE(DD, KK, CC) \
-    if (g.d == DD && g.kb == KK && (g.vb <= 2 ? 4 : 8) == CC) rc = launch<DD, KK, CC>(s, J, (unsigned)wgs, ev);
+    if (g.d == DD && g.kb == KK && (g.vb <= 2 ? 4 : 8) == CC) run = launch<DD, KK, CC>;
 #define INSITU_WINDOW_D(DD)                                                                           \
     INSITU_WINDOW_CASE(DD, 2, 4) INSITU_WINDOW_CASE(DD, 3, 4) INSITU_WINDOW_CASE(DD, 4, 4)            \
     INSITU_WINDOW_CASE(DD, 2, 8) INSITU_WINDOW_CASE(DD, 3, 8) INSITU_WINDOW_CASE(DD, 4, 8)
@@ -988,7 +1012,14 @@ hipError_t launch_attend_window_spans(hipStream_t s, const Geom &g, const Tables
     INSITU_WINDOW_D(128)
 #undef INSITU_WINDOW_D
 #undef INSITU_WINDOW_CASE
-    return rc;
+    if (!run) return hipErrorInvalidValue;
+    for (int64_t first = 0; first < all; first += LAUNCH) {
+        J.first = (uint32_t)first;
+        const LaunchEv e{first == 0 ? ev.start : nullptr, first + LAUNCH >= all ? ev.stop : nullptr};
+        const hipError_t rc = run(s, J, (unsigned)std::min(all - first, LAUNCH), e);
+        if (rc != hipSuccess) return rc;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_attend_window_serial(hipStream_t s, const Geom &g, const Tables *t, const WindowJob &w, LaunchEv ev,

@@ -393,6 +393,7 @@ struct WindowJob {
 // On the prefill kernel (attend_prefill.hip), where prefill_supported and up to PREFILL_MAX_ROWS of capacity.
 hipError_t launch_attend_window_prompt(hipStream_t s, const Geom &g, const Tables *t, const WindowJob &w, LaunchEv ev, DevStats *st);
 // A workgroup a few rows, its waves sharing out what they see (attend_window.hip), where prefill_supported.
+int64_t window_tiles(const Geom &g, int64_t n, int64_t nseq);          // its workgroups
 size_t window_scratch_bytes(const Geom &g, int64_t n, int64_t nseq);
 hipError_t launch_attend_window_spans(hipStream_t s, const Geom &g, const Tables *t, const Tables &host, const WindowJob &w, bool count,
                                       void *scratch, size_t scratch_bytes, LaunchEv ev, DevStats *st);
