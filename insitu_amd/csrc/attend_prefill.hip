@@ -164,7 +164,7 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
         q += (int64_t)(rest % (unsigned)w->nseq) * n_q * g.n_q * D;
         out += (int64_t)(rest % (unsigned)w->nseq) * n_q * g.n_q * D;
         rest /= (unsigned)w->nseq;
-        const int64_t T = w->len[seq];
+        const int64_t T = uni64(w->len[seq]);
         base = (T > n_q ? T : n_q) - n_q;
     }
     const int64_t blk = nblk - 1 - (int64_t)rest;
@@ -266,6 +266,7 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
         if (rerr) atomicAdd(&S.rerr, rerr);
 #pragma unroll
         for (int o = 1; o < 16; o <<= 1) bq = fmax(bq, __shfl_xor(bq, o));
+        bq = __longlong_as_double(uni64(__double_as_longlong(bq)));
     }
     const int32_t wmin = (int32_t)(base + (row0 < rows ? row0 : rows - 1) / G + 1);       // the wave's contexts
     // (WIN: the first and the last of the wave's windows)
@@ -617,74 +618,86 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
                 if (__ballot((uint32_t)m - (uint32_t)mx < delta_max) == 0) return;   // every p is 0
             }
         }
-        if (P != ONLINE || (plain && (WIN || !diag))) {
+        if constexpr (P != ONLINE) {
             const uint32_t dl[4] = {clip(m, s[0]), clip(m, s[1]), clip(m, s[2]), clip(m, s[3])};
-            terms((WIN || P != ONLINE) && diag, dl);
+            terms(diag, dl);
             lp += (p[0] + p[1]) + (p[2] + p[3]);
             accumulate(A, bf, tl);
             return;
         }
-        if constexpr (P != ONLINE) return;
-        // a tile with events, or at a row's end: its tokens in segments (bits 8 i of seg the segment
-        // of token i)
-        uint32_t dl[4], fe[4], seg = 0;
-        SC e = m;                                      // the maximum before this lane's tokens
+        // a tile with events: its tokens in segments (bits 8 i of seg the segment of token i). Both kinds of tile meet at
+        // the terms and the products: apart, the accumulators of d = 128 go through memory between them.
+        uint32_t dl[4], fe[4] = {0, 0, 0, 0}, seg = 0;
+        int row_ev = 0;                                // the row's events
         const unsigned long long evl = __ballot(mx > m);
         const bool single = (evl & (evl - 1)) == 0;    // at most one lane holds events
-        if (!single) {
-            const SC a = shfl_s<SC>(mx, lane - 16), b = shfl_s<SC>(mx, lane - 32), c = shfl_s<SC>(mx, lane - 48);
-            if (grp > 0) e = a > e ? a : e;
-            if (grp > 1) e = b > e ? b : e;
-            if (grp > 2) e = c > e ? c : e;
-        } else if (evl) {                              // the row's later tokens see its maximum
-            const int l = __ffsll((long long)evl) - 1;
-            const SC t = rdlane<SC>(mx, l);
-            if (col == (l & 15)) e = grp > (l >> 4) ? t : e;
-        }
-        uint32_t n = 0;
+        if (plain) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool ev = s[i] > e;
-            const uint32_t dd = clip(ev ? s[i] : e, ev ? e : s[i]);
-            fe[i] = ev ? dd + 1u : 0u;                 // an event's distance, + 1
-            dl[i] = ev ? 0u : dd;
-            e = ev ? s[i] : e;
-            n += ev ? 1 : 0;
-            seg |= n << (8 * i);
-        }
-        int row_ev = 0;                                // the row's events
-        if (!single) {
-            const uint32_t n1 = (uint32_t)__shfl((int)n, lane - 16), n2 = (uint32_t)__shfl((int)n, lane - 32),
-                           n3 = (uint32_t)__shfl((int)n, lane - 48);
-            const uint32_t off = (grp > 0 ? n1 : 0) + (grp > 1 ? n2 : 0) + (grp > 2 ? n3 : 0);
-            seg += off * 0x01010101u;                  // at most 16
-            row_ev = __shfl((int)(off + n), 48 + col);
-            m = shfl_s<SC>(e, 48 + col);
-        } else if (evl) {
-            const int l = __ffsll((long long)evl) - 1;
-            const uint32_t nl = (uint32_t)__builtin_amdgcn_readlane((int)n, l);
-            const SC t = rdlane<SC>(mx, l);
-            if (col == (l & 15)) {
-                if (grp > (l >> 4)) seg += nl * 0x01010101u;
-                row_ev = (int)nl;
-                m = t;
+            for (int i = 0; i < 4; ++i) dl[i] = clip(m, s[i]);
+        } else {
+            SC e = m;                                  // the maximum before this lane's tokens
+            if (!single) {
+                const SC a = shfl_s<SC>(mx, lane - 16), b = shfl_s<SC>(mx, lane - 32), c = shfl_s<SC>(mx, lane - 48);
+                if (grp > 0) e = a > e ? a : e;
+                if (grp > 1) e = b > e ? b : e;
+                if (grp > 2) e = c > e ? c : e;
+            } else if (evl) {                              // the row's later tokens see its maximum
+                const int l = __ffsll((long long)evl) - 1;
+                const SC t = rdlane<SC>(mx, l);
+                if (col == (l & 15)) e = grp > (l >> 4) ? t : e;
             }
-        }
-        n_events += n;
-        terms(true, dl);
-        for (int sg = 0;; ++sg) {
-            v4i B[WIDE ? 4 : 3][C::PVK];
+            uint32_t n = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool in = ((seg >> (8 * i)) & 0xFFu) == (uint32_t)sg;
-                lp += in ? p[i] : 0u;
+                const bool ev = s[i] > e;
+                const uint32_t dd = clip(ev ? s[i] : e, ev ? e : s[i]);
+                fe[i] = ev ? dd + 1u : 0u;                 // an event's distance, + 1
+                dl[i] = ev ? 0u : dd;
+                e = ev ? s[i] : e;
+                n += ev ? 1 : 0;
+                seg |= n << (8 * i);
+            }
+            if (!single) {
+                const uint32_t n1 = (uint32_t)__shfl((int)n, lane - 16), n2 = (uint32_t)__shfl((int)n, lane - 32),
+                               n3 = (uint32_t)__shfl((int)n, lane - 48);
+                const uint32_t off = (grp > 0 ? n1 : 0) + (grp > 1 ? n2 : 0) + (grp > 2 ? n3 : 0);
+                seg += off * 0x01010101u;                  // at most 16
+                row_ev = __shfl((int)(off + n), 48 + col);
+                m = shfl_s<SC>(e, 48 + col);
+            } else if (evl) {
+                const int l = __ffsll((long long)evl) - 1;
+                const uint32_t nl = (uint32_t)__builtin_amdgcn_readlane((int)n, l);
+                const SC t = rdlane<SC>(mx, l);
+                if (col == (l & 15)) {
+                    if (grp > (l >> 4)) seg += nl * 0x01010101u;
+                    row_ev = (int)nl;
+                    m = t;
+                }
+            }
+            n_events += n;
+        }
+        terms(diag, dl);
+        for (int sg = 0;; ++sg) {
+            v4i B[WIDE ? 4 : 3][C::PVK];
+            if (plain) {
+                lp += (p[0] + p[1]) + (p[2] + p[3]);
 #pragma unroll
-                for (int l = 0; l < (WIDE ? 4 : 3); ++l) {
-                    if constexpr (NC == 4) {
-                        B[l][0][i] = in ? A[l][0][i] : 0;
-                    } else {
-                        B[l][i >> 1][2 * (i & 1)] = in ? A[l][i >> 1][2 * (i & 1)] : 0;
-                        B[l][i >> 1][2 * (i & 1) + 1] = in ? A[l][i >> 1][2 * (i & 1) + 1] : 0;
+                for (int l = 0; l < (WIDE ? 4 : 3); ++l)
+#pragma unroll
+                    for (int k = 0; k < C::PVK; ++k) B[l][k] = A[l][k];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = ((seg >> (8 * i)) & 0xFFu) == (uint32_t)sg;
+                    lp += in ? p[i] : 0u;
+#pragma unroll
+                    for (int l = 0; l < (WIDE ? 4 : 3); ++l) {
+                        if constexpr (NC == 4) {
+                            B[l][0][i] = in ? A[l][0][i] : 0;
+                        } else {
+                            B[l][i >> 1][2 * (i & 1)] = in ? A[l][i >> 1][2 * (i & 1)] : 0;
+                            B[l][i >> 1][2 * (i & 1) + 1] = in ? A[l][i >> 1][2 * (i & 1) + 1] : 0;
+                        }
                     }
                 }
             }
@@ -749,14 +762,20 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
             }
             int32_t ts = s * C::ST;
             if constexpr (WIN) ts += ts >= skip_at ? skip : 0;
-            for (int tl = 0; tl < C::NT && ts + tl * 16 < wmax; ++tl) {
+            auto at = [&](int tl) __attribute__((always_inline)) {
                 const int32_t t0 = ts + tl * 16;
                 bool diag = t0 + 16 > wmin;
                 if constexpr (WIN) {
-                    if (t0 >= sinks && t0 + 16 <= first_lo) continue;
+                    if (t0 >= sinks && t0 + 16 <= first_lo) return;
                     diag = diag || (t0 < last_lo && t0 + 16 > sinks);
                 }
                 tile(passc, bf, tl, t0, diag, check, tight);
+            };
+            if constexpr (P == ONLINE) {               // (two tiles with events side by side spill)
+#pragma unroll 1
+                for (int tl = 0; tl < C::NT && ts + tl * 16 < wmax; ++tl) at(tl);
+            } else {
+                for (int tl = 0; tl < C::NT && ts + tl * 16 < wmax; ++tl) at(tl);
             }
             // a stage adds at most 16 tokens of 2^15 to a lane's 32 bits
             if (P != MAXONLY && (s & 4095) == 4095) {
@@ -844,12 +863,17 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
     return false;
 }
 
-// Not inlined, so that its registers are its own: it is entered when narrow scores did not do.
-template <int D, int NC, int W, int ST, bool TWO_PASS, bool WIN = false>
-__device__ __attribute__((noinline)) void prefill_rows_wide(const Geom *g, const Tables *tabs, const int32_t *q, int32_t *out,
-                                                            int64_t base, int64_t n_q, DevStats *st, Lds<D, NC, W, ST> *S,
-                                                            const WindowJob *w = nullptr) {
-    prefill_rows<D, NC, W, ST, TWO_PASS, true, WIN>(*g, tabs, q, out, base, n_q, st, *S, w);
+// Not inlined, so that its registers are its own: it is entered when narrow scores did not do. (Its arguments are values: a
+// kernel that gives an argument's address away reads it from memory, a lane at a time, wherever it uses it.)
+template <int D, int NC, int W, int ST, bool TWO_PASS>
+__device__ __attribute__((noinline)) void prefill_rows_wide(Geom g, const Tables *tabs, const int32_t *q, int32_t *out, int64_t base,
+                                                            int64_t n_q, DevStats *st, Lds<D, NC, W, ST> *S) {
+    prefill_rows<D, NC, W, ST, TWO_PASS, true, false>(g, tabs, q, out, base, n_q, st, *S, nullptr);
+}
+template <int D, int NC, int W, int ST, bool TWO_PASS>
+__device__ __attribute__((noinline)) void window_rows_wide(Geom g, const Tables *tabs, WindowJob w, DevStats *st,
+                                                           Lds<D, NC, W, ST> *S) {
+    prefill_rows<D, NC, W, ST, TWO_PASS, true, true>(g, tabs, w.q, w.out, 0, w.n, st, *S, &w);
 }
 
 template <int D, int NC, int W, int ST, bool TWO_PASS>
@@ -858,7 +882,7 @@ __global__ void __launch_bounds__(W * 64, D == 64 && ST == 32 && NC == 4 ? 3 : 2
                                                            int64_t base, int64_t n_q, DevStats *st) {
     __shared__ Lds<D, NC, W, ST> S;
     if (prefill_rows<D, NC, W, ST, TWO_PASS, false, false>(g, tabs, q, out, base, n_q, st, S, nullptr))
-        prefill_rows_wide<D, NC, W, ST, TWO_PASS>(&g, tabs, q, out, base, n_q, st, &S);
+        prefill_rows_wide<D, NC, W, ST, TWO_PASS>(g, tabs, q, out, base, n_q, st, &S);
 }
 
 // The same for queries that see a window and the first rows.
@@ -867,7 +891,7 @@ __global__ void __launch_bounds__(W * 64, D == 64 && ST == 32 && NC == 4 ? 3 : 2
                                                                                                 WindowJob w, DevStats *st) {
     __shared__ Lds<D, NC, W, ST> S;
     if (prefill_rows<D, NC, W, ST, TWO_PASS, false, true>(g, tabs, w.q, w.out, 0, w.n, st, S, &w))
-        prefill_rows_wide<D, NC, W, ST, TWO_PASS, true>(&g, tabs, w.q, w.out, 0, w.n, st, &S, &w);
+        window_rows_wide<D, NC, W, ST, TWO_PASS>(g, tabs, w, st, &S);
 }
 
 template <int D, int NC, int W, int ST>
