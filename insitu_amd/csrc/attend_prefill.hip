@@ -40,11 +40,16 @@
 // random rows drawn as the benchmark's). A short prompt, two waves a SIMD or one, is bound by the
 // longest walk's own latency: 0.1 us a row at d = 64, 0.1 a row and pass at d = 128. One accumulator
 // instead of one a digit costs two VALU instructions a register and tile and frees 32 registers at
-// d = 64 (64 at 128); the walk still spills some: 46 registers online and 42 two-pass at the 168 of three
-// workgroups a CU, 26 to 62 at d = 128's 256.
+// d = 64 (64 at 128). What is spilled at the 168 registers of three workgroups a CU (256 at d = 128) lies outside
+// the walk, as long as its branches are a wave's: an argument whose address escapes makes them a lane's, which cost a
+// window's prompt 631 us against 486. Six waves a workgroup do not sit two workgroups a CU (924).
 // Measured (the kernel, Llama-3.2-1B shape, queries scaled as a model's): 4,096 tokens 883 us (the
 // call 8,632 on the virtual batch of decode attends before); 333 tokens behind 2,000 219 us (797);
-// 1,000 tokens at d = 128, 3b/3b, two-pass 201 us (1,923).
+// 1,000 tokens at d = 128, 3b/3b, two-pass 190 us (1,923).
+//
+// A window (WIN): the workgroup's stages are those of the first rows and of its rows' windows, masked at their edges. A
+// window of 1,024 over 4,096 tokens takes 486 us, its events half as often again as a context's (31 of a wave's 65 tiles
+// hold some: 71 segments); in two passes, without them, 388. d = 128, window 2,048, 4,096 tokens behind 4,096: 1,981.
 #include <type_traits>
 
 #include "digits.h"

@@ -4,8 +4,9 @@
 // on those rows. The reference attends all of a context and has no counterpart.
 //
 // Many queries run on the prefill kernel (attend_prefill.hip), a wave 16 (query, head) rows over all they see.
-// Here are the few of decode steps and short turns (span_kernel): a workgroup holds one tile of R rows, 4, 8 or
-// 16, of a KV head, and its eight waves share out what the tile sees, in order; behind barriers follow
+// Here are the few of decode steps and short turns (span_kernel), which leave the chip to so few such waves that
+// the walk of one is the time: a workgroup holds one tile of R rows, 4, 8 or 16, of a KV head, and its eight or
+// twelve waves share out what the tile sees, in order; behind barriers follow
 //   the scores     of each wave's span, kept in LDS, and their largest a row;
 //   the walk       with the maximum of the spans before (online) or of all (two-pass). The terms
 //                  floor(v_norm p c / 2^23) between two rises of the maximum (events) are only added: such a run
@@ -25,6 +26,15 @@
 // The terms' digits are summed apart and put together where a run ends. A lane's channels lie together in the
 // value codes (channel col D / 16 + c in product c), so that it reads a word of a row, not all of it.
 #include <algorithm>
+//
+// What bounds it: VALU issue, and in a small call the chain of one workgroup's phases. A decode token of 32 sequences
+// of 8 KV heads over 4,096 rows (53.7 us; 11.8 to read them at the rate of a copy) is a workgroup a CU and three waves a
+// SIMD, which issue VALU 60 % of the time: tables and queries 3 us, keys expanded and scores 16, the walk 22 (10 of it
+// events: two-pass, which has none, takes 43), the runs 2. A wave a (token, head), token by token, takes 1,807 us; the
+// prefill kernel, whose workgroup's 64 rows are 4 here, 326. One query over a window of 128 in 300 rows, 15.8 us with the
+// call, is mostly instructions that come from memory once: loops that are not unrolled are faster there. At d = 128, or
+// with 8 codes a value, eight waves: twelve have too few registers.
+
 #include <cmath>
 
 #include "digits.h"
@@ -118,7 +128,8 @@ __device__ __forceinline__ uint32_t row_sum(uint32_t v) {
 
 // Lane i <= FW: the tile that span i of FW begins with (of nt; span FW is the end). Events thin out as 1 / x along what
 // a tile of rows sees, so that its first x tiles take about x + a ln(1 + x / EVENTS_FROM) times a tile without any: the
-// spans share that out evenly (Newton; its start is behind the cut, and the steps after the first stay before it).
+// spans share that out evenly (Newton; its start is behind the cut, and the steps after the first stay before it). Equal
+// spans take 62 us where these take 55 (a decode token of 32 sequences, window 4,096), 38.8 where 37 (16 tokens, 1,024).
 template <int FW>
 __device__ __forceinline__ int span_start(int nt, float a) {
     const int i = threadIdx.x & 63;
@@ -951,7 +962,8 @@ int64_t workgroups(const Geom &g, int64_t n, int64_t nseq) {
     return nseq * g.n_kv * ((rows + R - 1) / R);
 }
 constexpr int64_t LAUNCH = 1024;                       // workgroups a launch, which bounds the scratch
-// runs a workgroup has in the scratch beside those in LDS: up to 1,024 in 16 MiB, but 192 at least
+// runs a workgroup has in the scratch beside those in LDS: up to 1,024 in 16 MiB, but 192 at least. (Random scores take a
+// tile of 16 rows some 60 over 4,096 rows; one that is out of runs goes token by token, at 100 times the cost.)
 int64_t extra_runs(const Geom &g, int64_t wgs) {
     return std::max<int64_t>(192, std::min<int64_t>(1024, ((int64_t)16 << 20) / (wgs * (g.d * 4 + 16))));
 }

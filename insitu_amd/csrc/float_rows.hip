@@ -7,6 +7,12 @@
 // centroid are three balanced digits, 16 rows a wave and product, and the outputs' order is chosen so that a lane
 // holds D / 4 channels of a row side by side. What it loads, packs or stores are then whole words, with no
 // exchange through LDS.
+//
+// What bounds it. Reading: memory, 32,767 tokens of 8 heads of 64 into bfloat16 19.0 us, 4.25 TB/s where a copy has 4.68
+// (a wave a row and its butterfly in floating point 292 us). Writing: VALU issue, 76 % of the SIMDs' cycles in 40 of
+// 41.9 us for the same rows (405 a wave a row), 1,200 instructions a tile of 16 rows: the cast and its digits, the
+// exact norm, the codes by a bisection of the boundaries and their packing. Comparisons in place of signs 49 us; the boundaries' selects as v_bfi by hand 49; a norm in 32 bits with the exact one where it is close 40.5, not
+// worth a second way. Small calls are the host's: 65 tokens 6.6 us of kernel in 16, 100 read 4.5 in 13.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
