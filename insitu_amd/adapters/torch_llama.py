@@ -272,23 +272,23 @@ def graft(model, layers, *, past_key_values=None, **kw) -> dict:
     """torch_llama.py:206-219: replace model.model.layers[i].self_attn for each i;
     returns the replaced modules, so the graft can be undone. past_key_values: a dense cache of a
     sequence that has begun, whose rows the blocks take over."""
-    original = {}
+    original, blocks = {}, {}
     for i in layers:
-        layer = model.model.layers[i]
-        block = build_from_layer(layer.self_attn, model.config, layer_idx=i, **kw)
+        original[i] = model.model.layers[i].self_attn
+        blocks[i] = build_from_layer(original[i], model.config, layer_idx=i, **kw)
         if past_key_values is not None:
-            block.take(past_key_values)
-        original[i] = layer.self_attn
-        layer.self_attn = block
+            blocks[i].take(past_key_values)
+    for i, block in blocks.items():                   # (all of them or, where one is refused, none)
+        model.model.layers[i].self_attn = block
     return original
 
 
 def ungraft(model, original: dict, *, past_key_values=None) -> None:
     """past_key_values: the sequence's dense cache, which receives the blocks' rows for the model to go on with."""
+    if past_key_values is not None:
+        for i in original:
+            model.model.layers[i].self_attn.give(past_key_values)
     for i, module in original.items():
-        block = model.model.layers[i].self_attn
-        if past_key_values is not None and isinstance(block, KernelAttention):
-            block.give(past_key_values)
         model.model.layers[i].self_attn = module
 
 

@@ -140,7 +140,7 @@ class CompressedAttention:
         sequence (seq, or a batch of one). The query at row p attends the rows t <= p with t < sinks or
         t > p - window, in row order: the integers that `attend` gives in a cache of those rows alone,
         in every mode. n = 1 is a decode step. Returns (out torch int32 of q_rot's shape,
-        AttentionStats or None). With stats=False nothing synchronises."""
+        which may be q_rot itself, and AttentionStats or None). With stats=False nothing synchronises."""
         import torch
         c = self.cache
         q = self.ctx.to_device(q_rot, torch.int32)
@@ -155,6 +155,8 @@ class CompressedAttention:
         elif tuple(out.shape) != tuple(q.shape) or out.dtype != torch.int32 or not out.is_contiguous() or \
                 out.device != q.device:
             raise ValueError(f"out must be a contiguous int32 tensor {tuple(q.shape)} on {q.device}")
+        elif q.data_ptr() != out.data_ptr() and abs(q.data_ptr() - out.data_ptr()) < 4 * q.numel():
+            raise ValueError("out may be q_rot's memory, but not part of it")
         if seq is not None and not 0 <= seq < c.batch:
             raise ValueError(f"sequence {seq} of {c.batch}")
         st = _lib.Stats() if stats else None

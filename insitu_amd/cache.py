@@ -435,6 +435,8 @@ class CompressedCache(KVCache):
             if len(out) != 2 or dtype not in (None, out[0].dtype) or out[0].dtype != out[1].dtype:
                 raise ValueError("out is two tensors of one dtype")
             _float_type(out[0].dtype)
+            if out[0].numel() and out[0].data_ptr() == out[1].data_ptr():
+                raise ValueError("out's keys and values are in one place")
             for x in out:
                 if tuple(x.shape) != shape or x.device != self.ctx.torch_device or _overlaps(x):
                     raise ValueError(f"out must be two tensors {shape} on {self.ctx.torch_device}, a head's channels "

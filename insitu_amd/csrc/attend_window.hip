@@ -25,7 +25,6 @@
 // 4 of the step's 16 J tokens; for one token's four query heads a quarter of what 16 rows a tile would take.
 // The terms' digits are summed apart and put together where a run ends. A lane's channels lie together in the
 // value codes (channel col D / 16 + c in product c), so that it reads a word of a row, not all of it.
-#include <algorithm>
 //
 // What bounds it: VALU issue, and in a small call the chain of one workgroup's phases. A decode token of 32 sequences
 // of 8 KV heads over 4,096 rows (53.7 us; 11.8 to read them at the rate of a copy) is a workgroup a CU and three waves a
@@ -34,7 +33,7 @@
 // prefill kernel, whose workgroup's 64 rows are 4 here, 326. One query over a window of 128 in 300 rows, 15.8 us with the
 // call, is mostly instructions that come from memory once: loops that are not unrolled are faster there. At d = 128, or
 // with 8 codes a value, eight waves: twelve have too few registers.
-
+#include <algorithm>
 #include <cmath>
 
 #include "digits.h"

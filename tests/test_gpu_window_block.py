@@ -292,3 +292,66 @@ def test_take_and_give_refusals(ctx):
     one.update(torch.zeros(1, 2, 1, 64), torch.zeros(1, 2, 1, 64), 0)
     with pytest.raises(ValueError, match="not of the block's sequence"):
         adapter.give(one)
+
+
+def test_a_graft_is_whole_or_not_at_all(ctx):
+    """A cache that no block can take: the layers stay the model's own."""
+    import torch
+    from insitu_amd.adapters.torch_llama import graft, ungraft
+    from transformers import DynamicCache
+    model = _mistral(None)
+    before = [layer.self_attn for layer in model.model.layers]
+    cache = DynamicCache()
+    cache.update(torch.randn(1, 2, 5, 64), torch.randn(1, 2, 5, 64), 0)
+    cache.update(torch.randn(1, 2, 70, 64), torch.randn(1, 2, 70, 64), 1)     # more rows than there is room for
+    with pytest.raises(ValueError):
+        graft(model, [0, 1], capacity=64, past_key_values=cache, ctx=ctx)
+    assert [layer.self_attn for layer in model.model.layers] == before
+    orig = graft(model, [0, 0, 1], capacity=80, past_key_values=cache, ctx=ctx)
+    assert [orig[0], orig[1]] == before
+    ungraft(model, orig, past_key_values=cache)
+    assert [layer.self_attn for layer in model.model.layers] == before
+
+
+def test_a_window_step_is_its_parts(ctx):
+    """insitu_step_window's statistics and appended rows against append_wire and attend_window."""
+    import torch
+    from insitu_amd.attention import CompressedAttention
+    rng = np.random.default_rng(6)
+    a, b = _block(ctx, batch=3, window=9, sinks=2), _block(ctx, batch=3)
+    fill = _draw(rng, 3, 30, N_KV, 64), _draw(rng, 3, 30, N_KV, 64)
+    for blk in (a, b):
+        blk.cache.append_wire(*fill)
+    for softmax in ("online", "two_pass", "serial"):
+        a.softmax = softmax
+        q, k, v = (torch.as_tensor(_draw(rng, 3, h, 64), dtype=torch.int32).to(ctx.torch_device) for h in (8, N_KV, N_KV))
+        out = a.step(q, k, v)
+        b.cache.append_wire(k[:, None].contiguous(), v[:, None].contiguous())
+        want, st = CompressedAttention(b.cache).attend_window(b.rotation.apply(q, ctx).reshape(3, 1, 8, 64), 9, 2, softmax)
+        assert torch.equal(out.reshape(want.shape), want)
+        assert (a.last_stats.rescale_events, a.last_stats.max_abs_score, a.last_stats.max_abs_acc, a.last_stats.n_tokens) == \
+            (st.rescale_events, st.max_abs_score, st.max_abs_acc, st.n_tokens)
+        n = a.cache.lengths()[0]
+        for s in range(3):
+            for h in range(N_KV):
+                np.testing.assert_array_equal(a.cache.read_rows(h, 0, n, s), b.cache.read_rows(h, 0, n, s))
+
+
+def test_outputs_in_one_place(ctx):
+    """Memory that two rows would be written to, or read from and written to."""
+    import torch
+    from insitu_amd.attention import CompressedAttention
+    rng = np.random.default_rng(7)
+    blk = _block(ctx)
+    blk.cache.append_wire(_draw(rng, 30, N_KV, 64), _draw(rng, 30, N_KV, 64))
+    whole = torch.zeros(6, 8, 64, dtype=torch.int32, device=ctx.torch_device)
+    for q, out in ((whole[:5], whole[1:]), (whole[1:], whole[:5])):
+        with pytest.raises(ValueError, match="part of it"):
+            CompressedAttention(blk.cache).attend_window(q, 9, 2, out=out)
+    x = torch.zeros(30, N_KV, 64, device=ctx.torch_device)
+    with pytest.raises(ValueError, match="one place"):
+        blk.cache.read_float(seq=0, out=(x, x))
+    both = torch.zeros(30, N_KV, 2, 64, device=ctx.torch_device)              # (side by side is apart)
+    blk.cache.read_float(seq=0, out=(both[:, :, 0], both[:, :, 1]))
+    k, v = blk.cache.read_float(seq=0)
+    assert torch.equal(both[:, :, 0], k) and torch.equal(both[:, :, 1], v)
