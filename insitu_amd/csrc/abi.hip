@@ -1251,11 +1251,11 @@ static int window_ok(int64_t window, int64_t sinks) {
 
 // Whether a window attend takes the few queries' kernel (workgroups of one tile of up to 16 rows, that run one a CU) or
 // the prompts' (waves of 16 rows). Few rows leave most of a prompt workgroup's 64 or 128 empty: a decode token of 160
-// sequences, 8 KV heads, window 1,024, takes 133 us against 356, of 4 tokens each 192 against 425. Else the spans win by a
-// factor 2 to 5 while two rounds of tiles fill the chip (512 tiles, window 1,024: 79 us against 145 at d = 64, 118 against
-// 235 at d = 128; window 128: 38 against 44 and 65 against 67), to about four rounds where a row sees more (1,024 tiles,
-// window 4,096: 374 against 433 and 561 against 701, window 1,024 148 against 149 and 222 against 238, window 128 72
-// against 50 and 118 against 69), and lose from there on (2,048 tiles, window 1,024: 300 against 235 and 430 against 255).
+// sequences, 8 KV heads, window 1,024, takes 126 us against 330, of 4 tokens each 196 against 387. Else the spans win by a
+// factor 2 to 5 while two rounds of tiles fill the chip (512 tiles, window 1,024: 82 us against 140 at d = 64, 120 against
+// 234 at d = 128; window 128: 42 against 44 and 67 against 67), to about four rounds where a row sees more (1,024 tiles,
+// window 4,096: 371 against 403 and 556 against 690, window 1,024 148 against 141 and 218 against 232, window 128 71
+// against 48 and 120 against 70), and lose from there on (2,048 tiles, window 1,024: 294 against 181 and 431 against 242).
 static bool window_spans(const insitu_cache *k, int64_t n, int64_t nseq, int64_t window) {
     const Geom &g = k->g;
     if (k->window_path) return k->window_path == 1;

@@ -42,14 +42,14 @@
 // instead of one a digit costs two VALU instructions a register and tile and frees 32 registers at
 // d = 64 (64 at 128). What is spilled at the 168 registers of three workgroups a CU (256 at d = 128) lies outside
 // the walk, as long as its branches are a wave's: an argument whose address escapes makes them a lane's, which cost a
-// window's prompt 631 us against 486. Six waves a workgroup do not sit two workgroups a CU (924).
-// Measured (the kernel, Llama-3.2-1B shape, queries scaled as a model's): 4,096 tokens 883 us (the
-// call 8,632 on the virtual batch of decode attends before); 333 tokens behind 2,000 219 us (797);
-// 1,000 tokens at d = 128, 3b/3b, two-pass 190 us (1,923).
+// window's prompt 631 us against 486 (472 with the scores' two chains in turn). Six waves a workgroup do not sit two workgroups a CU (924).
+// Measured (the call, Llama-3.2-1B shape, queries scaled as a model's): 4,096 tokens 884 us (9,928 on
+// the virtual batch of decode attends); 333 tokens behind 2,000 235 us (797 the kernel's); 1,000 tokens at
+// d = 128, 3b/3b, two-pass 260 us (2,020).
 //
 // A window (WIN): the workgroup's stages are those of the first rows and of its rows' windows, masked at their edges. A
-// window of 1,024 over 4,096 tokens takes 486 us, its events half as often again as a context's (31 of a wave's 65 tiles
-// hold some: 71 segments); in two passes, without them, 388. d = 128, window 2,048, 4,096 tokens behind 4,096: 1,981.
+// window of 1,024 over 4,096 tokens takes 472 us, its events half as often again as a context's (31 of a wave's 65 tiles
+// hold some: 71 segments); in two passes, without them, 370. d = 128, window 2,048, 4,096 tokens behind 4,096: 1,942.
 #include <type_traits>
 
 #include "digits.h"
@@ -412,8 +412,8 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
         return (double)(o > mx ? o : mx);
     };
     auto lut = [&](uint32_t d) __attribute__((always_inline)) -> uint32_t {
-        // floor(d * log2e / 2^24), at most LUT_SPAN (d <= delta_max)
-        return S.lut[__umulhi(d, (uint32_t)LOG2E_Q16 << 8)];
+        // floor(d * log2e / 2^24), at most LUT_SPAN (d <= delta_max, 20 bits: a 24-bit product's upper half)
+        return S.lut[(uint32_t)(((uint64_t)((d << 1) & 0xFFFFFFu) * (((uint32_t)LOG2E_Q16 << 7) & 0xFFFFFFu)) >> 32)];
     };
     // a distance, at most delta_max
     auto clip = [&](SC hi, SC lo) __attribute__((always_inline)) -> uint32_t {
@@ -482,24 +482,22 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
             for (int b = 0; b < C::KBLK; ++b)
 #pragma unroll
                 for (int l = 0; l < 3; ++l) a[b][l] = S.u.op.ka[bf][tl][l][b][lane];
-#pragma unroll
-            for (int k = 4; k >= 2; --k) {
-                if (k < 4) H = H << 8;
+            const int4 k4 = *(const int4 *)&S.kn[bf][tl * 16 + grp * 4];
+            auto weight = [&](int k, v4i &x) __attribute__((always_inline)) {      // the digits' products of that weight
 #pragma unroll
                 for (int b = 0; b < C::KBLK; ++b)
 #pragma unroll
                     for (int l = 0; l < 3; ++l)
-                        if (k - l >= 0 && k - l < 3) H = mma(a[b][l], qd[k - l][b], H);
-            }
-#pragma unroll
-            for (int k = 1; k >= 0; --k) {
-                if (k < 1) L = L << 8;
-#pragma unroll
-                for (int b = 0; b < C::KBLK; ++b)
-#pragma unroll
-                    for (int l = 0; l <= k; ++l) L = mma(a[b][l], qd[k - l][b], L);
-            }
-            const int4 k4 = *(const int4 *)&S.kn[bf][tl * 16 + grp * 4];
+                        if (k - l >= 0 && k - l < 3) x = mma(a[b][l], qd[k - l][b], x);
+            };
+            weight(4, H);                              // (two chains in turn: one's products cover the other's latency)
+            weight(1, L);
+            H = H << 8;
+            weight(3, H);
+            L = L << 8;
+            weight(0, L);
+            H = H << 8;
+            weight(2, H);
             const int32_t kn[4] = {k4.x, k4.y, k4.z, k4.w};
             int64_t x[4];
 #pragma unroll
@@ -630,6 +628,9 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
             accumulate(A, bf, tl);
             return;
         }
+        // Tiles without events need no masks, but where leaving them out makes the compiler put the accumulators into memory
+        // (4,096 tokens, 3b/2b at d = 128: 3,884 us against 1,483).
+        constexpr bool MASKED = D == 128 && NC == 4 && !WIN;
         // a tile with events: its tokens in segments (bits 8 i of seg the segment of token i). Both kinds of tile meet at
         // the terms and the products: apart, the accumulators of d = 128 go through memory between them.
         uint32_t dl[4], fe[4] = {0, 0, 0, 0}, seg = 0;
@@ -684,7 +685,7 @@ __device__ __forceinline__ bool prefill_rows(const Geom &g, const Tables *__rest
         terms(diag, dl);
         for (int sg = 0;; ++sg) {
             v4i B[WIDE ? 4 : 3][C::PVK];
-            if (plain) {
+            if (plain && !MASKED) {
                 lp += (p[0] + p[1]) + (p[2] + p[3]);
 #pragma unroll
                 for (int l = 0; l < (WIDE ? 4 : 3); ++l)
