@@ -40,16 +40,17 @@
 // random rows drawn as the benchmark's). A short prompt, two waves a SIMD or one, is bound by the
 // longest walk's own latency: 0.1 us a row at d = 64, 0.1 a row and pass at d = 128. One accumulator
 // instead of one a digit costs two VALU instructions a register and tile and frees 32 registers at
-// d = 64 (64 at 128). What is spilled at the 168 registers of three workgroups a CU (256 at d = 128) lies outside
-// the walk, as long as its branches are a wave's: an argument whose address escapes makes them a lane's, which cost a
-// window's prompt 631 us against 486 (472 with the scores' two chains in turn). Six waves a workgroup do not sit two workgroups a CU (924).
+// d = 64 (64 at 128). What is spilled at the 168 registers of three workgroups a CU (256 at d = 128) lies
+// outside the walk, as long as its branches are a wave's: an argument whose address escapes makes them a lane's,
+// which cost a window's prompt 631 us against 486 (472 with the scores' two chains in turn). Of workgroups of
+// six waves a CU holds one (924).
 // Measured (the call, Llama-3.2-1B shape, queries scaled as a model's): 4,096 tokens 884 us (9,928 on
 // the virtual batch of decode attends); 333 tokens behind 2,000 235 us (797 the kernel's); 1,000 tokens at
 // d = 128, 3b/3b, two-pass 260 us (2,020).
 //
 // A window (WIN): the workgroup's stages are those of the first rows and of its rows' windows, masked at their edges. A
 // window of 1,024 over 4,096 tokens takes 472 us, its events half as often again as a context's (31 of a wave's 65 tiles
-// hold some: 71 segments); in two passes, without them, 370. d = 128, window 2,048, 4,096 tokens behind 4,096: 1,942.
+// hold some: 71 segments); in two passes, without them, 380. d = 128, window 2,048, 4,096 tokens behind 4,096: 1,942.
 #include <type_traits>
 
 #include "digits.h"
