@@ -22,7 +22,7 @@ the reference keeps it:
     compressed cache is the block's own.
   * a sequence that has begun can change sides: graft(..., past_key_values=cache) takes a dense cache's rows
     into the blocks' own, ungraft(..., past_key_values=cache) writes the blocks' rows where the zeros are. A
-    layer with a sliding window is grafted as one with window="layer"; by default the block attends every row.
+    cache whose tensors have room behind the sequence (a static one that is not full) is refused. A layer with a sliding window is grafted as one with window="layer"; by default the block attends every row.
   * `attention_mask` and `position_embeddings` are ignored: the block is causal
     by construction and applies RoPE itself. A batch of more than one sequence
     is refused rather than attended across.
@@ -121,12 +121,10 @@ class KernelAttention(nn.Module):
     def give(self, past_key_values) -> int:
         """The block's rows into a dense cache, in the place of the last it holds of this layer (which
         _advance_hf_cache filled with zeros): the model goes on without the graft. Returns their number."""
-        k, v = _dense(past_key_values, self.layer_idx)
-        n = 0 if k is None else min(int(k.shape[2]), self.kernel.cache.length)
+        n = self.check_give(past_key_values)
         if not n:
             return 0
-        if k.shape[0] != 1 or int(past_key_values.get_seq_length(self.layer_idx)) != self.kernel.first + self.kernel.cache.length:
-            raise ValueError(f"past_key_values is not of the block's sequence of {self.kernel.cache.length} rows")
+        k, v = _dense(past_key_values, self.layer_idx)
         types = (torch.float32, torch.float16, torch.bfloat16)
         rows = self.kernel.cache.read_float(self.kernel.cache.length - n, n, seq=0,
                                             dtype=k.dtype if k.dtype in types else torch.float32)
@@ -134,6 +132,23 @@ class KernelAttention(nn.Module):
             for dense, x in zip((k, v), rows):
                 dense[0, :, -n:].copy_(x.transpose(0, 1))
         return n
+
+    def check_give(self, past_key_values) -> int:
+        """How many rows give writes; raises where it cannot. They go to the end of the layer's tensors, which
+        therefore end with the sequence, and what they do not hold is what a window has left."""
+        k, _ = _dense(past_key_values, self.layer_idx)
+        length = self.kernel.cache.length
+        if not length:
+            return 0
+        written = int(past_key_values.get_seq_length(self.layer_idx))
+        if written != self.kernel.first + length or (k is not None and k.shape[0] != 1):
+            raise ValueError(f"past_key_values is not of the block's sequence of {length} rows")
+        rows = 0 if k is None else int(k.shape[2])
+        if rows > written:
+            raise NotImplementedError(f"{type(past_key_values).__name__}: room for {rows} rows, {written} of them written")
+        if rows < written and not _sliding(past_key_values, self.layer_idx):
+            raise NotImplementedError(f"{type(past_key_values).__name__}: {rows} of {written} rows in its tensors")
+        return min(rows, length)
 
     def reset(self) -> None:
         self.kernel.reset()
@@ -156,6 +171,12 @@ def _dense(past_key_values, layer_idx: int):
     if not isinstance(k, torch.Tensor) or k.dim() != 4 or not k.numel():
         return None, None
     return k, v
+
+
+def _sliding(past_key_values, layer_idx: int) -> bool:
+    """Whether a transformers cache keeps the last rows of a layer alone, as a window needs them."""
+    layers = getattr(past_key_values, "layers", None)
+    return layers is not None and bool(getattr(layers[layer_idx], "is_sliding", False))
 
 
 def _window(attn_module, model_config, layer_idx: int):
@@ -286,8 +307,11 @@ def graft(model, layers, *, past_key_values=None, **kw) -> dict:
 def ungraft(model, original: dict, *, past_key_values=None) -> None:
     """past_key_values: the sequence's dense cache, which receives the blocks' rows for the model to go on with."""
     if past_key_values is not None:
-        for i in original:
-            model.model.layers[i].self_attn.give(past_key_values)
+        blocks = [model.model.layers[i].self_attn for i in original]
+        for block in blocks:                          # (all of them or, where one is refused, none)
+            block.check_give(past_key_values)
+        for block in blocks:
+            block.give(past_key_values)
     for i, module in original.items():
         model.model.layers[i].self_attn = module
 
