@@ -103,19 +103,24 @@ class KernelAttention(nn.Module):
     def take(self, past_key_values) -> int:
         """The rows that a dense cache holds of this layer into the block's own, which is empty: a graft in
         the middle of a sequence goes on where the model was. Returns their number. A cache that keeps
-        a window's rows alone is taken over with those."""
+        a window's rows alone is taken over with those, where the block's window needs no others."""
         k, v = _dense(past_key_values, self.layer_idx)
-        if k is None:
+        name = type(past_key_values).__name__
+        n = 0 if k is None else int(k.shape[2])
+        written = int(past_key_values.get_seq_length(self.layer_idx))
+        if not written and not n:
             return 0
-        if k.shape[0] != 1:
+        if k is not None and k.shape[0] != 1:
             raise NotImplementedError(f"batch of {k.shape[0]}: this adapter holds one sequence's cache")
         if self.kernel.cache.length:
             raise ValueError(f"the block's cache holds {self.kernel.cache.length} rows already")
-        n = int(k.shape[2])
-        first = int(past_key_values.get_seq_length(self.layer_idx)) - n
-        if first < 0:
-            raise NotImplementedError(f"{type(past_key_values).__name__}: room for {n} rows, {n + first} of them written")
-        self.kernel.take(k[0].detach().transpose(0, 1), v[0].detach().transpose(0, 1), first=first)
+        if n > written:
+            raise NotImplementedError(f"{name}: room for {n} rows, {written} of them written")
+        window = self.kernel.window
+        if n < written and (not n or not _sliding(past_key_values, self.layer_idx) or window is None or n < window - 1):
+            raise NotImplementedError(f"{name}: {n} of {written} rows in its tensors, and the block's queries see "
+                                      f"{'all' if window is None else window}")
+        self.kernel.take(k[0].detach().transpose(0, 1), v[0].detach().transpose(0, 1), first=written - n)
         return n
 
     def give(self, past_key_values) -> int:

@@ -125,3 +125,34 @@ def test_layers_are_put_back_all_or_none():
     with pytest.raises(NotImplementedError):
         ungraft(model, {0: "own 0", 1: "own 1"}, past_key_values=cache)
     assert not any(_held(cache)[0]) and [x.self_attn for x in model.model.layers] == blocks
+
+
+@pytest.mark.parametrize("n", [1, 4, 5, 6, 9, 16])
+@pytest.mark.parametrize("window", [None, 1, 6, 7, 40])
+@pytest.mark.parametrize("kind", list(CACHES))
+def test_rows_are_taken_where_the_block_needs_no_others(kind, window, n):
+    """A block without a window needs every row, one with a window the last window - 1 of them (and the query's own)."""
+    cache = CACHES[kind]()
+    x = _rows(0, n).transpose(0, 1)[None]
+    cache.update(x, -x, 0)
+    a = KernelAttention(_Block(window))
+    room = {"static": 16, "static_window": 6}.get(kind, 0)
+    there = min(n, {"dynamic_window": 5, "static_window": 6}.get(kind, n))
+    if n < room or (there < n and (window is None or there < window - 1)):
+        with pytest.raises(NotImplementedError, match="room for" if n < room else f"{there} of {n} rows"):
+            a.take(cache)
+        assert not a.kernel.cache.length and a.kernel.first == 0
+        return
+    assert a.take(cache) == there and a.kernel.first == n - there
+    assert torch.equal(a.kernel.cache.k, _rows(n - there, n)) and torch.equal(a.kernel.cache.v, -_rows(n - there, n))
+
+
+@pytest.mark.parametrize("window", [None, 2, 3])
+@pytest.mark.parametrize("rows", [0, 3])
+def test_rows_that_the_tensors_do_not_hold_are_not_taken(rows, window):
+    """Few rows of a long sequence in a layer that is not a window's, or none of them."""
+    a = KernelAttention(_Block(window))
+    with pytest.raises(NotImplementedError, match=f"{rows} of 27 rows"):
+        a.take(_Residual(rows, 27))
+    assert not a.kernel.cache.length and a.kernel.first == 0
+    assert a.take(_Residual(0, 0)) == 0 and a.take(DynamicCache()) == 0
