@@ -87,7 +87,6 @@ class AttentionBlock:
         self.sinks = _lib.int64(sinks, "sinks")
         if (self.window is not None and self.window < 1) or self.sinks < 0:
             raise ValueError(f"window={window}, sinks={sinks}: a window holds 1 row at least, sinks are 0 or more")
-        self.first = 0                    # position of the cache's row 0 (take)
         self.quant = quant or QuantConfig()
         self.fmt = fmt or FixedFormat()
         self.ctx = ctx or default_context()
@@ -113,6 +112,11 @@ class AttentionBlock:
     @property
     def batch(self) -> int:
         return self.cache.batch
+
+    @property
+    def first(self) -> int:
+        """Position of the cache's row 0: 0, or where rows taken over into the empty cache began (take)."""
+        return self.cache.first
 
     def step(self, qi, ki, vi, *, stats: bool = True):
         """One decode token per sequence.
@@ -171,12 +175,14 @@ class AttentionBlock:
         """A dense cache's post-RoPE keys and values behind what the block's cache holds
         (CompressedCache.append_float), the first of them at position `first` of an empty cache: forward
         goes on behind them."""
-        if first < 0 or (first and any(self.cache.lengths())):
+        empty = not any(self.cache.lengths())
+        if first < 0 or (first and not empty):
             raise ValueError("first is the position of an empty cache's first row")
         if first and self.sinks:
             raise ValueError(f"rows from position {first} on do not hold the {self.sinks} first ones that stay visible")
         self.cache.append_float(k, v, seq=seq)
-        self.first = self.first or int(first)
+        if empty and any(self.cache.lengths()):
+            self.cache.first = int(first)
 
     def step_tree(self, qi, ki, vi, parents, *, stats: bool = True):
         """A draft of n nodes for every sequence: qi (batch, n, num_heads, d), ki/vi (batch, n,
@@ -330,4 +336,3 @@ class AttentionBlock:
     def reset(self) -> None:
         """kernel.py:454-456: a new sequence; tables survive."""
         self.cache.reset()
-        self.first = 0

@@ -236,6 +236,7 @@ class CompressedCache(KVCache):
         self.fmt = fmt or FixedFormat()
         self.batch = batch
         self.n_q_heads = n_q_heads if n_q_heads is not None else n_kv_heads * 4
+        self.first = 0                    # position of row 0 (AttentionBlock.take), while there are rows
         self.rotation = Rotation.for_quant(quant, head_dim)
         self.key_codebook = Codebook.build(quant.codebook, quant.key_bits,
                                            self.fmt.centroid_frac, quant.symmetric)
@@ -320,6 +321,11 @@ class CompressedCache(KVCache):
     def length(self) -> int:
         """Sequence 0's length (the reference cache holds one sequence)."""
         return self.lengths()[0]
+
+    def _dropped(self) -> None:
+        """After calls that may drop rows: what an empty cache receives begins at position 0 again."""
+        if self.first and not any(self.lengths()):
+            self.first = 0
 
     def append_rotated(self, k_rot, v_rot, trace=None, *, seq: int | None = None) -> None:
         """compressed.py:64-86: encode, pack and write rows at `length`.
@@ -518,6 +524,7 @@ class CompressedCache(KVCache):
                 self.handle, len(dst), many(*srcs), many(*dst), n,
                 ptr(rows) if rows is not None else None, stride, (ctypes.c_int64 * len(dst))(*counts) if n else None))
         self._keep_rows = rows
+        self._dropped()
 
     def keep(self, n: int, rows=None, *, counts=None) -> None:
         """Of the last n rows of every sequence only the listed ones stay, in the order given, and the
@@ -528,6 +535,7 @@ class CompressedCache(KVCache):
             _lib.check(self.ctx.lib.insitu_cache_keep(self.handle, n, ptr(rows) if rows is not None else None, stride,
                                                       (ctypes.c_int64 * self.batch)(*counts)))
         self._keep_rows = rows
+        self._dropped()
 
     def device_image(self):
         """The plane image of every sequence where it lies: a uint8 tensor (batch, seq_stride) over the
@@ -576,6 +584,7 @@ class CompressedCache(KVCache):
 
     def set_length(self, n: int, seq: int = 0) -> None:
         _lib.check(self.ctx.lib.insitu_cache_set_length(self.handle, seq, n))
+        self._dropped()
 
     def pin_kernel(self, path: str) -> None:
         """Test hook: the kernel of sequential-mode attends on this cache, "auto" (the
@@ -612,6 +621,7 @@ class CompressedCache(KVCache):
 
     def reset(self) -> None:
         _lib.check(self.ctx.lib.insitu_cache_reset(self.handle))
+        self._dropped()
 
     def layout(self) -> dict:
         """hw/ddr_layout.py:261-274 describe(), per sequence region."""
