@@ -193,14 +193,25 @@ def _float_rows(x) -> "_lib.FloatRows":
     return _lib.FloatRows(x.data_ptr() or None, s[0] if x.dim() == 4 else 0, s[-3], s[-2])
 
 
-def _overlaps(x) -> bool:
-    """Whether a tensor's last dimension has a stride, or two of its elements may lie in one place."""
+def _overlaps(x, y=None) -> bool:
+    """Whether a tensor's last dimension has a stride, or two of its elements may lie in one place; or an element of
+    it and one of y, a tensor of its shape and type."""
     if x.numel() == 0:
         return False
     if x.shape[-1] > 1 and x.stride(-1) != 1:
         return True
+    dims = [(s, n) for s, n in zip(x.stride(), x.shape) if n > 1]
+    if y is not None:
+        size = x.element_size()
+        lo, hi = sorted((x, y), key=lambda t: t.data_ptr())
+        step = hi.data_ptr() - lo.data_ptr()
+        if step >= size * (1 + sum(s * (n - 1) for s, n in zip(lo.stride(), lo.shape))):
+            return False                              # one ends before the other begins
+        if step % size or [s for s, n in zip(y.stride(), y.shape) if n > 1] != [s for s, _ in dims]:
+            return True
+        dims.append((step // size, 2))                # side by side: one more dimension
     reach = 0
-    for stride, size in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+    for stride, size in sorted(dims):
         if stride <= reach:
             return True
         reach += stride * (size - 1)
@@ -441,12 +452,12 @@ class CompressedCache(KVCache):
             if len(out) != 2 or dtype not in (None, out[0].dtype) or out[0].dtype != out[1].dtype:
                 raise ValueError("out is two tensors of one dtype")
             _float_type(out[0].dtype)
-            if out[0].numel() and out[0].data_ptr() == out[1].data_ptr():
-                raise ValueError("out's keys and values are in one place")
             for x in out:
                 if tuple(x.shape) != shape or x.device != self.ctx.torch_device or _overlaps(x):
                     raise ValueError(f"out must be two tensors {shape} on {self.ctx.torch_device}, a head's channels "
                                      f"together and no two elements in one place")
+            if _overlaps(*out):
+                raise ValueError("out's keys and values are in one place, or parts of them")
         if n == 0:
             return out
         with self.ctx.ordered(*out):
