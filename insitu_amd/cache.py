@@ -413,13 +413,16 @@ class CompressedCache(KVCache):
             (self.batch, "tokens", self.n_kv_heads, self.head_dim)
         if k.dim() != len(want) or any(a != b for a, b in zip(k.shape, want) if b != "tokens"):
             raise ValueError(f"expected {want}, got {tuple(k.shape)}")
+        n = int(k.shape[-3])
+        if n > self.capacity:                         # (a repeated row may have any number of tokens: more than 32 bits)
+            raise _lib.CapacityError(_lib.ECAPACITY, f"cache of {self.capacity} tokens; cannot append {n}")
         lost = ctypes.c_uint64() if counts else None
         if k.numel() == 0:
             return 0 if counts else None
         with self.ctx.ordered(k, v):
             _lib.check(self.ctx.lib.insitu_append_float(
                 self.handle, -1 if seq is None else self._seq(seq), ctypes.byref(_float_rows(k)), ctypes.byref(_float_rows(v)),
-                _float_type(k.dtype), int(k.shape[-3]), ctypes.byref(lost) if counts else None))
+                _float_type(k.dtype), n, ctypes.byref(lost) if counts else None))
         self._keep = (k, v)
         return int(lost.value) if counts else None
 
