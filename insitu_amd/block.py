@@ -133,12 +133,13 @@ class AttentionBlock:
         out = torch.empty_like(q)
         st = _lib.Stats() if stats else None
         stp = ctypes.byref(st) if st is not None else None
-        if self.window is None:
-            _lib.check(self.ctx.lib.insitu_step(self.cache.handle, ptr(q), ptr(k), ptr(v), ptr(out),
-                                                _lib.MODES[self.softmax], stp))
-        else:
-            _lib.check(self.ctx.lib.insitu_step_window(self.cache.handle, ptr(q), ptr(k), ptr(v), ptr(out), self.window,
-                                                       self.sinks, _lib.MODES[self.softmax], stp))
+        with self.ctx.ordered(q, k, v, out):
+            if self.window is None:
+                _lib.check(self.ctx.lib.insitu_step(self.cache.handle, ptr(q), ptr(k), ptr(v), ptr(out),
+                                                    _lib.MODES[self.softmax], stp))
+            else:
+                _lib.check(self.ctx.lib.insitu_step_window(self.cache.handle, ptr(q), ptr(k), ptr(v), ptr(out), self.window,
+                                                           self.sinks, _lib.MODES[self.softmax], stp))
         self._keep = (q, k, v)
         self.last_stats = AttentionStats.from_c(st) if st is not None else None
         return out.reshape(self.batch, m.num_heads * m.head_dim)
@@ -158,12 +159,14 @@ class AttentionBlock:
         k = self.ctx.to_device(ki, torch.int32).reshape(n, m.num_kv_heads, m.head_dim)
         v = self.ctx.to_device(vi, torch.int32).reshape(n, m.num_kv_heads, m.head_dim)
         base = self.cache.length
-        qr = self.rotation.apply(q, self.ctx)
-        self.cache.append_wire(k, v)            # rotate and append in one launch
-        if self._hides(base + n):
-            out, st = self.attn.attend_window(qr, self.window, self.sinks, self.softmax, stats=stats)
-        else:
-            out, st = self.attn.attend_prefill(qr, base, self.softmax, stats=stats)
+        # (what is made in here lies in the caller's stream's pool, whose later work comes behind the block's)
+        with self.ctx.ordered(q, k, v):
+            qr = self.rotation.apply(q, self.ctx)
+            self.cache.append_wire(k, v)        # rotate and append in one launch
+            if self._hides(base + n):
+                out, st = self.attn.attend_window(qr, self.window, self.sinks, self.softmax, stats=stats)
+            else:
+                out, st = self.attn.attend_prefill(qr, base, self.softmax, stats=stats)
         self.last_stats = st
         return out.reshape(n, m.num_heads * m.head_dim)
 
@@ -312,7 +315,8 @@ class AttentionBlock:
         if positions.shape != (n,):
             raise ValueError(f"expected {n} positions, got {positions.shape}")
         host = self.host
-        qi, ki, vi = host.wire(x, positions, counts=stats)
+        with self.ctx.ordered(x):
+            qi, ki, vi = host.wire(x, positions, counts=stats)
         self.taps = {"wire.q": qi, "wire.k": ki, "wire.v": vi}
         report = StepReport(n_tokens=n)
         if stats:
@@ -331,7 +335,9 @@ class AttentionBlock:
             out = rows[0] if n == 1 else torch.cat(rows, dim=0)
         self.taps["out"] = out
         report.context = base + n
-        return host.output(out), report
+        with self.ctx.ordered(out):
+            y = host.output(out)
+        return y, report
 
     def reset(self) -> None:
         """kernel.py:454-456: a new sequence; tables survive."""
