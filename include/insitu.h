@@ -248,14 +248,15 @@ int insitu_attend_tree(insitu_cache *cache, int32_t n, const int32_t *parents_de
  * counterpart in the reference, which attends all of a context). The last n rows of the sequence
  * are the queries' own, appended before: the query at row p attends, in row order, the rows t <= p
  * with t < sinks or t > p - window (its own among them: window is at least 1), exactly as
- * insitu_attend would in a cache that held those rows alone. A decode step is n = 1, a prompt its
+ * insitu_attend would in a cache that held those rows alone (SPLIT with SEQUENTIAL's integers). A decode step is n = 1, a prompt its
  * n tokens, a chunk of one the chunk's. q_rot_dev int32 (batch, n, n_q_heads, d) rotated, or (n,
  * n_q_heads, d) for one sequence; out_dev int32, the same shape, Q16 (q_rot_dev itself may be
  * given). EBADLEN when a sequence holds fewer than n rows. stats_host may be NULL: then nothing
  * synchronises, and once a call of the shape has allocated the cache's scratch nothing allocates
  * either, so that such a call may be captured into a graph. Its replays attend the lengths that the
  * cache has by then (n at least), share the scratch with insitu_attend_tree and with each other, and run one at a time,
- * in order with the cache's other calls. */
+ * in order with the cache's other calls. The scratch is the cache's, so each layer's: 17 MB for up to 256 tiles of 16
+ * query heads that share a KV head, 53 MB (d = 64) or 104 MB (d = 128) from 1,024 of them on; it is kept as a tree's is. */
 int insitu_attend_window(insitu_cache *cache, int32_t seq, int64_t n, int64_t window, int64_t sinks,
                          const int32_t *q_rot_dev, int32_t *out_dev, int32_t mode, insitu_stats *stats_host);
 

@@ -138,8 +138,8 @@ class CompressedAttention:
         """Queries of a layer with a sliding window, whose own rows are the last n of every sequence
         (or of sequence `seq`): q_rot (batch, n, n_q_heads, d) rotated, or (n, n_q_heads, d) of one
         sequence (seq, or a batch of one). The query at row p attends the rows t <= p with t < sinks or
-        t > p - window, in row order: the integers that `attend` gives in a cache of those rows alone,
-        in every mode. n = 1 is a decode step. Returns (out torch int32 of q_rot's shape,
+        t > p - window, in row order: the integers that `attend` gives in a cache of those rows alone
+        ("split" gives those of "online"). n = 1 is a decode step. Returns (out torch int32 of q_rot's shape,
         which may be q_rot itself, and AttentionStats or None). With stats=False nothing synchronises."""
         import torch
         c = self.cache

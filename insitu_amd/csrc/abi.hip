@@ -1256,6 +1256,9 @@ static int window_ok(int64_t window, int64_t sinks) {
 // 234 at d = 128; window 128: 42 against 44 and 67 against 67), to about four rounds where a row sees more (1,024 tiles,
 // window 4,096: 371 against 403 and 556 against 690, window 1,024 148 against 141 and 218 against 232, window 128 71
 // against 48 and 120 against 70), and lose from there on (2,048 tiles, window 1,024: 294 against 181 and 431 against 242).
+// Neither spreads a tile over workgroups, so that a token of one sequence has as many CUs as KV heads: 25 us against 99 over
+// a window of 1,024 (8 KV heads, d = 64), 52 against 322 over 4,096, 177 against 1,196 over 16,384, where an attend of all
+// of 32,768 rows, on the whole chip, takes 66.
 static bool window_spans(const insitu_cache *k, int64_t n, int64_t nseq, int64_t window) {
     const Geom &g = k->g;
     if (k->window_path) return k->window_path == 1;

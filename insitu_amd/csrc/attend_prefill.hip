@@ -35,8 +35,8 @@
 // proven is recomputed on the serial path (serial_head.h), as is one whose scores are not exact.
 //
 // What bounds it (SQ counters): VALU issue. A 4,096-token prompt takes a wave
-// some 330 VALU and 25 matrix instructions a 16 x 16 tile, its share of the staging and its events
-// included; they fill 62 % and 19 % of the SIMDs' cycles. 28 % of its tiles hold events (a count of
+// some 355 VALU and 25 matrix instructions a 16 x 16 tile, its share of the staging and its events
+// included; they fill 67 % and 19 % of the SIMDs' cycles. 28 % of its tiles hold events (a count of
 // random rows drawn as the benchmark's). A short prompt, two waves a SIMD or one, is bound by the
 // longest walk's own latency: 0.1 us a row at d = 64, 0.1 a row and pass at d = 128. One accumulator
 // instead of one a digit costs two VALU instructions a register and tile and frees 32 registers at

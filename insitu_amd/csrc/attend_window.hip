@@ -33,6 +33,9 @@
 // prefill kernel, whose workgroup's 64 rows are 4 here, 326. One query over a window of 128 in 300 rows, 15.8 us with the
 // call, is mostly instructions that come from memory once: loops that are not unrolled are faster there. At d = 128, or
 // with 8 codes a value, eight waves: twelve have too few registers.
+// A tile's window stays on one CU however long it is, so that one sequence's token takes as long as that of 32 (52 us of
+// 4,096 rows, on 8 CUs) and longer than all of a long context, which the dense attends spread over the chip (16,384 rows
+// 177 us, 32,768 rows there 66). Nothing in the integers asks for that, two-pass least of all, whose sums have no order.
 #include <algorithm>
 #include <cmath>
 
