@@ -118,6 +118,10 @@ class AttentionBlock:
         """Position of the cache's row 0: 0, or where rows taken over into the empty cache began (take)."""
         return self.cache.first
 
+    @first.setter
+    def first(self, position: int) -> None:
+        self.cache.first = int(position)
+
     def step(self, qi, ki, vi, *, stats: bool = True):
         """One decode token per sequence.
 

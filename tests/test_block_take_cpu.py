@@ -119,3 +119,14 @@ def test_a_batch_is_empty_when_every_sequence_is():
     b.take(_rows(5), _rows(5), first=7, seq=0)
     b.cache.fork(1, [0])                              # the empty sequence over the one with rows
     assert b.cache.lengths() == [0, 0] and b.first == 0
+
+
+def test_a_position_that_is_set():
+    """Of rows that came another way: until they are dropped."""
+    b = _block()
+    b.cache.append_float(_rows(3), _rows(3))
+    b.first = 30
+    b.take(_rows(2), _rows(2))
+    assert b.first == 30
+    b.cache.reset()
+    assert b.first == 0
