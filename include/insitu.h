@@ -255,8 +255,8 @@ int insitu_attend_tree(insitu_cache *cache, int32_t n, const int32_t *parents_de
  * synchronises, and once a call of the shape has allocated the cache's scratch nothing allocates
  * either, so that such a call may be captured into a graph. Its replays attend the lengths that the
  * cache has by then (n at least), share the scratch with insitu_attend_tree and with each other, and run one at a time,
- * in order with the cache's other calls. The scratch is the cache's, so each layer's: 17 MB for up to 256 tiles of 16
- * query heads that share a KV head, 53 MB (d = 64) or 104 MB (d = 128) from 1,024 of them on; it is kept as a tree's is. */
+ * in order with the cache's other calls. The scratch is the cache's, so each layer's: 17 MB (d = 64) or 26 MB (d = 128) for
+ * 256 tiles of up to 16 query heads that share a KV head, 53 MB or 104 MB from 1,024 tiles on; it is kept as a tree's is. */
 int insitu_attend_window(insitu_cache *cache, int32_t seq, int64_t n, int64_t window, int64_t sinks,
                          const int32_t *q_rot_dev, int32_t *out_dev, int32_t mode, insitu_stats *stats_host);
 
